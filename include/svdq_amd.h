@@ -39,7 +39,7 @@ extern "C" {
 #define SVDQ_EUNSUPPORTED -2 /* valid request that this build does not implement */
 #define SVDQ_ELAUNCH -3      /* the HIP runtime refused the launch */
 
-#define SVDQ_ABI_VERSION 5
+#define SVDQ_ABI_VERSION 6
 
 int svdq_abi_version(void);
 const char *svdq_last_error(void);
@@ -277,7 +277,78 @@ typedef struct svdq_awq_gemv_args {
 
 int svdq_awq_gemv_w4a16(const svdq_awq_gemv_args *args, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * 8-bit linear layers: int8 codes with one fp32 scale per token (activations) and per output channel (weights).
+ * The types of activations, outputs, norm weights and biases: */
+#define SVDQ_BF16 0
+#define SVDQ_FP16 1
 
+/* Rows to codes.  svdq_quantize_w8a8_act: g = input.  svdq_rms_norm_quantize_w8a8: h = input + residual, rounded to the type and
+ * stored in residual_out (h = input without a residual), g = h * weight.  For every row
+ *   a = max(max_k |g|, 2^-100),  output = rne(g * fl32(127 / a)),  oscales = a * f / 127,
+ * with f = 1, or 1 / sqrt(mean(h^2) + eps) behind the norm (a factor of the whole row, which cancels in the codes).  A row in which g
+ * holds an infinity or a NaN, or whose sum of squares overflows fp32, gets the scale NaN and codes 0. */
+typedef struct svdq_quantize_w8a8_args {
+    const void *input;      /* [M, K], rows ld_input elements apart                                  */
+    const void *residual;   /* [M, K], rows ld_residual apart, or NULL (plain form: always NULL)     */
+    const void *weight;     /* [K]; the plain form ignores it                                        */
+    void *residual_out;     /* [M, K], rows ld_residual_out apart; may be residual or input itself; NULL without residual */
+    void *output;           /* int8 [M, K] row-major                                                 */
+    float *oscales;         /* fp32 [M]                                                              */
+    int64_t M, K;           /* K: a multiple of 16 up to 65536                                       */
+    int64_t ld_input, ld_residual, ld_residual_out; /* elements, multiples of 8                      */
+    float eps;
+    int32_t dtype;          /* SVDQ_BF16 or SVDQ_FP16                                                */
+} svdq_quantize_w8a8_args;
+
+int svdq_quantize_w8a8_act(const svdq_quantize_w8a8_args *args, void *stream);
+int svdq_rms_norm_quantize_w8a8(const svdq_quantize_w8a8_args *args, void *stream);
+
+/* out[m, n] = T(float(sum_k act[m, k] * wgt[n, k]) * (ascales[m] * wscales[n]) + bias[n]).  The integer sums are exact. */
+typedef struct svdq_gemm_w8a8_args {
+    const void *act;        /* int8 [M, K], rows ld_act bytes apart                                  */
+    const void *wgt;        /* int8 [N, K], rows ld_wgt bytes apart                                  */
+    const float *ascales;   /* fp32 [M]                                                              */
+    const float *wscales;   /* fp32 [N]                                                              */
+    const void *bias;       /* [N] of the type of out, or NULL                                       */
+    void *out;              /* bf16 or fp16 [M, N], rows ld_out elements apart                       */
+    int64_t M, N, K;        /* K: a multiple of 16 below 131072; M and N: any                        */
+    int64_t ld_act, ld_wgt, ld_out; /* ld_act, ld_wgt: multiples of 16 below 2^23                    */
+    int32_t dtype;          /* of out and bias: SVDQ_BF16 or SVDQ_FP16                               */
+} svdq_gemm_w8a8_args;
+
+int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Softmax attention of q_len queries per batch entry to the keys of an encoder, which have a length of their own:
+ *   out[b][t][h] = sum_j p_j v[b][j][h / G],  p = softmax over the valid j of scale * q[b][t][h] . k[b][j][h / G],  G = heads / kv_heads.
+ * A query without a valid key gets zeros.  Keys are valid up to key_lengths[b] or where key_mask[b] says so; what k and v hold in
+ * other places (NaN, infinities) is not read into any result.  With cu_seqlens_k the sequences of keys stand one behind the other.
+ * No global state: a call that divides the keys among workgroups puts its partial sums where the caller says.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct svdq_cross_attention_args {
+    const void *q;          /* [batch][q_len][heads][head_dim] by strides                            */
+    const void *k, *v;      /* [batch][k_len][kv_heads][head_dim] by strides; with cu_seqlens_k: k_len is the number of
+                               rows of all sequences together and the batch strides are ignored       */
+    void *out;              /* as q                                                                  */
+    const int32_t *key_lengths;  /* [batch] or NULL; values outside 0..k_len count as the nearer of the two   */
+    const void *key_mask;   /* bytes [batch][k_len], batch entries mask_stride apart, 0: masked; or NULL      */
+    const int32_t *cu_seqlens_k; /* [batch + 1] ascending offsets, or NULL (offsets out of range or order give fewer keys) */
+    void *workspace;        /* svdq_cross_attention_workspace bytes (16-byte aligned), not shared with a call that may run at
+                               the same time; NULL if that is 0                                       */
+    int64_t workspace_bytes;
+    int64_t batch, heads, kv_heads, head_dim; /* head_dim: a multiple of 8 up to 128                 */
+    int64_t q_len, k_len;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head: elements, multiples of 8; elements
+                                                                     of a head are next to each other             */
+    int64_t mask_stride;
+    float scale;            /* positive                                                              */
+    int32_t dtype;          /* of q, k, v, out: SVDQ_BF16 or SVDQ_FP16                               */
+} svdq_cross_attention_args;
+
+/* What a call with these arguments on the current device needs as its workspace (depends on shapes alone). */
+int svdq_cross_attention_workspace(const svdq_cross_attention_args *args, int64_t *bytes);
+int svdq_cross_attention(const svdq_cross_attention_args *args, void *stream);
 
 
 #ifdef __cplusplus

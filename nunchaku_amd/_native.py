@@ -18,19 +18,20 @@ import torch
 _PKG_DIR = Path(__file__).resolve().parent
 _CSRC = _PKG_DIR / "csrc"
 LIB_PATH = _PKG_DIR / "libsvdq_amd.so"
-SOURCES = ["repack.hip", "quantize.hip", "gemm.hip", "awq_gemv.hip", "litela.hip"]
+SOURCES = ["repack.hip", "quantize.hip", "gemm.hip", "awq_gemv.hip", "litela.hip", "w8a8_quantize.hip", "w8a8_gemm.hip", "attention.hip"]
 HIPCC_FLAGS = [
     "-shared", "-fPIC", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
-SVDQ_ABI_VERSION = 5
+SVDQ_ABI_VERSION = 6
 EXPORTED_SYMBOLS = [
     "svdq_abi_version", "svdq_last_error",
     "svdq_repack_qweight", "svdq_repack_wscales", "svdq_repack_wmscales", "svdq_repack_vector",
     "svdq_repack_smooth", "svdq_repack_lora_down", "svdq_repack_lora_up", "svdq_repack_rotemb",
     "svdq_quantize_w4a4_act_fuse_lora", "svdq_gemm_w4a4", "svdq_gemm_w4a4_noalloc", "svdq_awq_gemv_w4a16",
     "svdq_linearattn_vk_mul_q", "svdq_release_workspaces",
+    "svdq_quantize_w8a8_act", "svdq_rms_norm_quantize_w8a8", "svdq_gemm_w8a8", "svdq_cross_attention_workspace", "svdq_cross_attention",
 ]
 
 
@@ -81,6 +82,41 @@ class AwqGemvArgs(ctypes.Structure):
         ("x", ctypes.c_void_p), ("qweight", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
         ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
         ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("group_size", ctypes.c_int32),
+    ]
+
+
+class QuantizeW8A8Args(ctypes.Structure):
+    """Mirror of ``svdq_quantize_w8a8_args``."""
+
+    _fields_ = [
+        ("input", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("residual_out", ctypes.c_void_p),
+        ("output", ctypes.c_void_p), ("oscales", ctypes.c_void_p), ("M", ctypes.c_int64), ("K", ctypes.c_int64),
+        ("ld_input", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ld_residual_out", ctypes.c_int64),
+        ("eps", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class GemmW8A8Args(ctypes.Structure):
+    """Mirror of ``svdq_gemm_w8a8_args``."""
+
+    _fields_ = [
+        ("act", ctypes.c_void_p), ("wgt", ctypes.c_void_p), ("ascales", ctypes.c_void_p), ("wscales", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64),
+        ("ld_act", ctypes.c_int64), ("ld_wgt", ctypes.c_int64), ("ld_out", ctypes.c_int64), ("dtype", ctypes.c_int32),
+    ]
+
+
+class CrossAttentionArgs(ctypes.Structure):
+    """Mirror of ``svdq_cross_attention_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("key_lengths", ctypes.c_void_p), ("key_mask", ctypes.c_void_p), ("cu_seqlens_k", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+        ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+        ("q_len", ctypes.c_int64), ("k_len", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3), ("out_stride", ctypes.c_int64 * 3),
+        ("mask_stride", ctypes.c_int64), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
     ]
 
 
@@ -177,6 +213,11 @@ def lib() -> ctypes.CDLL:
         L.svdq_awq_gemv_w4a16.argtypes = [ctypes.POINTER(AwqGemvArgs), vp]
         L.svdq_linearattn_vk_mul_q.argtypes = [vp, vp, i64, i64, i64, i64, ctypes.c_float, vp]
         L.svdq_release_workspaces.argtypes = []
+        L.svdq_quantize_w8a8_act.argtypes = [ctypes.POINTER(QuantizeW8A8Args), vp]
+        L.svdq_rms_norm_quantize_w8a8.argtypes = [ctypes.POINTER(QuantizeW8A8Args), vp]
+        L.svdq_gemm_w8a8.argtypes = [ctypes.POINTER(GemmW8A8Args), vp]
+        L.svdq_cross_attention_workspace.argtypes = [ctypes.POINTER(CrossAttentionArgs), ctypes.POINTER(i64)]
+        L.svdq_cross_attention.argtypes = [ctypes.POINTER(CrossAttentionArgs), vp]
         for name in EXPORTED_SYMBOLS:
             getattr(L, name)
             if name not in ("svdq_last_error",):

@@ -1,0 +1,585 @@
+// Softmax attention of queries to the keys of an encoder: out[b][t][h] = sum_j p_j v[b][j][h / G], p = softmax over the valid keys j
+// of scale * q[b][t][h] . k[b][j][h / G]; zero where no key is valid.  G = heads / kv_heads query heads share a head of keys and
+// values: a "row" below is one (token, head of the group) pair, row r = t * G + g of key head h / G.
+//
+// One pass over the keys, 64 at a time, with the running maximum and sum of the softmax in fp32.  The scores are formed as K q^T on
+// v_mfma_f32_32x32x16: a lane then holds 32 keys' scores of ONE row (the other 32 are 32 lanes away), so the maximum and the sum
+// take one exchange between lanes, and the scores, rounded to the inputs' type, are the right operand of v^T p^T as they are: the
+// instruction contracts 8 keys per lane, which 8 is free, as long as the left operand holds the same.  That operand is v down the
+// columns, which LDS reads that transpose 4 x 16 blocks (ds_read_b64_tr_b16) make of plain rows.
+// The probabilities are rounded to the inputs' type for that product (half a step relative each, like the result), sums stay in fp32.
+//
+// Rows of K and V in LDS: pieces of 16 bytes, piece c of row r at place c ^ f(r), so that neither 16 lanes that read one piece of 16
+// rows (K) nor 32 lanes that read 64 bytes of 4 rows (V) meet in a bank.  What no key stands for (rows behind the last key, masked
+// ones, columns behind the head's) is read from a block of zeros, whatever the tensors hold there.
+#include "svdq_common.h"
+
+using namespace svdq;
+
+namespace {
+
+struct AttentionParams {
+    const char *q, *k, *v;
+    char *out;
+    const int *key_lengths, *cu_seqlens;
+    const uint8_t *mask;
+    float *partial;                                // keys-split form with several parts: [part][b][hkv][rows] x D, then {maximum, sum} pairs
+    long long qs[3], ks[3], vs[3], os[3], mask_b;  // bytes: batch, token, head
+    int B, Hkv, G, D, Tq, Tk, rows, row_blocks, parts;
+    float scale2;  // scale * log2(e)
+};
+
+__device__ const u32x4_t zeros16 = {0, 0, 0, 0};
+
+constexpr int KEYS = 64;  // per step
+
+template <bool BF16>
+struct Elem;
+template <>
+struct Elem<true> {
+    typedef bf16x8_t vec;
+    static __device__ inline float16_t mfma(vec a, vec b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ inline uint32_t pair(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <>
+struct Elem<false> {
+    typedef half8_t vec;
+    static __device__ inline float16_t mfma(vec a, vec b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ inline uint32_t pair(float lo, float hi) {
+        typedef float float2_t __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{lo, hi}, half2_t));
+    }
+};
+
+// A head of DP elements (rounded up): KS steps of 16 in the first product, DB blocks of 32 in the second; rows PITCH bytes apart in LDS.
+template <int DP>
+struct Head {
+    static constexpr int KS = DP / 16, DB = (DP + 31) / 32, PITCH = DP <= 32 ? 64 : DP <= 64 ? 128 : 256, PIECES = PITCH / 16;
+    static constexpr int TILE = KEYS * PITCH, REQ = TILE / 1024, RPR = 1024 / PITCH;  // a tile of K or V: bytes, requests of a KB, rows per request
+    static __host__ __device__ constexpr int fk(int row) { return PITCH == 256 ? row & 15 : PITCH == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+    static __host__ __device__ constexpr int fv(int row) { return PITCH == 256 ? 4 * (row & 3) : PITCH == 128 ? 4 * ((row >> 1) & 1) : 0; }
+};
+
+__device__ inline void copy16(uint32_t dst, const char *base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ inline void copy16(uint32_t dst, const char *src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
+}
+
+__device__ inline float exchange_max(float x) {
+    const float o = __shfl_xor(x, 32);
+    return x > o ? x : o;
+}
+
+// The keys of batch entry b: the first one's row in the tensors (packed sequences) and how many there are.
+__device__ inline void keys_of(const AttentionParams &p, int b, long long &first, int &count) {
+    first = 0;
+    count = p.Tk;
+    if (p.cu_seqlens) {  // (offsets that are not in order or beyond the end give fewer keys, never others)
+        int lo = p.cu_seqlens[b], hi = p.cu_seqlens[b + 1];
+        lo = lo < 0 ? 0 : lo > p.Tk ? p.Tk : lo;
+        hi = hi < lo ? lo : hi > p.Tk ? p.Tk : hi;
+        first = lo;
+        count = hi - lo;
+    } else if (p.key_lengths) {
+        const int n = p.key_lengths[b];
+        count = n < 0 ? 0 : n < p.Tk ? n : p.Tk;
+    }
+    count = __builtin_amdgcn_readfirstlane(count);
+}
+
+// Running softmax and output of 32 rows: lane l holds row l % 32; of the output's block db element e is column 32 db + 8 (e / 4) + 4 (l / 32) + e % 4.
+template <bool BF16, int DP>
+struct State {
+    using H = Head<DP>;
+    using E = Elem<BF16>;
+    using vec = typename E::vec;
+    float16_t o[H::DB];
+    float top, sum;  // in units of log2; this lane's part of the sum
+    __device__ inline void clear() {
+#pragma unroll
+        for (int d = 0; d < H::DB; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+        top = -__builtin_huge_valf();
+        sum = 0.f;
+    }
+    // one step of 64 keys: scores s (block kb, element e: key 32 kb + 8 (e / 4) + 4 (lane / 32) + e % 4), v in LDS
+    __device__ inline void add(float16_t (&s)[2], float scale2, const char *v, int lane) {
+        float m = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) m = __builtin_fmaxf(m, s[i][e]);
+        m = exchange_max(m) * scale2;
+        if (__any(m > top)) {
+            const float now = m > top ? m : top;
+            const float f = top == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < H::DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= f;
+        }
+        const float ref = top == -__builtin_huge_valf() ? 0.f : top;  // (no valid key yet)
+        const int g = lane >> 4, i = lane & 15, h = lane >> 5;
+        const char *vrow = v + (4 * h + (i >> 2)) * H::PITCH + (i & 1) * 8;
+        const int piece = (g & 1) * 2 + ((i >> 1) & 1), f = H::fv(i >> 2);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                uint32_t w[4];
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + e], scale2, -ref));
+                    sum += x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = E::pair(x[2 * e], x[2 * e + 1]);
+                const vec pr = __builtin_bit_cast(vec, u32x4_t{w[0], w[1], w[2], w[3]});
+                typedef short short4_t __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) short4_t *lds_t;
+#pragma unroll
+                for (int d = 0; d < H::DB; d++) {
+                    const char *at = vrow + (32 * kb + 16 * st) * H::PITCH + ((4 * d + piece) ^ f) * 16;
+                    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
+                    const vec vv = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[d] = E::mfma(vv, pr, o[d]);
+                }
+            }
+    }
+};
+
+// This lane's row of queries as the right operand: elements 16 ks + 8 (lane / 32) ... + 7
+template <bool BF16, int DP>
+__device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec (&qf)[Head<DP>::KS], int b, int hk, int row, int lane) {
+    const int t = row / p.G, gq = row - t * p.G;
+    const char *q = p.q + b * p.qs[0] + t * p.qs[1] + (long long)(hk * p.G + gq) * p.qs[2];
+#pragma unroll
+    for (int ks = 0; ks < Head<DP>::KS; ks++) {
+        const int c = 16 * ks + 8 * (lane >> 5);
+        u32x4_t w = u32x4_t{0, 0, 0, 0};
+        if (row < p.rows && c < p.D) w = *(const u32x4_t *)(q + c * 2);
+        qf[ks] = __builtin_bit_cast(typename Elem<BF16>::vec, w);
+    }
+}
+
+// This lane's row of the output, normalised: 8 consecutive columns per lane and 16-byte store
+template <bool BF16, int DP>
+__device__ inline void store_row(const AttentionParams &p, State<BF16, DP> &s, float sum, int b, int hk, int row, int lane) {
+    const int t = row / p.G, gq = row - t * p.G, h = lane >> 5;
+    char *out = p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
+    const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;  // (a NaN stays one)
+#pragma unroll
+    for (int d = 0; d < Head<DP>::DB; d++)
+#pragma unroll
+        for (int gp = 0; gp < 2; gp++) {
+            // columns 32 d + 16 gp + [0, 4) + 4 h and 8 more: the half-waves exchange, so that each has 8 in a row
+            uint32_t lo[2], hi[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                lo[j] = Elem<BF16>::pair(s.o[d][8 * gp + 2 * j] * r, s.o[d][8 * gp + 2 * j + 1] * r);
+                hi[j] = Elem<BF16>::pair(s.o[d][8 * gp + 4 + 2 * j] * r, s.o[d][8 * gp + 4 + 2 * j + 1] * r);
+            }
+            u32x4_t w;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint32_t give = h ? lo[j] : hi[j], got = (uint32_t)__shfl_xor((int)give, 32);
+                w[j] = h ? got : lo[j];
+                w[2 + j] = h ? hi[j] : got;
+            }
+            const int c = 32 * d + 16 * gp + 8 * h;
+            if (row < p.rows && c < p.D) *(u32x4_t *)(out + c * 2) = w;
+        }
+}
+
+// Which (row block, head, batch entry) a workgroup takes: workgroups go round robin over 8 XCDs, each with an L2 of its own, and an
+// XCD gets a contiguous run, whose row blocks read the same keys.
+__device__ inline void block_of(const AttentionParams &p, int per_head, int &rb, int &hk, int &b) {
+    const int total = per_head * p.Hkv * p.B, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
+    const int at = xcd * per + (xcd < more ? xcd : more) + (id >> 3);
+    rb = at % per_head;
+    const int bh = at / per_head;
+    hk = bh % p.Hkv;
+    b = bh / p.Hkv;
+}
+
+// ---- rows form: 128 rows per workgroup, 32 per wave; all waves share the keys through LDS, two steps of them -------------------
+template <bool BF16, int DP, bool MASK>
+__global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams p) {
+    using H = Head<DP>;
+    using E = Elem<BF16>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    int rb, hk, b;
+    block_of(p, p.row_blocks, rb, hk, b);
+    long long first;
+    int count;
+    keys_of(p, b, first, count);
+    const int row = rb * 128 + wave * 32 + col;
+    typename E::vec qf[H::KS];
+    load_q<BF16, DP>(p, qf, b, hk, row, lane);
+    const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
+    const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
+    const uint8_t *mask = MASK ? p.mask + b * p.mask_b : nullptr;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    constexpr int REQ = H::REQ / 4;  // per wave, of K and of V
+    int rowi[REQ], ck[REQ], cv[REQ];
+    uint32_t ok[REQ], ov[REQ];
+#pragma unroll
+    for (int i = 0; i < REQ; i++) {
+        rowi[i] = (wave * REQ + i) * H::RPR + lane / H::PIECES;
+        ck[i] = ((lane % H::PIECES) ^ H::fk(rowi[i])) * 16;
+        cv[i] = ((lane % H::PIECES) ^ H::fv(rowi[i])) * 16;
+        ok[i] = (uint32_t)(rowi[i] * p.ks[1]) + ck[i];
+        ov[i] = (uint32_t)(rowi[i] * p.vs[1]) + cv[i];
+    }
+    const int steps = (count + KEYS - 1) / KEYS, bytes = p.D * 2;
+    const bool padded = bytes < H::PITCH;
+    auto request = [&](int step) __attribute__((always_inline)) {
+        const uint32_t dst = base + (step & 1) * 2 * H::TILE + wave * REQ * 1024;
+        const char *k = kp + (long long)step * KEYS * p.ks[1], *v = vp + (long long)step * KEYS * p.vs[1];
+        if (!MASK && !padded && (step + 1) * KEYS <= count) {
+#pragma unroll
+            for (int i = 0; i < REQ; i++) copy16(dst + i * 1024, k, ok[i]);
+#pragma unroll
+            for (int i = 0; i < REQ; i++) copy16(dst + H::TILE + i * 1024, v, ov[i]);
+        } else {
+            bool in[REQ];
+#pragma unroll
+            for (int i = 0; i < REQ; i++) {
+                const int key = step * KEYS + rowi[i];
+                in[i] = key < count;
+                if (MASK && in[i]) in[i] = mask[key] != 0;
+            }
+#pragma unroll
+            for (int i = 0; i < REQ; i++) copy16(dst + i * 1024, in[i] && ck[i] < bytes ? k + ok[i] : (const char *)&zeros16);
+#pragma unroll
+            for (int i = 0; i < REQ; i++) copy16(dst + H::TILE + i * 1024, in[i] && cv[i] < bytes ? v + ov[i] : (const char *)&zeros16);
+        }
+    };
+    State<BF16, DP> st;
+    st.clear();
+    if (steps > 0) request(0);
+    for (int step = 0; step < steps; step++) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + 1 < steps) request(step + 1);
+        const char *k = lds + (step & 1) * 2 * H::TILE, *v = k + H::TILE;
+        float16_t s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int ks = 0; ks < H::KS; ks++) {
+                const u32x4_t w = *(const u32x4_t *)(k + (kb * 32 + col) * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16);
+                s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[kb]);
+            }
+        if (MASK || (step + 1) * KEYS > count) {
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int key = step * KEYS + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
+                    bool in = key < count;
+                    if (MASK && in) in = mask[key] != 0;
+                    if (!in) s[kb][e] = -__builtin_huge_valf();
+                }
+        }
+        st.add(s, p.scale2, v, lane);
+    }
+    const float sum = st.sum + __shfl_xor(st.sum, 32);
+    store_row<BF16, DP>(p, st, sum, b, hk, row, lane);
+}
+
+// ---- keys form: 32 rows per workgroup, whose waves take every fourth step of the part's keys and meet in LDS; the parts of a row
+// block meet in attention_join_kernel -----------------------------------------------------------------------------------------------
+template <bool BF16, int DP, bool MASK>
+__global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams p) {
+    using H = Head<DP>;
+    using E = Elem<BF16>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    int rb, hk, b;
+    block_of(p, p.row_blocks * p.parts, rb, hk, b);
+    const int part = rb / p.row_blocks;
+    rb -= part * p.row_blocks;
+    long long first;
+    int count;
+    keys_of(p, b, first, count);
+    const int row = rb * 32 + col;
+    typename E::vec qf[H::KS];
+    load_q<BF16, DP>(p, qf, b, hk, row, lane);
+    const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
+    const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
+    const uint8_t *mask = MASK ? p.mask + b * p.mask_b : nullptr;
+    const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * H::TILE;
+    const char *varea = lds + wave * H::TILE;
+    const int steps = (count + KEYS - 1) / KEYS, bytes = p.D * 2;
+    const int begin = (int)((long long)steps * part / p.parts), end = (int)((long long)steps * (part + 1) / p.parts);
+    State<BF16, DP> st;
+    st.clear();
+    for (int step = begin + wave; step < end; step += 4) {
+        const char *k = kp + (long long)step * KEYS * p.ks[1], *v = vp + (long long)step * KEYS * p.vs[1];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads are done
+#pragma unroll
+        for (int i = 0; i < H::REQ; i++) {
+            const int r = i * H::RPR + lane / H::PIECES, c = ((lane % H::PIECES) ^ H::fv(r)) * 16, key = step * KEYS + r;
+            bool in = key < count && c < bytes;
+            if (MASK && in) in = mask[key] != 0;
+            copy16(area + i * 1024, in ? v + r * p.vs[1] + c : (const char *)&zeros16);
+        }
+        u32x4_t w[2][H::KS];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            const int key = step * KEYS + 32 * kb + col;
+            bool in = key < count;
+            if (MASK && in) in = mask[key] != 0;
+#pragma unroll
+            for (int ks = 0; ks < H::KS; ks++) {
+                const int c = (2 * ks + h) * 16;
+                w[kb][ks] = u32x4_t{0, 0, 0, 0};
+                if (in && c < bytes) w[kb][ks] = *(const u32x4_t *)(k + (32 * kb + col) * p.ks[1] + c);
+            }
+        }
+        float16_t s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < H::KS; ks++) s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w[kb][ks]), qf[ks], s[kb]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = step * KEYS + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
+                bool in = key < count;
+                if (MASK && in) in = mask[key] != 0;
+                if (!in) s[kb][e] = -__builtin_huge_valf();
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        st.add(s, p.scale2, varea, lane);
+    }
+    // the waves meet: {maximum, sum} first, then the outputs, in the place of V
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    float *stat = (float *)lds;  // [4][2][32]
+    const float own = st.sum + __shfl_xor(st.sum, 32);
+    if (h == 0) {
+        stat[wave * 64 + col] = st.top;
+        stat[wave * 64 + 32 + col] = own;
+    }
+    __syncthreads();
+    float top = -__builtin_huge_valf(), sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, stat[i * 64 + col]);
+    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum += stat[i * 64 + 32 + col] * __builtin_amdgcn_exp2f(stat[i * 64 + col] - ref);
+    const float f = __builtin_amdgcn_exp2f(st.top - ref);
+    float *sums = (float *)lds + 256;  // [32 DB][33] of one wave at a time
+    for (int i = 1; i < 4; i++) {
+        __syncthreads();
+        if (wave == i) {
+#pragma unroll
+            for (int d = 0; d < H::DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sums[((d * 16 + e) * 64) + lane] = st.o[d][e] * f;
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int d = 0; d < H::DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if (i == 1) st.o[d][e] *= f;
+                    st.o[d][e] += sums[((d * 16 + e) * 64) + lane];
+                }
+        }
+    }
+    if (wave > 0) return;
+    if (p.parts == 1) {
+        store_row<BF16, DP>(p, st, sum, b, hk, row, lane);
+        return;
+    }
+    if (row >= p.rows) return;
+    const long long heads = (long long)p.B * p.Hkv, at = ((long long)part * heads + (long long)b * p.Hkv + hk) * p.rows + row;
+    float *dst = p.partial + at * p.D;
+#pragma unroll
+    for (int d = 0; d < H::DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int c = 32 * d + 8 * g + 4 * h;
+            if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+        }
+    if (h == 0) {
+        float *ms = p.partial + (long long)p.parts * heads * p.rows * p.D + at * 2;
+        ms[0] = top;
+        ms[1] = sum;
+    }
+}
+
+// Adds the parts of every row: one wave per row, two columns per lane
+template <bool BF16>
+__global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) {
+    const int lane = threadIdx.x & 63;
+    const long long heads = (long long)p.B * p.Hkv, all = heads * p.rows, at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= all) return;
+    const float *ms = p.partial + p.parts * all * p.D;
+    float top = -__builtin_huge_valf();
+    for (int i = 0; i < p.parts; i++) top = __builtin_fmaxf(top, ms[(i * all + at) * 2]);
+    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+    float sum = 0.f, x = 0.f, y = 0.f;
+    const int c = lane * 2;
+    for (int i = 0; i < p.parts; i++) {
+        const float f = __builtin_amdgcn_exp2f(ms[(i * all + at) * 2] - ref);
+        sum += ms[(i * all + at) * 2 + 1] * f;
+        if (c < p.D) {
+            const float *src = p.partial + (i * all + at) * p.D + c;
+            x += src[0] * f;
+            y += src[1] * f;
+        }
+    }
+    const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
+    const int bh = (int)(at / p.rows), row = (int)(at - (long long)bh * p.rows), b = bh / p.Hkv, hk = bh - b * p.Hkv, t = row / p.G, g = row - t * p.G;
+    if (c < p.D) *(uint32_t *)(p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + g) * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
+}
+
+template <bool BF16, int DP, bool MASK>
+int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
+    using H = Head<DP>;
+    const int lds = keys ? 4 * H::TILE > 1024 + H::DB * 4096 ? 4 * H::TILE : 1024 + H::DB * 4096 : 4 * H::TILE;
+    const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
+    if (lds > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(SVDQ_ELAUNCH, "cross_attention: the device does not offer %d bytes of LDS", lds);
+    }
+    const dim3 grid((unsigned)((long long)p.row_blocks * p.parts * p.Hkv * p.B)), block(256);
+    if (!keys) {
+        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
+        return check_launch("cross_attention");
+    }
+    SVDQ_LAUNCH((attention_keys_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
+    int rc = check_launch("cross_attention");
+    if (rc || p.parts == 1) return rc;
+    SVDQ_LAUNCH((attention_join_kernel<BF16>), dim3((unsigned)(((long long)p.B * p.Hkv * p.rows + 3) / 4)), block, 0, st, p);
+    return check_launch("cross_attention");
+}
+
+template <bool BF16, bool MASK>
+int launch_heads(const AttentionParams &p, bool keys, hipStream_t st) {
+    if (p.D <= 32) return launch_kernels<BF16, 32, MASK>(p, keys, st);
+    if (p.D <= 64) return launch_kernels<BF16, 64, MASK>(p, keys, st);
+    if (p.D <= 80) return launch_kernels<BF16, 80, MASK>(p, keys, st);
+    if (p.D <= 96) return launch_kernels<BF16, 96, MASK>(p, keys, st);
+    return launch_kernels<BF16, 128, MASK>(p, keys, st);
+}
+
+// Which form a call takes and how many parts it divides the keys into.  The rows form reads K and V from memory once per 128 rows; it
+// wants enough of such blocks to fill the compute units.
+struct Plan {
+    bool keys;
+    long long row_blocks, parts, workspace;
+};
+Plan plan_of(const svdq_cross_attention_args *a, int cus) {
+    const long long rows = a->q_len * (a->heads / a->kv_heads), bh = a->batch * a->kv_heads;
+    const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len, steps = (keys_each + KEYS - 1) / KEYS;
+    Plan plan;
+    plan.keys = rows <= 32 || (rows + 127) / 128 * bh < cus;
+    plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
+    plan.parts = 1;
+    if (plan.keys) {
+        const long long want = (4 * cus + plan.row_blocks * bh - 1) / (plan.row_blocks * bh), most = (steps + 3) / 4;
+        plan.parts = want < most ? want : most;
+        if (plan.parts < 1) plan.parts = 1;
+    }
+    plan.workspace = plan.parts > 1 ? plan.parts * bh * rows * (a->head_dim + 2) * 4 : 0;
+    return plan;
+}
+
+int check_args(const svdq_cross_attention_args *a) {
+    SVDQ_REQUIRE(a && a->q && a->k && a->v && a->out, "cross_attention: q, k, v and out must not be null");
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "cross_attention: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
+    SVDQ_REQUIRE(a->batch > 0 && a->batch < 65536 && a->heads > 0 && a->heads < 65536 && a->kv_heads > 0 && a->heads % a->kv_heads == 0,
+                 "cross_attention: batch (%lld) and heads (%lld) must be in 1..65535, kv_heads (%lld) must divide heads", (long long)a->batch, (long long)a->heads, (long long)a->kv_heads);
+    SVDQ_REQUIRE(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, "cross_attention: head_dim (%lld) must be a multiple of 8 up to 128", (long long)a->head_dim);
+    SVDQ_REQUIRE(a->q_len > 0 && a->k_len > 0 && a->k_len < (1ll << 31) - 64, "cross_attention: q_len (%lld) and k_len (%lld) must be positive, k_len below 2^31 - 64", (long long)a->q_len,
+                 (long long)a->k_len);
+    SVDQ_REQUIRE(a->q_len * (a->heads / a->kv_heads) < (1ll << 31) - 128, "cross_attention: q_len (%lld) times the heads that share keys must be below 2^31 - 128", (long long)a->q_len);
+    SVDQ_REQUIRE(!a->key_lengths + !a->key_mask + !a->cu_seqlens_k >= 2, "cross_attention: at most one of key_lengths, key_mask and cu_seqlens_k can be given");
+    SVDQ_REQUIRE(a->scale > 0.f && a->scale < __builtin_huge_valf(), "cross_attention: scale must be a positive number");
+    for (int i = 0; i < 3; i++)
+        SVDQ_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->v_stride[i] >= 0 && a->out_stride[i] >= 0 &&
+                         (a->q_stride[i] | a->k_stride[i] | a->v_stride[i] | a->out_stride[i]) % 8 == 0,
+                     "cross_attention: strides must be multiples of 8 elements (16 bytes)");
+    SVDQ_REQUIRE(a->k_stride[1] < (1ll << 24) && a->v_stride[1] < (1ll << 24), "cross_attention: the tokens of k and v must be less than 2^24 elements apart");
+    SVDQ_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->workspace) % 16 == 0, "cross_attention: pointers must be 16-byte aligned");
+    SVDQ_REQUIRE(((uintptr_t)a->key_lengths | (uintptr_t)a->cu_seqlens_k) % 4 == 0, "cross_attention: key_lengths and cu_seqlens_k must be 4-byte aligned");
+    return SVDQ_OK;
+}
+
+int current_compute_units(int &cus) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || (cus = compute_units(dev)) == 0) {
+        (void)hipGetLastError();
+        return fail(SVDQ_ELAUNCH, "cross_attention: no current device");
+    }
+    return SVDQ_OK;
+}
+
+}  // namespace
+
+extern "C" int svdq_cross_attention_workspace(const svdq_cross_attention_args *a, int64_t *bytes) {
+    if (int rc = check_args(a)) return rc;
+    SVDQ_REQUIRE(bytes, "cross_attention: bytes must not be null");
+    int cus;
+    if (int rc = current_compute_units(cus)) return rc;
+    *bytes = plan_of(a, cus).workspace;
+    return SVDQ_OK;
+}
+
+extern "C" int svdq_cross_attention(const svdq_cross_attention_args *a, void *stream) {
+    if (int rc = check_args(a)) return rc;
+    int cus;
+    if (int rc = current_compute_units(cus)) return rc;
+    const Plan plan = plan_of(a, cus);
+    SVDQ_REQUIRE(plan.workspace == 0 || (a->workspace && a->workspace_bytes >= plan.workspace), "cross_attention: needs a workspace of %lld bytes, got %lld", plan.workspace,
+                 (long long)(a->workspace ? a->workspace_bytes : 0));
+    const long long grid = plan.row_blocks * plan.parts * a->kv_heads * a->batch;
+    if (grid >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "cross_attention: %lld workgroups are too many for one launch", grid);
+    AttentionParams p;
+    p.q = (const char *)a->q;
+    p.k = (const char *)a->k;
+    p.v = (const char *)a->v;
+    p.out = (char *)a->out;
+    p.key_lengths = a->key_lengths;
+    p.cu_seqlens = a->cu_seqlens_k;
+    p.mask = (const uint8_t *)a->key_mask;
+    p.partial = (float *)a->workspace;
+    for (int i = 0; i < 3; i++) {
+        p.qs[i] = a->q_stride[i] * 2;
+        p.ks[i] = a->k_stride[i] * 2;
+        p.vs[i] = a->v_stride[i] * 2;
+        p.os[i] = a->out_stride[i] * 2;
+    }
+    p.mask_b = a->mask_stride;
+    p.B = (int)a->batch;
+    p.Hkv = (int)a->kv_heads;
+    p.G = (int)(a->heads / a->kv_heads);
+    p.D = (int)a->head_dim;
+    p.Tq = (int)a->q_len;
+    p.Tk = (int)a->k_len;
+    p.rows = p.Tq * p.G;
+    p.row_blocks = (int)plan.row_blocks;
+    p.parts = (int)plan.parts;
+    p.scale2 = a->scale * 1.44269504088896340736f;
+    hipStream_t st = (hipStream_t)stream;
+    if (a->dtype == SVDQ_BF16) return p.mask ? launch_heads<true, true>(p, plan.keys, st) : launch_heads<true, false>(p, plan.keys, st);
+    return p.mask ? launch_heads<false, true>(p, plan.keys, st) : launch_heads<false, false>(p, plan.keys, st);
+}

@@ -1,0 +1,322 @@
+// out[m][n] = T(float(sum_k act[m][k] * wgt[n][k]) * (ascales[m] * wscales[n]) + bias[n]) on v_mfma_i32_32x32x32_i8 /
+// v_mfma_i32_16x16x64_i8.  The integer sums are exact, whatever their order; each factor, the product with it, the bias and the
+// result are rounded once.
+#include "svdq_common.h"
+
+using namespace svdq;
+
+namespace {
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int int16_t_ __attribute__((ext_vector_type(16)));
+
+struct W8A8Params {
+    const char *act, *wgt;
+    const float *ascales, *wscales;
+    const uint16_t *bias;
+    uint16_t *out;
+    long long ld_act, ld_wgt, ld_out;  // bytes, bytes, elements
+    int M, N, K, bf16;
+    int tiles_m, tiles_n;
+    int wide;  // rows of `out` and its first column are 16 bytes apart and aligned
+};
+
+// What copies of a piece behind a row's end read.
+__device__ const u32x4_t zeros16 = {0, 0, 0, 0};
+
+__device__ inline float value16(uint16_t b, int bf16) { return bf16 ? bf16_bits_to_f32(b) : (float)__builtin_bit_cast(_Float16, b); }
+__device__ inline uint32_t pair16(float lo, float hi, int bf16) {
+    if (bf16) return pack_bf16x2(lo, hi);
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
+}
+
+// Workgroup -> tile.  Workgroups go round robin over the 8 XCDs, each with an L2 of its own: an XCD gets one contiguous run of the
+// tiles, which are numbered down the rows inside bands of up to BAND row blocks, so that the tiles at work on an XCD share operands.
+constexpr int BAND = 8;
+__device__ inline void tile_of(const W8A8Params &p, int &tm, int &tn) {
+    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+    const int xcd = id & 7, per = total >> 3, more = total & 7;
+    const int tile = xcd * per + (xcd < more ? xcd : more) + (id >> 3);
+    const int band_tiles = BAND * p.tiles_n, band = tile / band_tiles, in = tile - band * band_tiles;
+    const int height = p.tiles_m - band * BAND < BAND ? p.tiles_m - band * BAND : BAND;
+    tm = band * BAND + in % height;
+    tn = in / height;
+}
+
+// ---- tiles through LDS --------------------------------------------------------------------------------------------------
+// BM x BN outputs by WM x WN waves.  128 bytes of K of every row make a stage of the ring; they come by asynchronous copies of
+// 16 bytes a lane, a KB (8 rows) a request.  Piece p of row r stands at place p ^ ((r / 2) % 8) of its row: 16 lanes that read the
+// same piece of 16 rows then touch every bank once.  The weights are the left operand, so that a lane holds four consecutive
+// columns of one row.
+constexpr int BK = 128;
+__device__ inline int swizzle(int row) { return (row >> 1) & 7; }
+
+template <int BM, int BN, int WM, int WN, int STAGES>
+struct Tiles {
+    static constexpr int THREADS = WM * WN * 64, WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr int A_REQ = BM / 8 / WAVES, B_REQ = BN / 8 / WAVES, REQ = A_REQ + B_REQ;
+    static constexpr int STAGE = (BM + BN) * BK, LDS = STAGE * STAGES;
+    static constexpr int SLAB_LD = TN * 32 + 8;  // elements
+    static_assert(WAVES * 32 * SLAB_LD * 2 <= LDS, "the epilogue's slabs reuse the ring");
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "");
+};
+
+template <int BM, int BN, int WM, int WN, int STAGES, int OCC>
+__global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params p) {
+    using T = Tiles<BM, BN, WM, WN, STAGES>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    int tm, tn;
+    tile_of(p, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    // copies: request i of this wave brings rows (wave * REQ + i) * 8 + lane / 8; rows behind the last are the last again
+    const int sub = lane >> 3;
+    const char *src_a = p.act + (long long)m0 * p.ld_act, *src_b = p.wgt + (long long)n0 * p.ld_wgt;
+    uint32_t off_a[T::A_REQ], off_b[T::B_REQ];
+    int piece_a[T::A_REQ], piece_b[T::B_REQ];
+#pragma unroll
+    for (int i = 0; i < T::A_REQ; i++) {
+        const int r = (wave * T::A_REQ + i) * 8 + sub, last = p.M - 1 - m0;
+        piece_a[i] = ((lane & 7) ^ swizzle(r)) * 16;
+        off_a[i] = (uint32_t)((r < last ? r : last) * p.ld_act) + piece_a[i];
+    }
+#pragma unroll
+    for (int i = 0; i < T::B_REQ; i++) {
+        const int r = (wave * T::B_REQ + i) * 8 + sub, last = p.N - 1 - n0;
+        piece_b[i] = ((lane & 7) ^ swizzle(r)) * 16;
+        off_b[i] = (uint32_t)((r < last ? r : last) * p.ld_wgt) + piece_b[i];
+    }
+    const int whole = p.K / BK, steps = (p.K + BK - 1) / BK;
+    const uint32_t dst_a = base + wave * T::A_REQ * 1024, dst_b = base + BM * BK + wave * T::B_REQ * 1024;
+    auto request = [&](int step) __attribute__((always_inline)) {
+        const uint32_t stage = (uint32_t)(step % STAGES) * T::STAGE;
+        const char *a = src_a + (long long)step * BK, *b = src_b + (long long)step * BK;
+        if (step < whole) {
+#pragma unroll
+            for (int i = 0; i < T::A_REQ; i++)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst_a + stage + i * 1024), "v"(off_a[i]), "s"(a) : "memory", "m0");
+#pragma unroll
+            for (int i = 0; i < T::B_REQ; i++)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst_b + stage + i * 1024), "v"(off_b[i]), "s"(b) : "memory", "m0");
+        } else {  // the last, partly filled step: zeros behind the row's end
+            const int left = p.K - step * BK;
+#pragma unroll
+            for (int i = 0; i < T::A_REQ; i++) {
+                const char *s = piece_a[i] < left ? a + off_a[i] : (const char *)&zeros16;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst_a + stage + i * 1024), "v"(s) : "memory", "m0");
+            }
+#pragma unroll
+            for (int i = 0; i < T::B_REQ; i++) {
+                const char *s = piece_b[i] < left ? b + off_b[i] : (const char *)&zeros16;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst_b + stage + i * 1024), "v"(s) : "memory", "m0");
+            }
+        }
+    };
+    int16_t_ acc[T::TM][T::TN];
+#pragma unroll
+    for (int i = 0; i < T::TM; i++)
+#pragma unroll
+        for (int j = 0; j < T::TN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++)
+        if (s < steps) request(s);
+    const int col = lane & 31, h = lane >> 5;
+    const char *row_a = lds + (wm * T::TM * 32 + col) * BK, *row_b = lds + BM * BK + (wn * T::TN * 32 + col) * BK;
+    for (int step = 0; step < steps; step++) {
+        // this step's copies have landed (of all waves), and nobody reads the stage that the next request overwrites
+        if (step + STAGES - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * T::REQ) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + STAGES - 1 < steps) request(step + STAGES - 1);
+        const int stage = (step % STAGES) * T::STAGE;
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ks++) {
+            const int at = ((2 * ks + h) ^ swizzle(col)) * 16;
+            int4_t a[T::TM], b[T::TN];
+#pragma unroll
+            for (int i = 0; i < T::TM; i++) a[i] = *(const int4_t *)(row_a + stage + i * 32 * BK + at);
+#pragma unroll
+            for (int j = 0; j < T::TN; j++) b[j] = *(const int4_t *)(row_b + stage + j * 32 * BK + at);
+#pragma unroll
+            for (int i = 0; i < T::TM; i++)
+#pragma unroll
+                for (int j = 0; j < T::TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[j], a[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    // epilogue: 32 rows at a time through the wave's slab in LDS, in the place of the ring
+    __syncthreads();
+    uint16_t *slab = (uint16_t *)lds + wave * 32 * T::SLAB_LD;
+    const int wave_n = n0 + wn * T::TN * 32;
+#pragma unroll
+    for (int i = 0; i < T::TM; i++) {
+        const int row0 = m0 + (wm * T::TM + i) * 32, row = row0 + col;
+        const float sa = row < p.M ? p.ascales[row] : 0.f;
+#pragma unroll
+        for (int j = 0; j < T::TN; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int c = j * 32 + 8 * g + 4 * h, n = wave_n + c;
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int ne = n + e < p.N ? n + e : p.N - 1;
+                    y[e] = (float)acc[i][j][4 * g + e] * (sa * p.wscales[ne]);
+                    if (p.bias) y[e] += value16(p.bias[ne], p.bf16);
+                }
+                *(u32x2_t *)(slab + col * T::SLAB_LD + c) = u32x2_t{pair16(y[0], y[1], p.bf16), pair16(y[2], y[3], p.bf16)};
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (p.wide) {
+            constexpr int LANES = T::TN * 4, PER = 64 / LANES;  // lanes per row, rows per pass
+#pragma unroll
+            for (int r = 0; r < 32; r += PER) {
+                const int rr = r + lane / LANES, cc = (lane % LANES) * 8;
+                const u32x4_t v = *(const u32x4_t *)(slab + rr * T::SLAB_LD + cc);
+                if (row0 + rr < p.M && wave_n + cc < p.N) __builtin_nontemporal_store(v, (u32x4_t *)(p.out + (row0 + rr) * p.ld_out + wave_n + cc));
+            }
+        } else {
+            for (int e = lane; e < 32 * T::TN * 32; e += 64) {
+                const int rr = e / (T::TN * 32), cc = e % (T::TN * 32);
+                if (row0 + rr < p.M && wave_n + cc < p.N) p.out[(row0 + rr) * p.ld_out + wave_n + cc] = slab[rr * T::SLAB_LD + cc];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+// 16 columns x 16 * MT rows per workgroup, whose WAVES waves split K in steps of 64 bytes and meet in LDS.  Operands go from
+// memory to the registers of the wave that multiplies them.
+template <int MT, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p) {
+    __shared__ int4_t sums[WAVES - 1][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    const char *w = p.wgt + (long long)(n0 + r < p.N ? n0 + r : p.N - 1) * p.ld_wgt + q * 16;
+    const char *a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = m0 + i * 16 + r;
+        a[i] = p.act + (long long)(m < p.M ? m : p.M - 1) * p.ld_act + q * 16;
+    }
+    int4_t acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) acc[i] = int4_t{0, 0, 0, 0};
+    const int whole = p.K / 64;
+    constexpr int UN = 4;
+    int s = wave * UN;
+    for (; s + UN <= whole; s += WAVES * UN) {
+        int4_t wv[UN], av[UN][MT];
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            wv[u] = *(const int4_t *)(w + (s + u) * 64);
+#pragma unroll
+            for (int i = 0; i < MT; i++) av[u][i] = *(const int4_t *)(a[i] + (s + u) * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], av[u][i], acc[i], 0, 0, 0);
+    }
+    // (the wave whose turn holds the last whole steps and the partly filled one)
+    for (; s * 64 < p.K && s < whole + 1; s++) {
+        const bool in = s * 64 + q * 16 < p.K;
+        int4_t wv = int4_t{0, 0, 0, 0};
+        if (in) wv = *(const int4_t *)(w + s * 64);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            int4_t av = int4_t{0, 0, 0, 0};
+            if (in) av = *(const int4_t *)(a[i] + s * 64);
+            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, av, acc[i], 0, 0, 0);
+        }
+        if ((s + 1) % UN == 0) break;
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) sums[wave - 1][i][lane] = acc[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+#pragma unroll
+        for (int v = 0; v < WAVES - 1; v++) acc[i] += sums[v][i][lane];
+        const int m = m0 + i * 16 + r;
+        if (m >= p.M) continue;
+        const float sa = p.ascales[m];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int n = n0 + 4 * q + e;
+            if (n >= p.N) continue;
+            float y = (float)acc[i][e] * (sa * p.wscales[n]);
+            if (p.bias) y += value16(p.bias[n], p.bf16);
+            p.out[m * p.ld_out + n] = (uint16_t)pair16(y, 0.f, p.bf16);
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int OCC>
+int launch_tiles(W8A8Params &p, hipStream_t st) {
+    using T = Tiles<BM, BN, WM, WN, STAGES>;
+    p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = (p.N + BN - 1) / BN;
+    if ((long long)p.tiles_m * p.tiles_n >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "gemm_w8a8: %d x %d tiles are too many for one launch", p.tiles_m, p.tiles_n);
+    auto *kernel = w8a8_tiles_kernel<BM, BN, WM, WN, STAGES, OCC>;
+    if (T::LDS > 65536 && hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(SVDQ_ELAUNCH, "gemm_w8a8: the device does not offer %d bytes of LDS", T::LDS);
+    }
+    SVDQ_LAUNCH(kernel, dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(T::THREADS), T::LDS, st, p);
+    return check_launch("gemm_w8a8");
+}
+
+template <int MT, int WAVES>
+int launch_few(W8A8Params &p, hipStream_t st) {
+    SVDQ_LAUNCH((w8a8_few_rows_kernel<MT, WAVES>), dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * MT - 1) / (16 * MT))), dim3(WAVES * 64), 0, st, p);
+    return check_launch("gemm_w8a8");
+}
+
+}  // namespace
+
+extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
+    SVDQ_REQUIRE(a && a->act && a->wgt && a->ascales && a->wscales && a->out, "gemm_w8a8: act, wgt, ascales, wscales and out must not be null");
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "gemm_w8a8: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
+    SVDQ_REQUIRE(a->M > 0 && a->N > 0 && a->M < (1ll << 31) - 256 && a->N < (1ll << 31) - 256, "gemm_w8a8: M (%lld) and N (%lld) must be positive and below 2^31 - 256",
+                 (long long)a->M, (long long)a->N);
+    // 127 * 127 * 131072 and 128 * 128 * 131056 stay below 2^31
+    SVDQ_REQUIRE(a->K > 0 && a->K % 16 == 0 && a->K < 131072, "gemm_w8a8: K (%lld) must be a multiple of 16 below 131072, so that the integer sums cannot overflow", (long long)a->K);
+    SVDQ_REQUIRE(a->ld_act >= a->K && a->ld_act % 16 == 0 && a->ld_act < (1ll << 23), "gemm_w8a8: rows of act must be at least K bytes, a multiple of 16 and less than 2^23 apart, got %lld",
+                 (long long)a->ld_act);
+    SVDQ_REQUIRE(a->ld_wgt >= a->K && a->ld_wgt % 16 == 0 && a->ld_wgt < (1ll << 23), "gemm_w8a8: rows of wgt must be at least K bytes, a multiple of 16 and less than 2^23 apart, got %lld",
+                 (long long)a->ld_wgt);
+    SVDQ_REQUIRE(a->ld_out >= a->N, "gemm_w8a8: rows of out must be at least N (%lld) elements apart, got %lld", (long long)a->N, (long long)a->ld_out);
+    SVDQ_REQUIRE(((uintptr_t)a->act | (uintptr_t)a->wgt) % 16 == 0, "gemm_w8a8: act and wgt must be 16-byte aligned");
+    SVDQ_REQUIRE(((uintptr_t)a->ascales | (uintptr_t)a->wscales) % 4 == 0 && ((uintptr_t)a->bias | (uintptr_t)a->out) % 2 == 0, "gemm_w8a8: scales, bias and out must be aligned to their elements");
+    W8A8Params p;
+    p.act = (const char *)a->act;
+    p.wgt = (const char *)a->wgt;
+    p.ascales = a->ascales;
+    p.wscales = a->wscales;
+    p.bias = (const uint16_t *)a->bias;
+    p.out = (uint16_t *)a->out;
+    p.ld_act = a->ld_act;
+    p.ld_wgt = a->ld_wgt;
+    p.ld_out = a->ld_out;
+    p.M = (int)a->M;
+    p.N = (int)a->N;
+    p.K = (int)a->K;
+    p.bf16 = a->dtype == SVDQ_BF16;
+    p.wide = a->N % 8 == 0 && a->ld_out % 8 == 0 && (uintptr_t)a->out % 16 == 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (a->M <= 16) return launch_few<1, 4>(p, st);
+    if (a->M <= 32) return launch_few<2, 4>(p, st);
+    if ((p.M + 255ll) / 256 * ((p.N + 255ll) / 256) >= 192) return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
+    if ((p.M + 127ll) / 128 * ((p.N + 127ll) / 128) >= 192) return launch_tiles<128, 128, 2, 2, 2, 2>(p, st);
+    return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
+}

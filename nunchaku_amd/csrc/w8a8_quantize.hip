@@ -1,0 +1,226 @@
+// Rows of bf16 / fp16 activations to 8-bit codes with one scale each, plain or behind a residual's addition and an RMS norm:
+//   plain: g = x;   norm: h = T(x + residual) (the stored residual stream; h = x without one), g = h * weight
+//   a = max(max_k |g|, 2^-100), code = rne(g * fl32(127 / a)), scale = fl32(a * f / 127), f = 1 or 1 / sqrt(mean(h^2) + eps).
+// The factor 1 / rms of a row is the same for all its elements, so it cancels in the codes: they depend on max |g| alone, and
+// g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32.  |code| <= 127 needs no clamp:
+// |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
+// scale NaN and codes 0: what a product makes of it is NaN.
+// Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.
+#include "svdq_common.h"
+
+using namespace svdq;
+
+namespace {
+
+constexpr float MIN_AMAX = 0x1p-100f;
+
+struct QuantizeParams {
+    const char *x, *residual, *weight;
+    char *residual_out, *codes;
+    float *scales;
+    long long M, ld_x, ld_residual, ld_residual_out, ld_codes;  // bytes
+    int pieces;                                                 // of 8 elements per row
+    float inv_k, eps;
+};
+
+template <bool BF16>
+__device__ inline void unpack(const u32x4_t w, float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (BF16) {
+            f[2 * j] = bits_f32(w[j] << 16);
+            f[2 * j + 1] = bits_f32(w[j] & 0xFFFF0000u);
+        } else {
+            const uint32_t pair = w[j];  // (a bit cast of w[j] itself takes element 0 whatever j)
+            const half2_t h = __builtin_bit_cast(half2_t, pair);
+            f[2 * j] = (float)h[0];
+            f[2 * j + 1] = (float)h[1];
+        }
+    }
+}
+template <bool BF16>
+__device__ inline uint32_t pack_pair(float lo, float hi) {
+    if (BF16) return pack_bf16x2(lo, hi);
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
+}
+
+// THREADS per row (64: four rows per workgroup), each with up to VECS pieces of 8 elements
+template <bool BF16, int THREADS, int VECS, bool NORM, bool RESIDUAL>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_kernel(QuantizeParams p) {
+    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, WAVES = THREADS / 64;
+    const int t = threadIdx.x % THREADS;
+    const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (row >= p.M) return;  // (a whole wave; rows of several waves are one per workgroup)
+    const char *x = p.x + row * p.ld_x;
+    u32x4_t w[VECS], r[RESIDUAL ? VECS : 1];
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * THREADS;
+        w[i] = u32x4_t{0, 0, 0, 0};
+        if (piece < p.pieces) w[i] = *(const u32x4_t *)(x + (size_t)piece * 16);
+    }
+    if constexpr (RESIDUAL) {
+        const char *res = p.residual + row * p.ld_residual;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int piece = t + i * THREADS;
+            r[i] = u32x4_t{0, 0, 0, 0};
+            if (piece < p.pieces) r[i] = *(const u32x4_t *)(res + (size_t)piece * 16);
+        }
+    }
+    uint32_t top = 0;
+    float squares = 0.f;
+    u32x4_t nw[NORM ? VECS : 1];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int piece = t + i * THREADS;
+            nw[i] = u32x4_t{0, 0, 0, 0};
+            if (piece < p.pieces) nw[i] = *(const u32x4_t *)(p.weight + (size_t)piece * 16);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * THREADS;
+        float f[8];
+        if constexpr (RESIDUAL) {
+            float a[8], b[8];
+            unpack<BF16>(w[i], a);
+            unpack<BF16>(r[i], b);
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[i][j] = pack_pair<BF16>(a[2 * j] + b[2 * j], a[2 * j + 1] + b[2 * j + 1]);
+            if (piece < p.pieces) *(u32x4_t *)(p.residual_out + row * p.ld_residual_out + (size_t)piece * 16) = w[i];
+        }
+        unpack<BF16>(w[i], f);
+        if constexpr (NORM) {
+            float g[8];
+            unpack<BF16>(nw[i], g);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                squares = __builtin_fmaf(f[j], f[j], squares);
+                f[j] *= g[j];
+            }
+        }
+        // magnitudes as integers: NaN is the largest, so that it is not lost
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t m = f32_bits(f[j]) & 0x7FFFFFFFu;
+            top = m > top ? m : top;
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)top, d);
+        top = o > top ? o : top;
+        if (NORM) squares += __shfl_xor(squares, d);
+    }
+    if constexpr (WAVES > 1) {
+        __shared__ uint32_t tops[WAVES];
+        __shared__ float sums[WAVES];
+        if ((t & 63) == 0) {
+            tops[t >> 6] = top;
+            sums[t >> 6] = squares;
+        }
+        __syncthreads();
+        top = 0;
+        squares = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) {
+            top = tops[i] > top ? tops[i] : top;
+            squares += sums[i];
+        }
+    }
+    const bool bad = top >= 0x7F800000u || !(squares < __builtin_huge_valf());
+    const float amax = bits_f32(top) > MIN_AMAX ? bits_f32(top) : MIN_AMAX;
+    const float factor = 127.0f / amax;
+    if (t == 0) {
+        float s = amax;
+        if (NORM) s *= 1.0f / __builtin_sqrtf(squares * p.inv_k + p.eps);
+        p.scales[row] = bad ? __builtin_nanf("") : s / 127.0f;
+    }
+    char *out = p.codes + row * p.ld_codes;
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * THREADS;
+        float f[8];
+        unpack<BF16>(w[i], f);
+        if constexpr (NORM) {
+            float g[8];
+            unpack<BF16>(nw[i], g);
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] *= g[j];
+        }
+        // adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves its two's complement in the low bits
+        uint32_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) b[j] = f32_bits(f[j] * factor + 12582912.0f) & 255u;
+        u32x2_t c;
+#pragma unroll
+        for (int j = 0; j < 2; j++) c[j] = bad ? 0u : b[4 * j] | b[4 * j + 1] << 8 | b[4 * j + 2] << 16 | b[4 * j + 3] << 24;
+        if (piece < p.pieces) *(u32x2_t *)(out + (size_t)piece * 8) = c;
+    }
+}
+
+template <bool BF16, int THREADS, int VECS>
+void launch_rows(const QuantizeParams &p, bool norm, hipStream_t st) {
+    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+    const dim3 grid((unsigned)((p.M + ROWS - 1) / ROWS)), block(THREADS < 256 ? 256 : THREADS);
+    if (!norm) SVDQ_LAUNCH((quantize_rows_kernel<BF16, THREADS, VECS, false, false>), grid, block, 0, st, p);
+    else if (!p.residual) SVDQ_LAUNCH((quantize_rows_kernel<BF16, THREADS, VECS, true, false>), grid, block, 0, st, p);
+    else SVDQ_LAUNCH((quantize_rows_kernel<BF16, THREADS, VECS, true, true>), grid, block, 0, st, p);
+}
+
+template <bool BF16>
+void dispatch(const QuantizeParams &p, bool norm, hipStream_t st) {
+    const int need = p.pieces;
+    if (need <= 64 * 4) launch_rows<BF16, 64, 4>(p, norm, st);
+    else if (need <= 256 * 2) launch_rows<BF16, 256, 2>(p, norm, st);
+    else if (need <= 256 * 4) launch_rows<BF16, 256, 4>(p, norm, st);
+    else if (need <= 1024 * 2) launch_rows<BF16, 1024, 2>(p, norm, st);
+    else launch_rows<BF16, 1024, 8>(p, norm, st);
+}
+
+int quantize_rows(const svdq_quantize_w8a8_args *a, bool norm, void *stream, const char *what) {
+    SVDQ_REQUIRE(a && a->input && a->output && a->oscales, "%s: input, output and oscales must not be null", what);
+    SVDQ_REQUIRE(!norm || a->weight, "%s: weight must not be null", what);
+    SVDQ_REQUIRE(!a->residual == !a->residual_out, "%s: residual and residual_out belong together", what);
+    SVDQ_REQUIRE(norm || !a->residual, "%s: takes no residual", what);
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "%s: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", what, (int)a->dtype);
+    SVDQ_REQUIRE(a->M > 0 && a->M < (1ll << 31), "%s: M (%lld) must be in 1..2^31-1", what, (long long)a->M);
+    SVDQ_REQUIRE(a->K > 0 && a->K <= 65536 && a->K % 16 == 0, "%s: K (%lld) must be a multiple of 16 up to 65536", what, (long long)a->K);
+    SVDQ_REQUIRE(a->ld_input >= a->K && a->ld_input % 8 == 0, "%s: rows of input must be at least K elements and a multiple of 8 apart, got %lld", what, (long long)a->ld_input);
+    SVDQ_REQUIRE(!a->residual || (a->ld_residual >= a->K && a->ld_residual % 8 == 0), "%s: rows of residual must be at least K elements and a multiple of 8 apart, got %lld", what,
+                 (long long)a->ld_residual);
+    SVDQ_REQUIRE(!a->residual || (a->ld_residual_out >= a->K && a->ld_residual_out % 8 == 0),
+                 "%s: rows of residual_out must be at least K elements and a multiple of 8 apart, got %lld", what, (long long)a->ld_residual_out);
+    SVDQ_REQUIRE(((uintptr_t)a->input | (uintptr_t)a->output | (uintptr_t)a->residual | (uintptr_t)a->residual_out | (uintptr_t)a->weight) % 16 == 0,
+                 "%s: pointers must be 16-byte aligned", what);
+    SVDQ_REQUIRE((uintptr_t)a->oscales % 4 == 0, "%s: oscales must be 4-byte aligned", what);
+    SVDQ_REQUIRE(!norm || (a->eps >= 0.f && a->eps < __builtin_huge_valf()), "%s: eps must be a finite number not below zero", what);
+    QuantizeParams p;
+    p.x = (const char *)a->input;
+    p.residual = (const char *)a->residual;
+    p.weight = (const char *)a->weight;
+    p.residual_out = (char *)a->residual_out;
+    p.codes = (char *)a->output;
+    p.scales = a->oscales;
+    p.M = a->M;
+    p.ld_x = a->ld_input * 2;
+    p.ld_residual = a->ld_residual * 2;
+    p.ld_residual_out = a->ld_residual_out * 2;
+    p.ld_codes = a->K;
+    p.pieces = (int)(a->K / 8);
+    p.inv_k = 1.0f / (float)a->K;
+    p.eps = a->eps;
+    if (a->dtype == SVDQ_BF16) dispatch<true>(p, norm, (hipStream_t)stream);
+    else dispatch<false>(p, norm, (hipStream_t)stream);
+    return check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int svdq_quantize_w8a8_act(const svdq_quantize_w8a8_args *args, void *stream) { return quantize_rows(args, false, stream, "quantize_w8a8_act"); }
+
+extern "C" int svdq_rms_norm_quantize_w8a8(const svdq_quantize_w8a8_args *args, void *stream) {
+    return quantize_rows(args, true, stream, "rms_norm_quantize_w8a8");
+}
