@@ -11,7 +11,7 @@
 //
 // Rows of K and V in LDS: pieces of 16 bytes, piece c of row r at place c ^ f(r), so that neither 16 lanes that read one piece of 16
 // rows (K) nor 32 lanes that read 64 bytes of 4 rows (V) meet in a bank.  What no key stands for (rows behind the last key, masked
-// ones, columns behind the head's) is read from a block of zeros, whatever the tensors hold there.
+// ones) is not read from V at all, whatever it holds: zeros stand there.
 #include "svdq_common.h"
 
 using namespace svdq;
@@ -28,8 +28,6 @@ struct AttentionParams {
     int B, Hkv, G, D, Tq, Tk, rows, row_blocks, parts;
     float scale2;  // scale * log2(e)
 };
-
-__device__ const u32x4_t zeros16 = {0, 0, 0, 0};
 
 constexpr int KEYS = 64;  // per step
 
@@ -63,13 +61,23 @@ struct Head {
 __device__ inline void copy16(uint32_t dst, const char *base, uint32_t off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
-__device__ inline void copy16(uint32_t dst, const char *src) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
+// zeros made on the spot: four registers that hold them through the whole loop are four too many
+__device__ inline void clear16(uint32_t dst) {
+    u32x4_t z;
+    asm volatile("v_mov_b32 %0, 0\n\tv_mov_b32 %1, 0" : "=v"(z[0]), "=v"(z[1]));
+    z[2] = z[0];
+    z[3] = z[1];
+    *(__attribute__((address_space(3))) u32x4_t *)dst = z;
 }
 
-__device__ inline float exchange_max(float x) {
-    const float o = __shfl_xor(x, 32);
-    return x > o ? x : o;
+// x of this lane and of the lane 32 further, in both
+__device__ inline float across_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(x), false, false);
+    return __builtin_fmaxf(bits_f32(r[0]), bits_f32(r[1]));
+}
+__device__ inline float across_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(x), false, false);
+    return bits_f32(r[0]) + bits_f32(r[1]);
 }
 
 // The keys of batch entry b: the first one's row in the tensors (packed sequences) and how many there are.
@@ -89,7 +97,47 @@ __device__ inline void keys_of(const AttentionParams &p, int b, long long &first
     count = __builtin_amdgcn_readfirstlane(count);
 }
 
+// The steps of 64 keys that hold any, in order, with a bit for every key that counts.  With a mask the bytes of the step behind the
+// next one are on their way while a step is worked on; steps without a key are left out.
+template <bool MASK>
+struct Steps {
+    const uint8_t *mask;
+    int count, steps, stride, at, lane;  // at: the next candidate
+    uint32_t byte;
+    uint64_t bits;  // of the step that next() returned
+    __device__ inline void fetch() {
+        if (MASK) {
+            const int key = at * KEYS + lane;
+            byte = 0;
+            if (key < count) byte = mask[key];
+        }
+    }
+    __device__ inline void start(const uint8_t *m, int count_, int first, int end, int stride_, int lane_) {
+        mask = m;
+        count = count_;
+        steps = end;
+        stride = stride_;
+        at = first;
+        lane = lane_;
+        byte = 0;
+        if (at < steps) fetch();
+    }
+    // the next step with a key, or -1
+    __device__ inline int next() {
+        while (at < steps) {
+            const int step = at, left = count - step * KEYS;
+            bits = MASK ? __ballot(byte != 0) : left >= KEYS ? ~0ull : (1ull << left) - 1;
+            at += stride;
+            if (at < steps) fetch();
+            if (!MASK || bits) return step;
+        }
+        bits = 0;
+        return -1;
+    }
+};
+
 // Running softmax and output of 32 rows: lane l holds row l % 32; of the output's block db element e is column 32 db + 8 (e / 4) + 4 (l / 32) + e % 4.
+// Scores s of a step: block kb, element e is key 32 kb + 8 (e / 4) + 4 (l / 32) + e % 4.
 template <bool BF16, int DP>
 struct State {
     using H = Head<DP>;
@@ -105,15 +153,28 @@ struct State {
         top = -__builtin_huge_valf();
         sum = 0.f;
     }
-    // one step of 64 keys: scores s (block kb, element e: key 32 kb + 8 (e / 4) + 4 (lane / 32) + e % 4), v in LDS
-    __device__ inline void add(float16_t (&s)[2], float scale2, const char *v, int lane) {
+    // keys without a bit get a score of minus infinity
+    static __device__ inline void mask(float16_t (&s)[2], uint64_t bits, int lane) {
+        if (bits == ~0ull) return;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            const uint32_t w = (uint32_t)(bits >> (32 * kb)) >> (4 * (lane >> 5));
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[kb][e] = w >> (8 * (e >> 2) + (e & 3)) & 1 ? s[kb][e] : -__builtin_huge_valf();
+        }
+    }
+    static __device__ inline float highest(const float16_t (&s)[2]) {
         float m = s[0][0];
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++) m = __builtin_fmaxf(m, s[i][e]);
-        m = exchange_max(m) * scale2;
-        if (__any(m > top)) {
+        return across_max(m);
+    }
+    // A new maximum of a row (in units of log2).  The one in use only has to keep the exponentials in range: it moves when a row's is
+    // more than 2^8 times off, so that the outputs are rarely scaled.
+    __device__ inline void raise(float m) {
+        if (__any(m > top + 8.f)) {
             const float now = m > top ? m : top;
             const float f = top == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(top - now);
             top = now;
@@ -123,34 +184,41 @@ struct State {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= f;
         }
-        const float ref = top == -__builtin_huge_valf() ? 0.f : top;  // (no valid key yet)
+    }
+    // scores to probabilities, rounded for the second product
+    __device__ inline void exponentials(const float16_t (&s)[2], float scale2, vec (&pr)[4]) {
+        const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float x[8];
+            u32x4_t w;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], scale2, -ref));
+                sum += x[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = E::pair(x[2 * e], x[2 * e + 1]);
+            pr[i] = __builtin_bit_cast(vec, w);
+        }
+    }
+    // o += v^T p of 64 keys, v in LDS
+    __device__ inline void product(const vec (&pr)[4], const char *v, int lane) {
         const int g = lane >> 4, i = lane & 15, h = lane >> 5;
         const char *vrow = v + (4 * h + (i >> 2)) * H::PITCH + (i & 1) * 8;
         const int piece = (g & 1) * 2 + ((i >> 1) & 1), f = H::fv(i >> 2);
+        typedef short short4_t __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) short4_t *lds_t;
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+        for (int st = 0; st < 4; st++) {
 #pragma unroll
-            for (int st = 0; st < 2; st++) {
-                uint32_t w[4];
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + e], scale2, -ref));
-                    sum += x[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = E::pair(x[2 * e], x[2 * e + 1]);
-                const vec pr = __builtin_bit_cast(vec, u32x4_t{w[0], w[1], w[2], w[3]});
-                typedef short short4_t __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) short4_t *lds_t;
-#pragma unroll
-                for (int d = 0; d < H::DB; d++) {
-                    const char *at = vrow + (32 * kb + 16 * st) * H::PITCH + ((4 * d + piece) ^ f) * 16;
-                    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
-                    const vec vv = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[d] = E::mfma(vv, pr, o[d]);
-                }
+            for (int d = 0; d < H::DB; d++) {
+                const char *at = vrow + 16 * st * H::PITCH + ((4 * d + piece) ^ f) * 16;
+                const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
+                o[d] = E::mfma(__builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pr[st], o[d]);
             }
+            if (st == 1) __builtin_amdgcn_sched_barrier(0);  // (all of V's reads at once would not fit the registers)
+        }
     }
 };
 
@@ -208,6 +276,19 @@ __device__ inline void block_of(const AttentionParams &p, int per_head, int &rb,
     b = bh / p.Hkv;
 }
 
+// Asks the scheduler for N times: an LDS read, a matrix instruction, VALU vector and TRANS transcendental instructions
+template <int N, int VALU, int TRANS>
+__device__ inline void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VALU - TRANS, 0);
+    }
+}
+
 // ---- rows form: 128 rows per workgroup, 32 per wave; all waves share the keys through LDS, two steps of them -------------------
 template <bool BF16, int DP, bool MASK>
 __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams p) {
@@ -225,77 +306,108 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     load_q<BF16, DP>(p, qf, b, hk, row, lane);
     const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
     const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
-    const uint8_t *mask = MASK ? p.mask + b * p.mask_b : nullptr;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     constexpr int REQ = H::REQ / 4;  // per wave, of K and of V
-    int rowi[REQ], ck[REQ], cv[REQ];
-    uint32_t ok[REQ], ov[REQ];
-#pragma unroll
-    for (int i = 0; i < REQ; i++) {
-        rowi[i] = (wave * REQ + i) * H::RPR + lane / H::PIECES;
-        ck[i] = ((lane % H::PIECES) ^ H::fk(rowi[i])) * 16;
-        cv[i] = ((lane % H::PIECES) ^ H::fv(rowi[i])) * 16;
-        ok[i] = (uint32_t)(rowi[i] * p.ks[1]) + ck[i];
-        ov[i] = (uint32_t)(rowi[i] * p.vs[1]) + cv[i];
+    const int bytes = p.D * 2;
+    // Request i of this wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
+    // two steps: the wave's rows start on a multiple of 16 where there are several requests).
+    const int row0 = wave * REQ * H::RPR + lane / H::PIECES;
+    const uint32_t ck = ((lane % H::PIECES) ^ H::fk(row0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(row0)) * 16;
+    const uint32_t ok = (uint32_t)(row0 * p.ks[1]), ov = (uint32_t)(row0 * p.vs[1]) + cv;
+    static_assert(REQ == 1 || (REQ * H::RPR == 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
+    const uint32_t dst = base + wave * REQ * 1024;
+    // Columns behind the head's end are zero in K for good: no copy writes there.
+    if (bytes < H::PITCH) {
+        for (int i = threadIdx.x; i < 2 * H::TILE / 16; i += 256) *(u32x4_t *)(lds + i * 16) = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
     }
-    const int steps = (count + KEYS - 1) / KEYS, bytes = p.D * 2;
-    const bool padded = bytes < H::PITCH;
-    auto request = [&](int step) __attribute__((always_inline)) {
-        const uint32_t dst = base + (step & 1) * 2 * H::TILE + wave * REQ * 1024;
-        const char *k = kp + (long long)step * KEYS * p.ks[1], *v = vp + (long long)step * KEYS * p.vs[1];
-        if (!MASK && !padded && (step + 1) * KEYS <= count) {
+    // K of step `step` to stage `slot`.  Rows behind the last key are not read: their scores are masked whatever they are.
+    auto request_k = [&](int step, int slot) __attribute__((always_inline)) {
+        const char *k = kp + (long long)step * KEYS * p.ks[1];
+        const int left = count - step * KEYS;
+        uint32_t c0 = ck;
+        asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
 #pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + i * 1024, k, ok[i]);
-#pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + H::TILE + i * 1024, v, ov[i]);
-        } else {
-            bool in[REQ];
-#pragma unroll
-            for (int i = 0; i < REQ; i++) {
-                const int key = step * KEYS + rowi[i];
-                in[i] = key < count;
-                if (MASK && in[i]) in[i] = mask[key] != 0;
-            }
-#pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + i * 1024, in[i] && ck[i] < bytes ? k + ok[i] : (const char *)&zeros16);
-#pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + H::TILE + i * 1024, in[i] && cv[i] < bytes ? v + ov[i] : (const char *)&zeros16);
+        for (int i = 0; i < REQ; i++) {
+            const uint32_t c = c0 ^ (64 * i);
+            if ((int)c < bytes && row0 < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * p.ks[1], ok + c);
         }
     };
-    State<BF16, DP> st;
-    st.clear();
-    if (steps > 0) request(0);
-    for (int step = 0; step < steps; step++) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + 1 < steps) request(step + 1);
-        const char *k = lds + (step & 1) * 2 * H::TILE, *v = k + H::TILE;
-        float16_t s[2];
+    // V: zeros for keys that do not count, since nothing times a NaN is one
+    auto request_v = [&](int step, int slot, uint64_t bits) __attribute__((always_inline)) {
+        const char *v = vp + (long long)step * KEYS * p.vs[1];
+        if ((int)cv >= bytes) return;
+        if (bits == ~0ull) {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+            for (int i = 0; i < REQ; i++) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * p.vs[1], ov);
+        } else {
+#pragma unroll
+            for (int i = 0; i < REQ; i++) {
+                if ((bits >> (i * H::RPR)) >> row0 & 1) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * p.vs[1], ov);
+                else clear16(dst + (2 + slot) * H::TILE + i * 1024 + lane * 16);
+            }
+        }
+    };
+    auto scores = [&](float16_t (&s)[2], int slot) __attribute__((always_inline)) {
+        const char *k = lds + slot * H::TILE;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int ks = 0; ks < H::KS; ks++) {
                 const u32x4_t w = *(const u32x4_t *)(k + (kb * 32 + col) * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16);
                 s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[kb]);
             }
-        if (MASK || (step + 1) * KEYS > count) {
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int key = step * KEYS + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
-                    bool in = key < count;
-                    if (MASK && in) in = mask[key] != 0;
-                    if (!in) s[kb][e] = -__builtin_huge_valf();
-                }
         }
-        st.add(s, p.scale2, v, lane);
+    };
+    // One step ahead: while the probabilities of step n are made and multiplied by V, the scores of step n + 1 are formed.
+    State<BF16, DP> st;
+    st.clear();
+    Steps<MASK> list;
+    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, 0, (count + KEYS - 1) / KEYS, 1, lane);
+    int step = list.next();
+    if (step >= 0) {
+        uint64_t bits = list.bits;
+        request_k(step, 0);
+        request_v(step, 0, bits);
+        int ahead = list.next();
+        uint64_t ahead_bits = list.bits;
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (ahead >= 0) request_k(ahead, 1);
+        float16_t even[2], odd[2];
+        scores(even, 0);
+        st.mask(even, bits, lane);
+        st.raise(st.highest(even) * p.scale2);
+        // one step: scores `s` of it, in stages `slot`; false behind the last
+        auto turn = [&](float16_t (&s)[2], float16_t (&next)[2], int slot) __attribute__((always_inline)) {
+            // K of the next step and V of this one have landed, of all waves; nobody reads what the requests below overwrite
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            typename E::vec pr[4];
+            if (ahead < 0) {
+                st.exponentials(s, p.scale2, pr);
+                st.product(pr, lds + (2 + slot) * H::TILE, lane);
+                return false;
+            }
+            request_v(ahead, slot ^ 1, ahead_bits);
+            const int after = list.next();
+            if (after >= 0) request_k(after, slot);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(next, slot ^ 1);
+            st.exponentials(s, p.scale2, pr);
+            interleave<2 * H::KS, 192 / (2 * H::KS), 32 / (2 * H::KS)>();
+            __builtin_amdgcn_sched_barrier(0);
+            st.product(pr, lds + (2 + slot) * H::TILE, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            st.mask(next, ahead_bits, lane);
+            st.raise(st.highest(next) * p.scale2);
+            ahead = after;
+            ahead_bits = list.bits;
+            return true;
+        };
+        while (turn(even, odd, 0) && turn(odd, even, 1)) {}
     }
-    const float sum = st.sum + __shfl_xor(st.sum, 32);
-    store_row<BF16, DP>(p, st, sum, b, hk, row, lane);
+    store_row<BF16, DP>(p, st, across_sum(st.sum), b, hk, row, lane);
 }
 
 // ---- keys form: 32 rows per workgroup, whose waves take every fourth step of the part's keys and meet in LDS; the parts of a row
@@ -318,29 +430,30 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
     load_q<BF16, DP>(p, qf, b, hk, row, lane);
     const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
     const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
-    const uint8_t *mask = MASK ? p.mask + b * p.mask_b : nullptr;
     const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * H::TILE;
     const char *varea = lds + wave * H::TILE;
     const int steps = (count + KEYS - 1) / KEYS, bytes = p.D * 2;
     const int begin = (int)((long long)steps * part / p.parts), end = (int)((long long)steps * (part + 1) / p.parts);
     State<BF16, DP> st;
     st.clear();
-    for (int step = begin + wave; step < end; step += 4) {
+    Steps<MASK> list;
+    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, begin + wave, end, 4, lane);
+    for (int step; (step = list.next()) >= 0;) {
+        const uint64_t bits = list.bits;
         const char *k = kp + (long long)step * KEYS * p.ks[1], *v = vp + (long long)step * KEYS * p.vs[1];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads are done
+        const int r0 = lane / H::PIECES, c = ((lane % H::PIECES) ^ H::fv(r0)) * 16;  // (f is the same in all requests)
+        const uint32_t ov = (uint32_t)(r0 * p.vs[1]) + c;
 #pragma unroll
         for (int i = 0; i < H::REQ; i++) {
-            const int r = i * H::RPR + lane / H::PIECES, c = ((lane % H::PIECES) ^ H::fv(r)) * 16, key = step * KEYS + r;
-            bool in = key < count && c < bytes;
-            if (MASK && in) in = mask[key] != 0;
-            copy16(area + i * 1024, in ? v + r * p.vs[1] + c : (const char *)&zeros16);
+            if (c >= bytes) continue;
+            if ((bits >> (i * H::RPR)) >> r0 & 1) copy16(area + i * 1024, v + i * H::RPR * p.vs[1], ov);
+            else clear16(area + i * 1024 + lane * 16);
         }
         u32x4_t w[2][H::KS];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            const int key = step * KEYS + 32 * kb + col;
-            bool in = key < count;
-            if (MASK && in) in = mask[key] != 0;
+            const bool in = step * KEYS + 32 * kb + col < count;
 #pragma unroll
             for (int ks = 0; ks < H::KS; ks++) {
                 const int c = (2 * ks + h) * 16;
@@ -355,22 +468,19 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
             for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < H::KS; ks++) s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w[kb][ks]), qf[ks], s[kb]);
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int key = step * KEYS + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
-                bool in = key < count;
-                if (MASK && in) in = mask[key] != 0;
-                if (!in) s[kb][e] = -__builtin_huge_valf();
-            }
         }
+        st.mask(s, bits, lane);
+        st.raise(st.highest(s) * p.scale2);
+        typename E::vec pr[4];
+        st.exponentials(s, p.scale2, pr);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        st.add(s, p.scale2, varea, lane);
+        st.product(pr, varea, lane);
     }
     // the waves meet: {maximum, sum} first, then the outputs, in the place of V
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
     float *stat = (float *)lds;  // [4][2][32]
-    const float own = st.sum + __shfl_xor(st.sum, 32);
+    const float own = across_sum(st.sum);
     if (h == 0) {
         stat[wave * 64 + col] = st.top;
         stat[wave * 64 + 32 + col] = own;

@@ -18,6 +18,7 @@ from .. import packing
 from ..ops import gemm as _gemm_op
 from ..ops.gemm import svdq_gemm_w4a4
 from ..ops.quantize import svdq_quantize_w4a4_act_fuse_lora
+from ..ops.w8a8 import gemm_w8a8, quantize_w8a8_act
 
 
 class _LayerCall:
@@ -335,3 +336,51 @@ class AWQW4A16Linear(nn.Module):
 
     def __repr__(self):
         return f"AWQW4A16Linear(in_features={self.in_features}, out_features={self.out_features}, group_size={self.group_size})"
+
+
+class W8A8Linear(nn.Module):
+    """8-bit linear layer: int8 codes with a scale for each output channel, activations quantized per token.  ``qweight`` int8
+    [N, K], ``wscales`` fp32 [N], ``bias`` [N]; bf16 or fp16 activations, K a multiple of 16.  Stands beside the 4-bit layers where
+    4 bits cost too much.  A caller that has codes already (``rms_norm_quantize_w8a8``) uses ``forward_quant``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, torch_dtype: torch.dtype = torch.bfloat16,
+                 device: str | torch.device | None = None):
+        super().__init__()
+        if in_features % 16 or in_features <= 0:
+            raise ValueError(f"in_features must be a multiple of 16, got {in_features}")
+        if device is None:
+            device = torch.device("cpu")
+        self.in_features, self.out_features, self.torch_dtype = in_features, out_features, torch_dtype
+        self.qweight = nn.Parameter(torch.empty(out_features, in_features, dtype=torch.int8, device=device), requires_grad=False)
+        self.wscales = nn.Parameter(torch.empty(out_features, dtype=torch.float32, device=device), requires_grad=False)
+        self.bias = nn.Parameter(torch.empty(out_features, dtype=torch_dtype, device=device), requires_grad=False) if bias else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [..., K] -> [..., N]"""
+        return self.forward_quant(*quantize_w8a8_act(x), out_dtype=x.dtype)
+
+    def forward_quant(self, codes: torch.Tensor, scales: torch.Tensor, output: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        """codes int8 [..., K] and scales fp32 [...] -> [..., N] of the layer's type"""
+        if output is None and out_dtype is None:
+            out_dtype = self.torch_dtype
+        return gemm_w8a8(codes, self.qweight, scales, self.wscales, bias=self.bias, out=output, out_dtype=out_dtype)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, torch_dtype: torch.dtype | None = None, device: str | torch.device | None = None, **kwargs):
+        """Quantizes the weights of ``linear``, each output channel like a row of activations (``quantize_w8a8_act``)."""
+        w = linear.weight.detach()
+        m = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, torch_dtype=torch_dtype or w.dtype,
+                device=w.device if device is None else device)
+        g = w.float()
+        if not torch.isfinite(g).all():
+            raise ValueError("the weights of the layer hold infinities or NaN")
+        a = g.abs().amax(1).clamp_min(2.0**-100)
+        with torch.no_grad():
+            m.qweight.copy_(torch.round(g * (torch.full_like(a, 127.0) / a)[:, None]).to(torch.int8))  # (`127.0 / a` is 127 times a reciprocal)
+            m.wscales.copy_(a / 127.0)
+            if m.bias is not None:
+                m.bias.copy_(linear.bias.detach())
+        return m
+
+    def __repr__(self):
+        return f"W8A8Linear(in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None})"
