@@ -58,7 +58,10 @@ struct Head {
     static __host__ __device__ constexpr int fv(int row) { return PITCH == 256 ? 4 * (row & 3) : PITCH == 128 ? 4 * ((row >> 1) & 1) : 0; }
 };
 
-__device__ inline void copy16(uint32_t dst, const char *base, uint32_t off) {
+__device__ inline void copy16(uint32_t dst, const char *src, uint32_t off) {
+    dst = __builtin_amdgcn_readfirstlane(dst);  // (the same in all lanes anyway)
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)src), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)src >> 32));
+    const char *base = (const char *)(((uintptr_t)hi << 32) | lo);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
 // zeros made on the spot: four registers that hold them through the whole loop are four too many
@@ -88,7 +91,7 @@ __device__ inline void keys_of(const AttentionParams &p, int b, long long &first
         int lo = p.cu_seqlens[b], hi = p.cu_seqlens[b + 1];
         lo = lo < 0 ? 0 : lo > p.Tk ? p.Tk : lo;
         hi = hi < lo ? lo : hi > p.Tk ? p.Tk : hi;
-        first = lo;
+        first = __builtin_amdgcn_readfirstlane(lo);
         count = hi - lo;
     } else if (p.key_lengths) {
         const int n = p.key_lengths[b];
@@ -164,12 +167,14 @@ struct State {
         }
     }
     static __device__ inline float highest(const float16_t (&s)[2]) {
-        float m = s[0][0];
+        float m[4];  // (four chains: a vector instruction waits for the one before it)
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < 4; i++) {
+            m[i] = s[i >> 1][8 * (i & 1)];
 #pragma unroll
-            for (int e = 0; e < 16; e++) m = __builtin_fmaxf(m, s[i][e]);
-        return across_max(m);
+            for (int e = 1; e < 8; e++) m[i] = __builtin_fmaxf(m[i], s[i >> 1][8 * (i & 1) + e]);
+        }
+        return across_max(__builtin_fmaxf(__builtin_fmaxf(m[0], m[1]), __builtin_fmaxf(m[2], m[3])));
     }
     // A new maximum of a row (in units of log2).  The one in use only has to keep the exponentials in range: it moves when a row's is
     // more than 2^8 times off, so that the outputs are rarely scaled.
@@ -185,39 +190,60 @@ struct State {
                 for (int e = 0; e < 16; e++) o[d][e] *= f;
         }
     }
-    // scores to probabilities, rounded for the second product
-    __device__ inline void exponentials(const float16_t (&s)[2], float scale2, vec (&pr)[4]) {
-        const float ref = top == -__builtin_huge_valf() ? 0.f : top;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float x[8];
-            u32x4_t w;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][8 * (i & 1) + e], scale2, -ref));
-                sum += x[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = E::pair(x[2 * e], x[2 * e + 1]);
-            pr[i] = __builtin_bit_cast(vec, w);
-        }
-    }
-    // o += v^T p of 64 keys, v in LDS
-    __device__ inline void product(const vec (&pr)[4], const char *v, int lane) {
+    // left operands of v^T p for 16 keys from row 16 n of the values in LDS on
+    static __device__ inline void read_v(vec (&vf)[H::DB], const char *v, int n, int lane) {
         const int g = lane >> 4, i = lane & 15, h = lane >> 5;
         const char *vrow = v + (4 * h + (i >> 2)) * H::PITCH + (i & 1) * 8;
         const int piece = (g & 1) * 2 + ((i >> 1) & 1), f = H::fv(i >> 2);
         typedef short short4_t __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) short4_t *lds_t;
 #pragma unroll
-        for (int st = 0; st < 4; st++) {
+        for (int d = 0; d < H::DB; d++) {
+            const char *at = vrow + 16 * n * H::PITCH + ((4 * d + piece) ^ f) * 16;
+            const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
+            vf[d] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+    // the right operand: probabilities of 16 keys, rounded
+    __device__ inline vec exponentials(const float16_t (&s)[2], int n, float scale2, float ref) {
+        float x[8];
+        u32x4_t w;
 #pragma unroll
-            for (int d = 0; d < H::DB; d++) {
-                const char *at = vrow + 16 * st * H::PITCH + ((4 * d + piece) ^ f) * 16;
-                const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
-                o[d] = E::mfma(__builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pr[st], o[d]);
+        for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n >> 1][8 * (n & 1) + e], scale2, -ref));
+        sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = E::pair(x[2 * e], x[2 * e + 1]);
+        return __builtin_bit_cast(vec, w);
+    }
+    __device__ inline float reference() const { return top == -__builtin_huge_valf() ? 0.f : top; }
+    // A step's scores and values (v in LDS) join the sums, 16 keys at a time: while the matrix cores multiply the probabilities of
+    // one 16, those of the next are made and the operands of the one behind it are on their way.
+    __device__ inline void attend(float16_t (&s)[2], uint64_t bits, float scale2, const char *v, int lane) {
+        vec vf[2][H::DB], pr[2];
+        read_v(vf[0], v, 0, lane);
+        mask(s, bits, lane);
+        raise(highest(s) * scale2);
+        const float ref = reference();
+        pr[0] = exponentials(s, 0, scale2, ref);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            if (n < 3) {
+                read_v(vf[(n + 1) & 1], v, n + 1, lane);
+                pr[(n + 1) & 1] = exponentials(s, n + 1, scale2, ref);
             }
-            if (st == 1) __builtin_amdgcn_sched_barrier(0);  // (all of V's reads at once would not fit the registers)
+#pragma unroll
+            for (int d = 0; d < H::DB; d++) o[d] = E::mfma(vf[n & 1][d], pr[n & 1], o[d]);
+            if (n < 3) {
+#pragma unroll
+                for (int d = 0; d < H::DB; d++) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 20 / H::DB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x400, 8 / H::DB, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -267,147 +293,197 @@ __device__ inline void store_row(const AttentionParams &p, State<BF16, DP> &s, f
 
 // Which (row block, head, batch entry) a workgroup takes: workgroups go round robin over 8 XCDs, each with an L2 of its own, and an
 // XCD gets a contiguous run, whose row blocks read the same keys.
-__device__ inline void block_of(const AttentionParams &p, int per_head, int &rb, int &hk, int &b) {
-    const int total = per_head * p.Hkv * p.B, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
+__device__ inline void block_of(int per_head, int heads, int &rb, int &hk, int &b) {
+    const int total = gridDim.x, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
     const int at = xcd * per + (xcd < more ? xcd : more) + (id >> 3);
     rb = at % per_head;
     const int bh = at / per_head;
-    hk = bh % p.Hkv;
-    b = bh / p.Hkv;
+    hk = bh % heads;
+    b = bh / heads;
 }
 
-// Asks the scheduler for N times: an LDS read, a matrix instruction, VALU vector and TRANS transcendental instructions
-template <int N, int VALU, int TRANS>
-__device__ inline void interleave() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, VALU - TRANS, 0);
-    }
-}
-
-// ---- rows form: 128 rows per workgroup, 32 per wave; all waves share the keys through LDS, two steps of them -------------------
-template <bool BF16, int DP, bool MASK>
-__global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams p) {
+// The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
+template <int DP, int WAVES>
+struct Copies {
     using H = Head<DP>;
-    using E = Elem<BF16>;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    int rb, hk, b;
-    block_of(p, p.row_blocks, rb, hk, b);
-    long long first;
-    int count;
-    keys_of(p, b, first, count);
-    const int row = rb * 128 + wave * 32 + col;
-    typename E::vec qf[H::KS];
-    load_q<BF16, DP>(p, qf, b, hk, row, lane);
-    const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
-    const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
-    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    constexpr int REQ = H::REQ / 4;  // per wave, of K and of V
-    const int bytes = p.D * 2;
-    // Request i of this wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
-    // two steps: the wave's rows start on a multiple of 16 where there are several requests).
-    const int row0 = wave * REQ * H::RPR + lane / H::PIECES;
-    const uint32_t ck = ((lane % H::PIECES) ^ H::fk(row0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(row0)) * 16;
-    const uint32_t ok = (uint32_t)(row0 * p.ks[1]), ov = (uint32_t)(row0 * p.vs[1]) + cv;
-    static_assert(REQ == 1 || (REQ * H::RPR == 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
-    const uint32_t dst = base + wave * REQ * 1024;
-    // Columns behind the head's end are zero in K for good: no copy writes there.
-    if (bytes < H::PITCH) {
-        for (int i = threadIdx.x; i < 2 * H::TILE / 16; i += 256) *(u32x4_t *)(lds + i * 16) = u32x4_t{0, 0, 0, 0};
-        __syncthreads();
+    // Request i of a wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
+    // two steps: the wave's rows start on a multiple of 16 where there are four requests, of 8 where there are two).
+    static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
+    static_assert(REQ == 1 || (REQ * H::RPR <= 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
+    const char *kp, *vp;
+    long long k_token, v_token;
+    uint32_t dst, ok, ov, ck;
+    int row0, count, bytes;
+    bool v_lane, any;
+    __device__ inline Copies(const AttentionParams &p, char *lds, int b, int hk, long long first, int count_, int wave, int lane) {
+        kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
+        vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
+        k_token = p.ks[1];
+        v_token = p.vs[1];
+        count = count_;
+        bytes = p.D * 2;
+        any = wave < ACTIVE;
+        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
+        row0 = wave * REQ * H::RPR + lane / H::PIECES;
+        ck = ((lane % H::PIECES) ^ H::fk(row0)) * 16;
+        const uint32_t cv = ((lane % H::PIECES) ^ H::fv(row0)) * 16;
+        ok = (uint32_t)(row0 * k_token);
+        ov = (uint32_t)(row0 * v_token) + cv;
+        v_lane = (int)cv < bytes;
+        // columns behind the head's end are zero in K for good: no copy writes there
+        if (bytes < H::PITCH) {
+            for (int i = threadIdx.x; i < 2 * H::TILE / 16; i += WAVES * 64) *(u32x4_t *)(lds + i * 16) = u32x4_t{0, 0, 0, 0};
+            __syncthreads();
+        }
     }
     // K of step `step` to stage `slot`.  Rows behind the last key are not read: their scores are masked whatever they are.
-    auto request_k = [&](int step, int slot) __attribute__((always_inline)) {
-        const char *k = kp + (long long)step * KEYS * p.ks[1];
+    __device__ __forceinline__ void k(int step, int slot) {
+        if (!any) return;
+        const char *k = kp + (long long)step * KEYS * k_token;
         const int left = count - step * KEYS;
         uint32_t c0 = ck;
         asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
+        if (left >= KEYS && bytes == H::PITCH) {
 #pragma unroll
-        for (int i = 0; i < REQ; i++) {
-            const uint32_t c = c0 ^ (64 * i);
-            if ((int)c < bytes && row0 < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * p.ks[1], ok + c);
-        }
-    };
-    // V: zeros for keys that do not count, since nothing times a NaN is one
-    auto request_v = [&](int step, int slot, uint64_t bits) __attribute__((always_inline)) {
-        const char *v = vp + (long long)step * KEYS * p.vs[1];
-        if ((int)cv >= bytes) return;
-        if (bits == ~0ull) {
-#pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * p.vs[1], ov);
+            for (int i = 0; i < REQ; i++) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok + (c0 ^ (64 * i)));
         } else {
 #pragma unroll
             for (int i = 0; i < REQ; i++) {
-                if ((bits >> (i * H::RPR)) >> row0 & 1) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * p.vs[1], ov);
-                else clear16(dst + (2 + slot) * H::TILE + i * 1024 + lane * 16);
+                const uint32_t c = c0 ^ (64 * i);
+                if ((int)c < bytes && row0 < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok + c);
             }
         }
-    };
-    auto scores = [&](float16_t (&s)[2], int slot) __attribute__((always_inline)) {
-        const char *k = lds + slot * H::TILE;
+    }
+    // V: zeros for keys that do not count, since nothing times a NaN is one
+    __device__ __forceinline__ void v(int step, int slot, uint64_t bits) {
+        if (!any || !v_lane) return;
+        const char *v = vp + (long long)step * KEYS * v_token;
+        if (bits == ~0ull) {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
+            for (int i = 0; i < REQ; i++) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * v_token, ov);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < H::KS; ks++) {
-                const u32x4_t w = *(const u32x4_t *)(k + (kb * 32 + col) * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16);
-                s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[kb]);
+            for (int i = 0; i < REQ; i++) {
+                if ((bits >> (i * H::RPR)) >> row0 & 1) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * v_token, ov);
+                else clear16(dst + (2 + slot) * H::TILE + i * 1024 + (threadIdx.x & 63) * 16);
             }
         }
-    };
-    // One step ahead: while the probabilities of step n are made and multiplied by V, the scores of step n + 1 are formed.
-    State<BF16, DP> st;
-    st.clear();
+    }
+};
+
+// ---- rows form: 4 waves of QB blocks of 32 rows each; all waves share the keys through LDS, two steps of them --------------------
+template <bool BF16, int DP, bool MASK, int QB>
+__global__ void __launch_bounds__(256, QB == 1 || DP <= 64 ? 2 : 1) attention_rows_kernel(AttentionParams p) {
+    using H = Head<DP>;
+    using E = Elem<BF16>;
+    using vec = typename E::vec;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    int rb, hk, b;
+    block_of(p.row_blocks, p.Hkv, rb, hk, b);
+    long long first;
+    int count;
+    keys_of(p, b, first, count);
+    const int row = (rb * 4 + wave) * 32 * QB + col;
+    vec qf[QB][H::KS];
+    State<BF16, DP> st[QB];
+#pragma unroll
+    for (int q = 0; q < QB; q++) {
+        load_q<BF16, DP>(p, qf[q], b, hk, row + 32 * q, lane);
+        st[q].clear();
+    }
+    Copies<DP, 4> copies(p, lds, b, hk, first, count, wave, lane);
     Steps<MASK> list;
     list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, 0, (count + KEYS - 1) / KEYS, 1, lane);
     int step = list.next();
+    uint64_t bits = list.bits;
     if (step >= 0) {
-        uint64_t bits = list.bits;
-        request_k(step, 0);
-        request_v(step, 0, bits);
-        int ahead = list.next();
-        uint64_t ahead_bits = list.bits;
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (ahead >= 0) request_k(ahead, 1);
-        float16_t even[2], odd[2];
-        scores(even, 0);
-        st.mask(even, bits, lane);
-        st.raise(st.highest(even) * p.scale2);
-        // one step: scores `s` of it, in stages `slot`; false behind the last
-        auto turn = [&](float16_t (&s)[2], float16_t (&next)[2], int slot) __attribute__((always_inline)) {
-            // K of the next step and V of this one have landed, of all waves; nobody reads what the requests below overwrite
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            typename E::vec pr[4];
-            if (ahead < 0) {
-                st.exponentials(s, p.scale2, pr);
-                st.product(pr, lds + (2 + slot) * H::TILE, lane);
-                return false;
-            }
-            request_v(ahead, slot ^ 1, ahead_bits);
-            const int after = list.next();
-            if (after >= 0) request_k(after, slot);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(next, slot ^ 1);
-            st.exponentials(s, p.scale2, pr);
-            interleave<2 * H::KS, 192 / (2 * H::KS), 32 / (2 * H::KS)>();
-            __builtin_amdgcn_sched_barrier(0);
-            st.product(pr, lds + (2 + slot) * H::TILE, lane);
-            __builtin_amdgcn_sched_barrier(0);
-            st.mask(next, ahead_bits, lane);
-            st.raise(st.highest(next) * p.scale2);
-            ahead = after;
-            ahead_bits = list.bits;
-            return true;
-        };
-        while (turn(even, odd, 0) && turn(odd, even, 1)) {}
+        copies.k(step, 0);
+        copies.v(step, 0, bits);
     }
-    store_row<BF16, DP>(p, st, across_sum(st.sum), b, hk, row, lane);
+    for (int slot = 0; step >= 0; slot ^= 1) {
+        // K and V of this step have landed, of all waves, and nobody reads what the next requests overwrite
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int next = list.next();
+        if (next >= 0) {
+            copies.k(next, slot ^ 1);
+            copies.v(next, slot ^ 1, list.bits);
+        }
+        const char *k = lds + slot * H::TILE + col * H::PITCH, *v = lds + (2 + slot) * H::TILE;
+        float16_t s[QB][2];
+        // operands of four matrix instructions a block at a time, the next four's on their way
+        constexpr int N = 2 * H::KS, GROUP = N % 4 == 0 ? 4 : 2;
+        vec kf[2][GROUP];
+        auto read_k = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                kf[g & 1][i] = __builtin_bit_cast(vec, *(const u32x4_t *)(k + kb * 32 * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16));
+            }
+        };
+#pragma unroll
+        for (int q = 0; q < QB; q++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[q][kb][e] = 0.f;
+        read_k(0);
+#pragma unroll
+        for (int g = 0; g < N / GROUP; g++) {
+            if (g + 1 < N / GROUP) read_k(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < GROUP; i++)
+#pragma unroll
+                for (int q = 0; q < QB; q++) {
+                    const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                    s[q][kb] = E::mfma(kf[g & 1][i], qf[q][ks], s[q][kb]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // 16 keys at a time: while the matrix cores multiply the probabilities of one 16, those of the next are made and the operands
+        // of the one behind it are on their way
+        vec vf[2][H::DB], pr[QB][2];
+        State<BF16, DP>::read_v(vf[0], v, 0, lane);
+        float ref[QB];
+#pragma unroll
+        for (int q = 0; q < QB; q++) {
+            st[q].mask(s[q], bits, lane);
+            st[q].raise(st[q].highest(s[q]) * p.scale2);
+            ref[q] = st[q].reference();
+            pr[q][0] = st[q].exponentials(s[q], 0, p.scale2, ref[q]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            if (n < 3) {
+                State<BF16, DP>::read_v(vf[(n + 1) & 1], v, n + 1, lane);
+#pragma unroll
+                for (int q = 0; q < QB; q++) pr[q][(n + 1) & 1] = st[q].exponentials(s[q], n + 1, p.scale2, ref[q]);
+            }
+#pragma unroll
+            for (int d = 0; d < H::DB; d++)
+#pragma unroll
+                for (int q = 0; q < QB; q++) st[q].o[d] = E::mfma(vf[n & 1][d], pr[q][n & 1], st[q].o[d]);
+            if (n < 3) {
+#pragma unroll
+                for (int d = 0; d < H::DB; d++) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                    for (int q = 0; q < QB; q++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 20 / H::DB, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 8 / H::DB, 0);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        step = next;
+        bits = list.bits;
+    }
+#pragma unroll
+    for (int q = 0; q < QB; q++) store_row<BF16, DP>(p, st[q], across_sum(st[q].sum), b, hk, row + 32 * q, lane);
 }
 
 // ---- keys form: 32 rows per workgroup, whose waves take every fourth step of the part's keys and meet in LDS; the parts of a row
@@ -419,7 +495,7 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     int rb, hk, b;
-    block_of(p, p.row_blocks * p.parts, rb, hk, b);
+    block_of(p.row_blocks * p.parts, p.Hkv, rb, hk, b);
     const int part = rb / p.row_blocks;
     rb -= part * p.row_blocks;
     long long first;
@@ -469,12 +545,8 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
 #pragma unroll
             for (int ks = 0; ks < H::KS; ks++) s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w[kb][ks]), qf[ks], s[kb]);
         }
-        st.mask(s, bits, lane);
-        st.raise(st.highest(s) * p.scale2);
-        typename E::vec pr[4];
-        st.exponentials(s, p.scale2, pr);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        st.product(pr, varea, lane);
+        st.attend(s, bits, p.scale2, varea, lane);
     }
     // the waves meet: {maximum, sum} first, then the outputs, in the place of V
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -562,17 +634,22 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) 
 }
 
 template <bool BF16, int DP, bool MASK>
-int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
+int launch_kernels(const AttentionParams &p, bool keys, bool groups, hipStream_t st) {
     using H = Head<DP>;
     const int lds = keys ? 4 * H::TILE > 1024 + H::DB * 4096 ? 4 * H::TILE : 1024 + H::DB * 4096 : 4 * H::TILE;
-    const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
+    const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK>
+                              : groups ? (const void *)attention_rows_kernel<BF16, DP, MASK, 2> : (const void *)attention_rows_kernel<BF16, DP, MASK, 1>;
     if (lds > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
         (void)hipGetLastError();
         return fail(SVDQ_ELAUNCH, "cross_attention: the device does not offer %d bytes of LDS", lds);
     }
     const dim3 grid((unsigned)((long long)p.row_blocks * p.parts * p.Hkv * p.B)), block(256);
+    if (groups) {
+        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK, 2>), grid, block, lds, st, p);
+        return check_launch("cross_attention");
+    }
     if (!keys) {
-        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
+        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK, 1>), grid, block, lds, st, p);
         return check_launch("cross_attention");
     }
     SVDQ_LAUNCH((attention_keys_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
@@ -583,18 +660,18 @@ int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
 }
 
 template <bool BF16, bool MASK>
-int launch_heads(const AttentionParams &p, bool keys, hipStream_t st) {
-    if (p.D <= 32) return launch_kernels<BF16, 32, MASK>(p, keys, st);
-    if (p.D <= 64) return launch_kernels<BF16, 64, MASK>(p, keys, st);
-    if (p.D <= 80) return launch_kernels<BF16, 80, MASK>(p, keys, st);
-    if (p.D <= 96) return launch_kernels<BF16, 96, MASK>(p, keys, st);
-    return launch_kernels<BF16, 128, MASK>(p, keys, st);
+int launch_heads(const AttentionParams &p, bool keys, bool groups, hipStream_t st) {
+    if (p.D <= 32) return launch_kernels<BF16, 32, MASK>(p, keys, groups, st);
+    if (p.D <= 64) return launch_kernels<BF16, 64, MASK>(p, keys, groups, st);
+    if (p.D <= 80) return launch_kernels<BF16, 80, MASK>(p, keys, groups, st);
+    if (p.D <= 96) return launch_kernels<BF16, 96, MASK>(p, keys, groups, st);
+    return launch_kernels<BF16, 128, MASK>(p, keys, groups, st);
 }
 
 // Which form a call takes and how many parts it divides the keys into.  The rows form reads K and V from memory once per 128 rows; it
 // wants enough of such blocks to fill the compute units.
 struct Plan {
-    bool keys;
+    bool keys, groups;
     long long row_blocks, parts, workspace;
 };
 Plan plan_of(const svdq_cross_attention_args *a, int cus) {
@@ -602,7 +679,8 @@ Plan plan_of(const svdq_cross_attention_args *a, int cus) {
     const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len, steps = (keys_each + KEYS - 1) / KEYS;
     Plan plan;
     plan.keys = rows <= 32 || (rows + 127) / 128 * bh < cus;
-    plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
+    plan.groups = !plan.keys && (rows + 255) / 256 * bh >= cus && false;
+    plan.row_blocks = plan.keys ? (rows + 31) / 32 : plan.groups ? (rows + 255) / 256 : (rows + 127) / 128;
     plan.parts = 1;
     if (plan.keys) {
         const long long want = (4 * cus + plan.row_blocks * bh - 1) / (plan.row_blocks * bh), most = (steps + 3) / 4;
@@ -690,6 +768,6 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args *a, void *st
     p.parts = (int)plan.parts;
     p.scale2 = a->scale * 1.44269504088896340736f;
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == SVDQ_BF16) return p.mask ? launch_heads<true, true>(p, plan.keys, st) : launch_heads<true, false>(p, plan.keys, st);
-    return p.mask ? launch_heads<false, true>(p, plan.keys, st) : launch_heads<false, false>(p, plan.keys, st);
+    if (a->dtype == SVDQ_BF16) return p.mask ? launch_heads<true, true>(p, plan.keys, plan.groups, st) : launch_heads<true, false>(p, plan.keys, plan.groups, st);
+    return p.mask ? launch_heads<false, true>(p, plan.keys, plan.groups, st) : launch_heads<false, false>(p, plan.keys, plan.groups, st);
 }

@@ -21,9 +21,12 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+#include <optional>
 #include <vector>
 
 #include "internal_api.h"
@@ -640,9 +643,191 @@ PyObject *vk_mul_q(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit linear layers and attention: the plain case of ops/w8a8.py and ops/attention.py, results allocated here ----------
+// (28 us of the caller's time for cross_attention, 13 .. 16 for the others in Python)
+int type_code(at::ScalarType t) { return t == at::kBFloat16 ? SVDQ_BF16 : t == at::kHalf ? SVDQ_FP16 : -1; }
+bool optional_tensor(PyObject *o, const at::Tensor **t) {
+    *t = nullptr;
+    return o == Py_None || as_tensor(o, t);
+}
+// rows [M, K] at one distance, the elements of a row next to each other; on the current device
+bool rows_of(const at::Tensor &x, int64_t *M, int64_t *K, int64_t *ld) {
+    if (!x.is_cuda() || x.dim() < 1 || x.numel() == 0 || x.device().index() != c10::hip::current_device()) return false;
+    *K = x.size(-1);
+    *M = x.numel() / *K;
+    if (x.is_contiguous()) {
+        *ld = *K;
+        return true;
+    }
+    if (x.dim() != 2 || x.stride(1) != 1 || *M < 2) return false;
+    *ld = x.stride(0);
+    return true;
+}
+PyObject *tuple_of(const at::Tensor &a, const at::Tensor &b, PyObject *third) {  // takes the reference to `third`, if any
+    PyObject *r = PyTuple_New(third ? 3 : 2);
+    if (!r) {
+        Py_XDECREF(third);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(a));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(b));
+    if (third) PyTuple_SET_ITEM(r, 2, third);
+    return r;
+}
+
+// w8a8_quantize(x) -> (codes, scales), or None
+PyObject *w8a8_quantize(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(1)
+    const at::Tensor *x;
+    svdq_quantize_w8a8_args a = {};
+    if (!as_tensor(args[0], &x) || (a.dtype = type_code(x->scalar_type())) < 0 || !rows_of(*x, &a.M, &a.K, &a.ld_input)) Py_RETURN_NONE;
+    at::Tensor codes = new_tensor(x->sizes(), at::kChar, *x), scales = new_tensor(x->sizes().slice(0, x->dim() - 1), at::kFloat, *x);
+    a.input = x->data_ptr();
+    a.output = codes.data_ptr();
+    a.oscales = (float *)scales.data_ptr();
+    hipStream_t st = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_quantize_w8a8_act(&a, st);
+    Py_END_ALLOW_THREADS
+    return rc != SVDQ_OK ? raise(rc) : tuple_of(codes, scales, nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
+// w8a8_norm(x, weight, residual or None, eps) -> (codes, scales, the sum with the residual or None), or None
+PyObject *w8a8_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(4)
+    const at::Tensor *x, *w, *r;
+    svdq_quantize_w8a8_args a = {};
+    if (!as_tensor(args[0], &x) || (a.dtype = type_code(x->scalar_type())) < 0 || !rows_of(*x, &a.M, &a.K, &a.ld_input) || !as_tensor(args[1], &w) ||
+        w->device() != x->device() || w->scalar_type() != x->scalar_type() || w->numel() != a.K || !w->is_contiguous() || !optional_tensor(args[2], &r) ||
+        !PyFloat_CheckExact(args[3])) Py_RETURN_NONE;
+    int64_t M, K;
+    if (r && (r->sizes() != x->sizes() || r->scalar_type() != x->scalar_type() || r->device() != x->device() || !rows_of(*r, &M, &K, &a.ld_residual))) Py_RETURN_NONE;
+    at::Tensor codes = new_tensor(x->sizes(), at::kChar, *x), scales = new_tensor(x->sizes().slice(0, x->dim() - 1), at::kFloat, *x), h;
+    a.input = x->data_ptr();
+    a.weight = w->data_ptr();
+    a.output = codes.data_ptr();
+    a.oscales = (float *)scales.data_ptr();
+    a.eps = (float)PyFloat_AS_DOUBLE(args[3]);
+    if (r) {
+        h = new_tensor(x->sizes(), x->scalar_type(), *x);
+        a.residual = r->data_ptr();
+        a.residual_out = h.data_ptr();
+        a.ld_residual_out = a.K;
+    }
+    hipStream_t st = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_rms_norm_quantize_w8a8(&a, st);
+    Py_END_ALLOW_THREADS
+    if (rc != SVDQ_OK) return raise(rc);
+    return tuple_of(codes, scales, r ? THPVariable_Wrap(h) : Py_NewRef(Py_None));
+    END_HANDLE_TH_ERRORS
+}
+
+// w8a8_gemm(act, wgt, ascales, wscales, bias or None, dtype or None) -> out, or None
+PyObject *w8a8_gemm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(6)
+    const at::Tensor *x, *w, *sa, *sw, *bias;
+    svdq_gemm_w8a8_args a = {};
+    int64_t K;
+    if (!as_tensor(args[0], &x) || x->scalar_type() != at::kChar || x->dim() < 2 || !rows_of(*x, &a.M, &a.K, &a.ld_act) || !as_tensor(args[1], &w) ||
+        w->scalar_type() != at::kChar || w->dim() != 2 || !rows_of(*w, &a.N, &K, &a.ld_wgt) || K != a.K || !as_tensor(args[2], &sa) || !as_tensor(args[3], &sw) ||
+        !plain_on(*sa, *x, at::kFloat, a.M) || !plain_on(*sw, *x, at::kFloat, a.N) || !optional_tensor(args[4], &bias)) Py_RETURN_NONE;
+    at::ScalarType dt = bias ? bias->scalar_type() : at::kBFloat16;
+    if (args[5] != Py_None) {
+        if (!THPDtype_Check(args[5])) Py_RETURN_NONE;
+        dt = ((THPDtype *)args[5])->scalar_type;
+    }
+    if ((a.dtype = type_code(dt)) < 0 || (bias && !plain_on(*bias, *x, dt, a.N))) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
+    sizes.back() = a.N;
+    at::Tensor out = new_tensor(sizes, dt, *x);
+    a.act = x->data_ptr();
+    a.wgt = w->data_ptr();
+    a.ascales = (const float *)sa->data_ptr();
+    a.wscales = (const float *)sw->data_ptr();
+    a.bias = bias ? bias->data_ptr() : nullptr;
+    a.out = out.data_ptr();
+    a.ld_out = a.N;
+    hipStream_t st = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_gemm_w8a8(&a, st);
+    Py_END_ALLOW_THREADS
+    return rc != SVDQ_OK ? raise(rc) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// batch, token and head strides of [B, T, H, D] (or [T, H, D]: batch stride 0); 0 for a dimension of one element
+bool head_strides(const at::Tensor &t, int64_t *s) {
+    const int64_t n = t.dim();
+    if (t.size(n - 1) > 1 && t.stride(n - 1) != 1) return false;
+    s[0] = 0;
+    for (int64_t i = 0; i < n - 1; i++) s[4 - n + i] = t.size(i) > 1 ? t.stride(i) : 0;
+    return true;
+}
+bool int_vector(const at::Tensor *t, const at::Tensor &x, int64_t n) { return !t || (t->dim() == 1 && plain_on(*t, x, at::kInt, n)); }
+
+// attention(q, k, v, key_lengths, key_mask, cu_seqlens_k, scale or None) -> out, or None
+PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(7)
+    const at::Tensor *q, *k, *v, *lengths, *mask, *cu;
+    svdq_cross_attention_args a = {};
+    if (!as_tensor(args[0], &q) || !as_tensor(args[1], &k) || !as_tensor(args[2], &v) || !optional_tensor(args[3], &lengths) || !optional_tensor(args[4], &mask) ||
+        !optional_tensor(args[5], &cu) || (lengths != nullptr) + (mask != nullptr) + (cu != nullptr) > 1) Py_RETURN_NONE;
+    if (!q->is_cuda() || q->device().index() != c10::hip::current_device() || (a.dtype = type_code(q->scalar_type())) < 0 || k->device() != q->device() ||
+        v->device() != q->device() || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || q->dim() != 4 || k->dim() != (cu ? 3 : 4) ||
+        k->sizes() != v->sizes() || q->numel() == 0 || k->numel() == 0) Py_RETURN_NONE;
+    a.batch = q->size(0);
+    a.q_len = q->size(1);
+    a.heads = q->size(2);
+    a.head_dim = q->size(3);
+    a.k_len = k->size(-3);
+    a.kv_heads = k->size(-2);
+    if (k->size(-1) != a.head_dim || (!cu && k->size(0) != a.batch) || a.heads % a.kv_heads || !head_strides(*q, a.q_stride) || !head_strides(*k, a.k_stride) ||
+        !head_strides(*v, a.v_stride) || !int_vector(lengths, *q, a.batch) || !int_vector(cu, *q, a.batch + 1)) Py_RETURN_NONE;
+    if (mask) {
+        if (mask->scalar_type() != at::kBool || mask->device() != q->device() || mask->sizes() != at::IntArrayRef({a.batch, a.k_len}) ||
+            (a.k_len > 1 && mask->stride(1) != 1)) Py_RETURN_NONE;
+        a.key_mask = mask->data_ptr();
+        a.mask_stride = a.batch > 1 ? mask->stride(0) : 0;
+    }
+    double scale = 1.0 / std::sqrt((double)a.head_dim);
+    if (args[6] != Py_None) {
+        if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+        scale = PyFloat_AS_DOUBLE(args[6]);
+    }
+    at::Tensor out = new_tensor(q->sizes(), q->scalar_type(), *q);
+    head_strides(out, a.out_stride);
+    a.q = q->data_ptr();
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.out = out.data_ptr();
+    a.key_lengths = lengths ? (const int32_t *)lengths->data_ptr() : nullptr;
+    a.cu_seqlens_k = cu ? (const int32_t *)cu->data_ptr() : nullptr;
+    a.scale = (float)scale;
+    hipStream_t st = c10::hip::getCurrentHIPStream(q->device().index()).stream();
+    int rc = svdq_cross_attention_workspace(&a, &a.workspace_bytes);
+    if (rc != SVDQ_OK) return raise(rc);
+    std::optional<Scratch> workspace;
+    if (a.workspace_bytes) a.workspace = workspace.emplace((size_t)a.workspace_bytes, st).ptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_cross_attention(&a, st);
+    Py_END_ALLOW_THREADS
+    return rc != SVDQ_OK ? raise(rc) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define SVDQ_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SVDQ_METHOD(make_layer), SVDQ_METHOD(linear), SVDQ_METHOD(gelu_mlp), SVDQ_METHOD(qkv_norm_rope), SVDQ_METHOD(awq_gemv), SVDQ_METHOD(awq_linear),
                          SVDQ_METHOD(quantize_call), SVDQ_METHOD(gemm_call), SVDQ_METHOD(vk_mul_q),
+                         SVDQ_METHOD(w8a8_quantize), SVDQ_METHOD(w8a8_norm), SVDQ_METHOD(w8a8_gemm), SVDQ_METHOD(attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Per-call host code of the quantized layers.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -45,6 +45,11 @@ def cross_attention(
     D is a multiple of 8 up to 128.  Tensors go by their strides (multiples of 8, elements of a head next to each other): the fp16
     [B, heads, tokens, 128] outputs of ``fused_qkv_norm_rottary`` are taken as ``t.transpose(1, 2)``.  ``out`` takes the result when
     given and must not overlap the inputs.  ``scale``: 1 / sqrt(D) by default, positive.  Forward only: the result carries no gradient."""
+    if out is None:
+        y = nv.host().attention(q, k, v, key_lengths, key_mask, cu_seqlens_k, scale)
+        if y is not None:
+            return y
+    # not the plain case: say what is wrong, or take the call with the caller's output or on another device than the current one
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
             raise RuntimeError(f"{name} must live on a GPU (got {t.device}); this path has no CPU implementation")

@@ -57,6 +57,11 @@ def quantize_w8a8_act(x: torch.Tensor, output: torch.Tensor | None = None, oscal
 
     K is a multiple of 16 up to 65536.  The rows of ``x`` may be parts of longer ones.  ``output`` and ``oscales`` take the results
     when given.  A weight [N, K] goes to its codes and channel scales the same way."""
+    if output is None and oscales is None:
+        y = nv.host().w8a8_quantize(x)
+        if y is not None:
+            return y
+    # not the plain case: say what is wrong, or take the call with the caller's outputs or on another device than the current one
     rows = _rows(x, "x")
     codes, scales = _outputs(rows, x.shape, output, oscales)
     M, K = rows.shape
@@ -81,6 +86,10 @@ def rms_norm_quantize_w8a8(
     h = ``x`` + ``residual``, rounded to the type (``x`` itself without a residual); y = h / sqrt(mean(h^2) + eps) * ``weight``, not
     rounded; codes and scales of y as in ``quantize_w8a8_act``.  Returns (codes int8 [..., K], scales fp32 [...], h), h None without
     a residual.  ``residual_out`` takes h when given; it may be ``residual`` or ``x`` itself (the stream is then updated in place)."""
+    if output is None and oscales is None and residual_out is None:
+        y = nv.host().w8a8_norm(x, weight, residual, eps)
+        if y is not None:
+            return y
     rows = _rows(x, "x")
     M, K = rows.shape
     if weight.device != x.device or weight.dtype != x.dtype or weight.numel() != K or not weight.is_contiguous():
@@ -140,6 +149,10 @@ def gemm_w8a8(
     output's type.  The integer sums are exact.  ``out_dtype``: bf16 by default, or the type of ``out`` or ``bias`` when given.
     K is a multiple of 16 below 131072; any numbers of rows and columns, from a single token on.  The rows of act, wgt and out may be
     parts of longer ones."""
+    if out is None:
+        y = nv.host().w8a8_gemm(act, wgt, ascales, wscales, bias, out_dtype)
+        if y is not None:
+            return y
     a, w = _code_rows(act, "act"), _code_rows(wgt, "wgt")
     M, K = a.shape
     N = w.shape[0]

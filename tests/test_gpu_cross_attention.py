@@ -54,7 +54,8 @@ SHAPES = [
     (1, 1, 1, 1, 1, 8), (2, 1, 63, 2, 1, 16), (1, 1, 64, 4, 4, 32), (3, 1, 65, 8, 2, 40), (1, 1, 1000, 5, 1, 64), (2, 1, 4097, 4, 2, 128), (1, 2, 513, 6, 3, 72),
     (1, 33, 130, 2, 2, 80), (2, 7, 257, 10, 2, 96), (1, 128, 128, 1, 1, 112), (1, 129, 77, 3, 3, 120), (2, 31, 1024, 2, 1, 24), (1, 300, 300, 2, 2, 104),
     (4, 1100, 77, 8, 8, 64), (2, 1024, 333, 20, 20, 72), (3, 260, 190, 16, 8, 128), (8, 500, 100, 8, 8, 32), (9, 130, 129, 30, 15, 96), (4, 1030, 64, 8, 8, 16),
-    (16, 128, 65, 16, 16, 88),
+    (16, 128, 65, 16, 16, 88), (4, 4090, 150, 4, 4, 32), (2, 2040, 65, 16, 4, 128), (1, 7937, 193, 8, 8, 72), (1, 4096, 128, 16, 16, 64), (2, 4000, 1, 8, 8, 96),
+    (1, 2550, 257, 96, 4, 112),
 ]
 
 
@@ -77,7 +78,8 @@ def test_all_keys(dev, shape, dtype):
     out.check("out")
 
 
-VALID_SHAPES = [(4, 1, 200, 4, 2, 128), (5, 3, 700, 2, 2, 72), (4, 260, 150, 16, 16, 64), (6, 257, 333, 12, 12, 80), (3, 40, 129, 4, 1, 32), (8, 1030, 70, 4, 4, 128)]
+VALID_SHAPES = [(4, 1, 200, 4, 2, 128), (5, 3, 700, 2, 2, 72), (4, 260, 150, 16, 16, 64), (6, 257, 333, 12, 12, 80), (3, 40, 129, 4, 1, 32), (8, 1030, 70, 4, 4, 128),
+                (8, 2030, 260, 4, 4, 128), (4, 4090, 150, 4, 4, 72), (3, 8000, 193, 3, 3, 24)]
 
 
 def spoil(t, keep):
