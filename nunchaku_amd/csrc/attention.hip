@@ -25,7 +25,7 @@ struct AttentionParams {
     const uint8_t *mask;
     float *partial;                                // keys-split form with several parts: [part][b][hkv][rows] x D, then {maximum, sum} pairs
     long long qs[3], ks[3], vs[3], os[3], mask_b;  // bytes: batch, token, head
-    int B, Hkv, G, D, Tq, Tk, rows, row_blocks, parts;
+    int B, Hkv, G, D, Tq, Tk, rows, row_blocks, parts, spread;
     float scale2;  // scale * log2(e)
 };
 
@@ -100,9 +100,9 @@ __device__ inline void keys_of(const AttentionParams &p, int b, long long &first
     count = __builtin_amdgcn_readfirstlane(count);
 }
 
-// The steps of 64 keys that hold any, in order, with a bit for every key that counts.  With a mask the bytes of the step behind the
+// The steps of SIZE keys that hold any, in order, with a bit for every key that counts.  With a mask the bytes of the step behind the
 // next one are on their way while a step is worked on; steps without a key are left out.
-template <bool MASK>
+template <bool MASK, int SIZE = KEYS>
 struct Steps {
     const uint8_t *mask;
     int count, steps, stride, at, lane;  // at: the next candidate
@@ -110,9 +110,9 @@ struct Steps {
     uint64_t bits;  // of the step that next() returned
     __device__ inline void fetch() {
         if (MASK) {
-            const int key = at * KEYS + lane;
+            const int key = at * SIZE + lane;
             byte = 0;
-            if (key < count) byte = mask[key];
+            if (lane < SIZE && key < count) byte = mask[key];
         }
     }
     __device__ inline void start(const uint8_t *m, int count_, int first, int end, int stride_, int lane_) {
@@ -128,8 +128,8 @@ struct Steps {
     // the next step with a key, or -1
     __device__ inline int next() {
         while (at < steps) {
-            const int step = at, left = count - step * KEYS;
-            bits = MASK ? __ballot(byte != 0) : left >= KEYS ? ~0ull : (1ull << left) - 1;
+            const int step = at, left = count - step * SIZE;
+            bits = MASK ? __ballot(byte != 0) : left >= SIZE ? ~0ull >> (64 - SIZE) : (1ull << left) - 1;
             at += stride;
             if (at < steps) fetch();
             if (!MASK || bits) return step;
@@ -157,24 +157,28 @@ struct State {
         sum = 0.f;
     }
     // keys without a bit get a score of minus infinity
-    static __device__ inline void mask(float16_t (&s)[2], uint64_t bits, int lane) {
-        if (bits == ~0ull) return;
+    template <int NB>
+    static __device__ inline void mask(float16_t (&s)[NB], uint64_t bits, int lane) {
+        if (bits == ~0ull >> (64 - 32 * NB)) return;
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
+        for (int kb = 0; kb < NB; kb++) {
             const uint32_t w = (uint32_t)(bits >> (32 * kb)) >> (4 * (lane >> 5));
 #pragma unroll
             for (int e = 0; e < 16; e++) s[kb][e] = w >> (8 * (e >> 2) + (e & 3)) & 1 ? s[kb][e] : -__builtin_huge_valf();
         }
     }
-    static __device__ inline float highest(const float16_t (&s)[2]) {
-        float m[4];  // (four chains: a vector instruction waits for the one before it)
+    template <int NB>
+    static __device__ inline float highest(const float16_t (&s)[NB]) {
+        float m[2 * NB];  // (as many chains: a vector instruction waits for the one before it)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 2 * NB; i++) {
             m[i] = s[i >> 1][8 * (i & 1)];
 #pragma unroll
             for (int e = 1; e < 8; e++) m[i] = __builtin_fmaxf(m[i], s[i >> 1][8 * (i & 1) + e]);
         }
-        return across_max(__builtin_fmaxf(__builtin_fmaxf(m[0], m[1]), __builtin_fmaxf(m[2], m[3])));
+        float top = __builtin_fmaxf(m[0], m[1]);
+        if constexpr (NB == 2) top = __builtin_fmaxf(top, __builtin_fmaxf(m[2], m[3]));
+        return across_max(top);
     }
     // A new maximum of a row (in units of log2).  The one in use only has to keep the exponentials in range: it moves when a row's is
     // more than 2^8 times off, so that the outputs are rarely scaled.
@@ -205,7 +209,8 @@ struct State {
         }
     }
     // the right operand: probabilities of 16 keys, rounded
-    __device__ inline vec exponentials(const float16_t (&s)[2], int n, float scale2, float ref) {
+    template <int NB>
+    __device__ inline vec exponentials(const float16_t (&s)[NB], int n, float scale2, float ref) {
         float x[8];
         u32x4_t w;
 #pragma unroll
@@ -218,7 +223,8 @@ struct State {
     __device__ inline float reference() const { return top == -__builtin_huge_valf() ? 0.f : top; }
     // A step's scores and values (v in LDS) join the sums, 16 keys at a time: while the matrix cores multiply the probabilities of
     // one 16, those of the next are made and the operands of the one behind it are on their way.
-    __device__ inline void attend(float16_t (&s)[2], uint64_t bits, float scale2, const char *v, int lane) {
+    template <int NB>
+    __device__ inline void attend(float16_t (&s)[NB], uint64_t bits, float scale2, const char *v, int lane) {
         vec vf[2][H::DB], pr[2];
         read_v(vf[0], v, 0, lane);
         mask(s, bits, lane);
@@ -227,14 +233,14 @@ struct State {
         pr[0] = exponentials(s, 0, scale2, ref);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-            if (n < 3) {
+        for (int n = 0; n < 2 * NB; n++) {
+            if (n < 2 * NB - 1) {
                 read_v(vf[(n + 1) & 1], v, n + 1, lane);
                 pr[(n + 1) & 1] = exponentials(s, n + 1, scale2, ref);
             }
 #pragma unroll
             for (int d = 0; d < H::DB; d++) o[d] = E::mfma(vf[n & 1][d], pr[n & 1], o[d]);
-            if (n < 3) {
+            if (n < 2 * NB - 1) {
 #pragma unroll
                 for (int d = 0; d < H::DB; d++) {
                     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
@@ -260,6 +266,10 @@ __device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec
         if (row < p.rows && c < p.D) w = *(const u32x4_t *)(q + c * 2);
         qf[ks] = __builtin_bit_cast(typename Elem<BF16>::vec, w);
     }
+    // The compiler waits for these loads where they are first used.  In the loop over the keys that wait would be for the copies
+    // that a step has just asked for, too, and at every step: they are waited for here.
+#pragma unroll
+    for (int ks = 0; ks < Head<DP>::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
 
 // This lane's row of the output, normalised: 8 consecutive columns per lane and 16-byte store
@@ -291,15 +301,22 @@ __device__ inline void store_row(const AttentionParams &p, State<BF16, DP> &s, f
         }
 }
 
-// Which (row block, head, batch entry) a workgroup takes: workgroups go round robin over 8 XCDs, each with an L2 of its own, and an
-// XCD gets a contiguous run, whose row blocks read the same keys.
-__device__ inline void block_of(int per_head, int heads, int &rb, int &hk, int &b) {
-    const int total = gridDim.x, id = blockIdx.x, xcd = id & 7, per = total >> 3, more = total & 7;
-    const int at = xcd * per + (xcd < more ? xcd : more) + (id >> 3);
-    rb = at % per_head;
-    const int bh = at / per_head;
-    hk = bh % heads;
-    b = bh / heads;
+// Which (row block, group) a workgroup takes, false: none.  A group's row blocks read the same keys (of a head, or of a part of its keys).
+// Workgroups go round robin over 8 XCDs, each with an L2 of its own.  The row blocks of a group go to one XCD, the groups in turn over
+// the XCDs (`spread`: a batch entry's keys may be many or few, and eight entries on an XCD each would leave some of them idle), or, where
+// there are too few groups for that to come out even, an XCD gets a contiguous run of all row blocks.
+__device__ inline bool block_of(const AttentionParams &p, int groups, int &rb, int &group) {
+    const int id = blockIdx.x, xcd = id & 7, j = id >> 3;
+    if (p.spread) {
+        group = j / p.row_blocks * 8 + xcd;
+        rb = j % p.row_blocks;
+        return group < groups;
+    }
+    const int total = groups * p.row_blocks, per = total >> 3, more = total & 7;
+    const int at = xcd * per + (xcd < more ? xcd : more) + j;
+    rb = at % p.row_blocks;
+    group = at / p.row_blocks;
+    return true;
 }
 
 // The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
@@ -371,27 +388,25 @@ struct Copies {
     }
 };
 
-// ---- rows form: 4 waves of QB blocks of 32 rows each; all waves share the keys through LDS, two steps of them --------------------
-template <bool BF16, int DP, bool MASK, int QB>
-__global__ void __launch_bounds__(256, QB == 1 || DP <= 64 ? 2 : 1) attention_rows_kernel(AttentionParams p) {
+// ---- rows form: 128 rows per workgroup, 32 per wave; all waves share the keys through LDS, two steps of them -------------------
+template <bool BF16, int DP, bool MASK>
+__global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams p) {
     using H = Head<DP>;
     using E = Elem<BF16>;
     using vec = typename E::vec;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    int rb, hk, b;
-    block_of(p.row_blocks, p.Hkv, rb, hk, b);
+    int rb, group;
+    if (!block_of(p, p.Hkv * p.B, rb, group)) return;
+    const int hk = group % p.Hkv, b = group / p.Hkv;
     long long first;
     int count;
     keys_of(p, b, first, count);
-    const int row = (rb * 4 + wave) * 32 * QB + col;
-    vec qf[QB][H::KS];
-    State<BF16, DP> st[QB];
-#pragma unroll
-    for (int q = 0; q < QB; q++) {
-        load_q<BF16, DP>(p, qf[q], b, hk, row + 32 * q, lane);
-        st[q].clear();
-    }
+    const int row = (rb * 4 + wave) * 32 + col;
+    vec qf[H::KS];
+    State<BF16, DP> st;
+    load_q<BF16, DP>(p, qf, b, hk, row, lane);
+    st.clear();
     Copies<DP, 4> copies(p, lds, b, hk, first, count, wave, lane);
     Steps<MASK> list;
     list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, 0, (count + KEYS - 1) / KEYS, 1, lane);
@@ -410,8 +425,8 @@ __global__ void __launch_bounds__(256, QB == 1 || DP <= 64 ? 2 : 1) attention_ro
             copies.v(next, slot ^ 1, list.bits);
         }
         const char *k = lds + slot * H::TILE + col * H::PITCH, *v = lds + (2 + slot) * H::TILE;
-        float16_t s[QB][2];
-        // operands of four matrix instructions a block at a time, the next four's on their way
+        float16_t s[2];
+        // operands of four matrix instructions at a time, the next four's on their way
         constexpr int N = 2 * H::KS, GROUP = N % 4 == 0 ? 4 : 2;
         vec kf[2][GROUP];
         auto read_k = [&](int g) __attribute__((always_inline)) {
@@ -422,82 +437,39 @@ __global__ void __launch_bounds__(256, QB == 1 || DP <= 64 ? 2 : 1) attention_ro
             }
         };
 #pragma unroll
-        for (int q = 0; q < QB; q++)
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[q][kb][e] = 0.f;
+            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
         read_k(0);
 #pragma unroll
         for (int g = 0; g < N / GROUP; g++) {
             if (g + 1 < N / GROUP) read_k(g + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < GROUP; i++)
-#pragma unroll
-                for (int q = 0; q < QB; q++) {
-                    const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
-                    s[q][kb] = E::mfma(kf[g & 1][i], qf[q][ks], s[q][kb]);
-                }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // 16 keys at a time: while the matrix cores multiply the probabilities of one 16, those of the next are made and the operands
-        // of the one behind it are on their way
-        vec vf[2][H::DB], pr[QB][2];
-        State<BF16, DP>::read_v(vf[0], v, 0, lane);
-        float ref[QB];
-#pragma unroll
-        for (int q = 0; q < QB; q++) {
-            st[q].mask(s[q], bits, lane);
-            st[q].raise(st[q].highest(s[q]) * p.scale2);
-            ref[q] = st[q].reference();
-            pr[q][0] = st[q].exponentials(s[q], 0, p.scale2, ref[q]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int n = 0; n < 4; n++) {
-            if (n < 3) {
-                State<BF16, DP>::read_v(vf[(n + 1) & 1], v, n + 1, lane);
-#pragma unroll
-                for (int q = 0; q < QB; q++) pr[q][(n + 1) & 1] = st[q].exponentials(s[q], n + 1, p.scale2, ref[q]);
-            }
-#pragma unroll
-            for (int d = 0; d < H::DB; d++)
-#pragma unroll
-                for (int q = 0; q < QB; q++) st[q].o[d] = E::mfma(vf[n & 1][d], pr[q][n & 1], st[q].o[d]);
-            if (n < 3) {
-#pragma unroll
-                for (int d = 0; d < H::DB; d++) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-                    for (int q = 0; q < QB; q++) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 20 / H::DB, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x400, 8 / H::DB, 0);
-                    }
-                }
+            for (int i = 0; i < GROUP; i++) {
+                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                s[kb] = E::mfma(kf[g & 1][i], qf[ks], s[kb]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        st.attend(s, bits, p.scale2, v, lane);
         step = next;
         bits = list.bits;
     }
-#pragma unroll
-    for (int q = 0; q < QB; q++) store_row<BF16, DP>(p, st[q], across_sum(st[q].sum), b, hk, row + 32 * q, lane);
+    store_row<BF16, DP>(p, st, across_sum(st.sum), b, hk, row, lane);
 }
 
-// ---- keys form: 32 rows per workgroup, whose waves take every fourth step of the part's keys and meet in LDS; the parts of a row
-// block meet in attention_join_kernel -----------------------------------------------------------------------------------------------
+// ---- keys form: 32 rows per workgroup, whose waves take every fourth step (of 32 keys) of the part's keys, each through its own LDS, a
+// step ahead, and meet in LDS at the end; the parts of a row block meet in attention_join_kernel ------------------------------------
 template <bool BF16, int DP, bool MASK>
-__global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams p) {
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(AttentionParams p) {
     using H = Head<DP>;
     using E = Elem<BF16>;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    int rb, hk, b;
-    block_of(p.row_blocks * p.parts, p.Hkv, rb, hk, b);
-    const int part = rb / p.row_blocks;
-    rb -= part * p.row_blocks;
+    int rb, group;
+    if (!block_of(p, p.Hkv * p.B * p.parts, rb, group)) return;
+    const int part = group % p.parts, hk = group / p.parts % p.Hkv, b = group / p.parts / p.Hkv;
     long long first;
     int count;
     keys_of(p, b, first, count);
@@ -506,50 +478,63 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
     load_q<BF16, DP>(p, qf, b, hk, row, lane);
     const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
     const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
-    const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * H::TILE;
-    const char *varea = lds + wave * H::TILE;
-    const int steps = (count + KEYS - 1) / KEYS, bytes = p.D * 2;
+    constexpr int SIZE = 32, REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
+    char *mine = lds + wave * 2 * STAGE;
+    const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 2 * STAGE;
+    const int steps = (count + SIZE - 1) / SIZE, bytes = p.D * 2;
     const int begin = (int)((long long)steps * part / p.parts), end = (int)((long long)steps * (part + 1) / p.parts);
+    // Request i brings rows r0 + i * RPR: of V the same piece every time, of K the pieces that f has there
+    const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
+    const uint32_t ok = (uint32_t)(r0 * p.ks[1]), ov = (uint32_t)(r0 * p.vs[1]) + cv;
+    static_assert(H::fv(H::RPR) == 0 && (H::RPR == 16 || H::fk(H::RPR) == 4), "");
+    if (bytes < H::PITCH) {  // columns behind the head's end are zero in K for good
+        for (int i = lane; i < 2 * STAGE / 16; i += 64) *(u32x4_t *)(mine + i * 16) = u32x4_t{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    auto request = [&](int step, int slot, uint64_t bits) __attribute__((always_inline)) {
+        const char *k = kp + (long long)step * SIZE * p.ks[1], *v = vp + (long long)step * SIZE * p.vs[1];
+        const int left = count - step * SIZE;
+        const uint32_t dst = area + slot * STAGE;
+#pragma unroll
+        for (int i = 0; i < REQ; i++) {
+            const int c = ck ^ (64 * (i & (16 / H::RPR - 1)));
+            if (c < bytes && r0 < left - i * H::RPR) copy16(dst + i * 1024, k + i * H::RPR * p.ks[1], ok + c);
+        }
+#pragma unroll
+        for (int i = 0; i < REQ; i++) {
+            if (cv >= bytes) continue;
+            if ((bits >> (i * H::RPR)) >> r0 & 1) copy16(dst + STAGE / 2 + i * 1024, v + i * H::RPR * p.vs[1], ov);
+            else clear16(dst + STAGE / 2 + i * 1024 + lane * 16);
+        }
+    };
     State<BF16, DP> st;
     st.clear();
-    Steps<MASK> list;
+    Steps<MASK, SIZE> list;
     list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, begin + wave, end, 4, lane);
-    for (int step; (step = list.next()) >= 0;) {
-        const uint64_t bits = list.bits;
-        const char *k = kp + (long long)step * KEYS * p.ks[1], *v = vp + (long long)step * KEYS * p.vs[1];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last step's reads are done
-        const int r0 = lane / H::PIECES, c = ((lane % H::PIECES) ^ H::fv(r0)) * 16;  // (f is the same in all requests)
-        const uint32_t ov = (uint32_t)(r0 * p.vs[1]) + c;
+    int step = list.next();
+    uint64_t bits = list.bits;
+    if (step >= 0) request(step, 0, bits);
+    for (int slot = 0; step >= 0; slot ^= 1) {
+        const int next = list.next();
+        if (next >= 0) request(next, slot ^ 1, list.bits);
+        // This step's copies have landed when no more than the next one's are on their way.  Of a step with keys that do not count some
+        // requests may have had no lane to make them: then all have to land.
+        if (next >= 0 && list.bits == 0xFFFFFFFFull) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        const char *k = mine + slot * STAGE + col * H::PITCH;
+        float16_t s[1];
 #pragma unroll
-        for (int i = 0; i < H::REQ; i++) {
-            if (c >= bytes) continue;
-            if ((bits >> (i * H::RPR)) >> r0 & 1) copy16(area + i * 1024, v + i * H::RPR * p.vs[1], ov);
-            else clear16(area + i * 1024 + lane * 16);
+        for (int e = 0; e < 16; e++) s[0][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < H::KS; ks++) {
+            const u32x4_t w = *(const u32x4_t *)(k + ((2 * ks + h) ^ H::fk(col)) * 16);
+            s[0] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[0]);
         }
-        u32x4_t w[2][H::KS];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            const bool in = step * KEYS + 32 * kb + col < count;
-#pragma unroll
-            for (int ks = 0; ks < H::KS; ks++) {
-                const int c = (2 * ks + h) * 16;
-                w[kb][ks] = u32x4_t{0, 0, 0, 0};
-                if (in && c < bytes) w[kb][ks] = *(const u32x4_t *)(k + (32 * kb + col) * p.ks[1] + c);
-            }
-        }
-        float16_t s[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < H::KS; ks++) s[kb] = E::mfma(__builtin_bit_cast(typename E::vec, w[kb][ks]), qf[ks], s[kb]);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        st.attend(s, bits, p.scale2, varea, lane);
+        st.attend(s, bits, p.scale2, mine + slot * STAGE + STAGE / 2, lane);
+        step = next;
+        bits = list.bits;
     }
-    // the waves meet: {maximum, sum} first, then the outputs, in the place of V
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // the waves meet in the place of the stages: {maximum, sum} of all, then the outputs of the other three, scaled to the highest maximum
     __syncthreads();
     float *stat = (float *)lds;  // [4][2][32]
     const float own = across_sum(st.sum);
@@ -565,25 +550,23 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
 #pragma unroll
     for (int i = 0; i < 4; i++) sum += stat[i * 64 + 32 + col] * __builtin_amdgcn_exp2f(stat[i * 64 + col] - ref);
     const float f = __builtin_amdgcn_exp2f(st.top - ref);
-    float *sums = (float *)lds + 256;  // [32 DB][33] of one wave at a time
-    for (int i = 1; i < 4; i++) {
-        __syncthreads();
-        if (wave == i) {
+    float *sums = stat + 256 + lane;  // [3][16 DB][64]
+    if (wave > 0 && row < p.rows) {
 #pragma unroll
-            for (int d = 0; d < H::DB; d++)
+        for (int d = 0; d < H::DB; d++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) sums[((d * 16 + e) * 64) + lane] = st.o[d][e] * f;
-        }
-        __syncthreads();
-        if (wave == 0) {
+            for (int e = 0; e < 16; e++) sums[(((wave - 1) * H::DB + d) * 16 + e) * 64] = st.o[d][e] * f;
+    }
+    __syncthreads();
+    if (wave == 0 && row < p.rows) {
 #pragma unroll
-            for (int d = 0; d < H::DB; d++)
+        for (int d = 0; d < H::DB; d++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    if (i == 1) st.o[d][e] *= f;
-                    st.o[d][e] += sums[((d * 16 + e) * 64) + lane];
-                }
-        }
+            for (int e = 0; e < 16; e++) {
+                st.o[d][e] *= f;
+#pragma unroll
+                for (int i = 0; i < 3; i++) st.o[d][e] += sums[((i * H::DB + d) * 16 + e) * 64];
+            }
     }
     if (wave > 0) return;
     if (p.parts == 1) {
@@ -607,71 +590,94 @@ __global__ void __launch_bounds__(256, 2) attention_keys_kernel(AttentionParams 
     }
 }
 
-// Adds the parts of every row: one wave per row, two columns per lane
+// Adds the parts of every row (at most 64): one workgroup per row, two columns per lane, whose waves take every fourth part, all requested
+// at once.  Lane i of every wave holds part i's share of the row.
+constexpr int MAX_PARTS = 64;
 template <bool BF16>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) {
-    const int lane = threadIdx.x & 63;
-    const long long heads = (long long)p.B * p.Hkv, all = heads * p.rows, at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= all) return;
+    __shared__ float sums[4][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long all = (long long)p.B * p.Hkv * p.rows, at = blockIdx.x;
     const float *ms = p.partial + p.parts * all * p.D;
-    float top = -__builtin_huge_valf();
-    for (int i = 0; i < p.parts; i++) top = __builtin_fmaxf(top, ms[(i * all + at) * 2]);
-    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
-    float sum = 0.f, x = 0.f, y = 0.f;
-    const int c = lane * 2;
-    for (int i = 0; i < p.parts; i++) {
-        const float f = __builtin_amdgcn_exp2f(ms[(i * all + at) * 2] - ref);
-        sum += ms[(i * all + at) * 2 + 1] * f;
-        if (c < p.D) {
-            const float *src = p.partial + (i * all + at) * p.D + c;
-            x += src[0] * f;
-            y += src[1] * f;
-        }
+    const int c = lane * 2 < p.D ? lane * 2 : 0;
+    typedef float float2_t __attribute__((ext_vector_type(2)));
+    float2_t part[MAX_PARTS / 4];
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS / 4; i++) {
+        part[i] = float2_t{0.f, 0.f};
+        if (wave + 4 * i < p.parts) part[i] = *(const float2_t *)(p.partial + ((wave + 4 * i) * all + at) * p.D + c);
+    }
+    float top = -__builtin_huge_valf(), sum = 0.f;
+    if (lane < p.parts) {
+        const float2_t t = *(const float2_t *)(ms + (lane * all + at) * 2);
+        top = t[0];
+        sum = t[1];
+    }
+    float most = top;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    const float f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
+    sum *= f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAX_PARTS / 4; i++) {
+        if (wave + 4 * i >= p.parts) break;
+        const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), wave + 4 * i));
+        x = __builtin_fmaf(part[i][0], g, x);
+        y = __builtin_fmaf(part[i][1], g, y);
+    }
+    sums[wave][0][lane] = x;
+    sums[wave][1][lane] = y;
+    __syncthreads();
+    if (wave > 0 || lane * 2 >= p.D) return;
+#pragma unroll
+    for (int i = 1; i < 4; i++) {
+        x += sums[i][0][lane];
+        y += sums[i][1][lane];
     }
     const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
     const int bh = (int)(at / p.rows), row = (int)(at - (long long)bh * p.rows), b = bh / p.Hkv, hk = bh - b * p.Hkv, t = row / p.G, g = row - t * p.G;
-    if (c < p.D) *(uint32_t *)(p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + g) * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
+    *(uint32_t *)(p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + g) * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
 }
 
 template <bool BF16, int DP, bool MASK>
-int launch_kernels(const AttentionParams &p, bool keys, bool groups, hipStream_t st) {
+int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
     using H = Head<DP>;
-    const int lds = keys ? 4 * H::TILE > 1024 + H::DB * 4096 ? 4 * H::TILE : 1024 + H::DB * 4096 : 4 * H::TILE;
-    const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK>
-                              : groups ? (const void *)attention_rows_kernel<BF16, DP, MASK, 2> : (const void *)attention_rows_kernel<BF16, DP, MASK, 1>;
+    const int lds = (keys ? 8 : 4) * H::TILE;
+    static_assert(1024 + 3 * H::DB * 4096 <= 8 * H::TILE, "the waves' sums take the place of the stages");
+    const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
     if (lds > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
         (void)hipGetLastError();
         return fail(SVDQ_ELAUNCH, "cross_attention: the device does not offer %d bytes of LDS", lds);
     }
-    const dim3 grid((unsigned)((long long)p.row_blocks * p.parts * p.Hkv * p.B)), block(256);
-    if (groups) {
-        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK, 2>), grid, block, lds, st, p);
-        return check_launch("cross_attention");
-    }
+    const long long groups = (long long)p.parts * p.Hkv * p.B;
+    const dim3 grid((unsigned)((p.spread ? (groups + 7) / 8 * 8 : groups) * p.row_blocks)), block(256);
     if (!keys) {
-        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK, 1>), grid, block, lds, st, p);
+        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
         return check_launch("cross_attention");
     }
     SVDQ_LAUNCH((attention_keys_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
     int rc = check_launch("cross_attention");
     if (rc || p.parts == 1) return rc;
-    SVDQ_LAUNCH((attention_join_kernel<BF16>), dim3((unsigned)(((long long)p.B * p.Hkv * p.rows + 3) / 4)), block, 0, st, p);
+    SVDQ_LAUNCH((attention_join_kernel<BF16>), dim3((unsigned)((long long)p.B * p.Hkv * p.rows)), dim3(256), 0, st, p);
     return check_launch("cross_attention");
 }
 
 template <bool BF16, bool MASK>
-int launch_heads(const AttentionParams &p, bool keys, bool groups, hipStream_t st) {
-    if (p.D <= 32) return launch_kernels<BF16, 32, MASK>(p, keys, groups, st);
-    if (p.D <= 64) return launch_kernels<BF16, 64, MASK>(p, keys, groups, st);
-    if (p.D <= 80) return launch_kernels<BF16, 80, MASK>(p, keys, groups, st);
-    if (p.D <= 96) return launch_kernels<BF16, 96, MASK>(p, keys, groups, st);
-    return launch_kernels<BF16, 128, MASK>(p, keys, groups, st);
+int launch_heads(const AttentionParams &p, bool keys, hipStream_t st) {
+    if (p.D <= 32) return launch_kernels<BF16, 32, MASK>(p, keys, st);
+    if (p.D <= 64) return launch_kernels<BF16, 64, MASK>(p, keys, st);
+    if (p.D <= 80) return launch_kernels<BF16, 80, MASK>(p, keys, st);
+    if (p.D <= 96) return launch_kernels<BF16, 96, MASK>(p, keys, st);
+    return launch_kernels<BF16, 128, MASK>(p, keys, st);
 }
 
 // Which form a call takes and how many parts it divides the keys into.  The rows form reads K and V from memory once per 128 rows; it
 // wants enough of such blocks to fill the compute units.
 struct Plan {
-    bool keys, groups;
+    bool keys;
     long long row_blocks, parts, workspace;
 };
 Plan plan_of(const svdq_cross_attention_args *a, int cus) {
@@ -679,13 +685,14 @@ Plan plan_of(const svdq_cross_attention_args *a, int cus) {
     const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len, steps = (keys_each + KEYS - 1) / KEYS;
     Plan plan;
     plan.keys = rows <= 32 || (rows + 127) / 128 * bh < cus;
-    plan.groups = !plan.keys && (rows + 255) / 256 * bh >= cus && false;
-    plan.row_blocks = plan.keys ? (rows + 31) / 32 : plan.groups ? (rows + 255) / 256 : (rows + 127) / 128;
+    plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
     plan.parts = 1;
     if (plan.keys) {
-        const long long want = (4 * cus + plan.row_blocks * bh - 1) / (plan.row_blocks * bh), most = (steps + 3) / 4;
+        // one round of workgroups: two to a compute unit with heads up to 64, one with wider ones (LDS), and at least a step per wave
+        const long long slots = (a->head_dim <= 64 ? 2 : 1) * cus, want = slots / (plan.row_blocks * bh), most = (2 * steps + 3) / 4;
         plan.parts = want < most ? want : most;
         if (plan.parts < 1) plan.parts = 1;
+        if (plan.parts > MAX_PARTS) plan.parts = MAX_PARTS;
     }
     plan.workspace = plan.parts > 1 ? plan.parts * bh * rows * (a->head_dim + 2) * 4 : 0;
     return plan;
@@ -739,7 +746,7 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args *a, void *st
     const Plan plan = plan_of(a, cus);
     SVDQ_REQUIRE(plan.workspace == 0 || (a->workspace && a->workspace_bytes >= plan.workspace), "cross_attention: needs a workspace of %lld bytes, got %lld", plan.workspace,
                  (long long)(a->workspace ? a->workspace_bytes : 0));
-    const long long grid = plan.row_blocks * plan.parts * a->kv_heads * a->batch;
+    const long long grid = plan.row_blocks * (plan.parts * a->kv_heads * a->batch + 7);
     if (grid >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "cross_attention: %lld workgroups are too many for one launch", grid);
     AttentionParams p;
     p.q = (const char *)a->q;
@@ -766,8 +773,10 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args *a, void *st
     p.rows = p.Tq * p.G;
     p.row_blocks = (int)plan.row_blocks;
     p.parts = (int)plan.parts;
+    const long long groups = plan.parts * a->kv_heads * a->batch, turns = (groups + 7) / 8 * 8;
+    p.spread = turns * 15 <= groups * 16;  // (at most a fifteenth more than an even share)
     p.scale2 = a->scale * 1.44269504088896340736f;
     hipStream_t st = (hipStream_t)stream;
-    if (a->dtype == SVDQ_BF16) return p.mask ? launch_heads<true, true>(p, plan.keys, plan.groups, st) : launch_heads<true, false>(p, plan.keys, plan.groups, st);
-    return p.mask ? launch_heads<false, true>(p, plan.keys, plan.groups, st) : launch_heads<false, false>(p, plan.keys, plan.groups, st);
+    if (a->dtype == SVDQ_BF16) return p.mask ? launch_heads<true, true>(p, plan.keys, st) : launch_heads<true, false>(p, plan.keys, st);
+    return p.mask ? launch_heads<false, true>(p, plan.keys, st) : launch_heads<false, false>(p, plan.keys, st);
 }

@@ -18,6 +18,9 @@ struct W8A8Params {
     long long ld_act, ld_wgt, ld_out;  // bytes, bytes, elements
     int M, N, K, bf16;
     int tiles_m, tiles_n;
+    int parts;          // along K; with more than one, a workgroup leaves its sums in `partial` and a small kernel finishes
+    int *partial;       // [part][M][ld_partial]
+    long long ld_partial;
     int wide;  // rows of `out` and its first column are 16 bytes apart and aligned
 };
 
@@ -34,7 +37,7 @@ __device__ inline uint32_t pair16(float lo, float hi, int bf16) {
 // tiles, which are numbered down the rows inside bands of up to BAND row blocks, so that the tiles at work on an XCD share operands.
 constexpr int BAND = 8;
 __device__ inline void tile_of(const W8A8Params &p, int &tm, int &tn) {
-    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;
+    const int total = p.tiles_m * p.tiles_n, id = blockIdx.x;  // (of the part blockIdx.y)
     const int xcd = id & 7, per = total >> 3, more = total & 7;
     const int tile = xcd * per + (xcd < more ? xcd : more) + (id >> 3);
     const int band_tiles = BAND * p.tiles_n, band = tile / band_tiles, in = tile - band * band_tiles;
@@ -88,10 +91,13 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
         piece_b[i] = ((lane & 7) ^ swizzle(r)) * 16;
         off_b[i] = (uint32_t)((r < last ? r : last) * p.ld_wgt) + piece_b[i];
     }
-    const int whole = p.K / BK, steps = (p.K + BK - 1) / BK;
+    // this part's steps along K
+    const int whole = p.K / BK, all = (p.K + BK - 1) / BK;
+    const int begin = (int)((long long)all * blockIdx.y / p.parts), steps = (int)((long long)all * (blockIdx.y + 1) / p.parts) - begin;
     const uint32_t dst_a = base + wave * T::A_REQ * 1024, dst_b = base + BM * BK + wave * T::B_REQ * 1024;
-    auto request = [&](int step) __attribute__((always_inline)) {
-        const uint32_t stage = (uint32_t)(step % STAGES) * T::STAGE;
+    auto request = [&](int n) __attribute__((always_inline)) {
+        const uint32_t stage = (uint32_t)(n % STAGES) * T::STAGE;
+        const int step = begin + n;
         const char *a = src_a + (long long)step * BK, *b = src_b + (long long)step * BK;
         if (step < whole) {
 #pragma unroll
@@ -130,24 +136,50 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
         // this step's copies have landed (of all waves), and nobody reads the stage that the next request overwrites
         if (step + STAGES - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * T::REQ) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + STAGES - 1 < steps) request(step + STAGES - 1);
         const int stage = (step % STAGES) * T::STAGE;
+        // operands of one 32 of K ahead of the matrix instructions; the copies are asked for behind the first ones
+        int4_t a[2][T::TM], b[2][T::TN];
+        auto read = [&](int ks) __attribute__((always_inline)) {
+            const int at = ((2 * ks + h) ^ swizzle(col)) * 16;
+#pragma unroll
+            for (int i = 0; i < T::TM; i++) a[ks & 1][i] = *(const int4_t *)(row_a + stage + i * 32 * BK + at);
+#pragma unroll
+            for (int j = 0; j < T::TN; j++) b[ks & 1][j] = *(const int4_t *)(row_b + stage + j * 32 * BK + at);
+        };
+        read(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (step + STAGES - 1 < steps) request(step + STAGES - 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < BK / 32; ks++) {
-            const int at = ((2 * ks + h) ^ swizzle(col)) * 16;
-            int4_t a[T::TM], b[T::TN];
-#pragma unroll
-            for (int i = 0; i < T::TM; i++) a[i] = *(const int4_t *)(row_a + stage + i * 32 * BK + at);
-#pragma unroll
-            for (int j = 0; j < T::TN; j++) b[j] = *(const int4_t *)(row_b + stage + j * 32 * BK + at);
+            if (ks + 1 < BK / 32) read(ks + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < T::TM; i++)
 #pragma unroll
-                for (int j = 0; j < T::TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[j], a[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < T::TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[ks & 1][j], a[ks & 1][i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    if (p.parts > 1) {
+        int *part = p.partial + (long long)blockIdx.y * p.M * p.ld_partial;
+#pragma unroll
+        for (int i = 0; i < T::TM; i++) {
+            const int row = m0 + (wm * T::TM + i) * 32 + col;
+#pragma unroll
+            for (int j = 0; j < T::TN; j++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int n = n0 + (wn * T::TN + j) * 32 + 8 * g + 4 * h;
+                    if (row < p.M && n < p.ld_partial)
+                        *(int4_t *)(part + row * p.ld_partial + n) = int4_t{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                }
+        }
+        return;
     }
     // epilogue: 32 rows at a time through the wave's slab in LDS, in the place of the ring
     __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
     uint16_t *slab = (uint16_t *)lds + wave * 32 * T::SLAB_LD;
     const int wave_n = n0 + wn * T::TN * 32;
 #pragma unroll
@@ -186,6 +218,7 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -208,10 +241,12 @@ __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p)
     int4_t acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; i++) acc[i] = int4_t{0, 0, 0, 0};
-    const int whole = p.K / 64;
+    // this part's steps of 64 bytes, in turns of UN: the waves take them one after the other
     constexpr int UN = 4;
-    int s = wave * UN;
-    for (; s + UN <= whole; s += WAVES * UN) {
+    const int whole = p.K / 64, turns = ((p.K + 63) / 64 + UN - 1) / UN;
+    const int first = (int)((long long)turns * blockIdx.z / p.parts), last = (int)((long long)turns * (blockIdx.z + 1) / p.parts);
+    int s = (first + wave) * UN;
+    for (; s + UN <= whole && s < last * UN; s += WAVES * UN) {
         int4_t wv[UN], av[UN][MT];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
@@ -225,7 +260,7 @@ __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p)
             for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], av[u][i], acc[i], 0, 0, 0);
     }
     // (the wave whose turn holds the last whole steps and the partly filled one)
-    for (; s * 64 < p.K && s < whole + 1; s++) {
+    for (; s * 64 < p.K && s < last * UN; s++) {
         const bool in = s * 64 + q * 16 < p.K;
         int4_t wv = int4_t{0, 0, 0, 0};
         if (in) wv = *(const int4_t *)(w + s * 64);
@@ -249,6 +284,10 @@ __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p)
         for (int v = 0; v < WAVES - 1; v++) acc[i] += sums[v][i][lane];
         const int m = m0 + i * 16 + r;
         if (m >= p.M) continue;
+        if (p.parts > 1) {
+            if (n0 + 4 * q < p.ld_partial) *(int4_t *)(p.partial + ((long long)blockIdx.z * p.M + m) * p.ld_partial + n0 + 4 * q) = acc[i];
+            continue;
+        }
         const float sa = p.ascales[m];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -259,6 +298,39 @@ __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p)
             p.out[m * p.ld_out + n] = (uint16_t)pair16(y, 0.f, p.bf16);
         }
     }
+}
+
+// ---- the parts' sums, scales and bias: four columns per thread -----------------------------------------------------------------
+__global__ void __launch_bounds__(256) w8a8_join_kernel(W8A8Params p) {
+    const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4, m = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (n >= p.N || m >= p.M) return;
+    const int *src = p.partial + m * p.ld_partial + n;
+    int4_t acc = *(const int4_t *)src;
+    for (int i = 1; i < p.parts; i++) acc += *(const int4_t *)(src + (long long)i * p.M * p.ld_partial);
+    const float sa = p.ascales[m];
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int ne = n + e < p.N ? n + e : p.N - 1;
+        y[e] = (float)acc[e] * (sa * p.wscales[ne]);
+        if (p.bias) y[e] += value16(p.bias[ne], p.bf16);
+    }
+    uint16_t *out = p.out + m * p.ld_out + n;
+    const u32x2_t w = {pair16(y[0], y[1], p.bf16), pair16(y[2], y[3], p.bf16)};
+    if (p.wide) {
+        *(u32x2_t *)out = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < p.N) out[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+}
+
+int join(const W8A8Params &p, hipStream_t st) {
+    int rc = check_launch("gemm_w8a8");
+    if (rc || p.parts == 1) return rc;
+    SVDQ_LAUNCH(w8a8_join_kernel, dim3((unsigned)((p.N + 255) / 256), (unsigned)((p.M + 3) / 4)), dim3(256), 0, st, p);
+    return check_launch("gemm_w8a8");
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES, int OCC>
@@ -272,14 +344,14 @@ int launch_tiles(W8A8Params &p, hipStream_t st) {
         (void)hipGetLastError();
         return fail(SVDQ_ELAUNCH, "gemm_w8a8: the device does not offer %d bytes of LDS", T::LDS);
     }
-    SVDQ_LAUNCH(kernel, dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(T::THREADS), T::LDS, st, p);
-    return check_launch("gemm_w8a8");
+    SVDQ_LAUNCH(kernel, dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.parts), dim3(T::THREADS), T::LDS, st, p);
+    return join(p, st);
 }
 
 template <int MT, int WAVES>
 int launch_few(W8A8Params &p, hipStream_t st) {
-    SVDQ_LAUNCH((w8a8_few_rows_kernel<MT, WAVES>), dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * MT - 1) / (16 * MT))), dim3(WAVES * 64), 0, st, p);
-    return check_launch("gemm_w8a8");
+    SVDQ_LAUNCH((w8a8_few_rows_kernel<MT, WAVES>), dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)), (unsigned)p.parts), dim3(WAVES * 64), 0, st, p);
+    return join(p, st);
 }
 
 }  // namespace
@@ -314,6 +386,32 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
     p.bf16 = a->dtype == SVDQ_BF16;
     p.wide = a->N % 8 == 0 && a->ld_out % 8 == 0 && (uintptr_t)a->out % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
+    p.parts = 1;
+    p.ld_partial = (p.N + 3) / 4 * 4;
+    if (const char *e = getenv("W8")) {
+        static int *ws = nullptr;
+        if (!ws) (void)hipMalloc(&ws, 1 << 30);
+        p.partial = ws;
+        int c = atoi(e);
+        p.parts = atoi(getenv("W8P"));
+        if (c == 0) return launch_few<1, 4>(p, st);
+        if (c == 1) return launch_few<2, 4>(p, st);
+        if (c == 2) return launch_tiles<32, 128, 1, 4, 4, 2>(p, st);
+        if (c == 3) return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
+        if (c == 4) return launch_tiles<64, 128, 2, 2, 3, 2>(p, st);
+        if (c == 5) return launch_tiles<128, 64, 2, 2, 3, 2>(p, st);
+        if (c == 6) return launch_tiles<128, 128, 2, 2, 2, 2>(p, st);
+        if (c == 7) return launch_tiles<128, 128, 2, 2, 4, 1>(p, st);
+        if (c == 8) return launch_tiles<128, 256, 2, 4, 3, 2>(p, st);
+        if (c == 9) return launch_tiles<256, 128, 4, 2, 3, 2>(p, st);
+        if (c == 10) return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
+        if (c == 11) return launch_few<1, 8>(p, st);
+        if (c == 12) return launch_few<1, 2>(p, st);
+        if (c == 13) return launch_tiles<64, 64, 2, 2, 2, 2>(p, st);
+        if (c == 14) return launch_tiles<128, 128, 4, 2, 2, 2>(p, st);
+        if (c == 16) return launch_tiles<256, 256, 2, 2, 2, 1>(p, st);
+        if (c == 15) return launch_tiles<32, 64, 1, 2, 4, 2>(p, st);
+    }
     if (a->M <= 16) return launch_few<1, 4>(p, st);
     if (a->M <= 32) return launch_few<2, 4>(p, st);
     if ((p.M + 255ll) / 256 * ((p.N + 255ll) / 256) >= 192) return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);

@@ -377,4 +377,5 @@ def test_attention_on_the_outputs_of_the_fused_projection(dev):
     assert torch.isnan(k[:, T:]).all()
     got = cross_attention(q[:, :T], k, v, key_lengths=torch.tensor([T], dtype=torch.int32, device=dev))
     check(got, q[:, :T].cpu(), k[:, :T].cpu(), v[:, :T].cpu())
-    assert torch.equal(got, cross_attention(q[:, :T], k[:, :T], v[:, :T]))
+    # (not the same bits: into how many parts the keys are divided goes by the tensors' length)
+    check(cross_attention(q[:, :T], k[:, :T], v[:, :T]), q[:, :T].cpu(), k[:, :T].cpu(), v[:, :T].cpu())
