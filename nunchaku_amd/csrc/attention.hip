@@ -164,7 +164,10 @@ struct State {
         for (int kb = 0; kb < NB; kb++) {
             const uint32_t w = (uint32_t)(bits >> (32 * kb)) >> (4 * (lane >> 5));
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[kb][e] = w >> (8 * (e >> 2) + (e & 3)) & 1 ? s[kb][e] : -__builtin_huge_valf();
+            for (int e = 0; e < 16; e++) {  // (the bit over the whole word picks the score or minus infinity: two instructions)
+                const uint32_t in = (uint32_t)__builtin_amdgcn_sbfe((int)w, 8 * (e >> 2) + (e & 3), 1);
+                s[kb][e] = bits_f32((f32_bits(s[kb][e]) & in) | (0xFF800000u & ~in));
+            }
         }
     }
     template <int NB>
@@ -266,8 +269,12 @@ __device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec
         if (row < p.rows && c < p.D) w = *(const u32x4_t *)(q + c * 2);
         qf[ks] = __builtin_bit_cast(typename Elem<BF16>::vec, w);
     }
-    // The compiler waits for these loads where they are first used.  In the loop over the keys that wait would be for the copies
-    // that a step has just asked for, too, and at every step: they are waited for here.
+}
+
+// The compiler waits for these loads where they are first used.  In the loop over the keys that wait would be for the copies that a step
+// has just asked for, too, and at every step: this, in front of the loop and behind the first copies, is where they are waited for.
+template <bool BF16, int DP>
+__device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[Head<DP>::KS]) {
 #pragma unroll
     for (int ks = 0; ks < Head<DP>::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
@@ -416,6 +423,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
         copies.k(step, 0);
         copies.v(step, 0, bits);
     }
+    wait_for_q<BF16, DP>(qf);
     for (int slot = 0; step >= 0; slot ^= 1) {
         // K and V of this step have landed, of all waves, and nobody reads what the next requests overwrite
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -514,6 +522,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     int step = list.next();
     uint64_t bits = list.bits;
     if (step >= 0) request(step, 0, bits);
+    wait_for_q<BF16, DP>(qf);
     for (int slot = 0; step >= 0; slot ^= 1) {
         const int next = list.next();
         if (next >= 0) request(next, slot ^ 1, list.bits);
