@@ -314,9 +314,15 @@ typedef struct svdq_gemm_w8a8_args {
     void *out;              /* bf16 or fp16 [M, N], rows ld_out elements apart                       */
     int64_t M, N, K;        /* K: a multiple of 16 below 131072; M and N: any                        */
     int64_t ld_act, ld_wgt, ld_out; /* ld_act, ld_wgt: multiples of 16 below 2^23                    */
+    void *workspace;        /* svdq_gemm_w8a8_workspace bytes (16-byte aligned), not shared with a call that may run at the
+                               same time; NULL if that is 0                                          */
+    int64_t workspace_bytes;
     int32_t dtype;          /* of out and bias: SVDQ_BF16 or SVDQ_FP16                               */
 } svdq_gemm_w8a8_args;
 
+/* What a call with these arguments on the current device needs as its workspace (depends on M, N and K alone): calls with few output
+ * tiles and long rows divide K among workgroups, whose integer sums meet there. */
+int svdq_gemm_w8a8_workspace(const svdq_gemm_w8a8_args *args, int64_t *bytes);
 int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *args, void *stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -31,7 +31,7 @@ EXPORTED_SYMBOLS = [
     "svdq_repack_smooth", "svdq_repack_lora_down", "svdq_repack_lora_up", "svdq_repack_rotemb",
     "svdq_quantize_w4a4_act_fuse_lora", "svdq_gemm_w4a4", "svdq_gemm_w4a4_noalloc", "svdq_awq_gemv_w4a16",
     "svdq_linearattn_vk_mul_q", "svdq_release_workspaces",
-    "svdq_quantize_w8a8_act", "svdq_rms_norm_quantize_w8a8", "svdq_gemm_w8a8", "svdq_cross_attention_workspace", "svdq_cross_attention",
+    "svdq_quantize_w8a8_act", "svdq_rms_norm_quantize_w8a8", "svdq_gemm_w8a8_workspace", "svdq_gemm_w8a8", "svdq_cross_attention_workspace", "svdq_cross_attention",
 ]
 
 
@@ -102,7 +102,8 @@ class GemmW8A8Args(ctypes.Structure):
     _fields_ = [
         ("act", ctypes.c_void_p), ("wgt", ctypes.c_void_p), ("ascales", ctypes.c_void_p), ("wscales", ctypes.c_void_p),
         ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64),
-        ("ld_act", ctypes.c_int64), ("ld_wgt", ctypes.c_int64), ("ld_out", ctypes.c_int64), ("dtype", ctypes.c_int32),
+        ("ld_act", ctypes.c_int64), ("ld_wgt", ctypes.c_int64), ("ld_out", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("dtype", ctypes.c_int32),
     ]
 
 
@@ -215,6 +216,7 @@ def lib() -> ctypes.CDLL:
         L.svdq_release_workspaces.argtypes = []
         L.svdq_quantize_w8a8_act.argtypes = [ctypes.POINTER(QuantizeW8A8Args), vp]
         L.svdq_rms_norm_quantize_w8a8.argtypes = [ctypes.POINTER(QuantizeW8A8Args), vp]
+        L.svdq_gemm_w8a8_workspace.argtypes = [ctypes.POINTER(GemmW8A8Args), ctypes.POINTER(i64)]
         L.svdq_gemm_w8a8.argtypes = [ctypes.POINTER(GemmW8A8Args), vp]
         L.svdq_cross_attention_workspace.argtypes = [ctypes.POINTER(CrossAttentionArgs), ctypes.POINTER(i64)]
         L.svdq_cross_attention.argtypes = [ctypes.POINTER(CrossAttentionArgs), vp]
@@ -272,6 +274,21 @@ def launch(entry, args_ref, device: torch.device) -> None:
             rc = entry(args_ref, torch.cuda.current_stream(device).cuda_stream)
     if rc:
         check(rc)
+
+
+def launch_with_workspace(size_of, entry, args, device: torch.device) -> None:
+    """``entry(args, stream)`` with the workspace that ``size_of(args, &bytes)`` asks for: from torch's allocator on the caller's
+    stream, so that calls on other streams and captured graphs have their own."""
+    need = ctypes.c_int64()
+    if device.index == torch.cuda.current_device():
+        check(size_of(ctypes.byref(args), ctypes.byref(need)))
+    else:
+        with torch.cuda.device(device):
+            check(size_of(ctypes.byref(args), ctypes.byref(need)))
+    if need.value:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
+    launch(entry, ctypes.byref(args), device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

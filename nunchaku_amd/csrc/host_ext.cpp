@@ -755,7 +755,10 @@ PyObject *w8a8_gemm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     a.out = out.data_ptr();
     a.ld_out = a.N;
     hipStream_t st = c10::hip::getCurrentHIPStream(x->device().index()).stream();
-    int rc;
+    int rc = svdq_gemm_w8a8_workspace(&a, &a.workspace_bytes);
+    if (rc != SVDQ_OK) return raise(rc);
+    std::optional<Scratch> workspace;
+    if (a.workspace_bytes) a.workspace = workspace.emplace((size_t)a.workspace_bytes, st).ptr;
     Py_BEGIN_ALLOW_THREADS
     rc = svdq_gemm_w8a8(&a, st);
     Py_END_ALLOW_THREADS

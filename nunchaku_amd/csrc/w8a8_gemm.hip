@@ -120,6 +120,9 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
             }
         }
     };
+    // Eight waves are two on every SIMD: the second four ask for their copies behind their first matrix instructions, while the first four,
+    // which do it in front, are still at it (8192 x 8192 x 8192: 481 -> 475 us; with one wave each it costs up to 10 %)
+    const bool late = BM == 256 && BN == 256 && wave >= T::WAVES / 2;
     int16_t_ acc[T::TM][T::TN];
 #pragma unroll
     for (int i = 0; i < T::TM; i++)
@@ -148,7 +151,8 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
         };
         read(0);
         __builtin_amdgcn_sched_barrier(0);
-        if (step + STAGES - 1 < steps) request(step + STAGES - 1);
+        const bool more = step + STAGES - 1 < steps;
+        if (more && !late) request(step + STAGES - 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < BK / 32; ks++) {
@@ -158,6 +162,8 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
             for (int i = 0; i < T::TM; i++)
 #pragma unroll
                 for (int j = 0; j < T::TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[ks & 1][j], a[ks & 1][i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (BM == 256 && BN == 256 && ks == 0 && more && late) request(step + STAGES - 1);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -223,80 +229,60 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
-// 16 columns x 16 * MT rows per workgroup, whose WAVES waves split K in steps of 64 bytes and meet in LDS.  Operands go from
-// memory to the registers of the wave that multiplies them.
-template <int MT, int WAVES>
+// 16 columns x 16 rows per workgroup, whose WAVES waves split K in steps of 64 bytes and meet in LDS.  Operands go from memory to the
+// registers of the wave that multiplies them.
+template <int WAVES>
 __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p) {
-    __shared__ int4_t sums[WAVES - 1][MT][64];
+    __shared__ int4_t sums[WAVES - 1][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
     const char *w = p.wgt + (long long)(n0 + r < p.N ? n0 + r : p.N - 1) * p.ld_wgt + q * 16;
-    const char *a[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int m = m0 + i * 16 + r;
-        a[i] = p.act + (long long)(m < p.M ? m : p.M - 1) * p.ld_act + q * 16;
-    }
-    int4_t acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) acc[i] = int4_t{0, 0, 0, 0};
+    const char *a = p.act + (long long)(r < p.M ? r : p.M - 1) * p.ld_act + q * 16;
+    int4_t acc = int4_t{0, 0, 0, 0};
     // this part's steps of 64 bytes, in turns of UN: the waves take them one after the other
     constexpr int UN = 4;
     const int whole = p.K / 64, turns = ((p.K + 63) / 64 + UN - 1) / UN;
-    const int first = (int)((long long)turns * blockIdx.z / p.parts), last = (int)((long long)turns * (blockIdx.z + 1) / p.parts);
+    const int first = (int)((long long)turns * blockIdx.y / p.parts), last = (int)((long long)turns * (blockIdx.y + 1) / p.parts);
     int s = (first + wave) * UN;
     for (; s + UN <= whole && s < last * UN; s += WAVES * UN) {
-        int4_t wv[UN], av[UN][MT];
+        int4_t wv[UN], av[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             wv[u] = *(const int4_t *)(w + (s + u) * 64);
-#pragma unroll
-            for (int i = 0; i < MT; i++) av[u][i] = *(const int4_t *)(a[i] + (s + u) * 64);
+            av[u] = *(const int4_t *)(a + (s + u) * 64);
         }
 #pragma unroll
-        for (int u = 0; u < UN; u++)
-#pragma unroll
-            for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], av[u][i], acc[i], 0, 0, 0);
+        for (int u = 0; u < UN; u++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], av[u], acc, 0, 0, 0);
     }
     // (the wave whose turn holds the last whole steps and the partly filled one)
     for (; s * 64 < p.K && s < last * UN; s++) {
         const bool in = s * 64 + q * 16 < p.K;
-        int4_t wv = int4_t{0, 0, 0, 0};
-        if (in) wv = *(const int4_t *)(w + s * 64);
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            int4_t av = int4_t{0, 0, 0, 0};
-            if (in) av = *(const int4_t *)(a[i] + s * 64);
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, av, acc[i], 0, 0, 0);
+        int4_t wv = int4_t{0, 0, 0, 0}, av = int4_t{0, 0, 0, 0};
+        if (in) {
+            wv = *(const int4_t *)(w + s * 64);
+            av = *(const int4_t *)(a + s * 64);
         }
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, av, acc, 0, 0, 0);
         if ((s + 1) % UN == 0) break;
     }
-    if (wave > 0) {
-#pragma unroll
-        for (int i = 0; i < MT; i++) sums[wave - 1][i][lane] = acc[i];
-    }
+    if (wave > 0) sums[wave - 1][lane] = acc;
     __syncthreads();
-    if (wave > 0) return;
+    if (wave > 0 || r >= p.M) return;
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
+    for (int v = 0; v < WAVES - 1; v++) acc += sums[v][lane];
+    // four consecutive columns of row r
+    const int n = n0 + 4 * q;
+    if (p.parts > 1) {
+        if (n < p.ld_partial) *(int4_t *)(p.partial + ((long long)blockIdx.y * p.M + r) * p.ld_partial + n) = acc;
+        return;
+    }
+    const float sa = p.ascales[r];
 #pragma unroll
-        for (int v = 0; v < WAVES - 1; v++) acc[i] += sums[v][i][lane];
-        const int m = m0 + i * 16 + r;
-        if (m >= p.M) continue;
-        if (p.parts > 1) {
-            if (n0 + 4 * q < p.ld_partial) *(int4_t *)(p.partial + ((long long)blockIdx.z * p.M + m) * p.ld_partial + n0 + 4 * q) = acc[i];
-            continue;
-        }
-        const float sa = p.ascales[m];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int n = n0 + 4 * q + e;
-            if (n >= p.N) continue;
-            float y = (float)acc[i][e] * (sa * p.wscales[n]);
-            if (p.bias) y += value16(p.bias[n], p.bf16);
-            p.out[m * p.ld_out + n] = (uint16_t)pair16(y, 0.f, p.bf16);
-        }
+    for (int e = 0; e < 4; e++) {
+        if (n + e >= p.N) break;
+        float y = (float)acc[e] * (sa * p.wscales[n + e]);
+        if (p.bias) y += value16(p.bias[n + e], p.bf16);
+        p.out[r * p.ld_out + n + e] = (uint16_t)pair16(y, 0.f, p.bf16);
     }
 }
 
@@ -348,15 +334,72 @@ int launch_tiles(W8A8Params &p, hipStream_t st) {
     return join(p, st);
 }
 
-template <int MT, int WAVES>
+template <int WAVES>
 int launch_few(W8A8Params &p, hipStream_t st) {
-    SVDQ_LAUNCH((w8a8_few_rows_kernel<MT, WAVES>), dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)), (unsigned)p.parts), dim3(WAVES * 64), 0, st, p);
+    SVDQ_LAUNCH((w8a8_few_rows_kernel<WAVES>), dim3((unsigned)((p.N + 15) / 16), (unsigned)p.parts), dim3(WAVES * 64), 0, st, p);
     return join(p, st);
 }
 
-}  // namespace
+// ---- which kernel ----------------------------------------------------------------------------------------------------------------
+enum Form { FEW_4, FEW_8, T32x64, T64x64_DEEP, T64x64, T64x128, T128x128, T128x256, T256x256 };
+struct Plan {
+    Form form;
+    int parts;
+    long long workspace;
+};
 
-extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
+// A model of the busiest compute unit's time, in us, fitted to 20 shapes of 1 .. 8192 rows (each form and number of parts timed): a step of
+// 128 bytes of K takes a workgroup `alone` while it has its compute unit to itself and every one of several `share`; `slots` fit a compute
+// unit.  A tile ends with its output's way to memory (20 bytes a ns for a compute unit when all write) and 1.5 us of latencies; launch and
+// first loads take 4 us, the kernel that joins parts 3 us and its traffic.  Few rows are the weights' way from memory.
+// Chosen / next best, us: 505 x 2304 x 4608 14.9 (64 x 64) / 16.3, 256 x 4096 x 4096 13.7 (64 x 64, four stages) / 14.1, 1024 x 4096 x 4096 27.8
+// (64 x 128) / 29.4, 2048 x 4096 x 4096 39.6 (128 x 128) / 43.3, 7747 x 13984 x 156 44.7 (128 x 256 in four parts; whole 61), 17 x 13728 x 3213 14.8
+// (32 x 64 in four parts; whole 17), 4608 x 4096 x 16384 316 (256 x 256) / 340.
+struct Cost {
+    Form form;
+    int bm, bn, slots;
+    float alone, share;
+};
+constexpr Cost costs[] = {
+    {T32x64, 32, 64, 3, 0.30f, 0.17f},    {T64x64_DEEP, 64, 64, 2, 0.31f, 0.20f},  {T64x64, 64, 64, 5, 0.45f, 0.20f},      {T64x128, 64, 128, 2, 0.45f, 0.36f},
+    {T128x128, 128, 128, 2, 0.72f, 0.55f}, {T128x256, 128, 256, 1, 1.15f, 1.15f}, {T256x256, 256, 256, 1, 1.90f, 1.90f},
+};
+constexpr int MAX_PARTS = 16;
+
+Plan plan_of(long long M, long long N, long long K, int cus) {
+    const long long steps = (K + BK - 1) / BK;
+    Plan plan = {T256x256, 1, 0};
+    if (M <= 16) {
+        // 16 columns a workgroup: with few of them eight waves instead of four, and parts of at least a turn for each wave
+        // (1 x 4096 x 4096 8.3 -> 7.8 us with eight waves, 8 x 16384 x 512 14.2 -> 9.4 with eight parts; 1 x 4096 x 12288 13.3 with four, 13.6 with eight)
+        const long long tiles = (N + 15) / 16, most = K / 2048, want = cus / tiles;
+        plan.form = tiles >= 2 * cus ? FEW_4 : FEW_8;
+        if (want > 1 && most > 1) plan.parts = (int)(want < most ? want : most);
+        if (plan.parts > MAX_PARTS) plan.parts = MAX_PARTS;
+    } else {
+        float best = 0.f;
+        for (const Cost &c : costs) {
+            const long long tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+            const float last = c.bm * c.bn * 2 / 20000.f;  // a tile's output
+            for (int parts = 1; parts <= MAX_PARTS && (parts == 1 || (steps >= 4 * parts && tiles * (parts - 1) < c.slots * cus)); parts++) {
+                const long long most = (tiles * parts + cus - 1) / cus, rounds = most / c.slots, rest = most % c.slots;
+                const float n = (float)((steps + parts - 1) / parts);
+                auto round = [&](long long w) { return n * (c.alone > w * c.share ? c.alone : w * c.share) + 1.5f + w * last * (parts > 1 ? 2.f : 1.f); };
+                float t = rounds * round(c.slots) + (rest ? round(rest) : 0.f);
+                if (parts > 1) t += 3.f + M * N * 4.f * parts / 4.0e6f;
+                if (best == 0.f || t < best) {
+                    best = t;
+                    plan.form = c.form;
+                    plan.parts = parts;
+                }
+            }
+        }
+    }
+    plan.workspace = plan.parts > 1 ? plan.parts * M * ((N + 3) / 4 * 4) * 4 : 0;
+    return plan;
+}
+
+int plan_call(const svdq_gemm_w8a8_args *a, Plan &plan) {
     SVDQ_REQUIRE(a && a->act && a->wgt && a->ascales && a->wscales && a->out, "gemm_w8a8: act, wgt, ascales, wscales and out must not be null");
     SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "gemm_w8a8: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
     SVDQ_REQUIRE(a->M > 0 && a->N > 0 && a->M < (1ll << 31) - 256 && a->N < (1ll << 31) - 256, "gemm_w8a8: M (%lld) and N (%lld) must be positive and below 2^31 - 256",
@@ -368,8 +411,32 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
     SVDQ_REQUIRE(a->ld_wgt >= a->K && a->ld_wgt % 16 == 0 && a->ld_wgt < (1ll << 23), "gemm_w8a8: rows of wgt must be at least K bytes, a multiple of 16 and less than 2^23 apart, got %lld",
                  (long long)a->ld_wgt);
     SVDQ_REQUIRE(a->ld_out >= a->N, "gemm_w8a8: rows of out must be at least N (%lld) elements apart, got %lld", (long long)a->N, (long long)a->ld_out);
-    SVDQ_REQUIRE(((uintptr_t)a->act | (uintptr_t)a->wgt) % 16 == 0, "gemm_w8a8: act and wgt must be 16-byte aligned");
+    SVDQ_REQUIRE(((uintptr_t)a->act | (uintptr_t)a->wgt | (uintptr_t)a->workspace) % 16 == 0, "gemm_w8a8: act, wgt and workspace must be 16-byte aligned");
     SVDQ_REQUIRE(((uintptr_t)a->ascales | (uintptr_t)a->wscales) % 4 == 0 && ((uintptr_t)a->bias | (uintptr_t)a->out) % 2 == 0, "gemm_w8a8: scales, bias and out must be aligned to their elements");
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || (cus = compute_units(dev)) == 0) {
+        (void)hipGetLastError();
+        return fail(SVDQ_ELAUNCH, "gemm_w8a8: no current device");
+    }
+    plan = plan_of(a->M, a->N, a->K, cus);
+    return SVDQ_OK;
+}
+
+}  // namespace
+
+extern "C" int svdq_gemm_w8a8_workspace(const svdq_gemm_w8a8_args *a, int64_t *bytes) {
+    Plan plan;
+    if (int rc = plan_call(a, plan)) return rc;
+    SVDQ_REQUIRE(bytes, "gemm_w8a8: bytes must not be null");
+    *bytes = plan.workspace;
+    return SVDQ_OK;
+}
+
+extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
+    Plan plan;
+    if (int rc = plan_call(a, plan)) return rc;
+    SVDQ_REQUIRE(plan.workspace == 0 || (a->workspace && a->workspace_bytes >= plan.workspace), "gemm_w8a8: needs a workspace of %lld bytes, got %lld", plan.workspace,
+                 (long long)(a->workspace ? a->workspace_bytes : 0));
     W8A8Params p;
     p.act = (const char *)a->act;
     p.wgt = (const char *)a->wgt;
@@ -385,36 +452,19 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
     p.K = (int)a->K;
     p.bf16 = a->dtype == SVDQ_BF16;
     p.wide = a->N % 8 == 0 && a->ld_out % 8 == 0 && (uintptr_t)a->out % 16 == 0;
+    p.parts = plan.parts;
+    p.ld_partial = (a->N + 3) / 4 * 4;
+    p.partial = (int *)a->workspace;
     hipStream_t st = (hipStream_t)stream;
-    p.parts = 1;
-    p.ld_partial = (p.N + 3) / 4 * 4;
-    if (const char *e = getenv("W8")) {
-        static int *ws = nullptr;
-        if (!ws) (void)hipMalloc(&ws, 1 << 30);
-        p.partial = ws;
-        int c = atoi(e);
-        p.parts = atoi(getenv("W8P"));
-        if (c == 0) return launch_few<1, 4>(p, st);
-        if (c == 1) return launch_few<2, 4>(p, st);
-        if (c == 2) return launch_tiles<32, 128, 1, 4, 4, 2>(p, st);
-        if (c == 3) return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
-        if (c == 4) return launch_tiles<64, 128, 2, 2, 3, 2>(p, st);
-        if (c == 5) return launch_tiles<128, 64, 2, 2, 3, 2>(p, st);
-        if (c == 6) return launch_tiles<128, 128, 2, 2, 2, 2>(p, st);
-        if (c == 7) return launch_tiles<128, 128, 2, 2, 4, 1>(p, st);
-        if (c == 8) return launch_tiles<128, 256, 2, 4, 3, 2>(p, st);
-        if (c == 9) return launch_tiles<256, 128, 4, 2, 3, 2>(p, st);
-        if (c == 10) return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
-        if (c == 11) return launch_few<1, 8>(p, st);
-        if (c == 12) return launch_few<1, 2>(p, st);
-        if (c == 13) return launch_tiles<64, 64, 2, 2, 2, 2>(p, st);
-        if (c == 14) return launch_tiles<128, 128, 4, 2, 2, 2>(p, st);
-        if (c == 16) return launch_tiles<256, 256, 2, 2, 2, 1>(p, st);
-        if (c == 15) return launch_tiles<32, 64, 1, 2, 4, 2>(p, st);
+    switch (plan.form) {
+    case FEW_4: return launch_few<4>(p, st);
+    case FEW_8: return launch_few<8>(p, st);
+    case T32x64: return launch_tiles<32, 64, 1, 2, 4, 2>(p, st);
+    case T64x64_DEEP: return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
+    case T64x64: return launch_tiles<64, 64, 2, 2, 2, 2>(p, st);
+    case T64x128: return launch_tiles<64, 128, 2, 2, 3, 2>(p, st);
+    case T128x128: return launch_tiles<128, 128, 4, 2, 2, 2>(p, st);
+    case T128x256: return launch_tiles<128, 256, 2, 4, 3, 2>(p, st);
+    default: return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
     }
-    if (a->M <= 16) return launch_few<1, 4>(p, st);
-    if (a->M <= 32) return launch_few<2, 4>(p, st);
-    if ((p.M + 255ll) / 256 * ((p.N + 255ll) / 256) >= 192) return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
-    if ((p.M + 127ll) / 128 * ((p.N + 127ll) / 128) >= 192) return launch_tiles<128, 128, 2, 2, 2, 2>(p, st);
-    return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
 }

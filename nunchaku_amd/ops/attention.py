@@ -97,16 +97,5 @@ def cross_attention(
         B, H, Hkv, D, Tq, Tk, i64x3(*_strides(q, "q")), i64x3(*_strides(k, "k")), i64x3(*_strides(v, "v")), i64x3(*_strides(out, "out")),
         mask_stride, scale, DTYPES[q.dtype],
     )
-    L = nv.lib()
-    need = ctypes.c_int64()
-    if q.device.index == torch.cuda.current_device():
-        rc = L.svdq_cross_attention_workspace(ctypes.byref(args), ctypes.byref(need))
-    else:
-        with torch.cuda.device(q.device):
-            rc = L.svdq_cross_attention_workspace(ctypes.byref(args), ctypes.byref(need))
-    nv.check(rc)
-    if need.value:  # (from torch's allocator, on the caller's stream: calls on other streams and captured graphs have their own)
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-    nv.launch(L.svdq_cross_attention, ctypes.byref(args), q.device)
+    nv.launch_with_workspace(nv.lib().svdq_cross_attention_workspace, nv.lib().svdq_cross_attention, args, q.device)
     return out

@@ -182,7 +182,7 @@ def gemm_w8a8(
         return out
     args = nv.GemmW8A8Args(
         a.data_ptr(), w.data_ptr(), ascales.data_ptr(), wscales.data_ptr(), nv.ptr(bias), out.data_ptr(), M, N, K,
-        _row_stride(a), _row_stride(w), ld, DTYPES[out_dtype],
+        _row_stride(a), _row_stride(w), ld, None, 0, DTYPES[out_dtype],
     )
-    nv.launch(nv.lib().svdq_gemm_w8a8, ctypes.byref(args), a.device)
+    nv.launch_with_workspace(nv.lib().svdq_gemm_w8a8_workspace, nv.lib().svdq_gemm_w8a8, args, a.device)
     return out

@@ -82,7 +82,12 @@ def test_quantize_refusals(lib):
 
 def test_gemm_refusals(lib):
     good = nv.GemmW8A8Args(act=16, wgt=16, ascales=16, wscales=16, out=16, M=3, N=5, K=64, ld_act=64, ld_wgt=64, ld_out=5)
-    entry = lib.svdq_gemm_w8a8
+    need = ctypes.c_int64()
+    for entry in (lib.svdq_gemm_w8a8, lambda a, _: lib.svdq_gemm_w8a8_workspace(a, ctypes.byref(need))):
+        _gemm_refusals(entry, good, lib)
+
+
+def _gemm_refusals(entry, good, lib):
     assert entry(None, None) == -1
     for name in ("act", "wgt", "ascales", "wscales", "out"):
         assert b"null" in _refused(entry, good, lib, **{name: None})
