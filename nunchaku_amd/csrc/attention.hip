@@ -50,10 +50,12 @@ struct Elem<false> {
 };
 
 // A head of DP elements (rounded up): KS steps of 16 in the first product, DB blocks of 32 in the second; rows PITCH bytes apart in LDS.
-template <int DP>
+// Heads of 72 .. 96 take three quarters of the widest rows' LDS (WHOLE: the pitch is a power of two for them, too), which is a third
+// workgroup on a compute unit (4096 queries, 256 keys, 4 x 16 heads of 80: 35.9 -> 32.5 us).
+template <int DP_, bool WHOLE = false>
 struct Head {
-    static constexpr int KS = DP / 16, DB = (DP + 31) / 32, PITCH = DP <= 32 ? 64 : DP <= 64 ? 128 : 256, PIECES = PITCH / 16;
-    static constexpr int TILE = KEYS * PITCH, REQ = TILE / 1024, RPR = 1024 / PITCH;  // a tile of K or V: bytes, requests of a KB, rows per request
+    static constexpr int DP = DP_, KS = DP / 16, DB = (DP + 31) / 32, PITCH = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 96 && !WHOLE ? 192 : 256, PIECES = PITCH / 16;
+    static constexpr int TILE = KEYS * PITCH, REQ = TILE / 1024, RPR = 1024 / PITCH;  // a tile of K or V: bytes, requests of a KB, whole rows per request
     static __host__ __device__ constexpr int fk(int row) { return PITCH == 256 ? row & 15 : PITCH == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
     static __host__ __device__ constexpr int fv(int row) { return PITCH == 256 ? 4 * (row & 3) : PITCH == 128 ? 4 * ((row >> 1) & 1) : 0; }
 };
@@ -141,9 +143,8 @@ struct Steps {
 
 // Running softmax and output of 32 rows: lane l holds row l % 32; of the output's block db element e is column 32 db + 8 (e / 4) + 4 (l / 32) + e % 4.
 // Scores s of a step: block kb, element e is key 32 kb + 8 (e / 4) + 4 (l / 32) + e % 4.
-template <bool BF16, int DP>
+template <bool BF16, typename H>
 struct State {
-    using H = Head<DP>;
     using E = Elem<BF16>;
     using vec = typename E::vec;
     float16_t o[H::DB];
@@ -258,12 +259,12 @@ struct State {
 };
 
 // This lane's row of queries as the right operand: elements 16 ks + 8 (lane / 32) ... + 7
-template <bool BF16, int DP>
-__device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec (&qf)[Head<DP>::KS], int b, int hk, int row, int lane) {
+template <bool BF16, typename H>
+__device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec (&qf)[H::KS], int b, int hk, int row, int lane) {
     const int t = row / p.G, gq = row - t * p.G;
     const char *q = p.q + b * p.qs[0] + t * p.qs[1] + (long long)(hk * p.G + gq) * p.qs[2];
 #pragma unroll
-    for (int ks = 0; ks < Head<DP>::KS; ks++) {
+    for (int ks = 0; ks < H::KS; ks++) {
         const int c = 16 * ks + 8 * (lane >> 5);
         u32x4_t w = u32x4_t{0, 0, 0, 0};
         if (row < p.rows && c < p.D) w = *(const u32x4_t *)(q + c * 2);
@@ -273,20 +274,20 @@ __device__ inline void load_q(const AttentionParams &p, typename Elem<BF16>::vec
 
 // The compiler waits for these loads where they are first used.  In the loop over the keys that wait would be for the copies that a step
 // has just asked for, too, and at every step: this, in front of the loop and behind the first copies, is where they are waited for.
-template <bool BF16, int DP>
-__device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[Head<DP>::KS]) {
+template <bool BF16, typename H>
+__device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[H::KS]) {
 #pragma unroll
-    for (int ks = 0; ks < Head<DP>::KS; ks++) asm volatile("" : "+v"(qf[ks]));
+    for (int ks = 0; ks < H::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
 
 // This lane's row of the output, normalised: 8 consecutive columns per lane and 16-byte store
-template <bool BF16, int DP>
-__device__ inline void store_row(const AttentionParams &p, State<BF16, DP> &s, float sum, int b, int hk, int row, int lane) {
+template <bool BF16, typename H>
+__device__ inline void store_row(const AttentionParams &p, State<BF16, H> &s, float sum, int b, int hk, int row, int lane) {
     const int t = row / p.G, gq = row - t * p.G, h = lane >> 5;
     char *out = p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
     const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;  // (a NaN stays one)
 #pragma unroll
-    for (int d = 0; d < Head<DP>::DB; d++)
+    for (int d = 0; d < H::DB; d++)
 #pragma unroll
         for (int gp = 0; gp < 2; gp++) {
             // columns 32 d + 16 gp + [0, 4) + 4 h and 8 more: the half-waves exchange, so that each has 8 in a row
@@ -327,18 +328,21 @@ __device__ inline bool block_of(const AttentionParams &p, int groups, int &rb, i
 }
 
 // The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
-template <int DP, int WAVES>
+template <typename H, int WAVES>
 struct Copies {
-    using H = Head<DP>;
     // Request i of a wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
-    // two steps: the wave's rows start on a multiple of 16 where there are four requests, of 8 where there are two).
+    // two steps: the wave's rows start on a multiple of 16 where there are four requests, of 8 where there are two).  With 12 pieces in a
+    // row a request is five rows and a third: each has its own rows, pieces and offsets.
+    static constexpr bool EVEN = H::PITCH != 192;
     static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
-    static_assert(REQ == 1 || (REQ * H::RPR <= 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
+    static_assert(!EVEN || REQ == 1 || (REQ * H::RPR <= 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
+    static_assert(EVEN || (H::REQ % WAVES == 0 && H::fv(1) == 0 && H::fk(15) < 4), "");
+    static constexpr int OWN = EVEN ? 1 : REQ;
     const char *kp, *vp;
     long long k_token, v_token;
-    uint32_t dst, ok, ov, ck;
-    int row0, count, bytes;
-    bool v_lane, any;
+    uint32_t dst, ok[OWN], ov[OWN], ck[OWN];
+    int row[OWN], count, bytes;
+    bool any, in_row[OWN];  // (whether V's piece lies in the head)
     __device__ inline Copies(const AttentionParams &p, char *lds, int b, int hk, long long first, int count_, int wave, int lane) {
         kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
         vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
@@ -348,12 +352,16 @@ struct Copies {
         bytes = p.D * 2;
         any = wave < ACTIVE;
         dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
-        row0 = wave * REQ * H::RPR + lane / H::PIECES;
-        ck = ((lane % H::PIECES) ^ H::fk(row0)) * 16;
-        const uint32_t cv = ((lane % H::PIECES) ^ H::fv(row0)) * 16;
-        ok = (uint32_t)(row0 * k_token);
-        ov = (uint32_t)(row0 * v_token) + cv;
-        v_lane = (int)cv < bytes;
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const int piece = (wave * REQ + i) * 64 + lane, place = piece % H::PIECES;
+            row[i] = piece / H::PIECES;
+            ck[i] = (place ^ H::fk(row[i])) * 16;
+            ok[i] = (uint32_t)(row[i] * k_token);
+            ov[i] = (uint32_t)(row[i] * v_token) + (place ^ H::fv(row[i])) * 16;
+            in_row[i] = (place ^ H::fv(row[i])) * 16 < bytes;
+            if (!EVEN) ok[i] += ck[i];
+        }
         // columns behind the head's end are zero in K for good: no copy writes there
         if (bytes < H::PITCH) {
             for (int i = threadIdx.x; i < 2 * H::TILE / 16; i += WAVES * 64) *(u32x4_t *)(lds + i * 16) = u32x4_t{0, 0, 0, 0};
@@ -365,31 +373,48 @@ struct Copies {
         if (!any) return;
         const char *k = kp + (long long)step * KEYS * k_token;
         const int left = count - step * KEYS;
-        uint32_t c0 = ck;
-        asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
-        if (left >= KEYS && bytes == H::PITCH) {
+        if constexpr (EVEN) {
+            uint32_t c0 = ck[0];
+            asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
+            if (left >= KEYS && bytes == H::PITCH) {
 #pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok + (c0 ^ (64 * i)));
+                for (int i = 0; i < REQ; i++) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + (c0 ^ (64 * i)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) {
+                    const uint32_t c = c0 ^ (64 * i);
+                    if ((int)c < bytes && row[0] < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + c);
+                }
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < REQ; i++) {
-                const uint32_t c = c0 ^ (64 * i);
-                if ((int)c < bytes && row0 < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok + c);
-            }
+            for (int i = 0; i < REQ; i++)
+                if ((int)ck[i] < bytes && row[i] < left) copy16(dst + slot * H::TILE + i * 1024, k, ok[i]);
         }
     }
     // V: zeros for keys that do not count, since nothing times a NaN is one
     __device__ __forceinline__ void v(int step, int slot, uint64_t bits) {
-        if (!any || !v_lane) return;
+        if (!any) return;
         const char *v = vp + (long long)step * KEYS * v_token;
-        if (bits == ~0ull) {
+        const uint32_t to = dst + (2 + slot) * H::TILE;
+        if constexpr (EVEN) {
+            if (!in_row[0]) return;
+            if (bits == ~0ull) {
 #pragma unroll
-            for (int i = 0; i < REQ; i++) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * v_token, ov);
+                for (int i = 0; i < REQ; i++) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) {
+                    if ((bits >> (i * H::RPR)) >> row[0] & 1) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
+                    else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < REQ; i++) {
-                if ((bits >> (i * H::RPR)) >> row0 & 1) copy16(dst + (2 + slot) * H::TILE + i * 1024, v + i * H::RPR * v_token, ov);
-                else clear16(dst + (2 + slot) * H::TILE + i * 1024 + (threadIdx.x & 63) * 16);
+                if (!in_row[i]) continue;
+                if (bits == ~0ull || (bits >> row[i] & 1)) copy16(to + i * 1024, v, ov[i]);
+                else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
             }
         }
     }
@@ -411,10 +436,10 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     keys_of(p, b, first, count);
     const int row = (rb * 4 + wave) * 32 + col;
     vec qf[H::KS];
-    State<BF16, DP> st;
-    load_q<BF16, DP>(p, qf, b, hk, row, lane);
+    State<BF16, H> st;
+    load_q<BF16, H>(p, qf, b, hk, row, lane);
     st.clear();
-    Copies<DP, 4> copies(p, lds, b, hk, first, count, wave, lane);
+    Copies<H, 4> copies(p, lds, b, hk, first, count, wave, lane);
     Steps<MASK> list;
     list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, 0, (count + KEYS - 1) / KEYS, 1, lane);
     int step = list.next();
@@ -423,7 +448,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
         copies.k(step, 0);
         copies.v(step, 0, bits);
     }
-    wait_for_q<BF16, DP>(qf);
+    wait_for_q<BF16, H>(qf);
     for (int slot = 0; step >= 0; slot ^= 1) {
         // K and V of this step have landed, of all waves, and nobody reads what the next requests overwrite
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -464,14 +489,14 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
         step = next;
         bits = list.bits;
     }
-    store_row<BF16, DP>(p, st, across_sum(st.sum), b, hk, row, lane);
+    store_row<BF16, H>(p, st, across_sum(st.sum), b, hk, row, lane);
 }
 
 // ---- keys form: 32 rows per workgroup, whose waves take every fourth step (of 32 keys) of the part's keys, each through its own LDS, a
 // step ahead, and meet in LDS at the end; the parts of a row block meet in attention_join_kernel ------------------------------------
 template <bool BF16, int DP, bool MASK>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(AttentionParams p) {
-    using H = Head<DP>;
+    using H = Head<DP, true>;
     using E = Elem<BF16>;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
@@ -483,7 +508,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     keys_of(p, b, first, count);
     const int row = rb * 32 + col;
     typename E::vec qf[H::KS];
-    load_q<BF16, DP>(p, qf, b, hk, row, lane);
+    load_q<BF16, H>(p, qf, b, hk, row, lane);
     const char *kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
     const char *vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
     constexpr int SIZE = 32, REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
@@ -515,14 +540,14 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
             else clear16(dst + STAGE / 2 + i * 1024 + lane * 16);
         }
     };
-    State<BF16, DP> st;
+    State<BF16, H> st;
     st.clear();
     Steps<MASK, SIZE> list;
     list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, begin + wave, end, 4, lane);
     int step = list.next();
     uint64_t bits = list.bits;
     if (step >= 0) request(step, 0, bits);
-    wait_for_q<BF16, DP>(qf);
+    wait_for_q<BF16, H>(qf);
     for (int slot = 0; step >= 0; slot ^= 1) {
         const int next = list.next();
         if (next >= 0) request(next, slot ^ 1, list.bits);
@@ -579,7 +604,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     }
     if (wave > 0) return;
     if (p.parts == 1) {
-        store_row<BF16, DP>(p, st, sum, b, hk, row, lane);
+        store_row<BF16, H>(p, st, sum, b, hk, row, lane);
         return;
     }
     if (row >= p.rows) return;
@@ -653,8 +678,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) 
 
 template <bool BF16, int DP, bool MASK>
 int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
-    using H = Head<DP>;
-    const int lds = (keys ? 8 : 4) * H::TILE;
+    using H = Head<DP, true>;
+    const int lds = keys ? 8 * H::TILE : 4 * Head<DP>::TILE;
     static_assert(1024 + 3 * H::DB * 4096 <= 8 * H::TILE, "the waves' sums take the place of the stages");
     const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
     if (lds > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {

@@ -369,10 +369,13 @@ constexpr int MAX_PARTS = 16;
 Plan plan_of(long long M, long long N, long long K, int cus) {
     const long long steps = (K + BK - 1) / BK;
     Plan plan = {T256x256, 1, 0};
-    if (M <= 16) {
+    const long long few = (N + 15) / 16;
+    if (M <= 8 || (M <= 16 && few < 2 * cus)) {
         // 16 columns a workgroup: with few of them eight waves instead of four, and parts of at least a turn for each wave
-        // (1 x 4096 x 4096 8.3 -> 7.8 us with eight waves, 8 x 16384 x 512 14.2 -> 9.4 with eight parts; 1 x 4096 x 12288 13.3 with four, 13.6 with eight)
-        const long long tiles = (N + 15) / 16, most = K / 2048, want = cus / tiles;
+        // (1 x 4096 x 4096 8.3 -> 7.8 us with eight waves, 8 x 16384 x 512 14.2 -> 9.4 with eight parts; 1 x 4096 x 12288 13.3 with four, 13.6 with
+        // eight).  More than eight rows on many columns go to tiles, whose activations come once per 64 columns (16 x 4096 x 12288 15.1 -> 13.9;
+        // eight rows 12.5 here, 13.5 there)
+        const long long tiles = few, most = K / 2048, want = cus / tiles;
         plan.form = tiles >= 2 * cus ? FEW_4 : FEW_8;
         if (want > 1 && most > 1) plan.parts = (int)(want < most ? want : most);
         if (plan.parts > MAX_PARTS) plan.parts = MAX_PARTS;
