@@ -681,11 +681,9 @@ int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
     using H = Head<DP, true>;
     const int lds = keys ? 8 * H::TILE : 4 * Head<DP>::TILE;
     static_assert(1024 + 3 * H::DB * 4096 <= 8 * H::TILE, "the waves' sums take the place of the stages");
+    static bool reserved[2][64] = {{false}};
     const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
-    if (lds > 65536 && hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-        (void)hipGetLastError();
-        return fail(SVDQ_ELAUNCH, "cross_attention: the device does not offer %d bytes of LDS", lds);
-    }
+    if (int rc = reserve_lds(kernel, lds, reserved[keys], "cross_attention")) return rc;
     const long long groups = (long long)p.parts * p.Hkv * p.B;
     const dim3 grid((unsigned)((p.spread ? (groups + 7) / 8 * 8 : groups) * p.row_blocks)), block(256);
     if (!keys) {

@@ -52,6 +52,16 @@ inline int compute_units(int dev) {
     }
     return cached[dev];
 }
+// More than 64 KB of LDS for a kernel, asked for once per device (racing first calls both ask, which is harmless); `reserved`: the kernel's own
+inline int reserve_lds(const void *kernel, int bytes, bool (&reserved)[64], const char *what) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return fail(SVDQ_ELAUNCH, "%s: cannot identify the current device", what);
+    if (reserved[dev] || bytes <= 65536) return SVDQ_OK;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(SVDQ_ELAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    reserved[dev] = true;
+    return SVDQ_OK;
+}
 #define SVDQ_REQUIRE(cond, ...) \
     do {                        \
         if (!(cond)) return svdq::fail(SVDQ_EINVAL, __VA_ARGS__); \

@@ -78,18 +78,16 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
     const int sub = lane >> 3;
     const char *src_a = p.act + (long long)m0 * p.ld_act, *src_b = p.wgt + (long long)n0 * p.ld_wgt;
     uint32_t off_a[T::A_REQ], off_b[T::B_REQ];
-    int piece_a[T::A_REQ], piece_b[T::B_REQ];
+    auto piece = [&](int row) __attribute__((always_inline)) { return ((lane & 7) ^ swizzle(row)) * 16; };
 #pragma unroll
     for (int i = 0; i < T::A_REQ; i++) {
         const int r = (wave * T::A_REQ + i) * 8 + sub, last = p.M - 1 - m0;
-        piece_a[i] = ((lane & 7) ^ swizzle(r)) * 16;
-        off_a[i] = (uint32_t)((r < last ? r : last) * p.ld_act) + piece_a[i];
+        off_a[i] = (uint32_t)((r < last ? r : last) * p.ld_act) + piece(r);
     }
 #pragma unroll
     for (int i = 0; i < T::B_REQ; i++) {
         const int r = (wave * T::B_REQ + i) * 8 + sub, last = p.N - 1 - n0;
-        piece_b[i] = ((lane & 7) ^ swizzle(r)) * 16;
-        off_b[i] = (uint32_t)((r < last ? r : last) * p.ld_wgt) + piece_b[i];
+        off_b[i] = (uint32_t)((r < last ? r : last) * p.ld_wgt) + piece(r);
     }
     // this part's steps along K
     const int whole = p.K / BK, all = (p.K + BK - 1) / BK;
@@ -110,12 +108,12 @@ __global__ void __launch_bounds__(WM *WN * 64, OCC) w8a8_tiles_kernel(W8A8Params
             const int left = p.K - step * BK;
 #pragma unroll
             for (int i = 0; i < T::A_REQ; i++) {
-                const char *s = piece_a[i] < left ? a + off_a[i] : (const char *)&zeros16;
+                const char *s = piece((wave * T::A_REQ + i) * 8 + sub) < left ? a + off_a[i] : (const char *)&zeros16;
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst_a + stage + i * 1024), "v"(s) : "memory", "m0");
             }
 #pragma unroll
             for (int i = 0; i < T::B_REQ; i++) {
-                const char *s = piece_b[i] < left ? b + off_b[i] : (const char *)&zeros16;
+                const char *s = piece((wave * T::B_REQ + i) * 8 + sub) < left ? b + off_b[i] : (const char *)&zeros16;
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst_b + stage + i * 1024), "v"(s) : "memory", "m0");
             }
         }
@@ -326,10 +324,8 @@ int launch_tiles(W8A8Params &p, hipStream_t st) {
     p.tiles_n = (p.N + BN - 1) / BN;
     if ((long long)p.tiles_m * p.tiles_n >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "gemm_w8a8: %d x %d tiles are too many for one launch", p.tiles_m, p.tiles_n);
     auto *kernel = w8a8_tiles_kernel<BM, BN, WM, WN, STAGES, OCC>;
-    if (T::LDS > 65536 && hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) != hipSuccess) {
-        (void)hipGetLastError();
-        return fail(SVDQ_ELAUNCH, "gemm_w8a8: the device does not offer %d bytes of LDS", T::LDS);
-    }
+    static bool reserved[64] = {false};
+    if (int rc = reserve_lds((const void *)kernel, T::LDS, reserved, "gemm_w8a8")) return rc;
     SVDQ_LAUNCH(kernel, dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.parts), dim3(T::THREADS), T::LDS, st, p);
     return join(p, st);
 }
