@@ -237,8 +237,9 @@ __global__ void __launch_bounds__(WAVES * 64) w8a8_few_rows_kernel(W8A8Params p)
     const char *w = p.wgt + (long long)(n0 + r < p.N ? n0 + r : p.N - 1) * p.ld_wgt + q * 16;
     const char *a = p.act + (long long)(r < p.M ? r : p.M - 1) * p.ld_act + q * 16;
     int4_t acc = int4_t{0, 0, 0, 0};
-    // this part's steps of 64 bytes, in turns of UN: the waves take them one after the other
-    constexpr int UN = 4;
+    // this part's steps of 64 bytes, in turns of UN: the waves take them one after the other (UN = 4: 1 x 4096 x 12288 13.3 us against 12.2,
+    // 1 x 4096 x 4096 7.9 against 7.3; 8: 12.4 and 7.5 with eight waves)
+    constexpr int UN = 2;
     const int whole = p.K / 64, turns = ((p.K + 63) / 64 + UN - 1) / UN;
     const int first = (int)((long long)turns * blockIdx.y / p.parts), last = (int)((long long)turns * (blockIdx.y + 1) / p.parts);
     int s = (first + wave) * UN;
@@ -367,10 +368,10 @@ Plan plan_of(long long M, long long N, long long K, int cus) {
     Plan plan = {T256x256, 1, 0};
     const long long few = (N + 15) / 16;
     if (M <= 8 || (M <= 16 && few < 2 * cus)) {
-        // 16 columns a workgroup: with few of them eight waves instead of four, and parts of at least a turn for each wave
-        // (1 x 4096 x 4096 8.3 -> 7.8 us with eight waves, 8 x 16384 x 512 14.2 -> 9.4 with eight parts; 1 x 4096 x 12288 13.3 with four, 13.6 with
+        // 16 columns a workgroup: with few of them eight waves instead of four, and parts of at least two turns for each wave
+        // (1 x 4096 x 4096 7.5 -> 7.3 us with eight waves, 8 x 16384 x 512 14.2 -> 9.2 in parts; 1 x 4096 x 12288 12.2 with four, 13.1 with
         // eight).  More than eight rows on many columns go to tiles, whose activations come once per 64 columns (16 x 4096 x 12288 15.1 -> 13.9;
-        // eight rows 12.5 here, 13.5 there)
+        // eight rows 13.3 here, 13.1 there)
         const long long tiles = few, most = K / 2048, want = cus / tiles;
         plan.form = tiles >= 2 * cus ? FEW_4 : FEW_8;
         if (want > 1 && most > 1) plan.parts = (int)(want < most ? want : most);
