@@ -739,6 +739,10 @@ int check_args(const svdq_cross_attention_args *a) {
     SVDQ_REQUIRE(a->q_len > 0 && a->k_len > 0 && a->k_len < (1ll << 31) - 64, "cross_attention: q_len (%lld) and k_len (%lld) must be positive, k_len below 2^31 - 64", (long long)a->q_len,
                  (long long)a->k_len);
     SVDQ_REQUIRE(a->q_len * (a->heads / a->kv_heads) < (1ll << 31) - 128, "cross_attention: q_len (%lld) times the heads that share keys must be below 2^31 - 128", (long long)a->q_len);
+    // (a launch takes fewer than 2^32 threads, 256 for 32 rows at most)
+    const long long rows = a->q_len * (a->heads / a->kv_heads);
+    SVDQ_REQUIRE((rows + 31) / 32 * (a->batch * a->kv_heads + 7) < (1ll << 24), "cross_attention: batch times kv_heads (%lld) groups of %lld rows of queries are too many for one launch",
+                 (long long)(a->batch * a->kv_heads), rows);
     SVDQ_REQUIRE(!a->key_lengths + !a->key_mask + !a->cu_seqlens_k >= 2, "cross_attention: at most one of key_lengths, key_mask and cu_seqlens_k can be given");
     SVDQ_REQUIRE(a->scale > 0.f && a->scale < __builtin_huge_valf(), "cross_attention: scale must be a positive number");
     for (int i = 0; i < 3; i++)
@@ -778,8 +782,6 @@ extern "C" int svdq_cross_attention(const svdq_cross_attention_args *a, void *st
     const Plan plan = plan_of(a, cus);
     SVDQ_REQUIRE(plan.workspace == 0 || (a->workspace && a->workspace_bytes >= plan.workspace), "cross_attention: needs a workspace of %lld bytes, got %lld", plan.workspace,
                  (long long)(a->workspace ? a->workspace_bytes : 0));
-    const long long grid = plan.row_blocks * (plan.parts * a->kv_heads * a->batch + 7);
-    if (grid >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "cross_attention: %lld workgroups are too many for one launch", grid);
     AttentionParams p;
     p.q = (const char *)a->q;
     p.k = (const char *)a->k;

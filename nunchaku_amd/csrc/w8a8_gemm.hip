@@ -323,7 +323,6 @@ int launch_tiles(W8A8Params &p, hipStream_t st) {
     using T = Tiles<BM, BN, WM, WN, STAGES>;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
-    if ((long long)p.tiles_m * p.tiles_n >= (1ll << 31)) return fail(SVDQ_EUNSUPPORTED, "gemm_w8a8: %d x %d tiles are too many for one launch", p.tiles_m, p.tiles_n);
     auto *kernel = w8a8_tiles_kernel<BM, BN, WM, WN, STAGES, OCC>;
     static bool reserved[64] = {false};
     if (int rc = reserve_lds((const void *)kernel, T::LDS, reserved, "gemm_w8a8")) return rc;
@@ -338,28 +337,30 @@ int launch_few(W8A8Params &p, hipStream_t st) {
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------------------
-enum Form { FEW_4, FEW_8, T32x64, T64x64_DEEP, T64x64, T64x128, T128x128, T128x256, T256x256 };
+enum Form { FEW_4, FEW_8, T32x64, T64x64_DEEP, T64x64, T64x128, T128x128, T256x256 };
 struct Plan {
     Form form;
     int parts;
     long long workspace;
 };
 
-// A model of the busiest compute unit's time, in us, fitted to 20 shapes of 1 .. 8192 rows (each form and number of parts timed): a step of
-// 128 bytes of K takes a workgroup `alone` while it has its compute unit to itself and every one of several `share`; `slots` fit a compute
-// unit.  A tile ends with its output's way to memory (20 bytes a ns for a compute unit when all write) and 1.5 us of latencies; launch and
-// first loads take 4 us, the kernel that joins parts 3 us and its traffic.  Few rows are the weights' way from memory.
-// Chosen / next best, us: 505 x 2304 x 4608 14.9 (64 x 64) / 16.3, 256 x 4096 x 4096 13.7 (64 x 64, four stages) / 14.1, 1024 x 4096 x 4096 27.8
-// (64 x 128) / 29.4, 2048 x 4096 x 4096 39.6 (128 x 128) / 43.3, 7747 x 13984 x 156 44.7 (128 x 256 in four parts; whole 61), 17 x 13728 x 3213 14.8
-// (32 x 64 in four parts; whole 17), 4608 x 4096 x 16384 316 (256 x 256) / 340.
+// A model of the busiest compute unit's time, in us, fitted to 32 shapes of 17 .. 16384 rows (each form and number of parts timed; what it
+// chooses is 0.8 % behind the fastest on average, 13 % at most): a step of 128 bytes of K takes a workgroup `alone` while it has its compute
+// unit to itself and every one of several `share`; `slots` fit a compute unit.  A tile ends with its output's way to memory (20 bytes a ns for a
+// compute unit when all write) and 0.4 us of latencies; the kernel that joins parts takes 1.4 us and its traffic.  Few rows are the weights'
+// way from memory.
+// Chosen / next best form, us: 505 x 2304 x 4608 14.3 (64 x 64) / 15.9, 256 x 4096 x 4096 14.7 (64 x 64, four stages) / 16.1, 1024 x 4096 x 4096 28.1
+// (64 x 128) / 29.2, 2048 x 4096 x 4096 38.1 (128 x 128) / 51.1, 7747 x 13984 x 156 46.6 (128 x 128 in four parts; whole 89.8), 17 x 13728 x 3213 14.3
+// (32 x 64 in five parts; whole 33.1), 4608 x 4096 x 16384 306 (256 x 256) / 335.  Tiles of 128 x 256 in three stages were ahead at 3 of the shapes
+// only, those with the most operand bytes for a round of tiles (1024 x 8192 x 8192 72.3 / 79.1), behind at the others (2048 x 4096 x 4096 41.5).
 struct Cost {
     Form form;
     int bm, bn, slots;
     float alone, share;
 };
 constexpr Cost costs[] = {
-    {T32x64, 32, 64, 3, 0.30f, 0.17f},    {T64x64_DEEP, 64, 64, 2, 0.31f, 0.20f},  {T64x64, 64, 64, 5, 0.45f, 0.20f},      {T64x128, 64, 128, 2, 0.45f, 0.36f},
-    {T128x128, 128, 128, 2, 0.72f, 0.55f}, {T128x256, 128, 256, 1, 1.15f, 1.15f}, {T256x256, 256, 256, 1, 1.90f, 1.90f},
+    {T32x64, 32, 64, 3, 0.235f, 0.205f},   {T64x64_DEEP, 64, 64, 2, 0.265f, 0.19f}, {T64x64, 64, 64, 5, 0.475f, 0.195f},
+    {T64x128, 64, 128, 2, 0.415f, 0.325f}, {T128x128, 128, 128, 2, 0.65f, 0.455f},  {T256x256, 256, 256, 1, 1.48f, 1.48f},
 };
 constexpr int MAX_PARTS = 16;
 
@@ -384,9 +385,9 @@ Plan plan_of(long long M, long long N, long long K, int cus) {
             for (int parts = 1; parts <= MAX_PARTS && (parts == 1 || (steps >= 4 * parts && tiles * (parts - 1) < c.slots * cus)); parts++) {
                 const long long most = (tiles * parts + cus - 1) / cus, rounds = most / c.slots, rest = most % c.slots;
                 const float n = (float)((steps + parts - 1) / parts);
-                auto round = [&](long long w) { return n * (c.alone > w * c.share ? c.alone : w * c.share) + 1.5f + w * last * (parts > 1 ? 2.f : 1.f); };
+                auto round = [&](long long w) { return n * (c.alone > w * c.share ? c.alone : w * c.share) + 0.4f + w * last * (parts > 1 ? 2.f : 1.f); };
                 float t = rounds * round(c.slots) + (rest ? round(rest) : 0.f);
-                if (parts > 1) t += 3.f + M * N * 4.f * parts / 4.0e6f;
+                if (parts > 1) t += 1.4f + M * N * 4.f * parts / 4.0e6f;
                 if (best == 0.f || t < best) {
                     best = t;
                     plan.form = c.form;
@@ -402,8 +403,11 @@ Plan plan_of(long long M, long long N, long long K, int cus) {
 int plan_call(const svdq_gemm_w8a8_args *a, Plan &plan) {
     SVDQ_REQUIRE(a && a->act && a->wgt && a->ascales && a->wscales && a->out, "gemm_w8a8: act, wgt, ascales, wscales and out must not be null");
     SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "gemm_w8a8: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
-    SVDQ_REQUIRE(a->M > 0 && a->N > 0 && a->M < (1ll << 31) - 256 && a->N < (1ll << 31) - 256, "gemm_w8a8: M (%lld) and N (%lld) must be positive and below 2^31 - 256",
+    SVDQ_REQUIRE(a->M > 0 && a->N > 0 && a->M < (1ll << 31) - 256 && a->N < (1ll << 28) - 256, "gemm_w8a8: M (%lld) must be positive and below 2^31 - 256, N (%lld) below 2^28 - 256",
                  (long long)a->M, (long long)a->N);
+    // a launch takes fewer than 2^32 threads: no form has more than 16 columns (few rows) or one and a half such tiles for 256 of them
+    SVDQ_REQUIRE(((a->M + 31) / 32) * ((a->N + 63) / 64) < (1ll << 24), "gemm_w8a8: %lld x %lld outputs are too many for one launch (2^24 tiles of 32 x 64)", (long long)a->M,
+                 (long long)a->N);
     // 127 * 127 * 131072 and 128 * 128 * 131056 stay below 2^31
     SVDQ_REQUIRE(a->K > 0 && a->K % 16 == 0 && a->K < 131072, "gemm_w8a8: K (%lld) must be a multiple of 16 below 131072, so that the integer sums cannot overflow", (long long)a->K);
     SVDQ_REQUIRE(a->ld_act >= a->K && a->ld_act % 16 == 0 && a->ld_act < (1ll << 23), "gemm_w8a8: rows of act must be at least K bytes, a multiple of 16 and less than 2^23 apart, got %lld",
@@ -464,7 +468,6 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
     case T64x64: return launch_tiles<64, 64, 2, 2, 2, 2>(p, st);
     case T64x128: return launch_tiles<64, 128, 2, 2, 3, 2>(p, st);
     case T128x128: return launch_tiles<128, 128, 4, 2, 2, 2>(p, st);
-    case T128x256: return launch_tiles<128, 256, 2, 4, 3, 2>(p, st);
     default: return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
     }
 }

@@ -212,9 +212,22 @@ int quantize_rows(const svdq_quantize_w8a8_args *a, bool norm, void *stream, con
     p.pieces = (int)(a->K / 8);
     p.inv_k = 1.0f / (float)a->K;
     p.eps = a->eps;
-    if (a->dtype == SVDQ_BF16) dispatch<true>(p, norm, (hipStream_t)stream);
-    else dispatch<false>(p, norm, (hipStream_t)stream);
-    return check_launch(what);
+    // a launch takes fewer than 2^32 threads, of which a row has 1024 at most (with rows that long it would be 2^21 of them, 70 GB)
+    const long long most = p.pieces <= 256 ? 1ll << 25 : 1ll << 21;
+    for (long long first = 0; first < a->M; first += most) {
+        p.M = a->M - first < most ? a->M - first : most;
+        if (a->dtype == SVDQ_BF16) dispatch<true>(p, norm, (hipStream_t)stream);
+        else dispatch<false>(p, norm, (hipStream_t)stream);
+        if (int rc = check_launch(what)) return rc;
+        p.x += most * p.ld_x;
+        p.codes += most * p.ld_codes;
+        p.scales += most;
+        if (p.residual) {
+            p.residual += most * p.ld_residual;
+            p.residual_out += most * p.ld_residual_out;
+        }
+    }
+    return SVDQ_OK;
 }
 
 }  // namespace

@@ -151,7 +151,7 @@ def check_gemm(got, act, wgt, sa, sw, bias, dtype):
 GEMM_SIZES = [
     (1, 1, 16), (1, 7, 32), (1, 256, 4096), (2, 33, 80), (16, 48, 64), (17, 130, 1008), (32, 64, 528), (33, 64, 128), (33, 65, 144), (64, 7, 2064),
     (65, 200, 256), (127, 129, 112), (128, 384, 400), (200, 1000, 1040), (257, 513, 272), (505, 1152, 2304), (1000, 1, 640), (3, 5000, 2064),
-    (4096, 3072 // 2, 144), (2049, 6145, 96), (4100, 4104, 208),
+    (4096, 1536, 144), (2049, 6145, 96), (4100, 4104, 208),
 ]
 
 
@@ -168,6 +168,84 @@ def test_gemm(dev, M, N, K, dtype, bias):
     assert got is out.t
     check_gemm(got, act, wgt, sa, sw, b, dtype)
     out.check("out")
+
+
+# every form of the kernel, whole and with K in parts (of which a small kernel adds the sums)
+GEMM_FORMS = [
+    (8, 8810, 144), (5, 30, 8208), (13, 100, 4112), (19, 44, 1488), (64, 7, 2064), (17, 700, 13728), (3052, 5, 1936), (8311, 4, 16), (6594, 4, 14496),
+    (8483, 198, 48), (9971, 273, 48), (10, 8764, 10688), (8531, 643, 16), (67, 8993, 8928), (6615, 1807, 32), (414, 5461, 11840),
+]
+
+
+@pytest.mark.parametrize("M,N,K", GEMM_FORMS)
+def test_gemm_forms(dev, M, N, K):
+    """... and the same bits from run to run, and through a call that names its output."""
+    from nunchaku_amd.ops import gemm_w8a8
+
+    announce(f"gemm forms {M} x {N} x {K}")
+    (act, sa), (wgt, sw) = codes_of(M, K, M), codes_of(N, K, N + 1)
+    on = [t.to(dev) for t in (act, wgt, sa, sw)]
+    b = rand((N,), N, torch.bfloat16).to(dev)
+    got = gemm_w8a8(*on, bias=b)
+    check_gemm(got, act, wgt, sa, sw, b.cpu(), torch.bfloat16)
+    out = Guarded((M, N), torch.bfloat16, dev)
+    for _ in range(3):
+        assert torch.equal(gemm_w8a8(*on, bias=b, out=out.t), got)
+    out.check("out")
+
+
+def test_gemm_streams_and_graphs(dev):
+    """Products with K in parts on a user's stream and in two captured graphs replayed in turn: workspaces are the calls' own."""
+    from nunchaku_amd.ops import gemm_w8a8
+
+    announce("gemm streams and graphs")
+    sets = []
+    for i, (M, N, K) in enumerate([(5, 500, 16384), (64, 700, 8208)]):
+        (act, sa), (wgt, sw) = codes_of(M, K, i), codes_of(N, K, i + 7)
+        sets.append([t.to(dev) for t in (act, wgt, sa, sw)])
+    want = [gemm_w8a8(*s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [gemm_w8a8(*s) for s in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(gemm_w8a8(*s))
+        graphs.append(g)
+    for turn in range(4):
+        for s in sets:
+            s[0].bitwise_xor_(turn)
+            s[2].mul_(1.25)
+        eager = [gemm_w8a8(*s) for s in sets]
+        for o in outs:
+            o.zero_()
+        for g in graphs if turn % 2 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+def test_more_rows_than_a_launch_takes(dev):
+    """2^25 rows a launch: the rows around that one, and the last."""
+    from nunchaku_amd.ops import quantize_w8a8_act, rms_norm_quantize_w8a8
+
+    announce("2^25 + 77 rows")
+    M, K = (1 << 25) + 77, 16
+    x = torch.randn(M, K, device=dev, dtype=torch.bfloat16)
+    w = rand((K,), 1, torch.bfloat16, False)
+    picks = [slice(0, 9), slice((1 << 25) - 5, (1 << 25) + 6), slice(M - 3, M)]
+    codes, scales = quantize_w8a8_act(x)
+    for p in picks:
+        check_codes(codes[p], scales[p], *ow.quantize_rows(x[p].cpu()), 0.0)
+    codes, scales, h = rms_norm_quantize_w8a8(x, w.to(dev), x)
+    for p in picks:
+        want = ow.rms_norm_quantize(x[p].cpu(), w, x[p].cpu())
+        check_codes(codes[p], scales[p], want[0], want[1], 52 * U32)
+        assert torch.equal(h[p].cpu(), want[2])
 
 
 def test_gemm_largest_sums(dev):
@@ -300,3 +378,27 @@ def test_layer(dev, dtype):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, m(x))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_same_with_and_without_given_outputs(dev, dtype):
+    """Calls that name their outputs, or come with an integer eps, take another way to the kernels: the same bits."""
+    from nunchaku_amd.ops import gemm_w8a8, quantize_w8a8_act, rms_norm_quantize_w8a8
+
+    x, r, w = (rand(s, i, dtype).to(dev) for i, s in enumerate([(2, 11, 528), (2, 11, 528), (528,)]))
+    codes, scales = quantize_w8a8_act(x)
+    out = torch.empty_like(codes), torch.empty_like(scales)
+    quantize_w8a8_act(x, *out)
+    assert torch.equal(codes, out[0]) and torch.equal(scales, out[1])
+    wide = torch.zeros(22, 1056, dtype=dtype, device=dev)
+    wide[:, 528:] = x.view(22, 528)
+    again = quantize_w8a8_act(wide[:, 528:])
+    assert torch.equal(codes.view(22, 528), again[0]) and torch.equal(scales.view(22), again[1])
+    a = rms_norm_quantize_w8a8(x, w, r, 0.0)
+    b = rms_norm_quantize_w8a8(x, w, r, 0)
+    c = rms_norm_quantize_w8a8(x, w, r, 0.0, *out, residual_out=torch.empty_like(x))
+    assert all(torch.equal(p, q) and torch.equal(p, s) for p, q, s in zip(a, b, c))
+    wc, ws = quantize_w8a8_act(r[0])
+    y = gemm_w8a8(codes, wc, scales, ws, out_dtype=dtype)
+    z = torch.empty(2, 11, 11, dtype=dtype, device=dev)
+    assert gemm_w8a8(codes, wc, scales, ws, out=z) is z and torch.equal(y, z)

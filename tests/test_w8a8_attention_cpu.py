@@ -93,6 +93,8 @@ def _gemm_refusals(entry, good, lib):
         assert b"null" in _refused(entry, good, lib, **{name: None})
     for changes in (dict(M=0), dict(N=0), dict(M=1 << 31), dict(N=1 << 31)):
         assert b"M (" in _refused(entry, good, lib, **changes)
+    for changes in (dict(M=(1 << 29) + 1, N=1), dict(M=33, N=1 << 28), dict(M=1 << 20, N=1 << 15, ld_out=1 << 15)):
+        assert b"M (" in _refused(entry, good, lib, **changes) or b"outputs" in _refused(entry, good, lib, **changes)
     for k in (0, 8, 72, 131072):
         assert b"K (" in _refused(entry, good, lib, K=k, ld_act=131072, ld_wgt=131072)
     assert b"act" in _refused(entry, good, lib, ld_act=48)
@@ -123,6 +125,8 @@ def test_attention_refusals(lib):
         assert b"k_len" in _refused(entry, good, lib, k_len=0)
         assert b"k_len" in _refused(entry, good, lib, k_len=1 << 31)
         assert b"q_len" in _refused(entry, good, lib, q_len=1 << 30)
+        assert b"too many" in _refused(entry, good, lib, batch=65535, heads=512, kv_heads=512)
+        assert b"too many" in _refused(entry, good, lib, q_len=1 << 28)
         assert b"at most one" in _refused(entry, good, lib, key_lengths=16, key_mask=16)
         assert b"at most one" in _refused(entry, good, lib, key_lengths=16, cu_seqlens_k=16)
         for s in (0.0, -1.0, math.inf, math.nan):
