@@ -5,7 +5,8 @@
 // g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32.  |code| <= 127 needs no clamp:
 // |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
 // scale NaN and codes 0: what a product makes of it is NaN.
-// Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.
+// Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 69 us, 5.8 TB/s;
+// 9216 x 5120 with residual 56 us, 5.9 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
 #include "svdq_common.h"
 
 using namespace svdq;
@@ -44,13 +45,13 @@ __device__ inline uint32_t pack_pair(float lo, float hi) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
 }
 
-// THREADS per row (64: four rows per workgroup), each with up to VECS pieces of 8 elements
+// THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements
 template <bool BF16, int THREADS, int VECS, bool NORM, bool RESIDUAL>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_kernel(QuantizeParams p) {
-    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, WAVES = THREADS / 64;
+    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, WAVES = THREADS <= 64 ? 1 : THREADS / 64;
     const int t = threadIdx.x % THREADS;
     const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    if (row >= p.M) return;  // (a whole wave; rows of several waves are one per workgroup)
+    if (row >= p.M) return;  // (all threads of a row; rows of several waves are one per workgroup)
     const char *x = p.x + row * p.ld_x;
     u32x4_t w[VECS], r[RESIDUAL ? VECS : 1];
 #pragma unroll
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_k
         }
     }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) {
+    for (int d = THREADS < 64 ? THREADS / 2 : 32; d; d >>= 1) {
         const uint32_t o = (uint32_t)__shfl_xor((int)top, d);
         top = o > top ? o : top;
         if (NORM) squares += __shfl_xor(squares, d);
@@ -170,13 +171,24 @@ void launch_rows(const QuantizeParams &p, bool norm, hipStream_t st) {
     else SVDQ_LAUNCH((quantize_rows_kernel<BF16, THREADS, VECS, true, true>), grid, block, 0, st, p);
 }
 
+// The fewest threads that hold a row in one or two pieces each: more of them are more exchanges between waves, more pieces are more work for every
+// lane of a row that does not fill them (the last of several pieces of a norm's row is as much work as the first).  Us, this way / the next best,
+// 1.3e8 elements, plain and norm with residual: K = 512 73 / 78 (two pieces of 64), 156 / 157; 1024 69 / 70 (four), 159 / 169 (256 threads); 2048 70 / 77
+// (four pieces of 64 against 256 threads; with 300 rows 2.9 / 2.7), norm 154 / 168 (256 against four of 64); 4096 69 / 69 (256 threads with four), 154 / 155 (512); 8192 68 / 69, 154 / 155 (512 with four, which
+// with 300 rows takes 3.6 and 6.7 against 3.3 and 5.4); 16384 69 / 72, 161 / 158 (512 with four: 300 rows 5.6 and 8.9 against 5.9 and 8.4); 32768 71 / 91, 167 / 191
+// (eight pieces).
 template <bool BF16>
 void dispatch(const QuantizeParams &p, bool norm, hipStream_t st) {
     const int need = p.pieces;
-    if (need <= 64 * 4) launch_rows<BF16, 64, 4>(p, norm, st);
+    if (need <= 32) launch_rows<BF16, 32, 1>(p, norm, st);
+    else if (need <= 64) launch_rows<BF16, 64, 1>(p, norm, st);
+    else if (need <= 64 * 2) launch_rows<BF16, 64, 2>(p, norm, st);
+    else if (need <= 64 * 4 && !norm && p.M > 2048) launch_rows<BF16, 64, 4>(p, norm, st);
+    else if (need <= 256) launch_rows<BF16, 256, 1>(p, norm, st);
     else if (need <= 256 * 2) launch_rows<BF16, 256, 2>(p, norm, st);
-    else if (need <= 256 * 4) launch_rows<BF16, 256, 4>(p, norm, st);
+    else if (need <= 512 * 2) launch_rows<BF16, 512, 2>(p, norm, st);
     else if (need <= 1024 * 2) launch_rows<BF16, 1024, 2>(p, norm, st);
+    else if (need <= 1024 * 4) launch_rows<BF16, 1024, 4>(p, norm, st);
     else launch_rows<BF16, 1024, 8>(p, norm, st);
 }
 
@@ -212,8 +224,8 @@ int quantize_rows(const svdq_quantize_w8a8_args *a, bool norm, void *stream, con
     p.pieces = (int)(a->K / 8);
     p.inv_k = 1.0f / (float)a->K;
     p.eps = a->eps;
-    // a launch takes fewer than 2^32 threads, of which a row has 1024 at most (with rows that long it would be 2^21 of them, 70 GB)
-    const long long most = p.pieces <= 256 ? 1ll << 25 : 1ll << 21;
+    // a launch takes fewer than 2^32 threads: 2^31 for so many rows of at most 64 threads, of at most 1024
+    const long long most = p.pieces <= 128 ? 1ll << 25 : 1ll << 21;
     for (long long first = 0; first < a->M; first += most) {
         p.M = a->M - first < most ? a->M - first : most;
         if (a->dtype == SVDQ_BF16) dispatch<true>(p, norm, (hipStream_t)stream);

@@ -31,7 +31,7 @@ def check_codes(codes, scales, want_codes, want_scales, rel):
 
 
 # row lengths on both sides of every number of threads per row
-SIZES = [(1, 16), (3, 64), (5, 2032), (2, 2048), (4, 2064), (3, 4096), (2, 4112), (2, 8192), (1, 8208), (3, 16384), (2, 16400), (1, 65536), (1157, 256)]
+SIZES = [(1, 16), (3, 64), (5, 240), (9, 256), (7, 272), (9, 512), (5, 528), (6, 1024), (3, 1040), (2100, 1040), (2050, 2048), (5, 2032), (2, 2048), (4, 2064), (3, 4096), (2, 4112), (2, 8192), (1, 8208), (3, 16384), (2, 16400), (3, 32768), (2, 32784), (1, 65536), (1157, 256)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
