@@ -323,6 +323,7 @@ int launch_tiles(W8A8Params &p, hipStream_t st) {
     using T = Tiles<BM, BN, WM, WN, STAGES>;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
+    if ((long long)p.tiles_m * p.tiles_n * T::THREADS >= (1ll << 32)) return fail(SVDQ_EUNSUPPORTED, "gemm_w8a8: %d x %d tiles are too many for one launch", p.tiles_m, p.tiles_n);
     auto *kernel = w8a8_tiles_kernel<BM, BN, WM, WN, STAGES, OCC>;
     static bool reserved[64] = {false};
     if (int rc = reserve_lds((const void *)kernel, T::LDS, reserved, "gemm_w8a8")) return rc;
@@ -352,7 +353,9 @@ struct Plan {
 // Chosen / next best form, us: 505 x 2304 x 4608 14.3 (64 x 64) / 15.9, 256 x 4096 x 4096 14.7 (64 x 64, four stages) / 16.1, 1024 x 4096 x 4096 28.1
 // (64 x 128) / 29.2, 2048 x 4096 x 4096 38.1 (128 x 128) / 51.1, 7747 x 13984 x 156 46.6 (128 x 128 in four parts; whole 89.8), 17 x 13728 x 3213 14.3
 // (32 x 64 in five parts; whole 33.1), 4608 x 4096 x 16384 306 (256 x 256) / 335.  Tiles of 128 x 256 in three stages were ahead at 3 of the shapes
-// only, those with the most operand bytes for a round of tiles (1024 x 8192 x 8192 72.3 / 79.1), behind at the others (2048 x 4096 x 4096 41.5).
+// only, those with the most operand bytes for a round of tiles (1024 x 8192 x 8192 72.3 / 79.1), behind at the others (2048 x 4096 x 4096 41.5).  64 x 128
+// by eight waves instead of four: 512 x 4096 x 4096 18.3 / 20.2, 1300 x 2304 x 1152 12.1 / 13.8, 1157 x 2304 x 4608 26.8 / 28.7; 128 x 128 by four instead of
+// eight 26.9 / 25.3 (3000 x 640 x 5120); 64 x 64 in three stages 15.5 / 15.0 (505 x 2304 x 4608).
 struct Cost {
     Form form;
     int bm, bn, slots;
@@ -360,7 +363,7 @@ struct Cost {
 };
 constexpr Cost costs[] = {
     {T32x64, 32, 64, 3, 0.235f, 0.205f},   {T64x64_DEEP, 64, 64, 2, 0.265f, 0.19f}, {T64x64, 64, 64, 5, 0.475f, 0.195f},
-    {T64x128, 64, 128, 2, 0.415f, 0.325f}, {T128x128, 128, 128, 2, 0.65f, 0.455f},  {T256x256, 256, 256, 1, 1.48f, 1.48f},
+    {T64x128, 64, 128, 2, 0.36f, 0.325f}, {T128x128, 128, 128, 2, 0.65f, 0.455f},  {T256x256, 256, 256, 1, 1.48f, 1.48f},
 };
 constexpr int MAX_PARTS = 16;
 
@@ -405,7 +408,7 @@ int plan_call(const svdq_gemm_w8a8_args *a, Plan &plan) {
     SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "gemm_w8a8: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
     SVDQ_REQUIRE(a->M > 0 && a->N > 0 && a->M < (1ll << 31) - 256 && a->N < (1ll << 28) - 256, "gemm_w8a8: M (%lld) must be positive and below 2^31 - 256, N (%lld) below 2^28 - 256",
                  (long long)a->M, (long long)a->N);
-    // a launch takes fewer than 2^32 threads: no form has more than 16 columns (few rows) or one and a half such tiles for 256 of them
+    // (a launch takes fewer than 2^32 threads: 128 to 512 a tile, 32 x 64 the smallest of them; 512 for 16 columns of few rows)
     SVDQ_REQUIRE(((a->M + 31) / 32) * ((a->N + 63) / 64) < (1ll << 24), "gemm_w8a8: %lld x %lld outputs are too many for one launch (2^24 tiles of 32 x 64)", (long long)a->M,
                  (long long)a->N);
     // 127 * 127 * 131072 and 128 * 128 * 131056 stay below 2^31
@@ -466,7 +469,7 @@ extern "C" int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *a, void *stream) {
     case T32x64: return launch_tiles<32, 64, 1, 2, 4, 2>(p, st);
     case T64x64_DEEP: return launch_tiles<64, 64, 2, 2, 4, 2>(p, st);
     case T64x64: return launch_tiles<64, 64, 2, 2, 2, 2>(p, st);
-    case T64x128: return launch_tiles<64, 128, 2, 2, 3, 2>(p, st);
+    case T64x128: return launch_tiles<64, 128, 2, 4, 3, 2>(p, st);
     case T128x128: return launch_tiles<128, 128, 4, 2, 2, 2>(p, st);
     default: return launch_tiles<256, 256, 2, 4, 2, 2>(p, st);
     }
