@@ -6,7 +6,7 @@
 // |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
 // scale NaN and codes 0: what a product makes of it is NaN.
 // Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 69 us, 5.8 TB/s;
-// 9216 x 5120 with residual 56 us, 5.9 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
+// 9216 x 5120 with residual 54 us, 6.1 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
 #include "svdq_common.h"
 
 using namespace svdq;
