@@ -355,6 +355,16 @@ class W8A8Linear(nn.Module):
         self.wscales = nn.Parameter(torch.empty(out_features, dtype=torch.float32, device=device), requires_grad=False)
         self.bias = nn.Parameter(torch.empty(out_features, dtype=torch_dtype, device=device), requires_grad=False) if bias else None
 
+    def _apply(self, fn, recurse=True):
+        """Moves and casts like any module, but the scales stay fp32 (``.to(torch.bfloat16)`` of a whole model reaches this layer, too)."""
+        scales = self.wscales.data
+        super()._apply(fn, recurse)
+        if self.wscales.dtype != torch.float32:
+            self.wscales.data = scales.to(self.wscales.device)
+        if self.bias is not None:
+            self.torch_dtype = self.bias.dtype
+        return self
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x [..., K] -> [..., N]"""
         return self.forward_quant(*quantize_w8a8_act(x), out_dtype=x.dtype)
@@ -367,9 +377,12 @@ class W8A8Linear(nn.Module):
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, torch_dtype: torch.dtype | None = None, device: str | torch.device | None = None, **kwargs):
-        """Quantizes the weights of ``linear``, each output channel like a row of activations (``quantize_w8a8_act``)."""
+        """Quantizes the weights of ``linear``, each output channel like a row of activations (``quantize_w8a8_act``).  The layer's type
+        is ``torch_dtype``, or that of ``linear`` where it is one the operators take, or bf16."""
         w = linear.weight.detach()
-        m = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, torch_dtype=torch_dtype or w.dtype,
+        if torch_dtype is None:
+            torch_dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        m = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, torch_dtype=torch_dtype,
                 device=w.device if device is None else device)
         g = w.float()
         if not torch.isfinite(g).all():

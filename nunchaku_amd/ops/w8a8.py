@@ -122,7 +122,7 @@ def rms_norm_quantize_w8a8(
 def _code_rows(t: torch.Tensor, name: str) -> torch.Tensor:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on a GPU (got {t.device}); this path has no CPU implementation")
-    if t.dtype != torch.int8 or t.dim() < 2:
+    if t.dtype != torch.int8 or t.dim() == 0:
         raise ValueError(f"{name} must be int8 rows of codes, got {t.dtype} {tuple(t.shape)}")
     if t.dim() != 2:
         try:

@@ -402,3 +402,16 @@ def test_same_with_and_without_given_outputs(dev, dtype):
     y = gemm_w8a8(codes, wc, scales, ws, out_dtype=dtype)
     z = torch.empty(2, 11, 11, dtype=dtype, device=dev)
     assert gemm_w8a8(codes, wc, scales, ws, out=z) is z and torch.equal(y, z)
+
+
+def test_a_token_without_a_batch(dev):
+    """[K] -> [N], as a linear layer takes it; and a layer cast with its model."""
+    from nunchaku_amd.models import W8A8Linear
+
+    torch.manual_seed(2)
+    m = W8A8Linear.from_linear(torch.nn.Linear(528, 72)).to(dev).half()
+    x = rand((3, 528), 1, torch.float16).to(dev)
+    y = m(x)
+    assert y.dtype == torch.float16 and y.shape == (3, 72)
+    one = m(x[1])
+    assert one.shape == (72,) and torch.equal(one, y[1])

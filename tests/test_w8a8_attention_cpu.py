@@ -175,6 +175,20 @@ def test_layer_quantizes_its_weights():
         W8A8Linear.from_linear(lin)
 
 
+def test_layer_keeps_its_scales_when_the_model_is_cast():
+    from nunchaku_amd.models import W8A8Linear
+
+    torch.manual_seed(1)
+    m = W8A8Linear.from_linear(torch.nn.Linear(96, 40))  # fp32: the operators' default type
+    assert m.torch_dtype == m.bias.dtype == torch.bfloat16
+    scales, codes = m.wscales.clone(), m.qweight.clone()
+    model = torch.nn.Sequential(m, torch.nn.Linear(40, 8)).to(torch.float16)
+    assert model[1].weight.dtype == m.bias.dtype == m.torch_dtype == torch.float16
+    assert torch.equal(m.wscales, scales) and m.wscales.dtype == torch.float32 and isinstance(m.wscales, torch.nn.Parameter)
+    assert torch.equal(model.double()[0].wscales, scales) and torch.equal(m.qweight, codes)
+    assert m.to("meta").wscales.dtype == torch.float32
+
+
 def test_oracle_by_hand():
     """Literals: a tie goes to the even code, the floor keeps a row of zeros, a bad row is NaN, and softmax weights of 1 : 3."""
     codes, scales = ow.quantize_rows(torch.tensor([[127.0, 0.5, 1.5, -2.5], [0.0, 0.0, 0.0, 0.0], [1.0, math.inf, 2.0, 3.0], [math.nan, 1.0, 1.0, 1.0]]))
