@@ -142,7 +142,7 @@ def _host_commands(obj: Path, lib_path: Path, out: Path):
     includes = [*cpp_extension.include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]
     compile_ = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                 *[a for d in includes for a in ("-isystem", d)], "-c", str(_CSRC / "host_ext.cpp"), "-o", str(obj)]
-    link = ["g++", "-shared", str(obj), "-o", str(out), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+    link = ["g++", "-shared", str(obj), "-o", str(out), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
             f"-L{lib_path.parent}", f"-l:{lib_path.name}", "-Wl,-rpath,$ORIGIN"]
     return compile_, link
 

@@ -415,3 +415,21 @@ def test_a_token_without_a_batch(dev):
     assert y.dtype == torch.float16 and y.shape == (3, 72)
     one = m(x[1])
     assert one.shape == (72,) and torch.equal(one, y[1])
+
+
+def test_results_in_inference_mode_are_as_torch_makes_them(dev):
+    from nunchaku_amd.ops import cross_attention, gemm_w8a8, rms_norm_quantize_w8a8
+
+    def run():
+        x = rand((4, 1, 64), 3, torch.bfloat16).to(dev)
+        codes, scales, h = rms_norm_quantize_w8a8(x, x[0, 0], x)
+        y = gemm_w8a8(codes, codes.view(4, 64), scales, scales.view(4))
+        return codes, scales, h, y, cross_attention(x.view(1, 4, 1, 64), x.view(1, 4, 1, 64), x.view(1, 4, 1, 64))
+
+    with torch.inference_mode():
+        inside = run()
+    outside = run()
+    assert all(t.is_inference() and t.is_contiguous() for t in inside) and not any(t.is_inference() or t.requires_grad for t in outside)
+    assert all(torch.equal(a, b) for a, b in zip(inside, outside))
+    outside[3].add_(1)  # an ordinary tensor: changed in place, and counted
+    assert outside[3]._version == 1
