@@ -280,33 +280,26 @@ __device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[H::KS]) {
     for (int ks = 0; ks < H::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
 
-// This lane's row of the output, normalised: 8 consecutive columns per lane and 16-byte store
-template <bool BF16, typename H>
-__device__ inline void store_row(const AttentionParams &p, State<BF16, H> &s, float sum, int b, int hk, int row, int lane) {
-    const int t = row / p.G, gq = row - t * p.G, h = lane >> 5;
-    char *out = p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
-    const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;  // (a NaN stays one)
+// Sixteen columns from c0 on of this lane's row of the output: the lane has c0 + 4 (lane / 32) + [0, 4) in x[0 .. 3] and the same 8 further in
+// x[4 .. 7].  The half-waves exchange, so that each has 8 in a row and stores 16 bytes.
+template <bool BF16>
+__device__ inline void store_columns(char *out, const float (&x)[8], float r, int c0, int columns, int lane) {
+    const int h = lane >> 5;
+    u32x4_t w;
 #pragma unroll
-    for (int d = 0; d < H::DB; d++)
-#pragma unroll
-        for (int gp = 0; gp < 2; gp++) {
-            // columns 32 d + 16 gp + [0, 4) + 4 h and 8 more: the half-waves exchange, so that each has 8 in a row
-            uint32_t lo[2], hi[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                lo[j] = Elem<BF16>::pair(s.o[d][8 * gp + 2 * j] * r, s.o[d][8 * gp + 2 * j + 1] * r);
-                hi[j] = Elem<BF16>::pair(s.o[d][8 * gp + 4 + 2 * j] * r, s.o[d][8 * gp + 4 + 2 * j + 1] * r);
-            }
-            u32x4_t w;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint32_t give = h ? lo[j] : hi[j], got = (uint32_t)__shfl_xor((int)give, 32);
-                w[j] = h ? got : lo[j];
-                w[2 + j] = h ? hi[j] : got;
-            }
-            const int c = 32 * d + 16 * gp + 8 * h;
-            if (row < p.rows && c < p.D) *(u32x4_t *)(out + c * 2) = w;
-        }
+    for (int j = 0; j < 2; j++) {
+        const uint32_t lo = Elem<BF16>::pair(x[2 * j] * r, x[2 * j + 1] * r), hi = Elem<BF16>::pair(x[4 + 2 * j] * r, x[5 + 2 * j] * r);
+        const uint32_t give = h ? lo : hi, got = (uint32_t)__shfl_xor((int)give, 32);
+        w[j] = h ? got : lo;
+        w[2 + j] = h ? hi : got;
+    }
+    const int c = c0 + 8 * h;
+    if (c < columns) *(u32x4_t *)(out + c * 2) = w;
+}
+__device__ inline float inverse(float sum) { return sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum; }  // (a NaN stays one)
+__device__ inline char *row_of(const AttentionParams &p, int b, int hk, int row) {
+    const int t = row / p.G, gq = row - t * p.G;
+    return p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
 }
 
 // Which (row block, group) a workgroup takes, false: none.  A group's row blocks read the same keys (of a head, or of a part of its keys).
@@ -325,6 +318,13 @@ __device__ inline bool block_of(const AttentionParams &p, int groups, int &rb, i
     rb = at % p.row_blocks;
     group = at / p.row_blocks;
     return true;
+}
+
+// Pieces from `first` to the last that is multiplied, of ROWS rows of K in LDS (stages one behind the other): zeros
+template <typename H, int ROWS>
+__device__ inline void zero_columns(char *lds, int first, int thread, int threads) {
+    for (int r = thread; r < ROWS; r += threads)
+        for (int c = first; c < H::DP / 8; c++) *(u32x4_t *)(lds + r * H::PITCH + (c ^ H::fk(r % KEYS)) * 16) = u32x4_t{0, 0, 0, 0};
 }
 
 // The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
@@ -362,11 +362,9 @@ struct Copies {
             in_row[i] = (place ^ H::fv(row[i])) * 16 < bytes;
             if (!EVEN) ok[i] += ck[i];
         }
-        // columns behind the head's end are zero in K for good: no copy writes there
-        if (bytes < H::PITCH) {
-            for (int i = threadIdx.x; i < 2 * H::TILE / 16; i += WAVES * 64) *(u32x4_t *)(lds + i * 16) = u32x4_t{0, 0, 0, 0};
-            __syncthreads();
-        }
+        // columns behind the head's end, as far as they are multiplied, are zero in K for good: no copy writes there (all waves see it behind the
+        // first step's barrier)
+        zero_columns<H, 2 * KEYS>(lds, p.D / 8, threadIdx.x, WAVES * 64);
     }
     // K of step `step` to stage `slot`.  Rows behind the last key are not read: their scores are masked whatever they are.
     __device__ __forceinline__ void k(int step, int slot) {
@@ -492,7 +490,15 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
         step = next;
         bits = list.bits;
     }
-    store_row<BF16, H>(p, st, across_sum(st.sum), b, hk, row, lane);
+    const float r = inverse(across_sum(st.sum));
+    char *out = row_of(p, b, hk, row);
+#pragma unroll
+    for (int u = 0; u < 2 * H::DB; u++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = st.o[u >> 1][8 * (u & 1) + e];
+        store_columns<BF16>(out, x, r, 16 * u, row < p.rows ? p.D : 0, lane);
+    }
 }
 
 // ---- keys form: 32 rows per workgroup, whose waves take every fourth step (of 32 keys) of the part's keys, each through its own LDS, a
@@ -524,10 +530,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
     const uint32_t ok = (uint32_t)(r0 * p.ks[1]), ov = (uint32_t)(r0 * p.vs[1]) + cv;
     static_assert(H::fv(H::RPR) == 0 && (H::RPR == 16 || H::fk(H::RPR) == 4), "");
-    if (bytes < H::PITCH) {  // columns behind the head's end are zero in K for good
-        for (int i = lane; i < 2 * STAGE / 16; i += 64) *(u32x4_t *)(mine + i * 16) = u32x4_t{0, 0, 0, 0};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    // columns behind the head's end are zero in K for good (the wait for a step's copies is one for these, too)
+    zero_columns<H, SIZE>(mine, p.D / 8, lane, 64);
+    zero_columns<H, SIZE>(mine + STAGE, p.D / 8, lane, 64);
     auto request = [&](int step, int slot, uint64_t bits) __attribute__((always_inline)) {
         const char *k = kp + (long long)step * SIZE * p.ks[1], *v = vp + (long long)step * SIZE * p.vs[1];
         const int left = count - step * SIZE;
@@ -572,56 +577,58 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
         step = next;
         bits = list.bits;
     }
-    // the waves meet in the place of the stages: {maximum, sum} of all, then the outputs of the other three, scaled to the highest maximum
-    __syncthreads();
-    float *stat = (float *)lds;  // [4][2][32]
+    // The waves meet.  Each leaves its maximum, sum and outputs in the place of its own stages, 16 columns (a unit) of 64 lanes in 2 KB, and takes
+    // every fourth unit of all four, scaled to the highest maximum.  (All sums in one wave's registers: single tokens, 40 keys, D = 128 8.2 us
+    // against 6.1.)
+    constexpr int UNITS = 2 * H::DB, AREA = 2 * STAGE;
+    static_assert(256 + UNITS * 2048 <= AREA, "");
     const float own = across_sum(st.sum);
     if (h == 0) {
-        stat[wave * 64 + col] = st.top;
-        stat[wave * 64 + 32 + col] = own;
+        ((float *)mine)[col] = st.top;
+        ((float *)mine)[32 + col] = own;
     }
-    __syncthreads();
-    float top = -__builtin_huge_valf(), sum = 0.f;
+    if (row < p.rows) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, stat[i * 64 + col]);
-    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+        for (int u = 0; u < UNITS; u++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum += stat[i * 64 + 32 + col] * __builtin_amdgcn_exp2f(stat[i * 64 + col] - ref);
-    const float f = __builtin_amdgcn_exp2f(st.top - ref);
-    float *sums = stat + 256 + lane;  // [3][16 DB][64]
-    if (wave > 0 && row < p.rows) {
-#pragma unroll
-        for (int d = 0; d < H::DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) sums[(((wave - 1) * H::DB + d) * 16 + e) * 64] = st.o[d][e] * f;
-    }
-    __syncthreads();
-    if (wave == 0 && row < p.rows) {
-#pragma unroll
-        for (int d = 0; d < H::DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                st.o[d][e] *= f;
-#pragma unroll
-                for (int i = 0; i < 3; i++) st.o[d][e] += sums[((i * H::DB + d) * 16 + e) * 64];
+            for (int i = 0; i < 2; i++) {
+                const int d = u >> 1, e = 8 * (u & 1) + 4 * i;
+                ((float4_t *)(mine + 256 + u * 2048 + i * 1024))[lane] = float4_t{st.o[d][e], st.o[d][e + 1], st.o[d][e + 2], st.o[d][e + 3]};
             }
     }
-    if (wave > 0) return;
-    if (p.parts == 1) {
-        store_row<BF16, H>(p, st, sum, b, hk, row, lane);
-        return;
+    __syncthreads();
+    float top = -__builtin_huge_valf(), sum = 0.f, f[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, ((float *)(lds + i * AREA))[col]);
+    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f[i] = __builtin_amdgcn_exp2f(((float *)(lds + i * AREA))[col] - ref);
+        sum += ((float *)(lds + i * AREA))[32 + col] * f[i];
     }
-    if (row >= p.rows) return;
+    const float r = inverse(sum);
+    char *out = row_of(p, b, hk, row);
     const long long heads = (long long)p.B * p.Hkv, at = ((long long)part * heads + (long long)b * p.Hkv + hk) * p.rows + row;
-    float *dst = p.partial + at * p.D;
+    const int columns = row < p.rows ? p.D : 0;
+    for (int u = wave; u < UNITS; u += 4) {
+        float x[8];
 #pragma unroll
-    for (int d = 0; d < H::DB; d++)
+        for (int i = 0; i < 2; i++) {
+            float4_t y = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int c = 32 * d + 8 * g + 4 * h;
-            if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+            for (int w = 0; w < 4; w++) {
+                const float4_t o = ((float4_t *)(lds + w * AREA + 256 + u * 2048 + i * 1024))[lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(o[e], f[w], y[e]);
+            }
+            const int c = 16 * u + 8 * i + 4 * h;
+            if (p.parts > 1 && c < columns) *(float4_t *)(p.partial + at * p.D + c) = y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * i + e] = y[e];
         }
-    if (h == 0) {
+        if (p.parts == 1) store_columns<BF16>(out, x, r, 16 * u, columns, lane);
+    }
+    if (p.parts > 1 && wave == 0 && h == 0 && row < p.rows) {
         float *ms = p.partial + (long long)p.parts * heads * p.rows * p.D + at * 2;
         ms[0] = top;
         ms[1] = sum;
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) 
         x += sums[i][0][lane];
         y += sums[i][1][lane];
     }
-    const float r = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
+    const float r = inverse(sum);
     const int bh = (int)(at / p.rows), row = (int)(at - (long long)bh * p.rows), b = bh / p.Hkv, hk = bh - b * p.Hkv, t = row / p.G, g = row - t * p.G;
     *(uint32_t *)(p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + g) * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
 }
@@ -684,7 +691,6 @@ template <bool BF16, int DP, bool MASK>
 int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
     using H = Head<DP, true>;
     const int lds = keys ? 8 * H::TILE : 4 * Head<DP>::TILE;
-    static_assert(1024 + 3 * H::DB * 4096 <= 8 * H::TILE, "the waves' sums take the place of the stages");
     static bool reserved[2][64] = {{false}};
     const void *kernel = keys ? (const void *)attention_keys_kernel<BF16, DP, MASK> : (const void *)attention_rows_kernel<BF16, DP, MASK>;
     if (int rc = reserve_lds(kernel, lds, reserved[keys], "cross_attention")) return rc;
@@ -718,17 +724,26 @@ struct Plan {
 };
 Plan plan_of(const svdq_cross_attention_args *a, int cus) {
     const long long rows = a->q_len * (a->heads / a->kv_heads), bh = a->batch * a->kv_heads;
-    const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len, steps = (keys_each + KEYS - 1) / KEYS;
+    const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
     Plan plan;
     plan.keys = rows <= 32 || (rows + 127) / 128 * bh < cus;
     plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
     plan.parts = 1;
     if (plan.keys) {
-        // one round of workgroups: two to a compute unit with heads up to 64, one with wider ones (LDS), and at least a step per wave
-        const long long slots = (a->head_dim <= 64 ? 2 : 1) * cus, want = slots / (plan.row_blocks * bh), most = (2 * steps + 3) / 4;
-        plan.parts = want < most ? want : most;
-        if (plan.parts < 1) plan.parts = 1;
-        if (plan.parts > MAX_PARTS) plan.parts = MAX_PARTS;
+        // At most one workgroup to a compute unit: two (heads up to 64 leave room for them) were no faster alone (8 x 8 key heads of 64, 2048 keys 13.0 us
+        // in four parts, 13.6 in eight) and slower where the batch fills the machine (32 x 8 key heads, 2048 keys 25.7 in one part, 29.2 in two).
+        // A round of the four waves' 32 keys takes 0.8 us (heads above 64: 1.4), the join 3.1: single tokens, 8 key heads of 128, in one part / in as
+        // many as there are steps for the waves: 333 keys 9.1 / 9.3, 512 10.5 / 9.5, 4096 49 / 9.9; heads of 64: 512 7.0 / 7.7, 800 9.4 / 8.4.
+        const long long most = cus / (plan.row_blocks * bh), waves_steps = (keys_each + 31) / 32;
+        const float round = a->head_dim <= 64 ? 0.8f : 1.4f;
+        float best = (float)((waves_steps + 3) / 4) * round;
+        for (long long parts = 2; parts <= most && parts <= MAX_PARTS; parts++) {
+            const float t = (float)((waves_steps + 4 * parts - 1) / (4 * parts)) * round + 3.1f;
+            if (t < best) {
+                best = t;
+                plan.parts = parts;
+            }
+        }
     }
     plan.workspace = plan.parts > 1 ? plan.parts * bh * rows * (a->head_dim + 2) * 4 : 0;
     return plan;
