@@ -716,8 +716,7 @@ int launch_heads(const AttentionParams &p, bool keys, hipStream_t st) {
     return launch_kernels<BF16, 128, MASK>(p, keys, st);
 }
 
-// Which form a call takes and how many parts it divides the keys into.  The rows form reads K and V from memory once per 128 rows; it
-// wants enough of such blocks to fill the compute units.
+// Which form a call takes and how many parts it divides the keys into.
 struct Plan {
     bool keys;
     long long row_blocks, parts, workspace;
@@ -726,7 +725,10 @@ Plan plan_of(const svdq_cross_attention_args *a, int cus) {
     const long long rows = a->q_len * (a->heads / a->kv_heads), bh = a->batch * a->kv_heads;
     const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
     Plan plan;
-    plan.keys = rows <= 32 || (rows + 127) / 128 * bh < cus;
+    // The keys form where its blocks of 32 rows take their places all at once (two to a compute unit with heads up to 64, one with wider ones: LDS) and
+    // there are more keys than two steps of the rows form.  24 heads of 72, 1024 queries, 333 keys (768 blocks): 25.0 us, rows form 11.9; 64 heads of 128, 130
+    // queries, 1024 keys (320) 32.7, 24.4; of 64 (320) 13.6, 18.0; 24 heads of 128, 300 queries, 1024 keys (240) 17.8, 23.4; 8 heads of 72, 200 queries, 77 keys 6.4, 5.9.
+    plan.keys = rows <= 32 || (keys_each > 2 * KEYS && (rows + 31) / 32 * bh <= (a->head_dim <= 64 ? 2 : 1) * cus);
     plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
     plan.parts = 1;
     if (plan.keys) {
