@@ -5,7 +5,7 @@
 // g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32.  |code| <= 127 needs no clamp:
 // |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
 // scale NaN and codes 0: what a product makes of it is NaN.
-// Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 69 us, 5.8 TB/s;
+// Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 62 us, 6.5 TB/s;
 // 9216 x 5120 with residual 54 us, 6.1 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
 #include "svdq_common.h"
 
@@ -22,7 +22,24 @@ struct QuantizeParams {
     long long M, ld_x, ld_residual, ld_residual_out, ld_codes;  // bytes
     int pieces;                                                 // of 8 elements per row
     float inv_k, eps;
+    int once;  // the tensors do not fit the memory-side cache: what is read is not kept there
 };
+
+// This thread's pieces of a row; zeros behind its end
+template <int THREADS, int VECS>
+__device__ inline void load_row(u32x4_t (&w)[VECS], const char *row, const QuantizeParams &p, int t) {
+#pragma unroll
+    for (int i = 0; i < VECS; i++) w[i] = u32x4_t{0, 0, 0, 0};
+    if (p.once) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+            if (t + i * THREADS < p.pieces) w[i] = __builtin_nontemporal_load((const u32x4_t *)(row + (size_t)(t + i * THREADS) * 16));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+            if (t + i * THREADS < p.pieces) w[i] = *(const u32x4_t *)(row + (size_t)(t + i * THREADS) * 16);
+    }
+}
 
 template <bool BF16>
 __device__ inline void unpack(const u32x4_t w, float (&f)[8]) {
@@ -52,23 +69,9 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_k
     const int t = threadIdx.x % THREADS;
     const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
     if (row >= p.M) return;  // (all threads of a row; rows of several waves are one per workgroup)
-    const char *x = p.x + row * p.ld_x;
     u32x4_t w[VECS], r[RESIDUAL ? VECS : 1];
-#pragma unroll
-    for (int i = 0; i < VECS; i++) {
-        const int piece = t + i * THREADS;
-        w[i] = u32x4_t{0, 0, 0, 0};
-        if (piece < p.pieces) w[i] = *(const u32x4_t *)(x + (size_t)piece * 16);
-    }
-    if constexpr (RESIDUAL) {
-        const char *res = p.residual + row * p.ld_residual;
-#pragma unroll
-        for (int i = 0; i < VECS; i++) {
-            const int piece = t + i * THREADS;
-            r[i] = u32x4_t{0, 0, 0, 0};
-            if (piece < p.pieces) r[i] = *(const u32x4_t *)(res + (size_t)piece * 16);
-        }
-    }
+    load_row<THREADS, VECS>(w, p.x + row * p.ld_x, p, t);
+    if constexpr (RESIDUAL) load_row<THREADS, VECS>(r, p.residual + row * p.ld_residual, p, t);
     uint32_t top = 0;
     float squares = 0.f;
     u32x4_t nw[NORM ? VECS : 1];
@@ -224,6 +227,10 @@ int quantize_rows(const svdq_quantize_w8a8_args *a, bool norm, void *stream, con
     p.pieces = (int)(a->K / 8);
     p.inv_k = 1.0f / (float)a->K;
     p.eps = a->eps;
+    // Read past the memory-side cache (256 MB) what would not stay there anyway: 16384 x 8192 71 -> 62 us, 9216 x 5120 with residual 57.5 -> 54; where the
+    // tensors fit, or nearly, those that another kernel has left there would be fetched again: 16384 x 5600 (275 MB) 45.9 -> 47.3, 9216 x 4096 18.9 -> 20.9,
+    // 4608 x 4096 with residual 21.4 -> 24.0
+    p.once = a->M * a->K * (a->residual ? 7 : 3) > 300000000;
     // a launch takes fewer than 2^32 threads: 2^31 for so many rows of at most 64 threads, of at most 1024
     const long long most = p.pieces <= 128 ? 1ll << 25 : 1ll << 21;
     for (long long first = 0; first < a->M; first += most) {
