@@ -302,6 +302,17 @@ __device__ inline char *row_of(const AttentionParams &p, int b, int hk, int row)
     return p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
 }
 
+// With the keys in parts: where a part's share of a row goes, [part][b][hkv][row] x D, and its maximum and sum behind all of those
+__device__ inline long long part_index(const AttentionParams &p, int part, int b, int hk, int row) {
+    return (((long long)part * p.B + b) * p.Hkv + hk) * p.rows + row;
+}
+__device__ inline float *part_of(const AttentionParams &p, int part, int b, int hk, int row) { return p.partial + part_index(p, part, b, hk, row) * p.D; }
+__device__ inline void store_stats(const AttentionParams &p, int part, int b, int hk, int row, float top, float sum) {
+    float *ms = p.partial + (long long)p.parts * p.B * p.Hkv * p.rows * p.D + part_index(p, part, b, hk, row) * 2;
+    ms[0] = top;
+    ms[1] = sum;
+}
+
 // Which (row block, group) a workgroup takes, false: none.  A group's row blocks read the same keys (of a head, or of a part of its keys).
 // Workgroups go round robin over 8 XCDs, each with an L2 of its own.  The row blocks of a group go to one XCD, the groups in turn over
 // the XCDs (`spread`: a batch entry's keys may be many or few, and eight entries on an XCD each would leave some of them idle), or, where
@@ -430,8 +441,8 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     int rb, group;
-    if (!block_of(p, p.Hkv * p.B, rb, group)) return;
-    const int hk = group % p.Hkv, b = group / p.Hkv;
+    if (!block_of(p, p.Hkv * p.B * p.parts, rb, group)) return;
+    const int part = group % p.parts, hk = group / p.parts % p.Hkv, b = group / p.parts / p.Hkv;
     long long first;
     int count;
     keys_of(p, b, first, count);
@@ -442,7 +453,8 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     st.clear();
     Copies<H, 4> copies(p, lds, b, hk, first, count, wave, lane);
     Steps<MASK> list;
-    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, 0, (count + KEYS - 1) / KEYS, 1, lane);
+    const int steps = (count + KEYS - 1) / KEYS;
+    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, (int)((long long)steps * part / p.parts), (int)((long long)steps * (part + 1) / p.parts), 1, lane);
     int step = list.next();
     uint64_t bits = list.bits;
     if (step >= 0) {
@@ -490,7 +502,21 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
         step = next;
         bits = list.bits;
     }
-    const float r = inverse(across_sum(st.sum));
+    const float sum = across_sum(st.sum);
+    if (p.parts > 1) {
+        if (row >= p.rows) return;
+        float *dst = part_of(p, part, b, hk, row);
+#pragma unroll
+        for (int d = 0; d < H::DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int c = 32 * d + 8 * g + 4 * h;
+                if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+            }
+        if (h == 0) store_stats(p, part, b, hk, row, st.top, sum);
+        return;
+    }
+    const float r = inverse(sum);
     char *out = row_of(p, b, hk, row);
 #pragma unroll
     for (int u = 0; u < 2 * H::DB; u++) {
@@ -609,7 +635,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     }
     const float r = inverse(sum);
     char *out = row_of(p, b, hk, row);
-    const long long heads = (long long)p.B * p.Hkv, at = ((long long)part * heads + (long long)b * p.Hkv + hk) * p.rows + row;
+    float *dst = part_of(p, part, b, hk, row);
     const int columns = row < p.rows ? p.D : 0;
     for (int u = wave; u < UNITS; u += 4) {
         float x[8];
@@ -623,35 +649,33 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
                 for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(o[e], f[w], y[e]);
             }
             const int c = 16 * u + 8 * i + 4 * h;
-            if (p.parts > 1 && c < columns) *(float4_t *)(p.partial + at * p.D + c) = y;
+            if (p.parts > 1 && c < columns) *(float4_t *)(dst + c) = y;
 #pragma unroll
             for (int e = 0; e < 4; e++) x[4 * i + e] = y[e];
         }
         if (p.parts == 1) store_columns<BF16>(out, x, r, 16 * u, columns, lane);
     }
-    if (p.parts > 1 && wave == 0 && h == 0 && row < p.rows) {
-        float *ms = p.partial + (long long)p.parts * heads * p.rows * p.D + at * 2;
-        ms[0] = top;
-        ms[1] = sum;
-    }
+    if (p.parts > 1 && wave == 0 && h == 0 && row < p.rows) store_stats(p, part, b, hk, row, top, sum);
 }
 
-// Adds the parts of every row (at most 64): one workgroup per row, two columns per lane, whose waves take every fourth part, all requested
-// at once.  Lane i of every wave holds part i's share of the row.
+// Adds the parts of every row (at most 64): four waves a workgroup, PER of them to a row, two columns per lane; a wave takes every PER-th part, all
+// requested at once.  Lane i of every wave holds part i's share of the row.
 constexpr int MAX_PARTS = 64;
-template <bool BF16>
+template <bool BF16, int PER>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) {
-    __shared__ float sums[4][2][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long all = (long long)p.B * p.Hkv * p.rows, at = blockIdx.x;
+    constexpr int MOST = 16;  // parts a wave
+    __shared__ float sums[PER == 1 ? 1 : 4][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = wave % PER;
+    const long long all = (long long)p.B * p.Hkv * p.rows, at = (long long)blockIdx.x * (4 / PER) + wave / PER;
+    if (PER == 1 && at >= all) return;
     const float *ms = p.partial + p.parts * all * p.D;
     const int c = lane * 2 < p.D ? lane * 2 : 0;
     typedef float float2_t __attribute__((ext_vector_type(2)));
-    float2_t part[MAX_PARTS / 4];
+    float2_t part[MOST];
 #pragma unroll
-    for (int i = 0; i < MAX_PARTS / 4; i++) {
+    for (int i = 0; i < MOST; i++) {
         part[i] = float2_t{0.f, 0.f};
-        if (wave + 4 * i < p.parts) part[i] = *(const float2_t *)(p.partial + ((wave + 4 * i) * all + at) * p.D + c);
+        if (sub + PER * i < p.parts) part[i] = *(const float2_t *)(p.partial + ((sub + PER * i) * all + at) * p.D + c);
     }
     float top = -__builtin_huge_valf(), sum = 0.f;
     if (lane < p.parts) {
@@ -668,24 +692,26 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionParams p) 
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     float x = 0.f, y = 0.f;
 #pragma unroll
-    for (int i = 0; i < MAX_PARTS / 4; i++) {
-        if (wave + 4 * i >= p.parts) break;
-        const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), wave + 4 * i));
+    for (int i = 0; i < MOST; i++) {  // (zero times zero behind the last part)
+        const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), sub + PER * i));
         x = __builtin_fmaf(part[i][0], g, x);
         y = __builtin_fmaf(part[i][1], g, y);
     }
-    sums[wave][0][lane] = x;
-    sums[wave][1][lane] = y;
-    __syncthreads();
-    if (wave > 0 || lane * 2 >= p.D) return;
+    if constexpr (PER > 1) {
+        sums[wave][0][lane] = x;
+        sums[wave][1][lane] = y;
+        __syncthreads();
+        if (wave > 0) return;
 #pragma unroll
-    for (int i = 1; i < 4; i++) {
-        x += sums[i][0][lane];
-        y += sums[i][1][lane];
+        for (int i = 1; i < 4; i++) {
+            x += sums[i][0][lane];
+            y += sums[i][1][lane];
+        }
     }
+    if (lane * 2 >= p.D) return;
     const float r = inverse(sum);
-    const int bh = (int)(at / p.rows), row = (int)(at - (long long)bh * p.rows), b = bh / p.Hkv, hk = bh - b * p.Hkv, t = row / p.G, g = row - t * p.G;
-    *(uint32_t *)(p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + g) * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
+    const int bh = (int)(at / p.rows), row = (int)(at - (long long)bh * p.rows), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+    *(uint32_t *)(row_of(p, b, hk, row) + c * 2) = Elem<BF16>::pair(x * r, y * r);
 }
 
 template <bool BF16, int DP, bool MASK>
@@ -697,14 +723,13 @@ int launch_kernels(const AttentionParams &p, bool keys, hipStream_t st) {
     if (int rc = reserve_lds(kernel, lds, reserved[keys], "cross_attention")) return rc;
     const long long groups = (long long)p.parts * p.Hkv * p.B;
     const dim3 grid((unsigned)((p.spread ? (groups + 7) / 8 * 8 : groups) * p.row_blocks)), block(256);
-    if (!keys) {
-        SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
-        return check_launch("cross_attention");
-    }
-    SVDQ_LAUNCH((attention_keys_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
+    if (keys) SVDQ_LAUNCH((attention_keys_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
+    else SVDQ_LAUNCH((attention_rows_kernel<BF16, DP, MASK>), grid, block, lds, st, p);
     int rc = check_launch("cross_attention");
     if (rc || p.parts == 1) return rc;
-    SVDQ_LAUNCH((attention_join_kernel<BF16>), dim3((unsigned)((long long)p.B * p.Hkv * p.rows)), dim3(256), 0, st, p);
+    const long long all = (long long)p.B * p.Hkv * p.rows;
+    if (p.parts <= 16) SVDQ_LAUNCH((attention_join_kernel<BF16, 1>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
+    else SVDQ_LAUNCH((attention_join_kernel<BF16, 4>), dim3((unsigned)all), dim3(256), 0, st, p);
     return check_launch("cross_attention");
 }
 
@@ -717,37 +742,51 @@ int launch_heads(const AttentionParams &p, bool keys, hipStream_t st) {
     return launch_kernels<BF16, 128, MASK>(p, keys, st);
 }
 
-// Which form a call takes and how many parts it divides the keys into.
+// Which form a call takes and how many parts it divides the keys into: the least time by a model of the busiest compute unit, us, whose constants are those
+// of 192 shapes in both forms; of 240 shapes in both forms and 1 .. 32 parts what it chooses is 0.6 % behind the fastest on average, 15 % at most.  The rows form reads K and
+// V once per 128 rows, the keys form has its waves side by side on one 32; parts of the keys fill the compute units and cost a join.  Chosen / the other form or no
+// parts, us: 24 heads of 72, 1024 queries, 333 keys (768 blocks of 32) rows 11.9 / 25.0; 64 heads of 64, 130 queries, 1024 keys keys 13.6 / 18.0; 8 heads of 128, 512
+// queries, 4096 keys rows in eight parts 26.6 / keys in two 34.6, rows whole 78; single tokens, 8 key heads of 128: 333 keys 9.1 / 9.3 in three, 512 9.5 in four / 10.5, 4096
+// 9.9 in 32 / 49; 32 x 8 key heads of 64, 2048 keys 25.7 / 29.2 in two.
 struct Plan {
     bool keys;
     long long row_blocks, parts, workspace;
 };
+struct Cost {
+    int head_dim;                    // up to
+    float rows_base, alone, share;   // rows form: launch, first and last; a step of 64 keys of a workgroup by itself, of each of several
+    float keys_base, round;          // keys form: the same; a round of four waves' 32 keys
+};
+constexpr Cost costs[] = {{64, 3.7f, 0.84f, 0.63f, 4.3f, 0.8f}, {96, 3.9f, 1.03f, 0.85f, 5.0f, 1.3f}, {128, 5.2f, 1.12f, 1.08f, 5.4f, 1.4f}};
+
 Plan plan_of(const svdq_cross_attention_args *a, int cus) {
     const long long rows = a->q_len * (a->heads / a->kv_heads), bh = a->batch * a->kv_heads;
     const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
-    Plan plan;
-    // The keys form where its blocks of 32 rows take their places all at once (two to a compute unit with heads up to 64, one with wider ones: LDS) and
-    // there are more keys than two steps of the rows form.  24 heads of 72, 1024 queries, 333 keys (768 blocks): 25.0 us, rows form 11.9; 64 heads of 128, 130
-    // queries, 1024 keys (320) 32.7, 24.4; of 64 (320) 13.6, 18.0; 24 heads of 128, 300 queries, 1024 keys (240) 17.8, 23.4; 8 heads of 72, 200 queries, 77 keys 6.4, 5.9.
-    plan.keys = rows <= 32 || (keys_each > 2 * KEYS && (rows + 31) / 32 * bh <= (a->head_dim <= 64 ? 2 : 1) * cus);
-    plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
-    plan.parts = 1;
-    if (plan.keys) {
-        // At most one workgroup to a compute unit: two (heads up to 64 leave room for them) were no faster alone (8 x 8 key heads of 64, 2048 keys 13.0 us
-        // in four parts, 13.6 in eight) and slower where the batch fills the machine (32 x 8 key heads, 2048 keys 25.7 in one part, 29.2 in two).
-        // A round of the four waves' 32 keys takes 0.8 us (heads above 64: 1.4), the join 3.1: single tokens, 8 key heads of 128, in one part / in as
-        // many as there are steps for the waves: 333 keys 9.1 / 9.3, 512 10.5 / 9.5, 4096 49 / 9.9; heads of 64: 512 7.0 / 7.7, 800 9.4 / 8.4.
-        const long long most = cus / (plan.row_blocks * bh), waves_steps = (keys_each + 31) / 32;
-        const float round = a->head_dim <= 64 ? 0.8f : 1.4f;
-        float best = (float)((waves_steps + 3) / 4) * round;
-        for (long long parts = 2; parts <= most && parts <= MAX_PARTS; parts++) {
-            const float t = (float)((waves_steps + 4 * parts - 1) / (4 * parts)) * round + 3.1f;
-            if (t < best) {
+    const long long blocks[2] = {(rows + 127) / 128 * bh, (rows + 31) / 32 * bh}, steps[2] = {(keys_each + KEYS - 1) / KEYS, (keys_each + 31) / 32};
+    const Cost &c = a->head_dim <= 64 ? costs[0] : a->head_dim <= 96 ? costs[1] : costs[2];
+    Plan plan = {true, 1, 1, 0};
+    float best = 0.f;
+    for (int keys = rows <= 32; keys < 2; keys++) {
+        for (long long parts = 1; parts <= MAX_PARTS; parts++) {
+            if (parts > 1 && (blocks[keys] * parts > (keys ? 1 : 2) * cus || steps[keys] < (keys ? 4 : 1) * (parts - 1))) break;
+            float t;
+            if (keys) {
+                // two workgroups to a compute unit with heads up to 64, one with wider ones (LDS)
+                const long long rounds = (steps[1] + 4 * parts - 1) / (4 * parts), slots = a->head_dim <= 64 ? 2 * cus : cus;
+                t = (c.keys_base + (float)rounds * c.round * (blocks[1] * parts > cus && a->head_dim <= 64 ? 1.3f : 1.f)) * (float)((blocks[1] * parts + slots - 1) / slots);
+            } else {
+                const float each = (float)((blocks[0] * parts + cus - 1) / cus) * c.share;
+                t = c.rows_base + (float)((steps[0] + parts - 1) / parts) * (each > c.alone ? each : c.alone);
+            }
+            if (parts > 1) t += 3.1f + (float)(bh * rows) * (float)(a->head_dim * 8 * parts) / 4.0e6f;  // the join, and the parts' way there and back
+            if (best == 0.f || t < best) {
                 best = t;
+                plan.keys = keys;
                 plan.parts = parts;
             }
         }
     }
+    plan.row_blocks = plan.keys ? (rows + 31) / 32 : (rows + 127) / 128;
     plan.workspace = plan.parts > 1 ? plan.parts * bh * rows * (a->head_dim + 2) * 4 : 0;
     return plan;
 }

@@ -79,7 +79,9 @@ def test_all_keys(dev, shape, dtype):
 
 
 VALID_SHAPES = [(4, 1, 200, 4, 2, 128), (5, 3, 700, 2, 2, 72), (4, 260, 150, 16, 16, 64), (6, 257, 333, 12, 12, 80), (3, 40, 129, 4, 1, 32), (8, 1030, 70, 4, 4, 128),
-                (8, 2030, 260, 4, 4, 128), (4, 4090, 150, 4, 4, 72), (3, 8000, 193, 3, 3, 24)]
+                (8, 2030, 260, 4, 4, 128), (4, 4090, 150, 4, 4, 72), (3, 8000, 193, 3, 3, 24),
+                # blocks of 128 rows with the keys in parts
+                (3, 70, 1100, 4, 2, 72), (4, 45, 2000, 3, 1, 80), (4, 100, 1100, 6, 6, 128), (4, 33, 5000, 2, 2, 120), (3, 120, 2500, 5, 5, 56)]
 
 
 def spoil(t, keep):
@@ -255,6 +257,38 @@ def test_streams_and_graphs(dev):
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+def test_rows_in_parts_on_streams_and_in_graphs(dev):
+    """As above, with blocks of 128 rows; lengths change between the replays."""
+    from nunchaku_amd.ops import cross_attention
+
+    announce("rows in parts, graphs")
+    sets = [[t.to(dev) for t in inputs(2, 100 + i, 2000 + 700 * i, 4, 2, 128, torch.float16, i)] for i in range(2)]
+    lengths = [torch.tensor([n, 77], dtype=torch.int32, device=dev) for n in (2000, 1500)]
+    graphs, outs = [], []
+    for s, n in zip(sets, lengths):
+        cross_attention(*s, key_lengths=n)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(cross_attention(*s, key_lengths=n))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for turn in range(4):
+        for n in lengths:
+            n[1] += 311 * turn
+            n[0] //= 2
+        eager = [cross_attention(*s, key_lengths=n) for s, n in zip(sets, lengths)]
+        for g in graphs if turn % 2 else graphs[::-1]:
+            g.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            beside = [cross_attention(*s, key_lengths=n) for s, n in zip(sets, lengths)]
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(outs, eager, beside))
+    for i, (s, n) in enumerate(zip(sets, lengths)):
+        check(outs[i], *[t.cpu() for t in s], torch.arange(s[1].shape[1]) < n.cpu()[:, None])
 
 
 def test_same_from_run_to_run(dev):
