@@ -302,7 +302,20 @@ __device__ inline char *row_of(const AttentionParams &p, int b, int hk, int row)
     return p.out + b * p.os[0] + t * p.os[1] + (long long)(hk * p.G + gq) * p.os[2];
 }
 
-// With the keys in parts: where a part's share of a row goes, [part][b][hkv][row] x D, and its maximum and sum behind all of those
+// With the keys in parts: which one a workgroup has (taken out of its group), and its share of the steps 0 .. end
+__device__ inline int take_part(const AttentionParams &p, int &group) {
+    if (p.parts == 1) return 0;
+    const int whole = group / p.parts, part = group - whole * p.parts;
+    group = whole;
+    return part;
+}
+__device__ inline void share(const AttentionParams &p, int part, int &begin, int &end) {
+    if (p.parts == 1) return;
+    const int each = end / p.parts, more = end - each * p.parts;
+    begin = part * each + (part < more ? part : more);
+    end = begin + each + (part < more);
+}
+// Where a part's share of a row goes, [part][b][hkv][row] x D, and its maximum and sum behind all of those
 __device__ inline long long part_index(const AttentionParams &p, int part, int b, int hk, int row) {
     return (((long long)part * p.B + b) * p.Hkv + hk) * p.rows + row;
 }
@@ -442,7 +455,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     int rb, group;
     if (!block_of(p, p.Hkv * p.B * p.parts, rb, group)) return;
-    const int part = group % p.parts, hk = group / p.parts % p.Hkv, b = group / p.parts / p.Hkv;
+    const int part = take_part(p, group), hk = group % p.Hkv, b = group / p.Hkv;
     long long first;
     int count;
     keys_of(p, b, first, count);
@@ -453,8 +466,9 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     st.clear();
     Copies<H, 4> copies(p, lds, b, hk, first, count, wave, lane);
     Steps<MASK> list;
-    const int steps = (count + KEYS - 1) / KEYS;
-    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, (int)((long long)steps * part / p.parts), (int)((long long)steps * (part + 1) / p.parts), 1, lane);
+    int begin = 0, end = (count + KEYS - 1) / KEYS;
+    share(p, part, begin, end);
+    list.start(MASK ? p.mask + b * p.mask_b : nullptr, count, begin, end, 1, lane);
     int step = list.next();
     uint64_t bits = list.bits;
     if (step >= 0) {
@@ -539,7 +553,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     int rb, group;
     if (!block_of(p, p.Hkv * p.B * p.parts, rb, group)) return;
-    const int part = group % p.parts, hk = group / p.parts % p.Hkv, b = group / p.parts / p.Hkv;
+    const int part = take_part(p, group), hk = group % p.Hkv, b = group / p.Hkv;
     long long first;
     int count;
     keys_of(p, b, first, count);
@@ -551,8 +565,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) attention_keys_kernel(A
     constexpr int SIZE = 32, REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
     char *mine = lds + wave * 2 * STAGE;
     const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 2 * STAGE;
-    const int steps = (count + SIZE - 1) / SIZE, bytes = p.D * 2;
-    const int begin = (int)((long long)steps * part / p.parts), end = (int)((long long)steps * (part + 1) / p.parts);
+    const int bytes = p.D * 2;
+    int begin = 0, end = (count + SIZE - 1) / SIZE;
+    share(p, part, begin, end);
     // Request i brings rows r0 + i * RPR: of V the same piece every time, of K the pieces that f has there
     const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
     const uint32_t ok = (uint32_t)(r0 * p.ks[1]), ov = (uint32_t)(r0 * p.vs[1]) + cv;
