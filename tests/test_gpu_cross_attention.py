@@ -416,3 +416,39 @@ def test_attention_on_the_outputs_of_the_fused_projection(dev):
     check(got, q[:, :T].cpu(), k[:, :T].cpu(), v[:, :T].cpu())
     # (not the same bits: into how many parts the keys are divided goes by the tensors' length)
     check(cross_attention(q[:, :T], k[:, :T], v[:, :T]), q[:, :T].cpu(), k[:, :T].cpu(), v[:, :T].cpu())
+
+
+def test_calls_from_several_threads(dev):
+    """Every thread on a stream of its own, products and keys in parts among them: the results of one thread alone."""
+    import threading
+
+    from nunchaku_amd.ops import cross_attention, gemm_w8a8, quantize_w8a8_act
+
+    announce("threads")
+
+    def work(i):
+        q, k, v = (t.to(dev) for t in inputs(2, 1 + 60 * (i % 2), 1500 + i, 4, 2, 64 + 8 * i, torch.bfloat16, i))
+        o = cross_attention(q, k, v)
+        codes, scales = quantize_w8a8_act(k[0].reshape(k.shape[1], -1))
+        return [o, codes, scales, gemm_w8a8(codes[:5 + 40 * (i % 2)], codes[:300], scales[:5 + 40 * (i % 2)], scales[:300])]
+
+    want = [work(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = work(i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 (reported below, in the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
