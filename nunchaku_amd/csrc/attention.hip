@@ -190,11 +190,13 @@ struct State {
         if constexpr (NB == 2) top = __builtin_fmaxf(top, __builtin_fmaxf(m[2], m[3]));
         return across_max(top);
     }
-    // A new maximum of a row (in units of log2).  The one in use only has to keep the exponentials in range: it moves when a row's is
-    // more than 2^8 times off, so that the outputs are rarely scaled.
-    __device__ inline void raise(float m) {
-        if (__any(m > top + 8.f)) {
-            const float now = m > top ? m : top;
+    // A new maximum of a row (of scores; times scale2, in units of log2).  The one in use only has to keep the exponentials in range: it moves when a
+    // row's is more than 2^8 times off, so that the outputs are rarely scaled.  How far off goes by the exponentials' own fma, rounded once: around
+    // 2^27 neighbours in fp32 are 8 to 16 apart, where a rounded maximum compared with a rounded sum let an fp16 probability of 2^16 through, an
+    // infinity.  The maximum in use is a rounded number, too, half such a distance off, so that fp16 is in range for scores below 2^28, bf16 2^31.
+    __device__ inline void raise(float high, float scale2) {
+        if (__any(__builtin_fmaf(high, scale2, -top) > 8.f)) {
+            const float m = high * scale2, now = m > top ? m : top;
             const float f = top == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(top - now);
             top = now;
             sum *= f;
@@ -238,7 +240,7 @@ struct State {
         vec vf[2][H::DB], pr[2];
         read_v(vf[0], v, 0, lane);
         mask(s, bits, lane);
-        raise(highest(s) * scale2);
+        raise(highest(s), scale2);
         const float ref = reference();
         pr[0] = exponentials<NB, ONES>(s, 0, scale2, ref);
         __builtin_amdgcn_sched_barrier(0);
