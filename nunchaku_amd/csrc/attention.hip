@@ -40,11 +40,16 @@ struct Elem<true> {
     static constexpr uint32_t ONE = 0x3F80;
     static __device__ inline float16_t mfma(vec a, vec b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ inline uint32_t pair(float lo, float hi) { return pack_bf16x2(lo, hi); }
+    static constexpr float RAISED = 0.f;  // as wide a range as fp32
 };
 template <>
 struct Elem<false> {
     typedef half8_t vec;
     static constexpr uint32_t ONE = 0x3C00;
+    // Probabilities stand 2^7 times higher than the maximum in use has them, which with the 2^8 that it may lag behind is 2^15 at most.  What a small one
+    // loses at the type's end, 2^-25, is then 2^-32 of the sum: one key e^17.5 times as likely as each of 65535 others leaves these 1.6e-3 of the result,
+    // all of which was lost without.
+    static constexpr float RAISED = 7.f;
     static __device__ inline float16_t mfma(vec a, vec b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ inline uint32_t pair(float lo, float hi) {
         typedef float float2_t __attribute__((ext_vector_type(2)));
@@ -154,7 +159,7 @@ struct State {
     using E = Elem<BF16>;
     using vec = typename E::vec;
     float16_t o[H::DB];
-    float top, sum;  // in units of log2; this lane's part of the sum
+    float top, sum;  // what the exponentials refer to, RAISED below the maximum in use, in units of log2; this lane's part of the sum
     __device__ inline void clear() {
 #pragma unroll
         for (int d = 0; d < H::DB; d++)
@@ -195,8 +200,8 @@ struct State {
     // 2^27 neighbours in fp32 are 8 to 16 apart, where a rounded maximum compared with a rounded sum let an fp16 probability of 2^16 through, an
     // infinity.  The maximum in use is a rounded number, too, half such a distance off, so that fp16 is in range for scores below 2^28, bf16 2^31.
     __device__ inline void raise(float high, float scale2) {
-        if (__any(__builtin_fmaf(high, scale2, -top) > 8.f)) {
-            const float m = high * scale2, now = m > top ? m : top;
+        if (__any(__builtin_fmaf(high, scale2, -top) > E::RAISED + 8.f)) {
+            const float m = high * scale2 - E::RAISED, now = m > top ? m : top;
             const float f = top == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(top - now);
             top = now;
             sum *= f;
