@@ -2,8 +2,8 @@
 //   plain: g = x;   norm: h = T(x + residual) (the stored residual stream; h = x without one), g = h * weight
 //   a = max(max_k |g|, 2^-100), code = rne(g * fl32(127 / a)), scale = fl32(a * f / 127), f = 1 or 1 / sqrt(mean(h^2) + eps).
 // The factor 1 / rms of a row is the same for all its elements, so it cancels in the codes: they depend on max |g| alone, and
-// g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32.  |code| <= 127 needs no clamp:
-// |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
+// g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32, of h * 2^100 where squares would end below fp32's
+// smallest numbers and eps does not make up for them.  |code| <= 127 needs no clamp: |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
 // scale NaN and codes 0: what a product makes of it is NaN.
 // Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 62 us, 6.5 TB/s;
 // 9216 x 5120 with residual 54 us, 6.1 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
@@ -14,6 +14,7 @@ using namespace svdq;
 namespace {
 
 constexpr float MIN_AMAX = 0x1p-100f;
+constexpr float TINY_SQUARES = 0x1p-100f;  // fp32 rounds a square by 2^-150 at most, 65536 of them by 2^-134: from here on 2^-34 of the sum
 
 struct QuantizeParams {
     const char *x, *residual, *weight;
@@ -62,9 +63,10 @@ __device__ inline uint32_t pack_pair(float lo, float hi) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
 }
 
-// THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements
+// THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements.  A norm without a residual of 1024 threads with four
+// pieces fits two workgroups to a compute unit with 64 registers, which the compiler has to be told (2048 x 20000 31.3 -> 23.5 us).
 template <bool BF16, int THREADS, int VECS, bool NORM, bool RESIDUAL>
-__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_kernel(QuantizeParams p) {
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS, THREADS == 1024 && VECS == 4 && NORM && !RESIDUAL ? 8 : THREADS < 256 ? 1 : THREADS / 256) quantize_rows_kernel(QuantizeParams p) {
     constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, WAVES = THREADS <= 64 ? 1 : THREADS / 64;
     const int t = threadIdx.x % THREADS;
     const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
@@ -162,6 +164,32 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) quantize_rows_k
 #pragma unroll
         for (int j = 0; j < 2; j++) c[j] = bad ? 0u : b[4 * j] | b[4 * j + 1] << 8 | b[4 * j + 2] << 16 | b[4 * j + 3] << 24;
         if (piece < p.pieces) *(u32x2_t *)(out + (size_t)piece * 8) = c;
+    }
+    if constexpr (NORM && BF16) {  // (the smallest square in fp16 is 2^-48)
+        if (!(p.eps < TINY_SQUARES && squares < TINY_SQUARES)) return;  // (the same in all threads of a row)
+        // The squares once more, in units of 2^-200: from 2^-66 on (|h| < 2^-50, in units of 2^-100), sums up to 2^100.  h is read again, this thread's own
+        // pieces, and behind the codes: with the row in registers for it the longest ones spilled.
+        const char *h = RESIDUAL ? p.residual_out + row * p.ld_residual_out : p.x + row * p.ld_x;
+        squares = 0.f;
+#pragma unroll 1
+        for (int piece = t; piece < p.pieces; piece += THREADS) {
+            float f[8];
+            unpack<BF16>(*(const u32x4_t *)(h + (size_t)piece * 16), f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) squares = __builtin_fmaf(f[j] * 0x1p100f, f[j] * 0x1p100f, squares);
+        }
+#pragma unroll
+        for (int d = THREADS < 64 ? THREADS / 2 : 32; d; d >>= 1) squares += __shfl_xor(squares, d);
+        if constexpr (WAVES > 1) {
+            __shared__ float sums[WAVES];
+            if ((t & 63) == 0) sums[t >> 6] = squares;
+            __syncthreads();
+            squares = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) squares += sums[i];
+        }
+        // amax is below 2^78 with the largest weight, the root of the mean between 2^-41 and 2^50 (or zero): neither factor leaves fp32
+        if (t == 0 && !bad) p.scales[row] = (amax * 0x1p40f) * (0x1p60f / __builtin_sqrtf(squares * p.inv_k + p.eps * 0x1p100f * 0x1p100f)) / 127.0f;
     }
 }
 
