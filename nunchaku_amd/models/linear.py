@@ -361,8 +361,8 @@ class W8A8Linear(nn.Module):
         super()._apply(fn, recurse)
         if self.wscales.dtype != torch.float32:
             self.wscales.data = scales.to(self.wscales.device)
-        if self.bias is not None:
-            self.torch_dtype = self.bias.dtype
+        # the layer's type goes the way of its bias, or of what a bias would have been
+        self.torch_dtype = fn(torch.empty(1, dtype=self.torch_dtype, device=self.wscales.device)).dtype if self.bias is None else self.bias.dtype
         return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
