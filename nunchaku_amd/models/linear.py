@@ -365,9 +365,25 @@ class W8A8Linear(nn.Module):
         self.torch_dtype = fn(torch.empty(1, dtype=self.torch_dtype, device=self.wscales.device)).dtype if self.bias is None else self.bias.dtype
         return self
 
+    @staticmethod
+    def _rows(x: torch.Tensor) -> torch.Tensor:
+        """``x``, or a copy where the operator does not take it as it stands: its rows are not at one distance (a slice along tokens, say),
+        or not 16 bytes apart and aligned."""
+        if x.is_contiguous() and x.data_ptr() % 16 == 0:
+            return x
+        if x.dim() > 0 and x.numel() > 0:
+            try:
+                rows = x.view(-1, x.shape[-1])
+            except RuntimeError:
+                return x.contiguous()
+            apart = rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
+            if rows.stride(1) != 1 or apart < rows.shape[1] or apart % 8 or x.data_ptr() % 16:
+                return x.clone(memory_format=torch.contiguous_format)
+        return x
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """x [..., K] -> [..., N]"""
-        return self.forward_quant(*quantize_w8a8_act(x), out_dtype=x.dtype)
+        """x [..., K] -> [..., N], whatever the strides of x"""
+        return self.forward_quant(*quantize_w8a8_act(self._rows(x)), out_dtype=x.dtype)
 
     def forward_quant(self, codes: torch.Tensor, scales: torch.Tensor, output: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """codes int8 [..., K] and scales fp32 [...] -> [..., N] of the layer's type"""
