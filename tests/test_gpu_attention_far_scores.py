@@ -47,3 +47,26 @@ def test_scores_around_1e8(dev, dtype, Tq, sign, descending):
         u = torch.finfo(dtype).eps / 2
         bound = 1.01 * want * (2 * u + 2 * (2 * U32 * 15 * 13 + 16 * U32 + 960 * U32)) + (2.0**-25 if dtype == torch.float16 else 2.0**-126) * (1 + 4 * 960)
         assert ((got - want).abs() <= bound).all(), (scale, (got - want).abs().max().item())
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("Tq", [1, 200])
+def test_bf16_scores_around_1e9(dev, Tq, sign):
+    """Up to 1.39e9 a reference is up to 64 off its score, which bf16's range holds: the 64 keys of the highest step share the result (the next
+    step is e^-32 of it and less), so each column of V is its value there, rounded: probabilities, sums, division and result as above."""
+    from nunchaku_amd.ops import cross_attention
+
+    B, H, D, each, steps = 1, 2, 64, 64, 9
+    first = 29952.0
+    j = torch.arange(steps).repeat_interleave(each)
+    k = torch.zeros(B, steps * each, H, D, dtype=torch.float64)
+    k[..., 0], k[..., 1] = sign * first, 8.0 * j[None, :, None]
+    q = torch.zeros(B, Tq, H, D, dtype=torch.float64)
+    q[..., 0], q[..., 1] = first, 8.0
+    v = (1.0 + j.double())[None, :, None, None].expand(B, -1, H, D)
+    on = [t.to(torch.bfloat16).to(dev) for t in (q, k, v)]
+    for scale in (0.51, 0.6, 0.77, 0.9, 1.1, 1.3, 1.49, 1.55):
+        announce(f"scores around 1e9 {Tq} {sign} {scale}")
+        got = cross_attention(*on, scale=scale).cpu().double()
+        bound = steps * (2 * 2.0**-8 + 64 * U32 + 2 * 576 * U32) * 1.01 + steps * math.exp(-32)
+        assert ((got - steps).abs() <= bound).all(), (scale, got.min().item(), got.max().item())
