@@ -312,7 +312,7 @@ typedef struct svdq_gemm_w8a8_args {
     const float *wscales;   /* fp32 [N]                                                              */
     const void *bias;       /* [N] of the type of out, or NULL                                       */
     void *out;              /* bf16 or fp16 [M, N], rows ld_out elements apart                       */
-    int64_t M, N, K;        /* K: a multiple of 16 below 131072; M and N: any                        */
+    int64_t M, N, K;        /* K: a multiple of 16 below 131072; M and N: fewer than 2^24 tiles of 32 x 64 */
     int64_t ld_act, ld_wgt, ld_out; /* ld_act, ld_wgt: multiples of 16 below 2^23                    */
     void *workspace;        /* svdq_gemm_w8a8_workspace bytes (16-byte aligned), not shared with a call that may run at the
                                same time; NULL if that is 0                                          */
@@ -330,6 +330,8 @@ int svdq_gemm_w8a8(const svdq_gemm_w8a8_args *args, void *stream);
  *   out[b][t][h] = sum_j p_j v[b][j][h / G],  p = softmax over the valid j of scale * q[b][t][h] . k[b][j][h / G],  G = heads / kv_heads.
  * A query without a valid key gets zeros.  Keys are valid up to key_lengths[b] or where key_mask[b] says so; what k and v hold in
  * other places (NaN, infinities) is not read into any result.  With cu_seqlens_k the sequences of keys stand one behind the other.
+ * Scores, maxima, exponentials and sums are fp32; the probabilities are rounded to dtype for their product with v.  Scores (with the scale) of
+ * magnitudes up to 1.8e8 (fp16) and 1.4e9 (bf16) are in range.
  * No global state: a call that divides the keys among workgroups puts its partial sums where the caller says.
  * ------------------------------------------------------------------------------------------ */
 typedef struct svdq_cross_attention_args {
@@ -346,7 +348,8 @@ typedef struct svdq_cross_attention_args {
     int64_t batch, heads, kv_heads, head_dim; /* head_dim: a multiple of 8 up to 128                 */
     int64_t q_len, k_len;
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head: elements, multiples of 8; elements
-                                                                     of a head are next to each other             */
+                                                                     of a head are next to each other; the tokens
+                                                                     of k and v less than 2^24 elements apart      */
     int64_t mask_stride;
     float scale;            /* positive                                                              */
     int32_t dtype;          /* of q, k, v, out: SVDQ_BF16 or SVDQ_FP16                               */

@@ -6,7 +6,7 @@
 // smallest numbers and eps does not make up for them.  |code| <= 127 needs no clamp: |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
 // scale NaN and codes 0: what a product makes of it is NaN.
 // Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 62 us, 6.5 TB/s;
-// 9216 x 5120 with residual 54 us, 6.1 TB/s; one row of 4096 2.4 and 2.7 us, launch and latencies.
+// 9216 x 5120 with residual 53 us, 6.2 TB/s; one row of 4096 2.4 and 2.8 us, launch and latencies.
 #include "svdq_common.h"
 
 using namespace svdq;

@@ -84,7 +84,9 @@ def rms_norm_quantize_w8a8(
     """RMS norm of ``x`` bf16 / fp16 [..., K], behind the residual's addition, to int8 codes with a scale for each token.
 
     h = ``x`` + ``residual``, rounded to the type (``x`` itself without a residual); y = h / sqrt(mean(h^2) + eps) * ``weight``, not
-    rounded; codes and scales of y as in ``quantize_w8a8_act``.  Returns (codes int8 [..., K], scales fp32 [...], h), h None without
+    rounded; codes and scales of y as in ``quantize_w8a8_act``, but for the smallest rows: with a = max(max |h * weight|, 2^-100) a code is
+    round(h * weight * (127 / a)) and the scale a / 127 / sqrt(mean(h^2) + eps).  A row whose sum of squares overflows fp32 gets the
+    scale NaN and codes 0, too.  Returns (codes int8 [..., K], scales fp32 [...], h), h None without
     a residual.  ``residual_out`` takes h when given; it may be ``residual`` or ``x`` itself (the stream is then updated in place)."""
     if output is None and oscales is None and residual_out is None:
         y = nv.host().w8a8_norm(x, weight, residual, eps)
