@@ -845,7 +845,8 @@ int check_args(const svdq_cross_attention_args *a) {
     SVDQ_REQUIRE(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, "cross_attention: head_dim (%lld) must be a multiple of 8 up to 128", (long long)a->head_dim);
     SVDQ_REQUIRE(a->q_len > 0 && a->k_len > 0 && a->k_len < (1ll << 31) - 64, "cross_attention: q_len (%lld) and k_len (%lld) must be positive, k_len below 2^31 - 64", (long long)a->q_len,
                  (long long)a->k_len);
-    SVDQ_REQUIRE(a->q_len < (1ll << 31) && a->q_len * (a->heads / a->kv_heads) < (1ll << 31) - 128, "cross_attention: q_len (%lld) times the heads that share keys must be below 2^31 - 128", (long long)a->q_len);
+    SVDQ_REQUIRE(a->q_len < (1ll << 31) && a->q_len * (a->heads / a->kv_heads) < (1ll << 31) - 128,
+                 "cross_attention: q_len (%lld) times the heads that share keys must be below 2^31 - 128", (long long)a->q_len);
     // (a launch takes fewer than 2^32 threads, 256 for 32 rows at most)
     const long long rows = a->q_len * (a->heads / a->kv_heads);
     SVDQ_REQUIRE((rows + 31) / 32 * (a->batch * a->kv_heads + 7) < (1ll << 24), "cross_attention: batch times kv_heads (%lld) groups of %lld rows of queries are too many for one launch",

@@ -3,8 +3,8 @@
 //   a = max(max_k |g|, 2^-100), code = rne(g * fl32(127 / a)), scale = fl32(a * f / 127), f = 1 or 1 / sqrt(mean(h^2) + eps).
 // The factor 1 / rms of a row is the same for all its elements, so it cancels in the codes: they depend on max |g| alone, and
 // g is exact in fp32 (two significands of at most 11 bits).  The sum of squares is held in fp32, of h * 2^100 where squares would end below fp32's
-// smallest numbers and eps does not make up for them.  |code| <= 127 needs no clamp: |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an infinity or a NaN in g (or a sum of squares that is not finite) gets the
-// scale NaN and codes 0: what a product makes of it is NaN.
+// smallest numbers and eps does not make up for them.  |code| <= 127 needs no clamp: |g| * fl32(127 / a) <= 127 (1 + 2^-23).  A row with an
+// infinity or a NaN in g (or a sum of squares that is not finite) gets the scale NaN and codes 0: what a product makes of it is NaN.
 // Bound by the traffic, 3 bytes per element (7 with a residual): one pass, the row stays in registers.  16384 x 8192 plain 62 us, 6.5 TB/s;
 // 9216 x 5120 with residual 53 us, 6.2 TB/s; one row of 4096 2.4 and 2.8 us, launch and latencies.
 #include "svdq_common.h"
@@ -66,7 +66,8 @@ __device__ inline uint32_t pack_pair(float lo, float hi) {
 // THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements.  A norm without a residual of 1024 threads with four
 // pieces fits two workgroups to a compute unit with 64 registers, which the compiler has to be told (2048 x 20000 31.3 -> 23.5 us).
 template <bool BF16, int THREADS, int VECS, bool NORM, bool RESIDUAL>
-__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS, THREADS == 1024 && VECS == 4 && NORM && !RESIDUAL ? 8 : THREADS < 256 ? 1 : THREADS / 256) quantize_rows_kernel(QuantizeParams p) {
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS, THREADS == 1024 && VECS == 4 && NORM && !RESIDUAL ? 8 : THREADS < 256 ? 1 : THREADS / 256)
+    quantize_rows_kernel(QuantizeParams p) {
     constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, WAVES = THREADS <= 64 ? 1 : THREADS / 64;
     const int t = threadIdx.x % THREADS;
     const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;

@@ -47,9 +47,9 @@ def cross_attention(
     given and must not overlap the inputs.  ``scale``: 1 / sqrt(D) by default, positive.  Forward only: the result carries no gradient.
 
     Scores, maxima, exponentials and sums are fp32; the probabilities are rounded to the inputs' type for their product with v, which with
-    the result's own rounding is up to one and a half steps of the type, relative to sum(p |v|) (typically a relative error of 0.0023 in bf16 and
-    0.0003 in fp16, where the rounding of the result alone is 0.0017 and 0.0002).  Scores (scale * q k^T) up to 1.8e8 in fp16 and 1.4e9 in bf16 are in range; larger ones
-    may give infinities or NaN."""
+    the result's own rounding is up to one and a half steps of the type, relative to sum(p |v|) (typically a relative error of 0.0023 in bf16
+    and 0.0003 in fp16, where the rounding of the result alone is 0.0017 and 0.0002).  Scores (scale * q k^T) up to 1.8e8 in fp16 and 1.4e9 in
+    bf16 are in range; larger ones may give infinities or NaN."""
     if out is None:
         y = nv.host().attention(q, k, v, key_lengths, key_mask, cu_seqlens_k, scale)
         if y is not None:
