@@ -39,7 +39,7 @@ extern "C" {
 #define SVDQ_EUNSUPPORTED -2 /* valid request that this build does not implement */
 #define SVDQ_ELAUNCH -3      /* the HIP runtime refused the launch */
 
-#define SVDQ_ABI_VERSION 6
+#define SVDQ_ABI_VERSION 7
 
 int svdq_abi_version(void);
 const char *svdq_last_error(void);
@@ -359,6 +359,98 @@ typedef struct svdq_cross_attention_args {
 int svdq_cross_attention_workspace(const svdq_cross_attention_args *args, int64_t *bytes);
 int svdq_cross_attention(const svdq_cross_attention_args *args, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The end of one block and the beginning of the next, for rows of K channels (bf16 or fp16; everything between is fp32):
+ *   b = input, or input / sqrt(mean(input^2) + eps) * branch_weight
+ *   h = residual_scale * residual + gate * b                        (gate * b without a residual), stored in residual_out
+ *   output = (h - m) / sqrt(mean((h - m)^2) + eps) * weight * (1 + scale) + shift,   m = 0, or mean(h) with `layer`
+ * Vectors that are NULL are left out.  output is made of h before that is rounded.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct svdq_gated_norm_args {
+    const void *input;         /* [M, K], rows ld_input elements apart                               */
+    const void *residual;      /* [M, K], rows ld_residual apart, or NULL                            */
+    void *output;              /* [M, K], rows ld_output apart; may be input itself                  */
+    void *residual_out;        /* [M, K], rows ld_residual_out apart; may be residual or input itself (not output); may be NULL */
+    const void *weight, *branch_weight; /* [K] or NULL                                               */
+    const void *gate, *scale, *shift;   /* vectors of K elements, or NULL: of entry e, token t at e * stride[0] + t * stride[1] */
+    const int32_t *cu_seqlens; /* [sequences + 1] ascending offsets, or NULL.  With them an entry is a sequence (token 0); rows in no
+                                  sequence are left as they are, or zeros (zero_rest)                 */
+    int64_t M, K;              /* K: a multiple of 8 up to 32768                                     */
+    int64_t tokens;            /* rows of an entry, without cu_seqlens                               */
+    int64_t sequences;
+    int64_t ld_input, ld_residual, ld_output, ld_residual_out; /* elements, multiples of 8           */
+    int64_t gate_stride[2], scale_stride[2], shift_stride[2];  /* elements, multiples of 8           */
+    float residual_scale, eps;
+    int32_t layer;             /* layer norm instead of RMS norm                                     */
+    int32_t zero_rest;         /* 1: rows of output in no sequence become zeros, 2: those of residual_out, 3: both */
+    int32_t dtype;             /* SVDQ_BF16 or SVDQ_FP16                                             */
+} svdq_gated_norm_args;
+
+int svdq_gated_norm(const svdq_gated_norm_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions with up to four axes, for the queries and keys of a layer in one launch, behind the RMS norm of every head where its
+ * weights are given.  Of the R = sum(axis_dim) rotated channels of a head, pair i is (2 i, 2 i + 1) or, with `halves`, (i, i + R / 2); axis a
+ * has the next axis_dim[a] / 2 pairs.  Pair j of axis a turns by positions[b][t][a] * theta[a]^(-2 j / axis_dim[a]); with
+ * `whole_spectrum` pair i of the head by positions[b][t][a] * theta[a]^(-2 i / R).  Angles are 64 bits, the rest fp32.  The channels behind
+ * the R are not turned.
+ * ------------------------------------------------------------------------------------------ */
+#define SVDQ_POSITION_INT32 0
+#define SVDQ_POSITION_INT64 1
+#define SVDQ_POSITION_FP32 2
+
+typedef struct svdq_rotary_axes_args {
+    const void *q, *k;         /* [batch][tokens][heads, kv_heads][head_dim] by strides; k may be NULL */
+    void *q_out, *k_out;       /* the same shapes; may be q and k themselves                         */
+    const void *norm_q, *norm_k; /* [head_dim] or NULL                                               */
+    const void *positions;     /* [batch][tokens][axes] by strides                                   */
+    int64_t batch, tokens, heads, kv_heads, head_dim; /* head_dim: a multiple of 8 up to 256         */
+    int64_t axes;              /* 1..4                                                               */
+    int64_t axis_dim[4];       /* channels of each axis: even; with `halves` their sum is a multiple of 16 */
+    double theta[4];
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3]; /* batch, token, head: elements, multiples of 8 */
+    int64_t position_stride[3];  /* batch, token, axis: elements                                     */
+    float eps;
+    int32_t position_type;     /* SVDQ_POSITION_*                                                    */
+    int32_t halves, whole_spectrum;
+    int32_t dtype;             /* SVDQ_BF16 or SVDQ_FP16                                             */
+} svdq_rotary_axes_args;
+
+int svdq_rotary_axes(const svdq_rotary_axes_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Softmax attention of the queries of several sequences to the keys of the same sequence, causal or not.  Sequence s has n_q queries and n_k keys:
+ *   queries: rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] of q, or all q_len rows of batch entry s;
+ *   keys: rows cu_seqlens_k[s] .. cu_seqlens_k[s + 1] of k and v, or the first key_lengths[s] (NULL: all k_len) rows of batch entry s.
+ *   out[i][h] = sum_j p_j v[j][h / G],  p = softmax over j of scale * q[i][h] . k[j][h / G],  G = heads / kv_heads,
+ * over all keys j, or, causal, those with j <= i + n_k - n_q: the last query sees all keys, and one in front of all keys none.  Queries without
+ * a key get zeros.  What k and v hold for keys that a query does not see (NaN, infinities) has no effect on it.  Precision as in
+ * svdq_cross_attention.  Rows of q in no sequence are left as they are in out, or zeros (zero_rest).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct svdq_self_attention_args {
+    const void *q;          /* [batch][q_len][heads][head_dim] by strides; with cu_seqlens_q: q_len is the number of rows of all
+                               sequences together and the batch stride is ignored                     */
+    const void *k, *v;      /* [batch][k_len][kv_heads][head_dim] by strides; with cu_seqlens_k the same */
+    void *out;              /* as q                                                                  */
+    const int32_t *cu_seqlens_q, *cu_seqlens_k; /* [batch + 1] ascending offsets or NULL (offsets out of range or order give
+                               fewer rows or keys, never others)                                      */
+    const int32_t *key_lengths; /* [batch] or NULL, without cu_seqlens_k; values outside 0..k_len count as the nearer of the two */
+    void *workspace;        /* svdq_self_attention_workspace bytes (16-byte aligned), not shared with a call that may run at the same
+                               time; NULL if that is 0                                               */
+    int64_t workspace_bytes;
+    int64_t batch, heads, kv_heads, head_dim; /* head_dim: a multiple of 8 up to 128                 */
+    int64_t q_len, k_len;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head: elements, multiples of 8; elements
+                                                                     of a head are next to each other; the tokens
+                                                                     of k and v less than 2^24 elements apart      */
+    float scale;            /* positive                                                              */
+    int32_t causal, zero_rest;
+    int32_t dtype;          /* of q, k, v, out: SVDQ_BF16 or SVDQ_FP16                               */
+} svdq_self_attention_args;
+
+/* What a call with these arguments on the current device needs as its workspace (depends on shapes alone). */
+int svdq_self_attention_workspace(const svdq_self_attention_args *args, int64_t *bytes);
+int svdq_self_attention(const svdq_self_attention_args *args, void *stream);
 
 #ifdef __cplusplus
 }

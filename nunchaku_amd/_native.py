@@ -18,13 +18,14 @@ import torch
 _PKG_DIR = Path(__file__).resolve().parent
 _CSRC = _PKG_DIR / "csrc"
 LIB_PATH = _PKG_DIR / "libsvdq_amd.so"
-SOURCES = ["repack.hip", "quantize.hip", "gemm.hip", "awq_gemv.hip", "litela.hip", "w8a8_quantize.hip", "w8a8_gemm.hip", "attention.hip"]
+SOURCES = ["repack.hip", "quantize.hip", "gemm.hip", "awq_gemv.hip", "litela.hip", "w8a8_quantize.hip", "w8a8_gemm.hip", "attention.hip", "self_attention.hip",
+           "rotary_axes.hip", "gated_norm.hip"]
 HIPCC_FLAGS = [
     "-shared", "-fPIC", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
-SVDQ_ABI_VERSION = 6
+SVDQ_ABI_VERSION = 7
 EXPORTED_SYMBOLS = [
     "svdq_abi_version", "svdq_last_error",
     "svdq_repack_qweight", "svdq_repack_wscales", "svdq_repack_wmscales", "svdq_repack_vector",
@@ -32,6 +33,7 @@ EXPORTED_SYMBOLS = [
     "svdq_quantize_w4a4_act_fuse_lora", "svdq_gemm_w4a4", "svdq_gemm_w4a4_noalloc", "svdq_awq_gemv_w4a16",
     "svdq_linearattn_vk_mul_q", "svdq_release_workspaces",
     "svdq_quantize_w8a8_act", "svdq_rms_norm_quantize_w8a8", "svdq_gemm_w8a8_workspace", "svdq_gemm_w8a8", "svdq_cross_attention_workspace", "svdq_cross_attention",
+    "svdq_gated_norm", "svdq_rotary_axes", "svdq_self_attention_workspace", "svdq_self_attention",
 ]
 
 
@@ -118,6 +120,47 @@ class CrossAttentionArgs(ctypes.Structure):
         ("q_len", ctypes.c_int64), ("k_len", ctypes.c_int64),
         ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3), ("out_stride", ctypes.c_int64 * 3),
         ("mask_stride", ctypes.c_int64), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class GatedNormArgs(ctypes.Structure):
+    """Mirror of ``svdq_gated_norm_args``."""
+
+    _fields_ = [
+        ("input", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("output", ctypes.c_void_p), ("residual_out", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p), ("branch_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p), ("M", ctypes.c_int64), ("K", ctypes.c_int64), ("tokens", ctypes.c_int64), ("sequences", ctypes.c_int64),
+        ("ld_input", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ld_output", ctypes.c_int64), ("ld_residual_out", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64 * 2), ("scale_stride", ctypes.c_int64 * 2), ("shift_stride", ctypes.c_int64 * 2),
+        ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float), ("layer", ctypes.c_int32), ("zero_rest", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class RotaryAxesArgs(ctypes.Structure):
+    """Mirror of ``svdq_rotary_axes_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("norm_q", ctypes.c_void_p),
+        ("norm_k", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+        ("axes", ctypes.c_int64), ("axis_dim", ctypes.c_int64 * 4), ("theta", ctypes.c_double * 4),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("q_out_stride", ctypes.c_int64 * 3), ("k_out_stride", ctypes.c_int64 * 3),
+        ("position_stride", ctypes.c_int64 * 3), ("eps", ctypes.c_float), ("position_type", ctypes.c_int32), ("halves", ctypes.c_int32),
+        ("whole_spectrum", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class SelfAttentionArgs(ctypes.Structure):
+    """Mirror of ``svdq_self_attention_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("cu_seqlens_q", ctypes.c_void_p), ("cu_seqlens_k", ctypes.c_void_p), ("key_lengths", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+        ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+        ("q_len", ctypes.c_int64), ("k_len", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3), ("out_stride", ctypes.c_int64 * 3),
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("zero_rest", ctypes.c_int32), ("dtype", ctypes.c_int32),
     ]
 
 
@@ -220,6 +263,10 @@ def lib() -> ctypes.CDLL:
         L.svdq_gemm_w8a8.argtypes = [ctypes.POINTER(GemmW8A8Args), vp]
         L.svdq_cross_attention_workspace.argtypes = [ctypes.POINTER(CrossAttentionArgs), ctypes.POINTER(i64)]
         L.svdq_cross_attention.argtypes = [ctypes.POINTER(CrossAttentionArgs), vp]
+        L.svdq_gated_norm.argtypes = [ctypes.POINTER(GatedNormArgs), vp]
+        L.svdq_rotary_axes.argtypes = [ctypes.POINTER(RotaryAxesArgs), vp]
+        L.svdq_self_attention_workspace.argtypes = [ctypes.POINTER(SelfAttentionArgs), ctypes.POINTER(i64)]
+        L.svdq_self_attention.argtypes = [ctypes.POINTER(SelfAttentionArgs), vp]
         for name in EXPORTED_SYMBOLS:
             getattr(L, name)
             if name not in ("svdq_last_error",):

@@ -1,0 +1,303 @@
+// The end of one block and the beginning of the next, row by row of K channels:
+//   b = x, or x / sqrt(mean(x^2) + eps) * branch_weight;   h = residual_scale * residual + gate * b  (h = gate * b without a residual)
+//   y = (h - m) / sqrt(mean((h - m)^2) + eps) * weight * (1 + scale) + shift,   m = 0 (RMS norm) or mean(h) (layer norm)
+// Vectors that are not given are left out.  gate, scale and shift belong to a batch entry, a packed sequence or a token.  All of it is fp32 from
+// the first conversion to the last: y is made of h as it is, before h is rounded for the residual stream.
+// The mean is taken before the deviations' squares are summed, from registers: their difference in one pass would lose what a large mean leaves.
+// Squares whose sum leaves fp32's range, at either end, are summed once more in 64 bits: rows of finite numbers have finite norms.
+#include "svdq_common.h"
+
+using namespace svdq;
+
+namespace {
+
+struct NormParams {
+    const char *x, *residual, *weight, *branch_weight, *gate, *scale, *shift;
+    char *y, *h;
+    const int *cu_seqlens;
+    long long first, M, ld_x, ld_residual, ld_y, ld_h;   // bytes; rows first .. M are this launch's
+    long long gate_s[2], scale_s[2], shift_s[2];        // bytes: entry, token
+    long long tokens;                                   // rows of an entry
+    int sequences, pieces, zero_rest;                   // pieces of 8 elements per row
+    float inv_k, tiny, eps, residual_scale;
+};
+
+template <bool BF16>
+__device__ inline void unpack(const u32x4_t w, float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t pair = w[j];
+        if (BF16) {
+            f[2 * j] = bits_f32(pair << 16);
+            f[2 * j + 1] = bits_f32(pair & 0xFFFF0000u);
+        } else {
+            const half2_t h = __builtin_bit_cast(half2_t, pair);
+            f[2 * j] = (float)h[0];
+            f[2 * j + 1] = (float)h[1];
+        }
+    }
+}
+template <bool BF16>
+__device__ inline u32x4_t pack(const float (&f)[8]) {
+    u32x4_t w;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (BF16) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+        else w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]) << 16);
+    }
+    return w;
+}
+
+// The sum of x over a row's THREADS threads, in all of them.  `slot`: a place in LDS of its own for every sum, so that one barrier each is enough
+template <int THREADS, typename T>
+__device__ inline T row_sum(T x, T (*place)[16], int slot, int t) {
+#pragma unroll
+    for (int d = THREADS < 64 ? THREADS / 2 : 32; d; d >>= 1) x += __shfl_xor(x, d);
+    if constexpr (THREADS > 64) {
+        if ((t & 63) == 0) place[slot][t >> 6] = x;
+        __syncthreads();
+        x = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) x += place[slot][i];
+    }
+    return x;
+}
+
+// h <- (h - m) / sqrt(mean((h - m)^2) + eps), the pieces of this thread that lie in the row
+template <int THREADS, int VECS>
+__device__ inline void normalise(float (&h)[VECS][8], bool center, const NormParams &p, int t, int slot) {
+    __shared__ float sums[4][16];
+    __shared__ double wide[4][16];
+    float m = 0.f;
+    if (center) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) s += h[i][j];  // (zeros behind the row's end)
+        m = row_sum<THREADS>(s, sums, slot, t) * p.inv_k;
+    }
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        if (t + i * THREADS >= p.pieces) break;
+#pragma unroll
+        for (int j = 0; j < 8; j++) squares = __builtin_fmaf(h[i][j] - m, h[i][j] - m, squares);
+    }
+    squares = row_sum<THREADS>(squares, sums, slot + 1, t);
+    if (squares < 0x1p120f && squares >= p.tiny) {
+        const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_k, p.eps));
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] = (h[i][j] - m) * r;
+        return;
+    }
+    const double inv_k = 1.0 / (8.0 * p.pieces);
+    double mean = 0.0, s = 0.0;
+    if (center) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) s += (double)h[i][j];
+        mean = row_sum<THREADS>(s, wide, slot, t) * inv_k;
+        s = 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        if (t + i * THREADS >= p.pieces) break;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += ((double)h[i][j] - mean) * ((double)h[i][j] - mean);
+    }
+    const double r = 1.0 / __builtin_sqrt(row_sum<THREADS>(s, wide, slot + 1, t) * inv_k + (double)p.eps);
+#pragma unroll
+    for (int i = 0; i < VECS; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] = (float)(((double)h[i][j] - mean) * r);
+}
+
+// The sequence of a row: how many offsets are not behind it, less one (-1 or the number of sequences: none).  THREADS threads look together.
+template <int THREADS>
+__device__ inline int sequence_of(const NormParams &p, long long row, int t) {
+    constexpr int L = THREADS < 64 ? THREADS : 64;
+    const int li = t % L;
+    int n = 0;
+    for (int base = 0; base <= p.sequences; base += L) {
+        uint64_t in = __ballot(base + li <= p.sequences && p.cu_seqlens[base + li] <= row);
+        if (L == 32) in = (threadIdx.x & 32 ? in >> 32 : in) & 0xFFFFFFFFull;
+        n += __popcll(in);
+    }
+    return n - 1;
+}
+
+// THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements
+template <bool BF16, int THREADS, int VECS, bool LAYER>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) gated_norm_kernel(NormParams p) {
+    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+    const int t = threadIdx.x % THREADS;
+    const long long row = p.first + (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (row >= p.M) return;  // (all threads of a row; rows of several waves are one per workgroup)
+    long long entry = row / p.tokens, token = row - entry * p.tokens;
+    bool any = true;
+    if (p.cu_seqlens) {
+        entry = sequence_of<THREADS>(p, row, t);
+        token = 0;
+        any = entry >= 0 && entry < p.sequences;
+    }
+    if (!any) {
+        if (p.zero_rest) {
+#pragma unroll
+            for (int i = 0; i < VECS; i++) {
+                const int piece = t + i * THREADS;
+                if (piece >= p.pieces) break;
+                if (p.zero_rest & 1) *(u32x4_t *)(p.y + row * p.ld_y + (size_t)piece * 16) = u32x4_t{0, 0, 0, 0};
+                if (p.h && (p.zero_rest & 2)) *(u32x4_t *)(p.h + row * p.ld_h + (size_t)piece * 16) = u32x4_t{0, 0, 0, 0};
+            }
+        }
+        return;
+    }
+    u32x4_t w[VECS], r[VECS];
+    float h[VECS][8], f[8];
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * THREADS;
+        w[i] = r[i] = u32x4_t{0, 0, 0, 0};
+        if (piece < p.pieces) {
+            w[i] = *(const u32x4_t *)(p.x + row * p.ld_x + (size_t)piece * 16);
+            if (p.residual) r[i] = *(const u32x4_t *)(p.residual + row * p.ld_residual + (size_t)piece * 16);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; i++) unpack<BF16>(w[i], h[i]);
+    auto times = [&](const char *v, float add) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int piece = t + i * THREADS;
+            if (piece >= p.pieces) break;
+            unpack<BF16>(*(const u32x4_t *)(v + (size_t)piece * 16), f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] *= add + f[j];
+        }
+    };
+    if (p.branch_weight) {
+        normalise<THREADS, VECS>(h, false, p, t, 0);
+        times(p.branch_weight, 0.f);
+    }
+    if (p.gate) times(p.gate + entry * p.gate_s[0] + token * p.gate_s[1], 0.f);
+    if (p.residual) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const int piece = t + i * THREADS;
+            unpack<BF16>(r[i], f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] = __builtin_fmaf(p.residual_scale, f[j], h[i][j]);
+            if (piece < p.pieces && p.h) *(u32x4_t *)(p.h + row * p.ld_h + (size_t)piece * 16) = pack<BF16>(h[i]);
+        }
+    }
+    normalise<THREADS, VECS>(h, LAYER, p, t, 2);
+    if (p.weight) times(p.weight, 0.f);
+    if (p.scale) times(p.scale + entry * p.scale_s[0] + token * p.scale_s[1], 1.f);
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * THREADS;
+        if (piece >= p.pieces) break;
+        if (p.shift) {
+            unpack<BF16>(*(const u32x4_t *)(p.shift + entry * p.shift_s[0] + token * p.shift_s[1] + (size_t)piece * 16), f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[i][j] += f[j];
+        }
+        *(u32x4_t *)(p.y + row * p.ld_y + (size_t)piece * 16) = pack<BF16>(h[i]);
+    }
+}
+
+template <bool BF16, int THREADS, int VECS>
+void launch_rows(const NormParams &p, bool layer, hipStream_t st) {
+    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
+    const dim3 grid((unsigned)((p.M - p.first + ROWS - 1) / ROWS)), block(THREADS < 256 ? 256 : THREADS);
+    if (layer) SVDQ_LAUNCH((gated_norm_kernel<BF16, THREADS, VECS, true>), grid, block, 0, st, p);
+    else SVDQ_LAUNCH((gated_norm_kernel<BF16, THREADS, VECS, false>), grid, block, 0, st, p);
+}
+
+template <bool BF16>
+void dispatch(const NormParams &p, bool layer, hipStream_t st) {
+    const int need = p.pieces;
+    if (need <= 32) launch_rows<BF16, 32, 1>(p, layer, st);
+    else if (need <= 64) launch_rows<BF16, 64, 1>(p, layer, st);
+    else if (need <= 128) launch_rows<BF16, 64, 2>(p, layer, st);
+    else if (need <= 256) launch_rows<BF16, 256, 1>(p, layer, st);
+    else if (need <= 512) launch_rows<BF16, 256, 2>(p, layer, st);
+    else if (need <= 1024) launch_rows<BF16, 512, 2>(p, layer, st);
+    else if (need <= 2048) launch_rows<BF16, 1024, 2>(p, layer, st);
+    else launch_rows<BF16, 1024, 4>(p, layer, st);
+}
+
+bool vector_ok(const void *v, const int64_t *s) { return !v || ((uintptr_t)v % 16 == 0 && s[0] >= 0 && s[1] >= 0 && (s[0] | s[1]) % 8 == 0); }
+
+}  // namespace
+
+extern "C" int svdq_gated_norm(const svdq_gated_norm_args *a, void *stream) {
+    SVDQ_REQUIRE(a && a->input && a->output, "gated_norm: input and output must not be null");
+    SVDQ_REQUIRE(a->residual || !a->residual_out, "gated_norm: residual_out is the sum with a residual, which must not be null");
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "gated_norm: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
+    SVDQ_REQUIRE(a->M > 0 && a->M < (1ll << 31), "gated_norm: M (%lld) must be in 1..2^31-1", (long long)a->M);
+    SVDQ_REQUIRE(a->K > 0 && a->K <= 32768 && a->K % 8 == 0, "gated_norm: K (%lld) must be a multiple of 8 up to 32768", (long long)a->K);
+    const struct {
+        const char *name;
+        const void *p;
+        int64_t ld;
+    } rows[] = {{"input", a->input, a->ld_input}, {"residual", a->residual, a->ld_residual}, {"output", a->output, a->ld_output}, {"residual_out", a->residual_out, a->ld_residual_out}};
+    for (const auto &r : rows) {
+        if (!r.p) continue;
+        SVDQ_REQUIRE((uintptr_t)r.p % 16 == 0, "gated_norm: %s must be 16-byte aligned", r.name);
+        SVDQ_REQUIRE(r.ld >= a->K && r.ld % 8 == 0, "gated_norm: rows of %s must be at least K elements and a multiple of 8 apart, got %lld", r.name, (long long)r.ld);
+    }
+    SVDQ_REQUIRE(((uintptr_t)a->weight | (uintptr_t)a->branch_weight) % 16 == 0, "gated_norm: weight and branch_weight must be 16-byte aligned");
+    SVDQ_REQUIRE(vector_ok(a->gate, a->gate_stride) && vector_ok(a->scale, a->scale_stride) && vector_ok(a->shift, a->shift_stride),
+                 "gated_norm: gate, scale and shift must be 16-byte aligned, their strides multiples of 8");
+    if (a->cu_seqlens) {
+        SVDQ_REQUIRE((uintptr_t)a->cu_seqlens % 4 == 0 && a->sequences > 0 && a->sequences < (1ll << 24), "gated_norm: cu_seqlens must be 4-byte aligned, sequences (%lld) in 1..2^24-1",
+                     (long long)a->sequences);
+    } else {
+        SVDQ_REQUIRE(a->tokens > 0, "gated_norm: tokens (%lld), the rows of a batch entry, must be positive", (long long)a->tokens);
+    }
+    SVDQ_REQUIRE(a->eps >= 0.f && a->eps < __builtin_huge_valf(), "gated_norm: eps must be a finite number not below zero");
+    SVDQ_REQUIRE(a->residual_scale - a->residual_scale == 0.f, "gated_norm: residual_scale must be finite");
+    NormParams p;
+    p.x = (const char *)a->input;
+    p.residual = (const char *)a->residual;
+    p.weight = (const char *)a->weight;
+    p.branch_weight = (const char *)a->branch_weight;
+    p.gate = (const char *)a->gate;
+    p.scale = (const char *)a->scale;
+    p.shift = (const char *)a->shift;
+    p.y = (char *)a->output;
+    p.h = (char *)a->residual_out;
+    p.cu_seqlens = a->cu_seqlens;
+    p.ld_x = a->ld_input * 2;
+    p.ld_residual = a->ld_residual * 2;
+    p.ld_y = a->ld_output * 2;
+    p.ld_h = a->ld_residual_out * 2;
+    for (int i = 0; i < 2; i++) {
+        p.gate_s[i] = a->gate_stride[i] * 2;
+        p.scale_s[i] = a->scale_stride[i] * 2;
+        p.shift_s[i] = a->shift_stride[i] * 2;
+    }
+    p.tokens = a->cu_seqlens ? a->M : a->tokens;
+    p.sequences = (int)a->sequences;
+    p.pieces = (int)(a->K / 8);
+    p.zero_rest = a->zero_rest;
+    p.inv_k = 1.0f / (float)a->K;
+    // fp32 rounds a square by 2^-150 at most, K of them by K * 2^-150: from K * 2^-126 on 2^-24 of the sum, and nothing beside an eps of 2^-120
+    p.tiny = a->eps >= 0x1p-120f ? 0.f : 0x1p-100f;
+    p.eps = a->eps;
+    p.residual_scale = a->residual_scale;
+    // a launch takes fewer than 2^32 threads
+    const long long most = p.pieces <= 128 ? 1ll << 25 : 1ll << 21;
+    for (p.first = 0; p.first < a->M; p.first += most) {
+        p.M = a->M - p.first < most ? a->M : p.first + most;
+        if (a->dtype == SVDQ_BF16) dispatch<true>(p, a->layer != 0, (hipStream_t)stream);
+        else dispatch<false>(p, a->layer != 0, (hipStream_t)stream);
+        if (int rc = check_launch("gated_norm")) return rc;
+    }
+    return SVDQ_OK;
+}

@@ -832,10 +832,220 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- between the linear layers: the plain case of ops/norm.py, ops/rotary.py and ops/attention.py::self_attention ------------------
+// A gate, scale or shift of rows x: its address and its (entry, token) strides; `entries`: of packed sequences, or -1
+bool vector_of(PyObject *o, const at::Tensor &x, int64_t K, int64_t tokens, int64_t entries, const void **ptr, int64_t *s) {
+    const at::Tensor *v;
+    if (!optional_tensor(o, &v)) return false;
+    if (!v) return true;
+    const int64_t n = v->dim();
+    if (v->device() != x.device() || v->scalar_type() != x.scalar_type() || n < 1 || v->size(n - 1) != K || (K > 1 && v->stride(n - 1) != 1)) return false;
+    *ptr = v->data_ptr();
+    if (n == 1) return true;
+    if (entries >= 0) {
+        if (n != 2 || v->size(0) != entries) return false;
+        s[0] = entries > 1 ? v->stride(0) : 0;
+        return true;
+    }
+    if (v->sizes() == x.sizes()) {
+        if (!v->is_contiguous()) return false;
+        s[0] = tokens * K;
+        s[1] = K;
+        return true;
+    }
+    if (x.dim() < 3 || v->size(0) != x.size(0) || v->numel() != x.size(0) * K) return false;
+    s[0] = v->size(0) > 1 ? v->stride(0) : 0;
+    return true;
+}
+bool plain_vector(PyObject *o, const at::Tensor &x, int64_t n, const void **ptr) {
+    const at::Tensor *v;
+    if (!optional_tensor(o, &v)) return false;
+    if (!v) return true;
+    if (v->dim() != 1 || !plain_on(*v, x, x.scalar_type(), n)) return false;
+    *ptr = v->data_ptr();
+    return true;
+}
+bool number_of(PyObject *o, double *x) {
+    if (!PyFloat_CheckExact(o)) return false;
+    *x = PyFloat_AS_DOUBLE(o);
+    return true;
+}
+
+// gated_norm(x, residual, norm, weight, gate, scale, shift, branch_weight, residual_scale, eps, cu_seqlens) -> (y, h or None), or None
+PyObject *gated_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(11)
+    const at::Tensor *x, *r, *cu;
+    svdq_gated_norm_args a = {};
+    double residual_scale, eps;
+    if (!as_tensor(args[0], &x) || (a.dtype = type_code(x->scalar_type())) < 0 || !rows_of(*x, &a.M, &a.K, &a.ld_input) || !optional_tensor(args[1], &r) || !PyUnicode_Check(args[2]) ||
+        !plain_vector(args[3], *x, a.K, &a.weight) || !plain_vector(args[7], *x, a.K, &a.branch_weight) || !number_of(args[8], &residual_scale) || !number_of(args[9], &eps) ||
+        !optional_tensor(args[10], &cu)) Py_RETURN_NONE;
+    if (PyUnicode_CompareWithASCIIString(args[2], "layer") == 0) a.layer = 1;
+    else if (PyUnicode_CompareWithASCIIString(args[2], "rms") != 0) Py_RETURN_NONE;
+    int64_t entries = -1, M, K;
+    if (cu) {
+        entries = cu->numel() - 1;
+        if (cu->dim() != 1 || entries < 1 || !plain_on(*cu, *x, at::kInt, entries + 1) || x->dim() != 2) Py_RETURN_NONE;
+        a.cu_seqlens = (const int32_t *)cu->data_ptr();
+        a.sequences = entries;
+    }
+    a.tokens = x->dim() > 2 ? a.M / x->size(0) : 1;
+    if (!vector_of(args[4], *x, a.K, a.tokens, entries, &a.gate, a.gate_stride) || !vector_of(args[5], *x, a.K, a.tokens, entries, &a.scale, a.scale_stride) ||
+        !vector_of(args[6], *x, a.K, a.tokens, entries, &a.shift, a.shift_stride)) Py_RETURN_NONE;
+    if (r && (r->sizes() != x->sizes() || r->scalar_type() != x->scalar_type() || r->device() != x->device() || !rows_of(*r, &M, &K, &a.ld_residual))) Py_RETURN_NONE;
+    at::Tensor y = result_tensor(x->sizes(), x->scalar_type(), *x), h;
+    a.input = x->data_ptr();
+    a.output = y.data_ptr();
+    a.ld_output = a.ld_residual_out = a.K;
+    if (r) {
+        h = result_tensor(x->sizes(), x->scalar_type(), *x);
+        a.residual = r->data_ptr();
+        a.residual_out = h.data_ptr();
+    }
+    a.residual_scale = (float)residual_scale;
+    a.eps = (float)eps;
+    a.zero_rest = 3;
+    hipStream_t st = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_gated_norm(&a, st);
+    Py_END_ALLOW_THREADS
+    if (rc != SVDQ_OK) return raise(rc);
+    PyObject *second = r ? THPVariable_Wrap(h) : Py_NewRef(Py_None), *t = PyTuple_New(2);
+    if (!t) {
+        Py_XDECREF(second);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(y));
+    PyTuple_SET_ITEM(t, 1, second);
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary_axes(q, k, positions, axes, theta, norm_q, norm_k, eps, interleaved, spectrum) -> (q, k or None), or None
+PyObject *rotary_axes(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(10)
+    const at::Tensor *q, *k, *pos;
+    svdq_rotary_axes_args a = {};
+    double theta, eps;
+    if (!as_tensor(args[0], &q) || !optional_tensor(args[1], &k) || !as_tensor(args[2], &pos) || !number_of(args[4], &theta) || !number_of(args[7], &eps) || !PyBool_Check(args[8]) ||
+        !PyUnicode_Check(args[9]) || !(PyTuple_CheckExact(args[3]) || PyList_CheckExact(args[3]))) Py_RETURN_NONE;
+    const int64_t n = q->dim();
+    if (!q->is_cuda() || q->device().index() != c10::hip::current_device() || (a.dtype = type_code(q->scalar_type())) < 0 || (n != 3 && n != 4) || q->numel() == 0) Py_RETURN_NONE;
+    if (k && (k->device() != q->device() || k->scalar_type() != q->scalar_type() || k->dim() != n || k->numel() == 0 || k->size(n - 1) != q->size(n - 1) ||
+              k->size(n - 3) != q->size(n - 3) || k->size(0) != q->size(0))) Py_RETURN_NONE;
+    a.batch = n == 4 ? q->size(0) : 1;
+    a.tokens = q->size(n - 3);
+    a.heads = q->size(n - 2);
+    a.kv_heads = k ? k->size(n - 2) : 0;
+    a.head_dim = q->size(n - 1);
+    const Py_ssize_t count = Py_SIZE(args[3]);
+    if (count < 1 || count > 4) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < count; i++) {
+        PyObject *o = PyTuple_CheckExact(args[3]) ? PyTuple_GET_ITEM(args[3], i) : PyList_GET_ITEM(args[3], i);
+        if (!PyLong_CheckExact(o)) Py_RETURN_NONE;
+        a.axis_dim[i] = PyLong_AsLongLong(o);
+        if (a.axis_dim[i] == -1 && PyErr_Occurred()) {
+            PyErr_Clear();
+            Py_RETURN_NONE;
+        }
+        a.theta[i] = theta;
+    }
+    a.axes = count;
+    const at::ScalarType pt = pos->scalar_type();
+    a.position_type = pt == at::kInt ? SVDQ_POSITION_INT32 : pt == at::kLong ? SVDQ_POSITION_INT64 : SVDQ_POSITION_FP32;
+    const int64_t pn = pos->dim();
+    if ((pt != at::kInt && pt != at::kLong && pt != at::kFloat) || pos->device() != q->device() || pn < 2 || pn > n - 1 || pos->size(pn - 1) != count || pos->size(pn - 2) != a.tokens ||
+        (pn == 3 && pos->size(0) != a.batch)) Py_RETURN_NONE;
+    for (int64_t i = 0; i < pn; i++) a.position_stride[3 - pn + i] = pos->size(i) > 1 ? pos->stride(i) : 0;
+    if (!plain_vector(args[5], *q, a.head_dim, &a.norm_q) || !plain_vector(args[6], *q, a.head_dim, &a.norm_k) || (!k && a.norm_k) || !head_strides(*q, a.q_stride) ||
+        (k && !head_strides(*k, a.k_stride))) Py_RETURN_NONE;
+    if (PyUnicode_CompareWithASCIIString(args[9], "head") == 0) a.whole_spectrum = 1;
+    else if (PyUnicode_CompareWithASCIIString(args[9], "axis") != 0) Py_RETURN_NONE;
+    a.halves = args[8] == Py_False;
+    a.eps = (float)eps;
+    at::Tensor oq = result_tensor(q->sizes(), q->scalar_type(), *q), ok;
+    head_strides(oq, a.q_out_stride);
+    a.q = q->data_ptr();
+    a.q_out = oq.data_ptr();
+    a.positions = pos->data_ptr();
+    if (k) {
+        ok = result_tensor(k->sizes(), k->scalar_type(), *k);
+        head_strides(ok, a.k_out_stride);
+        a.k = k->data_ptr();
+        a.k_out = ok.data_ptr();
+    }
+    hipStream_t st = c10::hip::getCurrentHIPStream(q->device().index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_rotary_axes(&a, st);
+    Py_END_ALLOW_THREADS
+    if (rc != SVDQ_OK) return raise(rc);
+    PyObject *second = k ? THPVariable_Wrap(ok) : Py_NewRef(Py_None), *t = PyTuple_New(2);
+    if (!t) {
+        Py_XDECREF(second);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(oq));
+    PyTuple_SET_ITEM(t, 1, second);
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// self_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, key_lengths, causal, scale or None) -> out, or None
+PyObject *self_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    SVDQ_NARGS(8)
+    const at::Tensor *q, *k, *v, *cu_q, *cu_k, *lengths;
+    svdq_self_attention_args a = {};
+    if (!as_tensor(args[0], &q) || !as_tensor(args[1], &k) || !as_tensor(args[2], &v) || !optional_tensor(args[3], &cu_q) || !optional_tensor(args[4], &cu_k) ||
+        !optional_tensor(args[5], &lengths) || !PyBool_Check(args[6])) Py_RETURN_NONE;
+    if (!q->is_cuda() || q->device().index() != c10::hip::current_device() || (a.dtype = type_code(q->scalar_type())) < 0 || k->device() != q->device() ||
+        v->device() != q->device() || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || q->dim() != (cu_q ? 3 : 4) ||
+        (k->dim() != 3 && k->dim() != 4) || k->sizes() != v->sizes() || q->numel() == 0 || k->numel() == 0) Py_RETURN_NONE;
+    if (k->dim() == 3 && !cu_k) cu_k = cu_q;
+    if ((k->dim() == 3) != (cu_k != nullptr) || (cu_k && lengths)) Py_RETURN_NONE;
+    a.batch = cu_q ? cu_q->numel() - 1 : q->size(0);
+    a.q_len = q->size(-3);
+    a.heads = q->size(-2);
+    a.head_dim = q->size(-1);
+    a.k_len = k->size(-3);
+    a.kv_heads = k->size(-2);
+    if (a.batch < 1 || k->size(-1) != a.head_dim || (!cu_k && k->size(0) != a.batch) || a.heads % a.kv_heads || !head_strides(*q, a.q_stride) || !head_strides(*k, a.k_stride) ||
+        !head_strides(*v, a.v_stride) || !int_vector(cu_q, *q, a.batch + 1) || !int_vector(cu_k, *q, a.batch + 1) || !int_vector(lengths, *q, a.batch)) Py_RETURN_NONE;
+    double scale = 1.0 / std::sqrt((double)a.head_dim);
+    if (args[7] != Py_None && !number_of(args[7], &scale)) Py_RETURN_NONE;
+    at::Tensor out = result_tensor(q->sizes(), q->scalar_type(), *q);
+    head_strides(out, a.out_stride);
+    a.q = q->data_ptr();
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.out = out.data_ptr();
+    a.cu_seqlens_q = cu_q ? (const int32_t *)cu_q->data_ptr() : nullptr;
+    a.cu_seqlens_k = cu_k ? (const int32_t *)cu_k->data_ptr() : nullptr;
+    a.key_lengths = lengths ? (const int32_t *)lengths->data_ptr() : nullptr;
+    a.scale = (float)scale;
+    a.causal = args[6] == Py_True;
+    a.zero_rest = 1;
+    hipStream_t st = c10::hip::getCurrentHIPStream(q->device().index()).stream();
+    int rc = svdq_self_attention_workspace(&a, &a.workspace_bytes);
+    if (rc != SVDQ_OK) return raise(rc);
+    std::optional<Scratch> workspace;
+    if (a.workspace_bytes) a.workspace = workspace.emplace((size_t)a.workspace_bytes, st).ptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = svdq_self_attention(&a, st);
+    Py_END_ALLOW_THREADS
+    return rc != SVDQ_OK ? raise(rc) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define SVDQ_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SVDQ_METHOD(make_layer), SVDQ_METHOD(linear), SVDQ_METHOD(gelu_mlp), SVDQ_METHOD(qkv_norm_rope), SVDQ_METHOD(awq_gemv), SVDQ_METHOD(awq_linear),
                          SVDQ_METHOD(quantize_call), SVDQ_METHOD(gemm_call), SVDQ_METHOD(vk_mul_q),
                          SVDQ_METHOD(w8a8_quantize), SVDQ_METHOD(w8a8_norm), SVDQ_METHOD(w8a8_gemm), SVDQ_METHOD(attention),
+                         SVDQ_METHOD(gated_norm), SVDQ_METHOD(rotary_axes), SVDQ_METHOD(self_attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Per-call host code of the quantized layers.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

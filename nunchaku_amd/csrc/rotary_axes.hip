@@ -1,0 +1,228 @@
+// Rotary positions with several axes, behind the RMS norm of every head where its weights are given: channels come in pairs, (2 i, 2 i + 1) or
+// (i, i + R / 2) of the R rotated channels of a head, and the pairs in runs, one for each axis of the positions (time, height, width).  With the
+// angle phi = position[axis] * frequency[pair] a pair (x, y) becomes (x cos phi - y sin phi, x sin phi + y cos phi).  Channels behind the R pass.
+//
+// Angles.  A frequency in revolutions, theta^(-e) / (2 pi), comes from the host in 64 bits; position times frequency, less the nearest whole number of
+// revolutions, is right to 2^-24 revolutions for positions of 2^31 and to 2^-34 for those of 2^21, where 32 bits would have lost all but 2^-6.  Sine and
+// cosine see half a revolution at most.
+// They are the same for all heads of a token: a workgroup makes them once, in LDS.
+#include <math.h>
+
+#include "svdq_common.h"
+
+using namespace svdq;
+
+namespace {
+
+constexpr int MAX_PAIRS = 128, MAX_AXES = 4, MOST_TOKENS = 8;
+
+struct RotaryParams {
+    const char *in[2], *norm[2];   // q, k
+    char *out[2];
+    const void *positions;
+    long long in_s[2][3], out_s[2][3];  // bytes: batch, token, head
+    long long pos_s[3];                 // elements: batch, token, axis
+    long long rows, first;              // tokens of all entries; this launch's first
+    int T, heads[2], D, pairs, halves, position_type, tokens;  // tokens: a workgroup's
+    float inv_d, eps, tiny;
+    double freq[MAX_PAIRS];  // revolutions per position
+    uint8_t axis[MAX_PAIRS];
+};
+
+template <bool BF16>
+__device__ inline void unpack(const u32x4_t w, float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t pair = w[j];
+        if (BF16) {
+            f[2 * j] = bits_f32(pair << 16);
+            f[2 * j + 1] = bits_f32(pair & 0xFFFF0000u);
+        } else {
+            const half2_t h = __builtin_bit_cast(half2_t, pair);
+            f[2 * j] = (float)h[0];
+            f[2 * j + 1] = (float)h[1];
+        }
+    }
+}
+template <bool BF16>
+__device__ inline u32x4_t pack(const float (&f)[8]) {
+    u32x4_t w;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (BF16) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+        else w[j] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]) << 16);
+    }
+    return w;
+}
+
+// LANES threads to a head, a piece of 8 channels each
+template <bool BF16, int LANES>
+__global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
+    typedef float float2_t __attribute__((ext_vector_type(2)));
+    __shared__ float2_t turns[MOST_TOKENS * MAX_PAIRS];  // cosine, sine
+    const long long row0 = p.first + (long long)blockIdx.x * p.tokens;
+    const int count = (int)(p.rows - row0 < p.tokens ? p.rows - row0 : p.tokens);
+    for (int i = threadIdx.x; i < count * p.pairs; i += 256) {
+        const int n = i / p.pairs, pair = i - n * p.pairs;
+        const long long row = row0 + n, b = row / p.T, t = row - b * p.T, at = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
+        const double x = p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[at]
+                         : p.position_type == SVDQ_POSITION_INT64 ? (double)((const int64_t *)p.positions)[at] : (double)((const float *)p.positions)[at];
+        const double revolutions = x * p.freq[pair];
+        float s, c;
+        sincospif(2.0f * (float)(revolutions - __builtin_rint(revolutions)), &s, &c);
+        turns[i] = float2_t{c, s};
+    }
+    __syncthreads();
+    const int c = threadIdx.x % LANES, pieces = p.D / 8, heads = p.heads[0] + p.heads[1], half = p.pairs / 8;
+    const bool in = c < pieces;
+    constexpr int SLOTS = 256 / LANES;
+    for (int item = threadIdx.x / LANES; item < count * heads; item += SLOTS) {
+        const int n = item / heads, any = item - n * heads, which = any >= p.heads[0], head = which ? any - p.heads[0] : any;
+        const long long row = row0 + n, b = row / p.T, t = row - b * p.T;
+        u32x4_t w = u32x4_t{0, 0, 0, 0};
+        float x[8], y[8];
+        if (in) w = *(const u32x4_t *)(p.in[which] + b * p.in_s[which][0] + t * p.in_s[which][1] + head * p.in_s[which][2] + c * 16);
+        unpack<BF16>(w, x);
+        if (p.norm[which]) {
+            float squares = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) squares = __builtin_fmaf(x[j], x[j], squares);
+#pragma unroll
+            for (int d = LANES / 2; d; d >>= 1) squares += __shfl_xor(squares, d);
+            if (squares < 0x1p120f && squares >= p.tiny) {
+                const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_d, p.eps));
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] *= r;
+            } else {  // squares that leave fp32's range: once more in 64 bits
+                double s = 0.0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) s += (double)x[j] * (double)x[j];
+#pragma unroll
+                for (int d = LANES / 2; d; d >>= 1) s += __shfl_xor(s, d);
+                const double r = 1.0 / __builtin_sqrt(s / (double)p.D + (double)p.eps);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = (float)((double)x[j] * r);
+            }
+            u32x4_t g = u32x4_t{0, 0, 0, 0};
+            if (in) g = *(const u32x4_t *)(p.norm[which] + c * 16);
+            unpack<BF16>(g, y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= y[j];
+        }
+        const float2_t *turn = turns + n * p.pairs;
+        if (p.halves) {
+            const bool low = c < half;
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = __shfl(x[j], low ? c + half : c - half, LANES);
+            if (c < 2 * half) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float2_t cs = turn[(low ? c : c - half) * 8 + j];
+                    x[j] = low ? x[j] * cs[0] - y[j] * cs[1] : y[j] * cs[1] + x[j] * cs[0];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int pair = c * 4 + j;
+                const float2_t cs = pair < p.pairs ? turn[pair] : float2_t{1.f, 0.f};
+                const float a = x[2 * j], d = x[2 * j + 1];
+                if (pair < p.pairs) {
+                    x[2 * j] = a * cs[0] - d * cs[1];
+                    x[2 * j + 1] = a * cs[1] + d * cs[0];
+                }
+            }
+        }
+        if (in) *(u32x4_t *)(p.out[which] + b * p.out_s[which][0] + t * p.out_s[which][1] + head * p.out_s[which][2] + c * 16) = pack<BF16>(x);
+    }
+}
+
+template <bool BF16>
+void dispatch(const RotaryParams &p, unsigned blocks, hipStream_t st) {
+    const dim3 grid(blocks), block(256);
+    if (p.D <= 32) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 4>), grid, block, 0, st, p);
+    else if (p.D <= 64) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 8>), grid, block, 0, st, p);
+    else if (p.D <= 128) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 16>), grid, block, 0, st, p);
+    else SVDQ_LAUNCH((rotary_axes_kernel<BF16, 32>), grid, block, 0, st, p);
+}
+
+}  // namespace
+
+extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
+    SVDQ_REQUIRE(a && a->q && a->q_out && a->positions, "rotary_axes: q, q_out and positions must not be null");
+    SVDQ_REQUIRE(!a->k == !a->k_out && (a->k || !a->norm_k), "rotary_axes: k, k_out and norm_k belong together");
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "rotary_axes: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
+    SVDQ_REQUIRE(a->position_type >= SVDQ_POSITION_INT32 && a->position_type <= SVDQ_POSITION_FP32, "rotary_axes: position_type %d is unknown", (int)a->position_type);
+    SVDQ_REQUIRE(a->batch > 0 && a->tokens > 0 && a->batch < (1ll << 31) && a->tokens < (1ll << 31) && a->batch * a->tokens < (1ll << 31),
+                 "rotary_axes: batch (%lld) times tokens (%lld) must be in 1..2^31-1", (long long)a->batch, (long long)a->tokens);
+    SVDQ_REQUIRE(a->heads > 0 && a->heads < 65536 && (!a->k || (a->kv_heads > 0 && a->kv_heads < 65536)), "rotary_axes: heads (%lld, %lld) must be in 1..65535", (long long)a->heads,
+                 (long long)a->kv_heads);
+    SVDQ_REQUIRE(a->head_dim > 0 && a->head_dim <= 2 * MAX_PAIRS && a->head_dim % 8 == 0, "rotary_axes: head_dim (%lld) must be a multiple of 8 up to 256", (long long)a->head_dim);
+    SVDQ_REQUIRE(a->axes > 0 && a->axes <= MAX_AXES, "rotary_axes: axes (%lld) must be in 1..4", (long long)a->axes);
+    int64_t rotated = 0;
+    for (int i = 0; i < a->axes; i++) {
+        SVDQ_REQUIRE(a->axis_dim[i] > 0 && a->axis_dim[i] % 2 == 0 && a->axis_dim[i] <= a->head_dim, "rotary_axes: axis_dim[%d] (%lld) must be even and positive", i, (long long)a->axis_dim[i]);
+        SVDQ_REQUIRE(a->theta[i] > 0.0 && a->theta[i] < __builtin_huge_val(), "rotary_axes: theta must be a positive number");
+        rotated += a->axis_dim[i];
+    }
+    SVDQ_REQUIRE(rotated <= a->head_dim, "rotary_axes: the axes' channels (%lld) must not be more than head_dim (%lld)", (long long)rotated, (long long)a->head_dim);
+    SVDQ_REQUIRE(!a->halves || rotated % 16 == 0, "rotary_axes: halves of the rotated channels (%lld) must be multiples of 8", (long long)rotated);
+    for (int i = 0; i < 3; i++)
+        SVDQ_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->q_out_stride[i] >= 0 && a->k_out_stride[i] >= 0 &&
+                         (a->q_stride[i] | a->k_stride[i] | a->q_out_stride[i] | a->k_out_stride[i]) % 8 == 0,
+                     "rotary_axes: strides must be multiples of 8 elements (16 bytes)");
+    SVDQ_REQUIRE(a->position_stride[0] >= 0 && a->position_stride[1] >= 0 && a->position_stride[2] >= 0, "rotary_axes: strides of positions must not be negative");
+    SVDQ_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->q_out | (uintptr_t)a->k_out | (uintptr_t)a->norm_q | (uintptr_t)a->norm_k) % 16 == 0,
+                 "rotary_axes: pointers must be 16-byte aligned");
+    SVDQ_REQUIRE((uintptr_t)a->positions % (a->position_type == SVDQ_POSITION_INT64 ? 8 : 4) == 0, "rotary_axes: positions must be aligned to their type");
+    SVDQ_REQUIRE(a->eps >= 0.f && a->eps < __builtin_huge_valf(), "rotary_axes: eps must be a finite number not below zero");
+    RotaryParams p;
+    const void *ins[2] = {a->q, a->k}, *norms[2] = {a->norm_q, a->norm_k};
+    void *outs[2] = {a->q_out, a->k_out};
+    const int64_t *in_s[2] = {a->q_stride, a->k_stride}, *out_s[2] = {a->q_out_stride, a->k_out_stride};
+    for (int i = 0; i < 2; i++) {
+        p.in[i] = (const char *)ins[i];
+        p.norm[i] = (const char *)norms[i];
+        p.out[i] = (char *)outs[i];
+        for (int j = 0; j < 3; j++) {
+            p.in_s[i][j] = in_s[i][j] * 2;
+            p.out_s[i][j] = out_s[i][j] * 2;
+        }
+    }
+    p.positions = a->positions;
+    for (int j = 0; j < 3; j++) p.pos_s[j] = a->position_stride[j];
+    p.rows = a->batch * a->tokens;
+    p.T = (int)a->tokens;
+    p.heads[0] = (int)a->heads;
+    p.heads[1] = a->k ? (int)a->kv_heads : 0;
+    p.D = (int)a->head_dim;
+    p.pairs = (int)(rotated / 2);
+    p.halves = a->halves != 0;
+    p.position_type = a->position_type;
+    p.inv_d = 1.0f / (float)a->head_dim;
+    p.eps = a->eps;
+    p.tiny = a->eps >= 0x1p-120f ? 0.f : 0x1p-100f;
+    // An axis' frequencies are a geometric series; its products in 80 bits are right to more than the 64 bits they are rounded to
+    int pair = 0;
+    for (int i = 0; i < a->axes; i++) {
+        const long double span = a->whole_spectrum ? (long double)rotated : (long double)a->axis_dim[i], rate = -logl((long double)a->theta[i]);
+        const long double step = expl(rate * 2.0L / span);
+        long double f = (a->whole_spectrum ? expl(rate * 2.0L * pair / span) : 1.0L) / 6.283185307179586476925286766559L;
+        for (int j = 0; j < a->axis_dim[i] / 2; j++, pair++, f *= step) {
+            p.freq[pair] = (double)f;
+            p.axis[pair] = (uint8_t)i;
+        }
+    }
+    p.tokens = p.rows >= 4096 ? 4 : 1;
+    // a launch takes fewer than 2^32 threads
+    const long long most = (1ll << 23) * p.tokens;
+    const long long all = p.rows;
+    for (p.first = 0; p.first < all; p.first += most) {
+        p.rows = all - p.first < most ? all : p.first + most;
+        const unsigned blocks = (unsigned)((p.rows - p.first + p.tokens - 1) / p.tokens);
+        if (a->dtype == SVDQ_BF16) dispatch<true>(p, blocks, (hipStream_t)stream);
+        else dispatch<false>(p, blocks, (hipStream_t)stream);
+        if (int rc = check_launch("rotary_axes")) return rc;
+    }
+    return SVDQ_OK;
+}

@@ -1,0 +1,509 @@
+// Softmax attention of the queries of several sequences to the keys of the same sequence, causal or not: query i of a sequence with n_q queries and
+// n_k keys sees the keys j <= i + n_k - n_q (all of them where it is not causal).  G = heads / kv_heads query heads share a head of keys: a "row"
+// below is one (token, head of the group) pair, row r = t * G + g of a sequence and a key head, so that a few tokens fill the rows of a matrix
+// instruction, and the rows of a block end at nearly the same key.
+//
+// Which rows a workgroup has is worked out on the device: sequences' lengths are there, and a launch has as many blocks of rows as there may be at most.
+#include "attention_core.h"
+
+using namespace svdq;
+using namespace svdq::attention;
+
+namespace {
+
+struct Params {
+    const char *q, *k, *v;
+    char *out;
+    const int *cu_q, *cu_k, *lengths;
+    float *partial;                            // several parts: [part][key head][row of all sequences] x D, then {maximum, sum} pairs
+    long long qs[3], ks[3], vs[3], os[3];      // bytes: batch, token, head
+    long long all_rows;                        // rows of a key head, of all sequences
+    int S, Hkv, G, D, Tq, Tk, blocks, parts, causal, zero_rest;  // blocks: of rows, for every key head and part
+    float scale2;                              // scale * log2(e)
+};
+
+__device__ inline int clamped(int x, int lo, int hi) { return x < lo ? lo : x < hi ? x : hi; }
+
+// A sequence's queries: where they start in q and out (packed: rows of all of them), and how many.  Rows in no sequence, in front of the first and behind
+// the last, are the queries of two more, without keys: number S and S + 1.
+__device__ inline void queries_of(const Params &p, int s, int &first, int &count) {
+    first = 0;
+    count = p.Tq;
+    if (!p.cu_q) return;
+    int lo, hi;
+    if (s < p.S) {
+        lo = p.cu_q[s];
+        hi = p.cu_q[s + 1];
+    } else {
+        lo = s == p.S ? 0 : p.cu_q[p.S];
+        hi = s == p.S ? p.cu_q[0] : p.Tq;
+        if (!p.zero_rest) hi = lo;
+    }
+    first = clamped(lo, 0, p.Tq);
+    count = clamped(hi, first, p.Tq) - first;
+}
+
+struct Block {
+    int s, first, count, rb;  // sequence, its first query's row of q (of a batch entry: 0), its queries, block of rows
+    bool any;
+};
+
+// Block number `at` of all sequences' blocks of ROWS rows.  A sequence's last block comes first: with a causal mask it has the most keys.
+template <int ROWS>
+__device__ inline Block block_of(const Params &p, int at, int lane) {
+    Block b;
+    if (!p.cu_q) {
+        const int each = (int)(((long long)p.Tq * p.G + ROWS - 1) / ROWS);
+        b.s = at % p.S;
+        b.rb = each - 1 - at / p.S;
+        b.first = 0;
+        b.count = p.Tq;
+        b.any = true;
+        return b;
+    }
+    b.any = false;
+    b.s = b.first = b.count = b.rb = 0;
+    int left = at;
+    for (int base = 0; base < p.S + 2; base += 64) {  // 64 sequences at a time, one to a lane
+        int first = 0, count = 0;
+        if (base + lane < p.S + 2) queries_of(p, base + lane, first, count);
+        const int mine = (int)(((long long)count * p.G + ROWS - 1) / ROWS);
+        int upto = mine;  // blocks of this sequence and those in front of it
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d);
+            if (lane >= d) upto = upto + o < 1 << 29 ? upto + o : 1 << 29;  // (offsets that are not in order can make any sum)
+        }
+        const uint64_t behind = __ballot(left < upto);
+        if (behind) {
+            const int l = __builtin_ctzll(behind);
+            b.s = base + l;
+            b.first = __builtin_amdgcn_readlane(first, l);
+            b.count = __builtin_amdgcn_readlane(count, l);
+            b.rb = __builtin_amdgcn_readlane(upto, l) - 1 - left;
+            b.any = b.rb < __builtin_amdgcn_readlane(mine, l);
+            return b;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return b;
+}
+
+// The keys of sequence s: the row of k and v (of its batch entry, if they are not packed) that the first one has, and how many there are
+__device__ inline void keys_of(const Params &p, int s, long long &first, int &count) {
+    first = 0;
+    count = 0;
+    if (s >= p.S) return;
+    if (p.cu_k) {
+        const int lo = clamped(p.cu_k[s], 0, p.Tk);
+        count = clamped(p.cu_k[s + 1], lo, p.Tk) - lo;
+        first = __builtin_amdgcn_readfirstlane(lo);
+    } else {
+        count = p.lengths ? clamped(p.lengths[s], 0, p.Tk) : p.Tk;
+    }
+    count = __builtin_amdgcn_readfirstlane(count);
+}
+
+// Rows of a block and the keys they see
+struct Rows {
+    const char *q;
+    char *out;
+    long long index;   // of this lane's row among all
+    int row, limit;    // this lane's; it sees the keys in front of `limit`
+    int least, most;   // the limits of the block's first row and of its last
+    bool in;
+};
+template <int ROWS>
+__device__ inline Rows rows_of(const Params &p, const Block &b, int keys, int hk, int row, int lane) {
+    Rows r;
+    const int total = b.count * p.G, t = row / p.G, g = row - t * p.G, off = keys - b.count;
+    const long long head = hk * p.G + g, entry = p.cu_q ? 0 : b.s;
+    r.row = row;
+    r.in = row < total;
+    r.q = p.q + entry * p.qs[0] + (long long)(b.first + t) * p.qs[1] + head * p.qs[2];
+    r.out = p.out + entry * p.os[0] + (long long)(b.first + t) * p.os[1] + head * p.os[2];
+    r.index = (entry * p.Tq + b.first) * p.G + row;
+    const int t0 = b.rb * ROWS / p.G, last = b.rb * ROWS + ROWS < total ? b.rb * ROWS + ROWS - 1 : total - 1, t1 = last / p.G;
+    r.limit = p.causal ? clamped(t + off + 1, 0, keys) : keys;
+    r.least = p.causal ? clamped(t0 + off + 1, 0, keys) : keys;
+    r.most = p.causal ? clamped(t1 + off + 1, 0, keys) : keys;
+    return r;
+}
+
+template <bool BF16, typename H>
+__device__ inline void load_q(const Params &p, typename Elem<BF16>::vec (&qf)[H::KS], const Rows &r, int lane) {
+#pragma unroll
+    for (int ks = 0; ks < H::KS; ks++) {
+        const int c = 16 * ks + 8 * (lane >> 5);
+        u32x4_t w = u32x4_t{0, 0, 0, 0};
+        if (r.in && c < p.D) w = *(const u32x4_t *)(r.q + c * 2);
+        qf[ks] = __builtin_bit_cast(typename Elem<BF16>::vec, w);
+    }
+}
+template <bool BF16, typename H>
+__device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[H::KS]) {
+#pragma unroll
+    for (int ks = 0; ks < H::KS; ks++) asm volatile("" : "+v"(qf[ks]));
+}
+
+__device__ inline void share(const Params &p, int part, int &begin, int &end) {
+    if (p.parts == 1) return;
+    const int each = end / p.parts, more = end - each * p.parts;
+    begin = part * each + (part < more ? part : more);
+    end = begin + each + (part < more);
+}
+__device__ inline float *part_of(const Params &p, int part, int hk, long long index) { return p.partial + (((long long)part * p.Hkv + hk) * p.all_rows + index) * p.D; }
+__device__ inline void store_stats(const Params &p, int part, int hk, long long index, float top, float sum) {
+    float *ms = p.partial + (long long)p.parts * p.Hkv * p.all_rows * p.D + (((long long)part * p.Hkv + hk) * p.all_rows + index) * 2;
+    ms[0] = top;
+    ms[1] = sum;
+}
+
+// A step in which some rows do not see some keys, where what such a key has in V is an infinity or a NaN: zero times it is a NaN, too.  A key at a time; rows that
+// do not see it keep what they have.
+template <bool BF16, typename H, int NB>
+__device__ __attribute__((noinline)) void attend_key_by_key(State<BF16, H> &st, float16_t (&s)[NB], float scale2, const char *v, int first, int limit, int lane) {
+    using vec = typename Elem<BF16>::vec;
+    st.raise(st.highest(s), scale2);
+    const float ref = st.reference();
+#pragma unroll
+    for (int n = 0; n < 2 * NB; n++) {
+        vec vf[H::DB];
+        st.read_v(vf, v, n, lane);
+        const u32x4_t pr = __builtin_bit_cast(u32x4_t, st.template exponentials<NB, H::ONES>(s, n, scale2, ref));
+#pragma unroll 1
+        for (int j = 0; j < 16; j++) {  // (element 4 (j / 8) + j % 4 of the half-wave j / 4 % 2)
+            const int at = 4 * (j >> 3) + (j & 3);
+            const bool half = (lane >> 5) == ((j >> 2) & 1), seen = first + 16 * n + j < limit;
+            u32x4_t keep;
+#pragma unroll
+            for (int w = 0; w < 4; w++) keep[w] = half && at >> 1 == w ? (at & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
+            const vec p = __builtin_bit_cast(vec, pr & keep);
+#pragma unroll
+            for (int d = 0; d < H::DB; d++) {
+                const float16_t o = Elem<BF16>::mfma(__builtin_bit_cast(vec, __builtin_bit_cast(u32x4_t, vf[d]) & keep), p, st.o[d]);
+#pragma unroll
+                for (int e = 0; e < 16; e++) st.o[d][e] = seen ? o[e] : st.o[d][e];
+            }
+        }
+    }
+}
+// whether a sum of this wave's is a NaN or an infinity, of the head's columns (what stands behind them in LDS is nobody's)
+template <bool BF16, typename H>
+__device__ inline bool any_nan(const State<BF16, H> &st, int D) {
+    float x = 0.f;
+#pragma unroll
+    for (int d = 0; d < H::DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (32 * d + 8 * (e >> 2) < D) x = __builtin_fmaf(st.o[d][e], 0.f, x);
+    return __any(x != x);
+}
+
+// keys that a row does not see get a score of minus infinity: those from `limit` on, of NB blocks of 32 from key `first` on
+template <int NB>
+__device__ inline void hide(float16_t (&s)[NB], int first, int limit, int lane) {
+    const int left = limit - first - 4 * (lane >> 5);
+#pragma unroll
+    for (int kb = 0; kb < NB; kb++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (32 * kb + 8 * (e >> 2) + (e & 3) >= left) s[kb][e] = -__builtin_huge_valf();
+}
+
+// ---- keys form: 32 rows per workgroup, whose waves take every fourth step (of 32 keys) of the part's keys, each through its own LDS, a
+// step ahead, and meet in LDS at the end; the parts of a row block meet in self_attention_join_kernel ------------------------------------
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_kernel(Params p) {
+    using H = Head<DP, true>;
+    using E = Elem<BF16>;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, part = rest % p.parts;
+    const Block b = block_of<32>(p, rest / p.parts, lane);
+    if (!b.any) return;
+    long long first;
+    int count;
+    keys_of(p, b.s, first, count);
+    const Rows r = rows_of<32>(p, b, count, hk, b.rb * 32 + col, lane);
+    typename E::vec qf[H::KS];
+    load_q<BF16, H>(p, qf, r, lane);
+    const char *kp = p.k + (p.cu_k ? 0 : b.s) * p.ks[0] + first * p.ks[1] + hk * p.ks[2];
+    const char *vp = p.v + (p.cu_k ? 0 : b.s) * p.vs[0] + first * p.vs[1] + hk * p.vs[2];
+    constexpr int SIZE = 32, REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
+    char *mine = lds + wave * 2 * STAGE;
+    const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 2 * STAGE;
+    const int bytes = p.D * 2;
+    int begin = 0, end = (r.most + SIZE - 1) / SIZE;
+    share(p, part, begin, end);
+    // Request i brings rows r0 + i * RPR: of V the same piece every time, of K the pieces that f has there
+    const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
+    const uint32_t ok = (uint32_t)(r0 * p.ks[1]), ov = (uint32_t)(r0 * p.vs[1]) + cv;
+    static_assert(H::fv(H::RPR) == 0 && (H::RPR == 16 || H::fk(H::RPR) == 4), "");
+    // columns behind the head's end are zero in K for good (the wait for a step's copies is one for these, too)
+    zero_columns<H, SIZE>(mine, p.D / 8, lane, 64);
+    zero_columns<H, SIZE>(mine + STAGE, p.D / 8, lane, 64);
+    auto request = [&](int step, int slot) __attribute__((always_inline)) {
+        const char *k = kp + (long long)step * SIZE * p.ks[1], *v = vp + (long long)step * SIZE * p.vs[1];
+        const int left = r.most - step * SIZE;
+        const uint32_t dst = area + slot * STAGE;
+#pragma unroll
+        for (int i = 0; i < REQ; i++) {
+            const int c = ck ^ (64 * (i & (16 / H::RPR - 1)));
+            if (c < bytes && r0 < left - i * H::RPR) copy16(dst + i * 1024, k + i * H::RPR * p.ks[1], ok + c);
+        }
+#pragma unroll
+        for (int i = 0; i < REQ; i++) {
+            if (cv >= bytes) continue;
+            if (r0 < left - i * H::RPR) copy16(dst + STAGE / 2 + i * 1024, v + i * H::RPR * p.vs[1], ov);
+            else clear16(dst + STAGE / 2 + i * 1024 + lane * 16);
+        }
+    };
+    State<BF16, H> st;
+    // Once more, key by key where rows do not see all keys, if sums turn out to hold a NaN: rows that see none of its causes have none then
+    for (bool careful = false;; careful = true) {
+        st.clear();
+        int step = begin + wave;
+        if (step < end) request(step, 0);
+        wait_for_q<BF16, H>(qf);
+        for (int slot = 0; step < end; slot ^= 1) {
+            const int next = step + 4;
+            if (next < end) request(next, slot ^ 1);
+            // This step's copies have landed when no more than the next one's are on their way.  Of a step with keys behind the last one some
+            // requests may have had no lane to make them: then all have to land.
+            if (next < end && r.most - next * SIZE >= SIZE) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            const char *k = mine + slot * STAGE + col * H::PITCH, *v = mine + slot * STAGE + STAGE / 2;
+            float16_t s[1];
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[0][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < H::KS; ks++) {
+                const u32x4_t w = *(const u32x4_t *)(k + ((2 * ks + h) ^ H::fk(col)) * 16);
+                s[0] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[0]);
+            }
+            const bool some = r.least < (step + 1) * SIZE;
+            if (some) hide(s, step * SIZE, r.limit, lane);
+            if (some && careful) attend_key_by_key(st, s, p.scale2, v, step * SIZE, r.limit, lane);
+            else st.template attend<false>(s, 0xFFFFFFFFull, p.scale2, v, lane);
+            step = next;
+        }
+        if (careful || !p.causal || !any_nan(st, p.D)) break;
+    }
+    // The waves meet.  Each leaves its maximum, sum and outputs in the place of its own stages, 16 columns (a unit) of 64 lanes in 2 KB, and takes
+    // every fourth unit of all four, scaled to the highest maximum.
+    constexpr int UNITS = 2 * H::DB, AREA = 2 * STAGE;
+    static_assert(256 + UNITS * 2048 <= AREA, "");
+    const float own = across_sum(st.sum);
+    if (h == 0) {
+        ((float *)mine)[col] = st.top;
+        ((float *)mine)[32 + col] = own;
+    }
+    if (r.in) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int d = u >> 1, e = 8 * (u & 1) + 4 * i;
+                ((float4_t *)(mine + 256 + u * 2048 + i * 1024))[lane] = float4_t{st.o[d][e], st.o[d][e + 1], st.o[d][e + 2], st.o[d][e + 3]};
+            }
+    }
+    __syncthreads();
+    float top = -__builtin_huge_valf(), sum = 0.f, f[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, ((float *)(lds + i * AREA))[col]);
+    const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f[i] = __builtin_amdgcn_exp2f(((float *)(lds + i * AREA))[col] - ref);
+        sum += ((float *)(lds + i * AREA))[32 + col] * f[i];
+    }
+    const float inv = inverse(sum);
+    float *dst = part_of(p, part, hk, r.index);
+    const int columns = r.in ? p.D : 0;
+    for (int u = wave; u < UNITS; u += 4) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float4_t y = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4_t o = ((float4_t *)(lds + w * AREA + 256 + u * 2048 + i * 1024))[lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(o[e], f[w], y[e]);
+            }
+            const int c = 16 * u + 8 * i + 4 * h;
+            if (p.parts > 1 && c < columns) *(float4_t *)(dst + c) = y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * i + e] = y[e];
+        }
+        if (p.parts == 1) store_columns<BF16>(r.out, x, inv, 16 * u, columns, lane);
+    }
+    if (p.parts > 1 && wave == 0 && h == 0 && r.in) store_stats(p, part, hk, r.index, top, sum);
+}
+
+// Adds the parts of every row (at most 64): a wave to a row, two columns per lane; lane i holds part i's share of the row.
+constexpr int MAX_PARTS = 64;
+template <bool BF16>
+__global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long all = p.all_rows * p.Hkv, at = (long long)blockIdx.x * 4 + wave;
+    if (at >= all) return;
+    const int hk = (int)(at / p.all_rows);
+    const long long index = at - hk * p.all_rows, token = index / p.G;
+    if (p.cu_q && !p.zero_rest && (token < p.cu_q[0] || token >= p.cu_q[p.S])) return;
+    const float *ms = p.partial + p.parts * all * p.D;
+    const int c = lane * 2 < p.D ? lane * 2 : 0;
+    typedef float float2_t __attribute__((ext_vector_type(2)));
+    float top = -__builtin_huge_valf(), sum = 0.f;
+    if (lane < p.parts) {
+        const float2_t t = *(const float2_t *)(ms + (lane * all + at) * 2);
+        top = t[0];
+        sum = t[1];
+    }
+    float most = top;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    const float f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
+    sum *= f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    float x = 0.f, y = 0.f;
+    for (int i = 0; i < p.parts; i++) {
+        const float2_t part = *(const float2_t *)(p.partial + (i * all + at) * p.D + c);
+        const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), i));
+        x = __builtin_fmaf(part[0], g, x);
+        y = __builtin_fmaf(part[1], g, y);
+    }
+    if (lane * 2 >= p.D) return;
+    const float r = inverse(sum);
+    const long long entry = p.cu_q ? 0 : token / p.Tq, t = token - entry * p.Tq, head = hk * p.G + (index - token * p.G);
+    *(uint32_t *)(p.out + entry * p.os[0] + t * p.os[1] + head * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
+}
+
+template <bool BF16, int DP>
+int launch_kernels(const Params &p, hipStream_t st) {
+    const int lds = 8 * Head<DP, true>::TILE;
+    static bool reserved[64] = {false};
+    if (int rc = reserve_lds((const void *)self_attention_keys_kernel<BF16, DP>, lds, reserved, "self_attention")) return rc;
+    const dim3 grid((unsigned)((long long)p.blocks * p.parts * p.Hkv)), block(256);
+    SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, block, lds, st, p);
+    int rc = check_launch("self_attention");
+    if (rc || p.parts == 1) return rc;
+    const long long all = p.all_rows * p.Hkv;
+    SVDQ_LAUNCH((self_attention_join_kernel<BF16>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
+    return check_launch("self_attention");
+}
+
+template <bool BF16>
+int launch_heads(const Params &p, hipStream_t st) {
+    if (p.D <= 32) return launch_kernels<BF16, 32>(p, st);
+    if (p.D <= 64) return launch_kernels<BF16, 64>(p, st);
+    if (p.D <= 80) return launch_kernels<BF16, 80>(p, st);
+    if (p.D <= 96) return launch_kernels<BF16, 96>(p, st);
+    return launch_kernels<BF16, 128>(p, st);
+}
+
+struct Plan {
+    long long blocks, parts, workspace;
+};
+
+long long blocks_of(const svdq_self_attention_args *a, long long size) {
+    const long long rows = a->q_len * (a->heads / a->kv_heads);
+    // packed sequences: each, and the rows in front of them and behind, may end in the middle of a block
+    return a->cu_seqlens_q ? rows / size + (a->batch + 2 < a->q_len ? a->batch + 2 : a->q_len) : (rows + size - 1) / size * a->batch;
+}
+
+Plan plan_of(const svdq_self_attention_args *a, int cus) {
+    const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
+    Plan plan;
+    plan.blocks = blocks_of(a, 32);
+    plan.parts = 1;
+    while (plan.parts < MAX_PARTS && plan.blocks * a->kv_heads * plan.parts * 2 <= cus && keys_each >= 256 * plan.parts) plan.parts *= 2;
+    const long long rows = (a->cu_seqlens_q ? 1 : a->batch) * a->q_len * (a->heads / a->kv_heads);
+    plan.workspace = plan.parts > 1 ? plan.parts * a->kv_heads * rows * (a->head_dim + 2) * 4 : 0;
+    return plan;
+}
+
+int check_args(const svdq_self_attention_args *a) {
+    SVDQ_REQUIRE(a && a->q && a->k && a->v && a->out, "self_attention: q, k, v and out must not be null");
+    SVDQ_REQUIRE(a->dtype == SVDQ_BF16 || a->dtype == SVDQ_FP16, "self_attention: dtype must be SVDQ_BF16 or SVDQ_FP16, got %d", (int)a->dtype);
+    SVDQ_REQUIRE(a->batch > 0 && a->batch < 65536 && a->heads > 0 && a->heads < 65536 && a->kv_heads > 0 && a->heads % a->kv_heads == 0,
+                 "self_attention: batch (%lld) and heads (%lld) must be in 1..65535, kv_heads (%lld) must divide heads", (long long)a->batch, (long long)a->heads, (long long)a->kv_heads);
+    SVDQ_REQUIRE(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, "self_attention: head_dim (%lld) must be a multiple of 8 up to 128", (long long)a->head_dim);
+    SVDQ_REQUIRE(a->q_len > 0 && a->k_len > 0 && a->k_len < (1ll << 31) - 512, "self_attention: q_len (%lld) and k_len (%lld) must be positive, k_len below 2^31 - 512", (long long)a->q_len,
+                 (long long)a->k_len);
+    SVDQ_REQUIRE(a->q_len < (1ll << 31) && a->q_len * (a->heads / a->kv_heads) < (1ll << 31) - 512,
+                 "self_attention: q_len (%lld) times the heads that share keys must be below 2^31 - 512", (long long)a->q_len);
+    // (a launch takes fewer than 2^32 threads, 256 for 32 rows at most)
+    SVDQ_REQUIRE(blocks_of(a, 32) < (1ll << 24) && blocks_of(a, 32) * a->kv_heads < (1ll << 24), "self_attention: %lld queries of %lld heads are too many for one launch", (long long)a->q_len,
+                 (long long)a->heads);
+    SVDQ_REQUIRE(!a->key_lengths || !a->cu_seqlens_k, "self_attention: at most one of key_lengths and cu_seqlens_k can be given");
+    SVDQ_REQUIRE(a->scale > 0.f && a->scale < __builtin_huge_valf(), "self_attention: scale must be a positive number");
+    for (int i = 0; i < 3; i++)
+        SVDQ_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->v_stride[i] >= 0 && a->out_stride[i] >= 0 &&
+                         (a->q_stride[i] | a->k_stride[i] | a->v_stride[i] | a->out_stride[i]) % 8 == 0,
+                     "self_attention: strides must be multiples of 8 elements (16 bytes)");
+    SVDQ_REQUIRE(a->k_stride[1] < (1ll << 24) && a->v_stride[1] < (1ll << 24), "self_attention: the tokens of k and v must be less than 2^24 elements apart");
+    SVDQ_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)a->workspace) % 16 == 0, "self_attention: pointers must be 16-byte aligned");
+    SVDQ_REQUIRE(((uintptr_t)a->key_lengths | (uintptr_t)a->cu_seqlens_q | (uintptr_t)a->cu_seqlens_k) % 4 == 0,
+                 "self_attention: key_lengths, cu_seqlens_q and cu_seqlens_k must be 4-byte aligned");
+    return SVDQ_OK;
+}
+
+int current_compute_units(int &cus) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || (cus = compute_units(dev)) == 0) {
+        (void)hipGetLastError();
+        return fail(SVDQ_ELAUNCH, "self_attention: no current device");
+    }
+    return SVDQ_OK;
+}
+
+}  // namespace
+
+extern "C" int svdq_self_attention_workspace(const svdq_self_attention_args *a, int64_t *bytes) {
+    if (int rc = check_args(a)) return rc;
+    SVDQ_REQUIRE(bytes, "self_attention: bytes must not be null");
+    int cus;
+    if (int rc = current_compute_units(cus)) return rc;
+    *bytes = plan_of(a, cus).workspace;
+    return SVDQ_OK;
+}
+
+extern "C" int svdq_self_attention(const svdq_self_attention_args *a, void *stream) {
+    if (int rc = check_args(a)) return rc;
+    int cus;
+    if (int rc = current_compute_units(cus)) return rc;
+    const Plan plan = plan_of(a, cus);
+    SVDQ_REQUIRE(plan.workspace == 0 || (a->workspace && a->workspace_bytes >= plan.workspace), "self_attention: needs a workspace of %lld bytes, got %lld", plan.workspace,
+                 (long long)(a->workspace ? a->workspace_bytes : 0));
+    Params p;
+    p.q = (const char *)a->q;
+    p.k = (const char *)a->k;
+    p.v = (const char *)a->v;
+    p.out = (char *)a->out;
+    p.cu_q = a->cu_seqlens_q;
+    p.cu_k = a->cu_seqlens_k;
+    p.lengths = a->key_lengths;
+    p.partial = (float *)a->workspace;
+    for (int i = 0; i < 3; i++) {
+        p.qs[i] = a->q_stride[i] * 2;
+        p.ks[i] = a->k_stride[i] * 2;
+        p.vs[i] = a->v_stride[i] * 2;
+        p.os[i] = a->out_stride[i] * 2;
+    }
+    p.S = (int)a->batch;
+    p.Hkv = (int)a->kv_heads;
+    p.G = (int)(a->heads / a->kv_heads);
+    p.D = (int)a->head_dim;
+    p.Tq = (int)a->q_len;
+    p.Tk = (int)a->k_len;
+    p.all_rows = (a->cu_seqlens_q ? 1 : a->batch) * a->q_len * p.G;
+    p.blocks = (int)plan.blocks;
+    p.parts = (int)plan.parts;
+    p.causal = a->causal != 0;
+    p.zero_rest = a->zero_rest != 0;
+    p.scale2 = a->scale * 1.44269504088896340736f;
+    return a->dtype == SVDQ_BF16 ? launch_heads<true>(p, (hipStream_t)stream) : launch_heads<false>(p, (hipStream_t)stream);
+}
