@@ -104,30 +104,33 @@ __device__ inline void keys_of(const Params &p, int s, long long &first, int &co
     count = __builtin_amdgcn_readfirstlane(count);
 }
 
-// Rows of a block and the keys they see
+// This lane's row, and the keys that rows see
 struct Rows {
     const char *q;
     char *out;
-    long long index;   // of this lane's row among all
-    int row, limit;    // this lane's; it sees the keys in front of `limit`
-    int least, most;   // the limits of the block's first row and of its last
+    long long index;  // of the row among all
+    int total, off, limit;  // rows of the sequence; key of its first query; the row sees the keys in front of `limit`
     bool in;
 };
-template <int ROWS>
-__device__ inline Rows rows_of(const Params &p, const Block &b, int keys, int hk, int row, int lane) {
+__device__ inline int limit_of(const Params &p, const Rows &r, int row, int keys) { return p.causal ? clamped(row / p.G + r.off + 1, 0, keys) : keys; }
+__device__ inline Rows rows_of(const Params &p, const Block &b, int keys, int hk, int row) {
     Rows r;
-    const int total = b.count * p.G, t = row / p.G, g = row - t * p.G, off = keys - b.count;
+    const int t = row / p.G, g = row - t * p.G;
     const long long head = hk * p.G + g, entry = p.cu_q ? 0 : b.s;
-    r.row = row;
-    r.in = row < total;
+    r.total = b.count * p.G;
+    r.off = keys - b.count;
+    r.in = row < r.total;
     r.q = p.q + entry * p.qs[0] + (long long)(b.first + t) * p.qs[1] + head * p.qs[2];
     r.out = p.out + entry * p.os[0] + (long long)(b.first + t) * p.os[1] + head * p.os[2];
     r.index = (entry * p.Tq + b.first) * p.G + row;
-    const int t0 = b.rb * ROWS / p.G, last = b.rb * ROWS + ROWS < total ? b.rb * ROWS + ROWS - 1 : total - 1, t1 = last / p.G;
-    r.limit = p.causal ? clamped(t + off + 1, 0, keys) : keys;
-    r.least = p.causal ? clamped(t0 + off + 1, 0, keys) : keys;
-    r.most = p.causal ? clamped(t1 + off + 1, 0, keys) : keys;
+    r.limit = limit_of(p, r, row, keys);
     return r;
+}
+// The limits of the first of `count` rows from `row` on and of the last one of the sequence among them (none: zero keys)
+__device__ inline void limits_of(const Params &p, const Rows &r, int row, int count, int keys, int &least, int &most) {
+    const int last = row + count < r.total ? row + count - 1 : r.total - 1;
+    least = limit_of(p, r, row, keys);
+    most = last < row ? 0 : limit_of(p, r, last, keys);
 }
 
 template <bool BF16, typename H>
@@ -162,7 +165,7 @@ __device__ inline void store_stats(const Params &p, int part, int hk, long long 
 // A step in which some rows do not see some keys, where what such a key has in V is an infinity or a NaN: zero times it is a NaN, too.  A key at a time; rows that
 // do not see it keep what they have.
 template <bool BF16, typename H, int NB>
-__device__ __attribute__((noinline)) void attend_key_by_key(State<BF16, H> &st, float16_t (&s)[NB], float scale2, const char *v, int first, int limit, int lane) {
+__device__ inline void attend_key_by_key(State<BF16, H> &st, float16_t (&s)[NB], float scale2, const char *v, int first, int limit, int lane) {
     using vec = typename Elem<BF16>::vec;
     st.raise(st.highest(s), scale2);
     const float ref = st.reference();
@@ -225,7 +228,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     long long first;
     int count;
     keys_of(p, b.s, first, count);
-    const Rows r = rows_of<32>(p, b, count, hk, b.rb * 32 + col, lane);
+    const Rows r = rows_of(p, b, count, hk, b.rb * 32 + col);
+    int least, most;
+    limits_of(p, r, b.rb * 32, 32, count, least, most);
     typename E::vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
     const char *kp = p.k + (p.cu_k ? 0 : b.s) * p.ks[0] + first * p.ks[1] + hk * p.ks[2];
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     char *mine = lds + wave * 2 * STAGE;
     const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 2 * STAGE;
     const int bytes = p.D * 2;
-    int begin = 0, end = (r.most + SIZE - 1) / SIZE;
+    int begin = 0, end = (most + SIZE - 1) / SIZE;
     share(p, part, begin, end);
     // Request i brings rows r0 + i * RPR: of V the same piece every time, of K the pieces that f has there
     const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     zero_columns<H, SIZE>(mine + STAGE, p.D / 8, lane, 64);
     auto request = [&](int step, int slot) __attribute__((always_inline)) {
         const char *k = kp + (long long)step * SIZE * p.ks[1], *v = vp + (long long)step * SIZE * p.vs[1];
-        const int left = r.most - step * SIZE;
+        const int left = most - step * SIZE;
         const uint32_t dst = area + slot * STAGE;
 #pragma unroll
         for (int i = 0; i < REQ; i++) {
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
             if (next < end) request(next, slot ^ 1);
             // This step's copies have landed when no more than the next one's are on their way.  Of a step with keys behind the last one some
             // requests may have had no lane to make them: then all have to land.
-            if (next < end && r.most - next * SIZE >= SIZE) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ) : "memory");
+            if (next < end && most - next * SIZE >= SIZE) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * REQ) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             const char *k = mine + slot * STAGE + col * H::PITCH, *v = mine + slot * STAGE + STAGE / 2;
             float16_t s[1];
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
                 const u32x4_t w = *(const u32x4_t *)(k + ((2 * ks + h) ^ H::fk(col)) * 16);
                 s[0] = E::mfma(__builtin_bit_cast(typename E::vec, w), qf[ks], s[0]);
             }
-            const bool some = r.least < (step + 1) * SIZE;
+            const bool some = least < (step + 1) * SIZE;
             if (some) hide(s, step * SIZE, r.limit, lane);
             if (some && careful) attend_key_by_key(st, s, p.scale2, v, step * SIZE, r.limit, lane);
             else st.template attend<false>(s, 0xFFFFFFFFull, p.scale2, v, lane);
@@ -342,6 +347,258 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     if (p.parts > 1 && wave == 0 && h == 0 && r.in) store_stats(p, part, hk, r.index, top, sum);
 }
 
+// ---- rows form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
+// The two waves of a SIMD take turns: while one makes probabilities of its scores (vector instructions), the other multiplies (the probabilities before
+// those with V, the next keys with Q).  A phase is one or the other; waves 4 .. 7 are one phase behind waves 0 .. 3, and a barrier ends a phase for all.
+// In phase 2 j the first four waves make the probabilities of step j, in phase 2 j + 1 they multiply them and score step j + 1.  Keys and values of step i are
+// read in phases 2 i - 1 .. 2 i + 2; those of step i + 4 take their place, asked for in phase 2 i + 3, by all waves, and waited for at the end of phase 2 i + 6.
+constexpr int STAGES = 4, WAVES = 8;
+
+__device__ inline void phase_ends() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// A wave's share of the copies of K and V: the same requests at every step, one or two of K and as many of V
+template <typename H>
+struct RowCopies {
+    static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
+    const char *k, *v;
+    long long k_step, v_step;
+    uint32_t dst, ok[REQ], ov[REQ];
+    int row[REQ], most, steps;
+    bool any, in_k[REQ], in_v[REQ];  // whether the piece lies in the head
+    __device__ inline RowCopies(const Params &p, char *lds, const char *kp, const char *vp, int most_, int wave, int lane) {
+        k = kp;
+        v = vp;
+        k_step = KEYS * p.ks[1];
+        v_step = KEYS * p.vs[1];
+        most = most_;
+        steps = (most + KEYS - 1) / KEYS;
+        any = wave < ACTIVE;
+        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
+#pragma unroll
+        for (int i = 0; i < REQ; i++) {
+            const int piece = (wave * REQ + i) * 64 + lane, place = piece % H::PIECES;
+            row[i] = piece / H::PIECES;
+            const int ck = (place ^ H::fk(row[i])) * 16, cv = (place ^ H::fv(row[i])) * 16;
+            ok[i] = (uint32_t)(row[i] * p.ks[1]) + ck;
+            ov[i] = (uint32_t)(row[i] * p.vs[1]) + cv;
+            in_k[i] = ck < p.D * 2;
+            in_v[i] = cv < p.D * 2;
+        }
+    }
+    // Rows behind the last key are not read: their scores are masked whatever K holds, and V holds zeros there, since nothing times a NaN is one.
+    __device__ inline void ask(int step, int slot) const {
+        if (!any || step >= steps) return;
+        const char *ks = k + step * k_step, *vs = v + step * v_step;
+        const uint32_t to = dst + slot * H::TILE;
+        const int left = most - step * KEYS;
+        if (left >= KEYS) {
+#pragma unroll
+            for (int i = 0; i < REQ; i++)
+                if (in_k[i]) copy16(to + i * 1024, ks, ok[i]);
+#pragma unroll
+            for (int i = 0; i < REQ; i++)
+                if (in_v[i]) copy16(to + STAGES * H::TILE + i * 1024, vs, ov[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < REQ; i++) {
+                if (in_k[i] && row[i] < left) copy16(to + i * 1024, ks, ok[i]);
+                if (in_v[i]) {
+                    if (row[i] < left) copy16(to + STAGES * H::TILE + i * 1024, vs, ov[i]);
+                    else clear16(to + STAGES * H::TILE + i * 1024 + (threadIdx.x & 63) * 16);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a barrier alone does not wait for LDS)
+        }
+    }
+    // Step j + 1 has landed.  Step j + 2 alone has been asked for behind it; of the last step some requests may have had no lane to make them.
+    __device__ inline void wait_for_next(int j) const {
+        if (j + 3 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
+template <bool BF16, int DP, bool ONES>
+__global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
+    using H = Head<DP, true, ONES>;
+    using E = Elem<BF16>;
+    using vec = typename E::vec;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, part = rest % p.parts;
+    const Block b = block_of<32 * WAVES>(p, rest / p.parts, lane);
+    if (!b.any) return;
+    long long first;
+    int count;
+    keys_of(p, b.s, first, count);
+    const int row0 = b.rb * 32 * WAVES, wave0 = row0 + wave * 32;
+    Rows r = rows_of(p, b, count, hk, wave0 + col);
+    int least, most, wave_least, wave_most;
+    limits_of(p, r, row0, 32 * WAVES, count, least, most);
+    limits_of(p, r, wave0, 32, count, wave_least, wave_most);
+    vec qf[H::KS];
+    load_q<BF16, H>(p, qf, r, lane);
+    // a part's keys: limits from its first one on
+    int begin = 0, end = (most + KEYS - 1) / KEYS;
+    share(p, part, begin, end);
+    const int skip = begin * KEYS;
+    most = (most < end * KEYS ? most : end * KEYS) - skip;
+    wave_most = (wave_most < end * KEYS ? wave_most : end * KEYS) - skip;
+    wave_least -= skip;
+    r.limit -= skip;
+    first += skip;
+    const RowCopies<H> copies(p, lds, p.k + (p.cu_k ? 0 : b.s) * p.ks[0] + first * p.ks[1] + hk * p.ks[2], p.v + (p.cu_k ? 0 : b.s) * p.vs[0] + first * p.vs[1] + hk * p.vs[2], most, wave,
+                              lane);
+    const int steps = copies.steps;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) copies.ask(i, i);
+    // columns behind the head's end, as far as they are multiplied, are zero in K for good: no copy writes there
+    zero_columns<H, STAGES * KEYS>(lds, p.D / 8, threadIdx.x, 64 * WAVES);
+    if constexpr (H::ONES) {
+        for (int i = threadIdx.x; i < STAGES * KEYS; i += 64 * WAVES)
+            *(u32x4_t *)(lds + STAGES * H::TILE + i * H::PITCH + ((p.D / 8) ^ H::fv(i)) * 16) = u32x4_t{E::ONE, 0, 0, 0};
+    }
+    State<BF16, H> st;
+    st.clear();
+    float16_t s[2];
+    vec pr[4], vf[2][H::DB], kf[2][4];
+    constexpr int N = 2 * H::KS, GROUP = N % 4 == 0 ? 4 : 2;
+    const char *k0 = lds + col * H::PITCH, *v0 = lds + STAGES * H::TILE;
+    auto read_k = [&](int slot, int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < GROUP; i++) {
+            const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+            kf[g & 1][i] = __builtin_bit_cast(vec, *(const u32x4_t *)(k0 + slot * H::TILE + kb * 32 * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16));
+        }
+    };
+    // the scores of a step; its first operands are there or on their way
+    auto score = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+#pragma unroll
+        for (int g = 0; g < N / GROUP; g++) {
+            if (g + 1 < N / GROUP) read_k(slot, g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                s[kb] = E::mfma(kf[g & 1][i], qf[ks], s[kb]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // the probabilities of a step times its values, the first of these there or on their way
+    auto weigh = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            if (n < 3) st.read_v(vf[(n + 1) & 1], v0 + slot * H::TILE, n + 1, lane);
+            else read_k((slot + 1) % STAGES, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < H::DB; d++) st.o[d] = E::mfma(vf[n & 1][d], pr[n], st.o[d]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const bool late = wave >= WAVES / 2;
+    if (steps > 0) {
+        wait_for_q<BF16, H>(qf);
+        if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RowCopies<H>::REQ * (STAGES - 2)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        phase_ends();
+        if (late) phase_ends();
+        if (wave_most > 0) {
+            read_k(0, 0);
+            score(0);
+        }
+        if (late) copies.wait_for_next(0);
+        phase_ends();
+        for (int j = 0; j < steps; j++) {
+            const int slot = j % STAGES;
+            const bool here = j * KEYS < wave_most;
+            if (late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
+            if (here) {
+                if (wave_least < (j + 1) * KEYS) hide(s, j * KEYS, r.limit, lane);
+                st.raise(st.highest(s), p.scale2);
+                const float ref = st.reference();
+#pragma unroll
+                for (int n = 0; n < 4; n++) pr[n] = st.template exponentials<2, H::ONES>(s, n, p.scale2, ref);
+                st.read_v(vf[0], v0 + slot * H::TILE, 0, lane);
+            }
+            if (!late) copies.wait_for_next(j);
+            phase_ends();
+            if (!late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
+            if (here) {
+                weigh(slot);
+                if ((j + 1) * KEYS < wave_most) score((j + 1) % STAGES);
+            }
+            if (late) {
+                if (j + 1 == steps) break;
+                copies.wait_for_next(j + 1);
+            }
+            phase_ends();
+        }
+        // Once more, key by key where rows do not see all keys, if sums turn out to hold a NaN: rows that see none of its causes have none then
+        if (p.causal) {
+            int *flags = (int *)(lds + 2 * STAGES * H::TILE);
+            const bool nan = any_nan(st, p.D);
+            if (lane == 0) flags[wave] = nan;
+            __syncthreads();
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) any |= flags[i] != 0;
+            if (__builtin_amdgcn_readfirstlane(any)) {
+                st.clear();
+#pragma unroll 1
+                for (int j = 0; j < steps; j++) {
+                    phase_ends();
+                    copies.ask(j, 0);
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    phase_ends();
+                    if (j * KEYS >= wave_most) continue;
+                    read_k(0, 0);
+                    score(0);
+                    const bool some = wave_least < (j + 1) * KEYS;
+                    if (some) hide(s, j * KEYS, r.limit, lane);
+                    if (some) attend_key_by_key(st, s, p.scale2, v0, j * KEYS, r.limit, lane);
+                    else st.template attend<H::ONES>(s, ~0ull, p.scale2, v0, lane);
+                }
+            }
+        }
+    }
+    if constexpr (H::ONES) {
+#pragma unroll
+        for (int g = 0; g < 4 * H::DB; g++)
+            if (8 * g == p.D && h == 0) st.sum = st.o[g >> 2][4 * (g & 3)];
+    }
+    const float sum = across_sum(st.sum);
+    if (p.parts > 1) {
+        if (!r.in) return;
+        float *dst = part_of(p, part, hk, r.index);
+#pragma unroll
+        for (int d = 0; d < H::DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int c = 32 * d + 8 * g + 4 * h;
+                if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+            }
+        if (h == 0) store_stats(p, part, hk, r.index, st.top, sum);
+        return;
+    }
+    const float inv = inverse(sum);
+#pragma unroll
+    for (int u = 0; u < 2 * H::DB; u++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = st.o[u >> 1][8 * (u & 1) + e];
+        store_columns<BF16>(r.out, x, inv, 16 * u, r.in ? p.D : 0, lane);
+    }
+}
+
 // Adds the parts of every row (at most 64): a wave to a row, two columns per lane; lane i holds part i's share of the row.
 constexpr int MAX_PARTS = 64;
 template <bool BF16>
@@ -381,13 +638,15 @@ __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
     *(uint32_t *)(p.out + entry * p.os[0] + t * p.os[1] + head * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
 }
 
-template <bool BF16, int DP>
-int launch_kernels(const Params &p, hipStream_t st) {
-    const int lds = 8 * Head<DP, true>::TILE;
-    static bool reserved[64] = {false};
-    if (int rc = reserve_lds((const void *)self_attention_keys_kernel<BF16, DP>, lds, reserved, "self_attention")) return rc;
-    const dim3 grid((unsigned)((long long)p.blocks * p.parts * p.Hkv)), block(256);
-    SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, block, lds, st, p);
+template <bool BF16, int DP, bool ONES>
+int launch_kernels(const Params &p, bool keys, hipStream_t st) {
+    const int lds = keys ? 8 * Head<DP, true>::TILE : 2 * STAGES * Head<DP, true>::TILE + 64;
+    static bool reserved[2][64] = {{false}};
+    const void *kernel = keys ? (const void *)self_attention_keys_kernel<BF16, DP> : (const void *)self_attention_rows_kernel<BF16, DP, ONES>;
+    if (int rc = reserve_lds(kernel, lds, reserved[keys], "self_attention")) return rc;
+    const dim3 grid((unsigned)((long long)p.blocks * p.parts * p.Hkv));
+    if (keys) SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, dim3(256), lds, st, p);
+    else SVDQ_LAUNCH((self_attention_rows_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
     int rc = check_launch("self_attention");
     if (rc || p.parts == 1) return rc;
     const long long all = p.all_rows * p.Hkv;
@@ -395,16 +654,23 @@ int launch_kernels(const Params &p, hipStream_t st) {
     return check_launch("self_attention");
 }
 
+template <bool BF16, int DP>
+int launch_head(const Params &p, bool keys, hipStream_t st) {
+    if (p.D < 32 * Head<DP>::DB) return launch_kernels<BF16, DP, true>(p, keys, st);
+    if constexpr (DP % 32 == 0) return launch_kernels<BF16, DP, false>(p, keys, st);
+    return SVDQ_EUNSUPPORTED;  // (not reached: the blocks of 80 end at 96)
+}
 template <bool BF16>
-int launch_heads(const Params &p, hipStream_t st) {
-    if (p.D <= 32) return launch_kernels<BF16, 32>(p, st);
-    if (p.D <= 64) return launch_kernels<BF16, 64>(p, st);
-    if (p.D <= 80) return launch_kernels<BF16, 80>(p, st);
-    if (p.D <= 96) return launch_kernels<BF16, 96>(p, st);
-    return launch_kernels<BF16, 128>(p, st);
+int launch_heads(const Params &p, bool keys, hipStream_t st) {
+    if (p.D <= 32) return launch_head<BF16, 32>(p, keys, st);
+    if (p.D <= 64) return launch_head<BF16, 64>(p, keys, st);
+    if (p.D <= 80) return launch_head<BF16, 80>(p, keys, st);
+    if (p.D <= 96) return launch_head<BF16, 96>(p, keys, st);
+    return launch_head<BF16, 128>(p, keys, st);
 }
 
 struct Plan {
+    bool keys;
     long long blocks, parts, workspace;
 };
 
@@ -417,7 +683,9 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
     const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
     Plan plan;
-    plan.blocks = blocks_of(a, 32);
+    const long long rows_each = (a->cu_seqlens_q ? (a->q_len + a->batch - 1) / a->batch : a->q_len) * (a->heads / a->kv_heads);
+    plan.keys = rows_each <= 128;
+    plan.blocks = blocks_of(a, plan.keys ? 32 : 32 * WAVES);
     plan.parts = 1;
     while (plan.parts < MAX_PARTS && plan.blocks * a->kv_heads * plan.parts * 2 <= cus && keys_each >= 256 * plan.parts) plan.parts *= 2;
     const long long rows = (a->cu_seqlens_q ? 1 : a->batch) * a->q_len * (a->heads / a->kv_heads);
@@ -505,5 +773,5 @@ extern "C" int svdq_self_attention(const svdq_self_attention_args *a, void *stre
     p.causal = a->causal != 0;
     p.zero_rest = a->zero_rest != 0;
     p.scale2 = a->scale * 1.44269504088896340736f;
-    return a->dtype == SVDQ_BF16 ? launch_heads<true>(p, (hipStream_t)stream) : launch_heads<false>(p, (hipStream_t)stream);
+    return a->dtype == SVDQ_BF16 ? launch_heads<true>(p, plan.keys, (hipStream_t)stream) : launch_heads<false>(p, plan.keys, (hipStream_t)stream);
 }
