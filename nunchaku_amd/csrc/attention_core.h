@@ -142,7 +142,9 @@ struct State {
         }
     }
     // left operands of v^T p for 16 keys from row 16 n of the values in LDS on
-    static __device__ inline void read_v(vec (&vf)[H::DB], const char *v, int n, int lane) {
+    template <int S>
+    static __device__ inline void read_v(vec (&vf)[S], const char *v, int n, int lane) {
+        static_assert(S >= H::DB, "");
         const int g = lane >> 4, i = lane & 15, h = lane >> 5;
         const char *vrow = v + (4 * h + (i >> 2)) * H::PITCH + (i & 1) * 8;
         const int piece = (g & 1) * 2 + ((i >> 1) & 1), f = H::fv(i >> 2);

@@ -15,122 +15,197 @@ struct Params {
     const char *q, *k, *v;
     char *out;
     const int *cu_q, *cu_k, *lengths;
-    float *partial;                            // several parts: [part][key head][row of all sequences] x D, then {maximum, sum} pairs
-    long long qs[3], ks[3], vs[3], os[3];      // bytes: batch, token, head
-    long long all_rows;                        // rows of a key head, of all sequences
-    int S, Hkv, G, D, Tq, Tk, blocks, parts, causal, zero_rest;  // blocks: of rows, for every key head and part
-    float scale2;                              // scale * log2(e)
+    float *partial;                        // keys in parts: [item][key head][row of the block] x D, then {maximum, sum} pairs
+    long long qs[3], ks[3], vs[3], os[3];  // bytes: batch, token, head
+    int S, Hkv, G, D, Tq, Tk, causal, zero_rest;
+    int items, blocks;                     // per key head, at most
+    int target, least;                     // keys in parts (target > 0): about how many items in all, steps of one at least
+    float scale2;                          // scale * log2(e)
 };
 
 __device__ inline int clamped(int x, int lo, int hi) { return x < lo ? lo : x < hi ? x : hi; }
 
-// A sequence's queries: where they start in q and out (packed: rows of all of them), and how many.  Rows in no sequence, in front of the first and behind
-// the last, are the queries of two more, without keys: number S and S + 1.
-__device__ inline void queries_of(const Params &p, int s, int &first, int &count) {
-    first = 0;
-    count = p.Tq;
-    if (!p.cu_q) return;
-    int lo, hi;
-    if (s < p.S) {
-        lo = p.cu_q[s];
-        hi = p.cu_q[s + 1];
-    } else {
-        lo = s == p.S ? 0 : p.cu_q[p.S];
-        hi = s == p.S ? p.cu_q[0] : p.Tq;
-        if (!p.zero_rest) hi = lo;
+// Rows of q that belong together: those of a sequence (s in 0 .. S - 1), or, packed, those in front of the first (region 0) and behind the last, which are in none.
+// Offsets that are not in order give fewer rows and keys, never others.
+struct Region {
+    int s, first, count;  // sequence, its first query's row of q (of its batch entry, if they are not packed), its queries
+    int key, keys;        // the same of k and v
+};
+__device__ inline int regions(const Params &p) { return p.cu_q ? p.S + 2 : p.S; }
+__device__ inline int region_start(const Params &p, int i) { return i == 0 ? 0 : i > p.S + 1 ? p.Tq : clamped(p.cu_q[i - 1], 0, p.Tq); }  // (packed)
+__device__ inline Region region_of(const Params &p, int i) {
+    Region r;
+    r.s = p.cu_q ? i - 1 : i;
+    r.first = r.key = r.keys = 0;
+    r.count = p.Tq;
+    const bool any = r.s >= 0 && r.s < p.S;
+    if (p.cu_q) {
+        r.first = region_start(p, i);
+        const int n = region_start(p, i + 1) - r.first;
+        r.count = (any || p.zero_rest) && n > 0 ? n : 0;
     }
-    first = clamped(lo, 0, p.Tq);
-    count = clamped(hi, first, p.Tq) - first;
+    if (any) {
+        if (p.cu_k) {
+            r.key = clamped(p.cu_k[r.s], 0, p.Tk);
+            r.keys = clamped(p.cu_k[r.s + 1], r.key, p.Tk) - r.key;
+        } else {
+            r.keys = p.lengths ? clamped(p.lengths[r.s], 0, p.Tk) : p.Tk;
+        }
+    }
+    return r;
+}
+__device__ inline Region in_lane(const Region &r, int l) {
+    return Region{__builtin_amdgcn_readlane(r.s, l), __builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.count, l), __builtin_amdgcn_readlane(r.key, l),
+                  __builtin_amdgcn_readlane(r.keys, l)};
+}
+template <int ROWS>
+__device__ inline int blocks_of(const Params &p, int count) {
+    return (int)(((long long)count * p.G + ROWS - 1) / ROWS);
 }
 
-struct Block {
-    int s, first, count, rb;  // sequence, its first query's row of q (of a batch entry: 0), its queries, block of rows
+// A block of rows of a region and a part of its keys
+struct Item {
+    Region r;
+    int rb, part, parts;
+    int index, next;  // which of the items' partial results is its own, and how much further that of the next part is
     bool any;
 };
 
-// Block number `at` of all sequences' blocks of ROWS rows.  A sequence's last block comes first: with a causal mask it has the most keys.
+// Item `at`.  A region's last block comes first: with a causal mask it has the most keys.
+// Packed, region i has the numbers from f(i) = floor(start(i) * G / ROWS) + i to f(i + 1): one more than it needs, or two, but no sums over the regions in front of it.
+// Its own is the last region whose f is not behind `at`, found among 64 at a time.
 template <int ROWS>
-__device__ inline Block block_of(const Params &p, int at, int lane) {
-    Block b;
+__device__ inline Item item_of(const Params &p, int at, int lane) {
+    Item it;
+    it.part = 0;
+    it.parts = 1;
+    it.index = it.next = 0;
     if (!p.cu_q) {
-        const int each = (int)(((long long)p.Tq * p.G + ROWS - 1) / ROWS);
-        b.s = at % p.S;
-        b.rb = each - 1 - at / p.S;
-        b.first = 0;
-        b.count = p.Tq;
-        b.any = true;
-        return b;
+        it.r = region_of(p, at % p.S);
+        it.rb = blocks_of<ROWS>(p, p.Tq) - 1 - at / p.S;
+        it.any = true;
+        return it;
     }
-    b.any = false;
-    b.s = b.first = b.count = b.rb = 0;
-    int left = at;
-    for (int base = 0; base < p.S + 2; base += 64) {  // 64 sequences at a time, one to a lane
-        int first = 0, count = 0;
-        if (base + lane < p.S + 2) queries_of(p, base + lane, first, count);
-        const int mine = (int)(((long long)count * p.G + ROWS - 1) / ROWS);
-        int upto = mine;  // blocks of this sequence and those in front of it
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d);
-            if (lane >= d) upto = upto + o < 1 << 29 ? upto + o : 1 << 29;  // (offsets that are not in order can make any sum)
+    int lo = 0, n = regions(p);
+    for (;;) {
+        const int step = (n + 63) / 64, i = lo + lane * step;
+        Region r = Region{0, 0, 0, 0, 0};
+        bool in = i < lo + n;
+        if (in) {
+            if (step == 1) r = region_of(p, i);
+            else r.first = region_start(p, i);
+            in = (int)((long long)r.first * p.G / ROWS) + i <= at;
         }
-        const uint64_t behind = __ballot(left < upto);
-        if (behind) {
-            const int l = __builtin_ctzll(behind);
-            b.s = base + l;
-            b.first = __builtin_amdgcn_readlane(first, l);
-            b.count = __builtin_amdgcn_readlane(count, l);
-            b.rb = __builtin_amdgcn_readlane(upto, l) - 1 - left;
-            b.any = b.rb < __builtin_amdgcn_readlane(mine, l);
-            return b;
+        const uint64_t found = __ballot(in);
+        const int l = found ? 63 - __builtin_clzll(found) : 0;
+        if (step == 1) {
+            it.r = in_lane(r, l);
+            const int blocks = blocks_of<ROWS>(p, it.r.count), rel = at - ((int)((long long)it.r.first * p.G / ROWS) + lo + l);
+            it.rb = blocks - 1 - rel;
+            it.any = found && rel >= 0 && rel < blocks;
+            return it;
         }
-        left -= __builtin_amdgcn_readlane(upto, 63);
+        lo += l * step;
+        n = n - l * step < step ? n - l * step : step;
     }
-    return b;
 }
 
-// The keys of sequence s: the row of k and v (of its batch entry, if they are not packed) that the first one has, and how many there are
-__device__ inline void keys_of(const Params &p, int s, long long &first, int &count) {
-    first = 0;
-    count = 0;
-    if (s >= p.S) return;
-    if (p.cu_k) {
-        const int lo = clamped(p.cu_k[s], 0, p.Tk);
-        count = clamped(p.cu_k[s + 1], lo, p.Tk) - lo;
-        first = __builtin_amdgcn_readfirstlane(lo);
-    } else {
-        count = p.lengths ? clamped(p.lengths[s], 0, p.Tk) : p.Tk;
+// Item `at` where keys are divided into parts, or (BLOCK) the first of block `at`.  All regions' work together, in steps of SIZE keys, is divided by the number of items that
+// is aimed at: longer keys than that are divided, evenly.  At most 4 x 64 regions, four to a lane.
+constexpr int MAX_PARTS = 64, MAX_REGIONS = 256;
+template <int ROWS, int SIZE, bool BLOCK>
+__device__ inline Item part_of(const Params &p, int at, int lane) {
+    constexpr int C = MAX_REGIONS / 64;
+    Region r[C];
+    int blocks[C], steps[C], most = 0;
+    float work = 0.f;
+    const int n = regions(p);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        r[c] = Region{0, 0, 0, 0, 0};
+        if (c * 64 + lane < n) r[c] = region_of(p, c * 64 + lane);
     }
-    count = __builtin_amdgcn_readfirstlane(count);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        blocks[c] = blocks_of<ROWS>(p, r[c].count);
+        steps[c] = (r[c].keys + SIZE - 1) / SIZE;
+        if (blocks[c]) most = steps[c] > most ? steps[c] : most;
+        work += (float)blocks[c] * (float)steps[c];
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const int o = __shfl_xor(most, d);
+        most = o > most ? o : most;
+        work += __shfl_xor(work, d);
+    }
+    int chunk = (int)__builtin_fminf(work / (float)p.target, 1.0e9f) + 1;
+    chunk = chunk < p.least ? p.least : chunk;
+    chunk = chunk < (most + MAX_PARTS - 1) / MAX_PARTS ? (most + MAX_PARTS - 1) / MAX_PARTS : chunk;
+    Item it;
+    it.any = false;
+    int left = at, items_before = 0;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        if (c * 64 >= n || it.any) continue;
+        const int parts = steps[c] > chunk ? (steps[c] + chunk - 1) / chunk : 1;
+        int upto = blocks[c], items = blocks[c] * parts;  // of this region and those in front of it
+        const int mine = items;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d), i = __shfl_up(items, d);
+            if (lane >= d) {  // (offsets that are not in order can make any sum)
+                upto = upto + o < 1 << 29 ? upto + o : 1 << 29;
+                items = items + i < 1 << 29 ? items + i : 1 << 29;
+            }
+        }
+        const uint64_t behind = __ballot(left < (BLOCK ? upto : items));
+        if (behind) {
+            const int l = __builtin_ctzll(behind), b = __builtin_amdgcn_readlane(blocks[c], l), before = __builtin_amdgcn_readlane(items, l) - __builtin_amdgcn_readlane(mine, l);
+            it.r = in_lane(r[c], l);
+            it.parts = __builtin_amdgcn_readlane(parts, l);
+            const int rel = left - (BLOCK ? __builtin_amdgcn_readlane(upto, l) - b : before);  // (blocks of a part next to each other: they read the same keys)
+            it.any = rel >= 0 && b > 0 && rel < b * (BLOCK ? 1 : it.parts);
+            it.part = it.any ? rel / b : 0;
+            it.rb = b - 1 - (rel - it.part * b);
+            it.index = BLOCK ? items_before + before + rel : at;
+            it.next = b;
+        } else {
+            left -= __builtin_amdgcn_readlane(BLOCK ? upto : items, 63);
+            items_before += __builtin_amdgcn_readlane(items, 63);
+        }
+    }
+    return it;
 }
 
 // This lane's row, and the keys that rows see
 struct Rows {
     const char *q;
     char *out;
-    long long index;  // of the row among all
-    int total, off, limit;  // rows of the sequence; key of its first query; the row sees the keys in front of `limit`
+    int total, off, keys, limit;  // rows of the sequence; key of its first query; keys; the row sees the keys in front of `limit`
     bool in;
 };
-__device__ inline int limit_of(const Params &p, const Rows &r, int row, int keys) { return p.causal ? clamped(row / p.G + r.off + 1, 0, keys) : keys; }
-__device__ inline Rows rows_of(const Params &p, const Block &b, int keys, int hk, int row) {
+__device__ inline int limit_of(const Params &p, const Rows &r, int row) { return p.causal ? clamped(row / p.G + r.off + 1, 0, r.keys) : r.keys; }
+__device__ inline Rows rows_of(const Params &p, const Region &g, int hk, int row) {
     Rows r;
-    const int t = row / p.G, g = row - t * p.G;
-    const long long head = hk * p.G + g, entry = p.cu_q ? 0 : b.s;
-    r.total = b.count * p.G;
-    r.off = keys - b.count;
+    const int t = row / p.G, head = hk * p.G + (row - t * p.G);
+    const long long entry = p.cu_q ? 0 : g.s;
+    r.total = g.count * p.G;
+    r.off = g.keys - g.count;
+    r.keys = g.keys;
     r.in = row < r.total;
-    r.q = p.q + entry * p.qs[0] + (long long)(b.first + t) * p.qs[1] + head * p.qs[2];
-    r.out = p.out + entry * p.os[0] + (long long)(b.first + t) * p.os[1] + head * p.os[2];
-    r.index = (entry * p.Tq + b.first) * p.G + row;
-    r.limit = limit_of(p, r, row, keys);
+    r.q = p.q + entry * p.qs[0] + (long long)(g.first + t) * p.qs[1] + head * p.qs[2];
+    r.out = p.out + entry * p.os[0] + (long long)(g.first + t) * p.os[1] + head * p.os[2];
+    r.limit = limit_of(p, r, row);
     return r;
 }
 // The limits of the first of `count` rows from `row` on and of the last one of the sequence among them (none: zero keys)
-__device__ inline void limits_of(const Params &p, const Rows &r, int row, int count, int keys, int &least, int &most) {
+__device__ inline void limits_of(const Params &p, const Rows &r, int row, int count, int &least, int &most) {
     const int last = row + count < r.total ? row + count - 1 : r.total - 1;
-    least = limit_of(p, r, row, keys);
-    most = last < row ? 0 : limit_of(p, r, last, keys);
+    least = limit_of(p, r, row);
+    most = last < row ? 0 : limit_of(p, r, last);
+}
+__device__ inline const char *first_key(const Params &p, const Region &g, const char *t, const long long (&s)[3], int hk) {
+    return t + (p.cu_k || g.s < 0 || g.s >= p.S ? 0 : g.s) * s[0] + g.key * s[1] + hk * s[2];
 }
 
 template <bool BF16, typename H>
@@ -149,17 +224,25 @@ __device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[H::KS]) {
     for (int ks = 0; ks < H::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
 
-__device__ inline void share(const Params &p, int part, int &begin, int &end) {
-    if (p.parts == 1) return;
-    const int each = end / p.parts, more = end - each * p.parts;
-    begin = part * each + (part < more ? part : more);
-    end = begin + each + (part < more);
+// The steps of a part, of those that all of the sequence's keys make; no more than the first `most` keys
+template <int SIZE>
+__device__ inline void share(const Item &it, int most, int &begin, int &end) {
+    begin = 0;
+    end = (most + SIZE - 1) / SIZE;
+    if (it.parts == 1) return;
+    const int all = (it.r.keys + SIZE - 1) / SIZE, each = all / it.parts, more = all - each * it.parts;
+    begin = it.part * each + (it.part < more ? it.part : more);
+    const int stop = begin + each + (it.part < more);
+    end = stop < end ? stop : end;
 }
-__device__ inline float *part_of(const Params &p, int part, int hk, long long index) { return p.partial + (((long long)part * p.Hkv + hk) * p.all_rows + index) * p.D; }
-__device__ inline void store_stats(const Params &p, int part, int hk, long long index, float top, float sum) {
-    float *ms = p.partial + (long long)p.parts * p.Hkv * p.all_rows * p.D + (((long long)part * p.Hkv + hk) * p.all_rows + index) * 2;
-    ms[0] = top;
-    ms[1] = sum;
+// Where an item's share of a row goes, and its maximum and sum behind all of those
+template <int ROWS>
+__device__ inline float *share_of(const Params &p, int index, int hk, int row) {
+    return p.partial + (((long long)index * p.Hkv + hk) * ROWS + row) * p.D;
+}
+template <int ROWS>
+__device__ inline float *stats_of(const Params &p, int index, int hk, int row) {
+    return p.partial + (long long)p.items * p.Hkv * ROWS * p.D + (((long long)index * p.Hkv + hk) * ROWS + row) * 2;
 }
 
 // A step in which some rows do not see some keys, where what such a key has in V is an infinity or a NaN: zero times it is a NaN, too.  A key at a time; rows that
@@ -222,25 +305,21 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     using E = Elem<BF16>;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, part = rest % p.parts;
-    const Block b = block_of<32>(p, rest / p.parts, lane);
-    if (!b.any) return;
-    long long first;
-    int count;
-    keys_of(p, b.s, first, count);
-    const Rows r = rows_of(p, b, count, hk, b.rb * 32 + col);
-    int least, most;
-    limits_of(p, r, b.rb * 32, 32, count, least, most);
+    const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    constexpr int SIZE = 32;
+    const Item it = p.target ? part_of<32, SIZE, false>(p, at, lane) : item_of<32>(p, at, lane);
+    if (!it.any) return;
+    const Rows r = rows_of(p, it.r, hk, it.rb * 32 + col);
+    int least, most, begin, end;
+    limits_of(p, r, it.rb * 32, 32, least, most);
+    share<SIZE>(it, most, begin, end);
     typename E::vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
-    const char *kp = p.k + (p.cu_k ? 0 : b.s) * p.ks[0] + first * p.ks[1] + hk * p.ks[2];
-    const char *vp = p.v + (p.cu_k ? 0 : b.s) * p.vs[0] + first * p.vs[1] + hk * p.vs[2];
-    constexpr int SIZE = 32, REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
+    const char *kp = first_key(p, it.r, p.k, p.ks, hk), *vp = first_key(p, it.r, p.v, p.vs, hk);
+    constexpr int REQ = H::REQ / 2, STAGE = H::TILE;  // a stage: 32 rows of K, then of V
     char *mine = lds + wave * 2 * STAGE;
     const uint32_t area = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * 2 * STAGE;
     const int bytes = p.D * 2;
-    int begin = 0, end = (most + SIZE - 1) / SIZE;
-    share(p, part, begin, end);
     // Request i brings rows r0 + i * RPR: of V the same piece every time, of K the pieces that f has there
     const int r0 = lane / H::PIECES, ck = ((lane % H::PIECES) ^ H::fk(r0)) * 16, cv = ((lane % H::PIECES) ^ H::fv(r0)) * 16;
     const uint32_t ok = (uint32_t)(r0 * p.ks[1]), ov = (uint32_t)(r0 * p.vs[1]) + cv;
@@ -324,7 +403,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
         sum += ((float *)(lds + i * AREA))[32 + col] * f[i];
     }
     const float inv = inverse(sum);
-    float *dst = part_of(p, part, hk, r.index);
+    float *dst = share_of<32>(p, it.index, hk, col);
     const int columns = r.in ? p.D : 0;
     for (int u = wave; u < UNITS; u += 4) {
         float x[8];
@@ -338,13 +417,17 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
                 for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(o[e], f[w], y[e]);
             }
             const int c = 16 * u + 8 * i + 4 * h;
-            if (p.parts > 1 && c < columns) *(float4_t *)(dst + c) = y;
+            if (it.parts > 1 && c < columns) *(float4_t *)(dst + c) = y;
 #pragma unroll
             for (int e = 0; e < 4; e++) x[4 * i + e] = y[e];
         }
-        if (p.parts == 1) store_columns<BF16>(r.out, x, inv, 16 * u, columns, lane);
+        if (it.parts == 1) store_columns<BF16>(r.out, x, inv, 16 * u, columns, lane);
     }
-    if (p.parts > 1 && wave == 0 && h == 0 && r.in) store_stats(p, part, hk, r.index, top, sum);
+    if (it.parts > 1 && wave == 0 && h == 0 && r.in) {
+        float *ms = stats_of<32>(p, it.index, hk, col);
+        ms[0] = top;
+        ms[1] = sum;
+    }
 }
 
 // ---- rows form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
@@ -352,7 +435,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
 // those with V, the next keys with Q).  A phase is one or the other; waves 4 .. 7 are one phase behind waves 0 .. 3, and a barrier ends a phase for all.
 // In phase 2 j the first four waves make the probabilities of step j, in phase 2 j + 1 they multiply them and score step j + 1.  Keys and values of step i are
 // read in phases 2 i - 1 .. 2 i + 2; those of step i + 4 take their place, asked for in phase 2 i + 3, by all waves, and waited for at the end of phase 2 i + 6.
-constexpr int STAGES = 4, WAVES = 8;
+constexpr int STAGES = 4, WAVES = 8, ROWS = 32 * WAVES;
 
 __device__ inline void phase_ends() {
     __builtin_amdgcn_sched_barrier(0);
@@ -375,7 +458,7 @@ struct RowCopies {
         k_step = KEYS * p.ks[1];
         v_step = KEYS * p.vs[1];
         most = most_;
-        steps = (most + KEYS - 1) / KEYS;
+        steps = most > 0 ? (most + KEYS - 1) / KEYS : 0;  // (a part may lie behind all keys that are seen)
         any = wave < ACTIVE;
         dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
 #pragma unroll
@@ -428,30 +511,24 @@ __global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
     using vec = typename E::vec;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, part = rest % p.parts;
-    const Block b = block_of<32 * WAVES>(p, rest / p.parts, lane);
-    if (!b.any) return;
-    long long first;
-    int count;
-    keys_of(p, b.s, first, count);
-    const int row0 = b.rb * 32 * WAVES, wave0 = row0 + wave * 32;
-    Rows r = rows_of(p, b, count, hk, wave0 + col);
-    int least, most, wave_least, wave_most;
-    limits_of(p, r, row0, 32 * WAVES, count, least, most);
-    limits_of(p, r, wave0, 32, count, wave_least, wave_most);
+    const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    const Item it = p.target ? part_of<ROWS, KEYS, false>(p, at, lane) : item_of<ROWS>(p, at, lane);
+    if (!it.any) return;
+    const int wave0 = it.rb * ROWS + wave * 32;
+    Rows r = rows_of(p, it.r, hk, wave0 + col);
+    int least, most, wave_least, wave_most, begin, end;
+    limits_of(p, r, it.rb * ROWS, ROWS, least, most);
+    limits_of(p, r, wave0, 32, wave_least, wave_most);
     vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
     // a part's keys: limits from its first one on
-    int begin = 0, end = (most + KEYS - 1) / KEYS;
-    share(p, part, begin, end);
-    const int skip = begin * KEYS;
-    most = (most < end * KEYS ? most : end * KEYS) - skip;
-    wave_most = (wave_most < end * KEYS ? wave_most : end * KEYS) - skip;
+    share<KEYS>(it, most, begin, end);
+    const int skip = begin * KEYS, stop = end * KEYS;
+    most = (most < stop ? most : stop) - skip;
+    wave_most = (wave_most < stop ? wave_most : stop) - skip;
     wave_least -= skip;
     r.limit -= skip;
-    first += skip;
-    const RowCopies<H> copies(p, lds, p.k + (p.cu_k ? 0 : b.s) * p.ks[0] + first * p.ks[1] + hk * p.ks[2], p.v + (p.cu_k ? 0 : b.s) * p.vs[0] + first * p.vs[1] + hk * p.vs[2], most, wave,
-                              lane);
+    const RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], most, wave, lane);
     const int steps = copies.steps;
 #pragma unroll
     for (int i = 0; i < STAGES - 1; i++) copies.ask(i, i);
@@ -576,9 +653,9 @@ __global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
             if (8 * g == p.D && h == 0) st.sum = st.o[g >> 2][4 * (g & 3)];
     }
     const float sum = across_sum(st.sum);
-    if (p.parts > 1) {
+    if (it.parts > 1) {
         if (!r.in) return;
-        float *dst = part_of(p, part, hk, r.index);
+        float *dst = share_of<ROWS>(p, it.index, hk, wave * 32 + col);
 #pragma unroll
         for (int d = 0; d < H::DB; d++)
 #pragma unroll
@@ -586,7 +663,11 @@ __global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
                 const int c = 32 * d + 8 * g + 4 * h;
                 if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
             }
-        if (h == 0) store_stats(p, part, hk, r.index, st.top, sum);
+        if (h == 0) {
+            float *ms = stats_of<ROWS>(p, it.index, hk, wave * 32 + col);
+            ms[0] = st.top;
+            ms[1] = sum;
+        }
         return;
     }
     const float inv = inverse(sum);
@@ -599,43 +680,43 @@ __global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
     }
 }
 
-// Adds the parts of every row (at most 64): a wave to a row, two columns per lane; lane i holds part i's share of the row.
-constexpr int MAX_PARTS = 64;
-template <bool BF16>
+// Adds the parts of every row (at most 64): 32 rows of a block per workgroup, a wave to a row, two columns per lane; lane i holds part i's share of the row.
+template <bool BF16, int BLOCK_ROWS, int SIZE>
 __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
+    constexpr int SUBS = BLOCK_ROWS / 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long all = p.all_rows * p.Hkv, at = (long long)blockIdx.x * 4 + wave;
-    if (at >= all) return;
-    const int hk = (int)(at / p.all_rows);
-    const long long index = at - hk * p.all_rows, token = index / p.G;
-    if (p.cu_q && !p.zero_rest && (token < p.cu_q[0] || token >= p.cu_q[p.S])) return;
-    const float *ms = p.partial + p.parts * all * p.D;
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, sub = rest % SUBS;
+    const Item it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
+    if (!it.any || it.parts == 1 || (long long)it.index + (long long)(it.parts - 1) * it.next >= p.items) return;
     const int c = lane * 2 < p.D ? lane * 2 : 0;
     typedef float float2_t __attribute__((ext_vector_type(2)));
-    float top = -__builtin_huge_valf(), sum = 0.f;
-    if (lane < p.parts) {
-        const float2_t t = *(const float2_t *)(ms + (lane * all + at) * 2);
-        top = t[0];
-        sum = t[1];
-    }
-    float most = top;
+    for (int i = wave; i < 32; i += 4) {
+        const int at = sub * 32 + i, row = it.rb * BLOCK_ROWS + at;
+        const Rows r = rows_of(p, it.r, hk, row);
+        if (!r.in) break;
+        float top = -__builtin_huge_valf(), sum = 0.f;
+        if (lane < it.parts) {
+            const float2_t t = *(const float2_t *)stats_of<BLOCK_ROWS>(p, it.index + lane * it.next, hk, at);
+            top = t[0];
+            sum = t[1];
+        }
+        float most = top;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
-    const float f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
-    sum *= f;
+        for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+        const float f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
+        sum *= f;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    float x = 0.f, y = 0.f;
-    for (int i = 0; i < p.parts; i++) {
-        const float2_t part = *(const float2_t *)(p.partial + (i * all + at) * p.D + c);
-        const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), i));
-        x = __builtin_fmaf(part[0], g, x);
-        y = __builtin_fmaf(part[1], g, y);
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        float x = 0.f, y = 0.f;
+        for (int j = 0; j < it.parts; j++) {
+            const float2_t part = *(const float2_t *)(share_of<BLOCK_ROWS>(p, it.index + j * it.next, hk, at) + c);
+            const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), j));
+            x = __builtin_fmaf(part[0], g, x);
+            y = __builtin_fmaf(part[1], g, y);
+        }
+        const float inv = inverse(sum);
+        if (lane * 2 < p.D) *(uint32_t *)(r.out + c * 2) = Elem<BF16>::pair(x * inv, y * inv);
     }
-    if (lane * 2 >= p.D) return;
-    const float r = inverse(sum);
-    const long long entry = p.cu_q ? 0 : token / p.Tq, t = token - entry * p.Tq, head = hk * p.G + (index - token * p.G);
-    *(uint32_t *)(p.out + entry * p.os[0] + t * p.os[1] + head * p.os[2] + c * 2) = Elem<BF16>::pair(x * r, y * r);
 }
 
 template <bool BF16, int DP, bool ONES>
@@ -644,13 +725,13 @@ int launch_kernels(const Params &p, bool keys, hipStream_t st) {
     static bool reserved[2][64] = {{false}};
     const void *kernel = keys ? (const void *)self_attention_keys_kernel<BF16, DP> : (const void *)self_attention_rows_kernel<BF16, DP, ONES>;
     if (int rc = reserve_lds(kernel, lds, reserved[keys], "self_attention")) return rc;
-    const dim3 grid((unsigned)((long long)p.blocks * p.parts * p.Hkv));
+    const dim3 grid((unsigned)((long long)p.items * p.Hkv));
     if (keys) SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, dim3(256), lds, st, p);
     else SVDQ_LAUNCH((self_attention_rows_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
     int rc = check_launch("self_attention");
-    if (rc || p.parts == 1) return rc;
-    const long long all = p.all_rows * p.Hkv;
-    SVDQ_LAUNCH((self_attention_join_kernel<BF16>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st, p);
+    if (rc || !p.target) return rc;
+    if (keys) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * p.Hkv)), dim3(256), 0, st, p);
+    else SVDQ_LAUNCH((self_attention_join_kernel<BF16, ROWS, KEYS>), dim3((unsigned)(p.blocks * WAVES * p.Hkv)), dim3(256), 0, st, p);
     return check_launch("self_attention");
 }
 
@@ -671,25 +752,29 @@ int launch_heads(const Params &p, bool keys, hipStream_t st) {
 
 struct Plan {
     bool keys;
-    long long blocks, parts, workspace;
+    long long blocks, items, target, least, workspace;
 };
 
 long long blocks_of(const svdq_self_attention_args *a, long long size) {
     const long long rows = a->q_len * (a->heads / a->kv_heads);
     // packed sequences: each, and the rows in front of them and behind, may end in the middle of a block
-    return a->cu_seqlens_q ? rows / size + (a->batch + 2 < a->q_len ? a->batch + 2 : a->q_len) : (rows + size - 1) / size * a->batch;
+    return a->cu_seqlens_q ? rows / size + a->batch + 2 : (rows + size - 1) / size * a->batch;
 }
 
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
-    const long long keys_each = a->cu_seqlens_k ? (a->k_len + a->batch - 1) / a->batch : a->k_len;
     Plan plan;
     const long long rows_each = (a->cu_seqlens_q ? (a->q_len + a->batch - 1) / a->batch : a->q_len) * (a->heads / a->kv_heads);
     plan.keys = rows_each <= 128;
-    plan.blocks = blocks_of(a, plan.keys ? 32 : 32 * WAVES);
-    plan.parts = 1;
-    while (plan.parts < MAX_PARTS && plan.blocks * a->kv_heads * plan.parts * 2 <= cus && keys_each >= 256 * plan.parts) plan.parts *= 2;
-    const long long rows = (a->cu_seqlens_q ? 1 : a->batch) * a->q_len * (a->heads / a->kv_heads);
-    plan.workspace = plan.parts > 1 ? plan.parts * a->kv_heads * rows * (a->head_dim + 2) * 4 : 0;
+    const int size = plan.keys ? 32 : ROWS;
+    plan.blocks = plan.items = blocks_of(a, size);
+    plan.target = plan.workspace = 0;
+    plan.least = 512 / (plan.keys ? 32 : KEYS);
+    const long long slots = plan.keys && a->head_dim <= 64 ? 2 * cus : cus;
+    if (plan.keys && a->batch + 2 <= MAX_REGIONS && plan.blocks * a->kv_heads < 2 * slots && a->k_len > 512) {
+        plan.target = (slots * 3 / 2 + a->kv_heads - 1) / a->kv_heads;
+        plan.items = plan.blocks + plan.target + 1;
+        plan.workspace = plan.items * a->kv_heads * size * (a->head_dim + 2) * 4;
+    }
     return plan;
 }
 
@@ -767,9 +852,10 @@ extern "C" int svdq_self_attention(const svdq_self_attention_args *a, void *stre
     p.D = (int)a->head_dim;
     p.Tq = (int)a->q_len;
     p.Tk = (int)a->k_len;
-    p.all_rows = (a->cu_seqlens_q ? 1 : a->batch) * a->q_len * p.G;
+    p.items = (int)plan.items;
     p.blocks = (int)plan.blocks;
-    p.parts = (int)plan.parts;
+    p.target = (int)plan.target;
+    p.least = (int)plan.least;
     p.causal = a->causal != 0;
     p.zero_rest = a->zero_rest != 0;
     p.scale2 = a->scale * 1.44269504088896340736f;
