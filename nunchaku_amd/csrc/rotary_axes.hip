@@ -14,7 +14,7 @@ using namespace svdq;
 
 namespace {
 
-constexpr int MAX_PAIRS = 128, MAX_AXES = 4, MOST_TOKENS = 8;
+constexpr int MAX_PAIRS = 128, MAX_AXES = 4, MOST_TOKENS = 16;
 
 struct RotaryParams {
     const char *in[2], *norm[2];   // q, k
@@ -23,7 +23,8 @@ struct RotaryParams {
     long long in_s[2][3], out_s[2][3];  // bytes: batch, token, head
     long long pos_s[3];                 // elements: batch, token, axis
     long long rows, first;              // tokens of all entries; this launch's first
-    int T, heads[2], D, pairs, halves, position_type, tokens;  // tokens: a workgroup's
+    int T, heads[2], D, pairs, halves, position_type, tokens;  // T: 0: one entry, or entries whose tokens go on where those in front end; tokens: a workgroup's
+    int once;                           // the tensors do not fit the memory-side cache: what is read is not kept there
     float inv_d, eps, tiny;
     double freq[MAX_PAIRS];  // revolutions per position
     uint8_t axis[MAX_PAIRS];
@@ -55,95 +56,150 @@ __device__ inline u32x4_t pack(const float (&f)[8]) {
     return w;
 }
 
-// LANES threads to a head, a piece of 8 channels each
-template <bool BF16, int LANES>
+// x of the lanes that share a head, added: within quads, then mirrored halves of 8 and of 16
+template <int CONTROL>
+__device__ inline float moved(float x) {
+    return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), CONTROL, 0xF, 0xF, true));
+}
+template <int LANES>
+__device__ inline float head_sum(float x) {
+    x += moved<0xB1>(x);
+    x += moved<0x4E>(x);
+    if (LANES > 4) x += moved<0x141>(x);
+    if (LANES > 8) x += moved<0x140>(x);
+    if (LANES > 16) x += __shfl_xor(x, 16);
+    return x;
+}
+
+// LANES threads to a head, a piece of 8 channels each; ITEMS heads of a thread are on their way at once, the first ones while the angles are made
+template <bool BF16, int LANES, int ITEMS>
 __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
     typedef float float2_t __attribute__((ext_vector_type(2)));
-    __shared__ float2_t turns[MOST_TOKENS * MAX_PAIRS];  // cosine, sine
-    const long long row0 = p.first + (long long)blockIdx.x * p.tokens;
-    const int count = (int)(p.rows - row0 < p.tokens ? p.rows - row0 : p.tokens);
+    __shared__ __attribute__((aligned(16))) float2_t turns[MOST_TOKENS * MAX_PAIRS];  // cosine, sine
+    constexpr int SLOTS = 256 / LANES;
+    const int row0 = (int)(p.first + (long long)blockIdx.x * p.tokens);
+    const int count = p.rows - row0 < p.tokens ? (int)(p.rows - row0) : p.tokens;
+    const int c = threadIdx.x % LANES, heads = p.heads[0] + p.heads[1], half = p.pairs / 8;
+    const bool in = c < p.D / 8;
+    // this thread's heads: `head` of token `n` next
+    int n = 0, head = threadIdx.x / LANES;
+    u32x4_t w[ITEMS];
+    char *out[ITEMS];
+    int token[ITEMS], which[ITEMS];
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            while (head >= heads) {
+                head -= heads;
+                n++;
+            }
+            token[i] = n < count ? n : -1;
+            which[i] = head >= p.heads[0];
+            w[i] = u32x4_t{0, 0, 0, 0};
+            if (n < count && in) {
+                const int k = which[i], h = k ? head - p.heads[0] : head, row = row0 + n, b = p.T ? row / p.T : 0, t = row - b * p.T;
+                const char *src = p.in[k] + b * p.in_s[k][0] + t * p.in_s[k][1] + h * p.in_s[k][2] + c * 16;
+                out[i] = p.out[k] + b * p.out_s[k][0] + t * p.out_s[k][1] + h * p.out_s[k][2] + c * 16;
+                if (p.once) w[i] = __builtin_nontemporal_load((const u32x4_t *)src);
+                else w[i] = *(const u32x4_t *)src;
+            }
+            head += SLOTS;
+        }
+    };
+    load();
+    u32x4_t g[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        g[k] = u32x4_t{0, 0, 0, 0};
+        if (p.norm[k] && in) g[k] = *(const u32x4_t *)(p.norm[k] + c * 16);
+    }
     for (int i = threadIdx.x; i < count * p.pairs; i += 256) {
-        const int n = i / p.pairs, pair = i - n * p.pairs;
-        const long long row = row0 + n, b = row / p.T, t = row - b * p.T, at = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
+        const int m = i / p.pairs, pair = i - m * p.pairs, row = row0 + m, b = p.T ? row / p.T : 0, t = row - b * p.T;
+        const long long at = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
         const double x = p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[at]
                          : p.position_type == SVDQ_POSITION_INT64 ? (double)((const int64_t *)p.positions)[at] : (double)((const float *)p.positions)[at];
         const double revolutions = x * p.freq[pair];
-        float s, c;
-        sincospif(2.0f * (float)(revolutions - __builtin_rint(revolutions)), &s, &c);
-        turns[i] = float2_t{c, s};
+        float s, co;
+        sincospif(2.0f * (float)(revolutions - __builtin_rint(revolutions)), &s, &co);
+        turns[i] = float2_t{co, s};
     }
     __syncthreads();
-    const int c = threadIdx.x % LANES, pieces = p.D / 8, heads = p.heads[0] + p.heads[1], half = p.pairs / 8;
-    const bool in = c < pieces;
-    constexpr int SLOTS = 256 / LANES;
-    for (int item = threadIdx.x / LANES; item < count * heads; item += SLOTS) {
-        const int n = item / heads, any = item - n * heads, which = any >= p.heads[0], head = which ? any - p.heads[0] : any;
-        const long long row = row0 + n, b = row / p.T, t = row - b * p.T;
-        u32x4_t w = u32x4_t{0, 0, 0, 0};
-        float x[8], y[8];
-        if (in) w = *(const u32x4_t *)(p.in[which] + b * p.in_s[which][0] + t * p.in_s[which][1] + head * p.in_s[which][2] + c * 16);
-        unpack<BF16>(w, x);
-        if (p.norm[which]) {
-            float squares = 0.f;
+    for (;;) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) squares = __builtin_fmaf(x[j], x[j], squares);
+        for (int i = 0; i < ITEMS; i++) {
+            if (token[i] < 0) break;
+            float x[8], y[8];
+            unpack<BF16>(w[i], x);
+            const bool norm = p.norm[0] || p.norm[1];
+            if (norm) {
+                // (the sum is everybody's, also where this head has no norm: lanes of other heads may have one)
+                float squares = 0.f;
 #pragma unroll
-            for (int d = LANES / 2; d; d >>= 1) squares += __shfl_xor(squares, d);
-            if (squares < 0x1p120f && squares >= p.tiny) {
-                const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_d, p.eps));
+                for (int j = 0; j < 8; j++) squares = __builtin_fmaf(x[j], x[j], squares);
+                squares = head_sum<LANES>(squares);
+                if (p.norm[which[i]]) {
+                    if (squares < 0x1p120f && squares >= p.tiny) {
+                        const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_d, p.eps));
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] *= r;
-            } else {  // squares that leave fp32's range: once more in 64 bits
-                double s = 0.0;
+                        for (int j = 0; j < 8; j++) x[j] *= r;
+                    } else {  // squares that leave fp32's range: once more in 64 bits (all lanes of the head)
+                        double s = 0.0;
 #pragma unroll
-                for (int j = 0; j < 8; j++) s += (double)x[j] * (double)x[j];
+                        for (int j = 0; j < 8; j++) s += (double)x[j] * (double)x[j];
 #pragma unroll
-                for (int d = LANES / 2; d; d >>= 1) s += __shfl_xor(s, d);
-                const double r = 1.0 / __builtin_sqrt(s / (double)p.D + (double)p.eps);
+                        for (int d = LANES / 2; d; d >>= 1) s += __shfl_xor(s, d);
+                        const double r = 1.0 / __builtin_sqrt(s / (double)p.D + (double)p.eps);
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = (float)((double)x[j] * r);
-            }
-            u32x4_t g = u32x4_t{0, 0, 0, 0};
-            if (in) g = *(const u32x4_t *)(p.norm[which] + c * 16);
-            unpack<BF16>(g, y);
+                        for (int j = 0; j < 8; j++) x[j] = (float)((double)x[j] * r);
+                    }
+                    unpack<BF16>(which[i] ? g[1] : g[0], y);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] *= y[j];
-        }
-        const float2_t *turn = turns + n * p.pairs;
-        if (p.halves) {
-            const bool low = c < half;
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = __shfl(x[j], low ? c + half : c - half, LANES);
-            if (c < 2 * half) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float2_t cs = turn[(low ? c : c - half) * 8 + j];
-                    x[j] = low ? x[j] * cs[0] - y[j] * cs[1] : y[j] * cs[1] + x[j] * cs[0];
+                    for (int j = 0; j < 8; j++) x[j] *= y[j];
                 }
             }
-        } else {
+            const float2_t *turn = turns + token[i] * p.pairs;
+            if (p.halves) {
+                const bool low = c < half;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int pair = c * 4 + j;
-                const float2_t cs = pair < p.pairs ? turn[pair] : float2_t{1.f, 0.f};
-                const float a = x[2 * j], d = x[2 * j + 1];
-                if (pair < p.pairs) {
-                    x[2 * j] = a * cs[0] - d * cs[1];
-                    x[2 * j + 1] = a * cs[1] + d * cs[0];
+                for (int j = 0; j < 8; j++) y[j] = __shfl(x[j], low ? c + half : c - half, LANES);
+                if (c < 2 * half) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float2_t cs = turn[(low ? c : c - half) * 8 + j];
+                        x[j] = low ? x[j] * cs[0] - y[j] * cs[1] : y[j] * cs[1] + x[j] * cs[0];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int pair = c * 4 + j;
+                    if (pair < p.pairs) {
+                        const float2_t cs = turn[pair];
+                        const float a = x[2 * j], d = x[2 * j + 1];
+                        x[2 * j] = a * cs[0] - d * cs[1];
+                        x[2 * j + 1] = a * cs[1] + d * cs[0];
+                    }
                 }
             }
+            if (in) *(u32x4_t *)out[i] = pack<BF16>(x);
         }
-        if (in) *(u32x4_t *)(p.out[which] + b * p.out_s[which][0] + t * p.out_s[which][1] + head * p.out_s[which][2] + c * 16) = pack<BF16>(x);
+        if (n >= count) return;
+        load();
     }
 }
 
+template <bool BF16, int LANES>
+void launch_lanes(const RotaryParams &p, unsigned blocks, hipStream_t st) {
+    const dim3 grid(blocks), block(256);
+    if (p.tokens * (p.heads[0] + p.heads[1]) <= 256 / LANES) SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, 1>), grid, block, 0, st, p);
+    else SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, 4>), grid, block, 0, st, p);
+}
 template <bool BF16>
 void dispatch(const RotaryParams &p, unsigned blocks, hipStream_t st) {
-    const dim3 grid(blocks), block(256);
-    if (p.D <= 32) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 4>), grid, block, 0, st, p);
-    else if (p.D <= 64) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 8>), grid, block, 0, st, p);
-    else if (p.D <= 128) SVDQ_LAUNCH((rotary_axes_kernel<BF16, 16>), grid, block, 0, st, p);
-    else SVDQ_LAUNCH((rotary_axes_kernel<BF16, 32>), grid, block, 0, st, p);
+    if (p.D <= 32) launch_lanes<BF16, 4>(p, blocks, st);
+    else if (p.D <= 64) launch_lanes<BF16, 8>(p, blocks, st);
+    else if (p.D <= 128) launch_lanes<BF16, 16>(p, blocks, st);
+    else launch_lanes<BF16, 32>(p, blocks, st);
 }
 
 }  // namespace
@@ -192,7 +248,11 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
     p.positions = a->positions;
     for (int j = 0; j < 3; j++) p.pos_s[j] = a->position_stride[j];
     p.rows = a->batch * a->tokens;
-    p.T = (int)a->tokens;
+    // one row of tokens, where strides go on from an entry to the next
+    bool one = a->batch == 1 || a->position_stride[0] == a->tokens * a->position_stride[1];
+    for (int i = 0; i < 2; i++)
+        one = one && (a->batch == 1 || !ins[i] || (in_s[i][0] == a->tokens * in_s[i][1] && out_s[i][0] == a->tokens * out_s[i][1]));
+    p.T = one ? 0 : (int)a->tokens;
     p.heads[0] = (int)a->heads;
     p.heads[1] = a->k ? (int)a->kv_heads : 0;
     p.D = (int)a->head_dim;
@@ -213,7 +273,10 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
             p.axis[pair] = (uint8_t)i;
         }
     }
-    p.tokens = p.rows >= 4096 ? 4 : 1;
+    const int lanes = p.D <= 32 ? 4 : p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, heads = p.heads[0] + p.heads[1];
+    p.tokens = 1;
+    while (p.tokens < MOST_TOKENS && p.rows >= 2048 * p.tokens && p.tokens * heads < 4 * 256 / lanes) p.tokens *= 2;
+    p.once = p.rows * heads * p.D * 4 > 300000000;
     // a launch takes fewer than 2^32 threads
     const long long most = (1ll << 23) * p.tokens;
     const long long all = p.rows;
