@@ -5,7 +5,7 @@
 // Angles.  A frequency in revolutions, theta^(-e) / (2 pi), comes from the host in 64 bits; position times frequency, less the nearest whole number of
 // revolutions, is right to 2^-24 revolutions for positions of 2^31 and to 2^-34 for those of 2^21, where 32 bits would have lost all but 2^-6.  Sine and
 // cosine see half a revolution at most.
-// They are the same for all heads of a token: a workgroup makes them once, in LDS.
+// They are the same for all heads of a token: a wave makes those of its token once, a pair to a lane, and hands them round through LDS.
 #include <math.h>
 
 #include "svdq_common.h"
@@ -14,7 +14,7 @@ using namespace svdq;
 
 namespace {
 
-constexpr int MAX_PAIRS = 128, MAX_AXES = 4, MOST_TOKENS = 16;
+constexpr int MAX_PAIRS = 128, MAX_AXES = 4, ITEMS = 4;
 
 struct RotaryParams {
     const char *in[2], *norm[2];   // q, k
@@ -22,8 +22,8 @@ struct RotaryParams {
     const void *positions;
     long long in_s[2][3], out_s[2][3];  // bytes: batch, token, head
     long long pos_s[3];                 // elements: batch, token, axis
-    long long rows, first;              // tokens of all entries; this launch's first
-    int T, heads[2], D, pairs, halves, position_type, tokens;  // T: 0: one entry, or entries whose tokens go on where those in front end; tokens: a workgroup's
+    long long work, first;              // tokens of all entries times the waves that share one; this launch's first
+    int T, heads[2], D, pairs, halves, position_type, share;  // share: waves to a token
     int once;                           // the tensors do not fit the memory-side cache: what is read is not kept there
     float inv_d, eps, tiny;
     double freq[MAX_PAIRS];  // revolutions per position
@@ -71,128 +71,132 @@ __device__ inline float head_sum(float x) {
     return x;
 }
 
-// LANES threads to a head, a piece of 8 channels each; ITEMS heads of a thread are on their way at once, the first ones while the angles are made
-template <bool BF16, int LANES, int ITEMS>
+// A wave to a token, or several, each with some of its heads: 64 / LANES heads at a time, LANES threads to a head, a piece of 8 channels each, ITEMS times on their way.
+template <bool BF16, int LANES, bool NORM, bool HALVES>
 __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
     typedef float float2_t __attribute__((ext_vector_type(2)));
-    __shared__ __attribute__((aligned(16))) float2_t turns[MOST_TOKENS * MAX_PAIRS];  // cosine, sine
-    constexpr int SLOTS = 256 / LANES;
-    const int row0 = (int)(p.first + (long long)blockIdx.x * p.tokens);
-    const int count = p.rows - row0 < p.tokens ? (int)(p.rows - row0) : p.tokens;
-    const int c = threadIdx.x % LANES, heads = p.heads[0] + p.heads[1], half = p.pairs / 8;
+    __shared__ __attribute__((aligned(16))) float2_t table[4][MAX_PAIRS];  // cosine, sine
+    constexpr int SLOTS = 64 / LANES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LANES, slot = lane / LANES;
+    const long long at = p.first + (long long)blockIdx.x * 4 + wave;
+    if (at >= p.work) return;
+    const int row = (int)(at / p.share), part = (int)(at - (long long)row * p.share), b = row / p.T, t = row - b * p.T;
     const bool in = c < p.D / 8;
-    // this thread's heads: `head` of token `n` next
-    int n = 0, head = threadIdx.x / LANES;
-    u32x4_t w[ITEMS];
-    char *out[ITEMS];
-    int token[ITEMS], which[ITEMS];
-    auto load = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            while (head >= heads) {
-                head -= heads;
-                n++;
-            }
-            token[i] = n < count ? n : -1;
-            which[i] = head >= p.heads[0];
-            w[i] = u32x4_t{0, 0, 0, 0};
-            if (n < count && in) {
-                const int k = which[i], h = k ? head - p.heads[0] : head, row = row0 + n, b = p.T ? row / p.T : 0, t = row - b * p.T;
-                const char *src = p.in[k] + b * p.in_s[k][0] + t * p.in_s[k][1] + h * p.in_s[k][2] + c * 16;
-                out[i] = p.out[k] + b * p.out_s[k][0] + t * p.out_s[k][1] + h * p.out_s[k][2] + c * 16;
-                if (p.once) w[i] = __builtin_nontemporal_load((const u32x4_t *)src);
-                else w[i] = *(const u32x4_t *)src;
-            }
-            head += SLOTS;
-        }
-    };
-    load();
-    u32x4_t g[2];
+    // turns of SLOTS heads: those of q, then those of k
+    const int nq = (p.heads[0] + SLOTS - 1) / SLOTS, all = nq + (p.heads[1] + SLOTS - 1) / SLOTS;
+    int turn = part * all / p.share;
+    const int end = (part + 1) * all / p.share;
+    const char *src[2];
+    char *dst[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        g[k] = u32x4_t{0, 0, 0, 0};
-        if (p.norm[k] && in) g[k] = *(const u32x4_t *)(p.norm[k] + c * 16);
+        src[k] = p.in[k] + b * p.in_s[k][0] + t * p.in_s[k][1] + (slot * p.in_s[k][2] + c * 16);
+        dst[k] = p.out[k] + b * p.out_s[k][0] + t * p.out_s[k][1] + (slot * p.out_s[k][2] + c * 16);
     }
-    for (int i = threadIdx.x; i < count * p.pairs; i += 256) {
-        const int m = i / p.pairs, pair = i - m * p.pairs, row = row0 + m, b = p.T ? row / p.T : 0, t = row - b * p.T;
-        const long long at = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
-        const double x = p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[at]
-                         : p.position_type == SVDQ_POSITION_INT64 ? (double)((const int64_t *)p.positions)[at] : (double)((const float *)p.positions)[at];
+    u32x4_t w[ITEMS];
+    auto load = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int k = first + i >= nq, head = (first + i - (k ? nq : 0)) * SLOTS;
+            w[i] = u32x4_t{0, 0, 0, 0};
+            if (first + i < end && in && head + slot < p.heads[k]) {
+                const u32x4_t *from = (const u32x4_t *)(src[k] + head * p.in_s[k][2]);
+                if (p.once) w[i] = __builtin_nontemporal_load(from);
+                else w[i] = *from;
+            }
+        }
+    };
+    load(turn);
+    u32x4_t g[2];
+    if (NORM) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            g[k] = u32x4_t{0, 0, 0, 0};
+            if (p.norm[k] && in) g[k] = *(const u32x4_t *)(p.norm[k] + c * 16);
+        }
+    }
+    for (int pair = lane; pair < p.pairs; pair += 64) {
+        const long long from = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
+        const double x = p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[from]
+                         : p.position_type == SVDQ_POSITION_INT64 ? (double)((const int64_t *)p.positions)[from] : (double)((const float *)p.positions)[from];
         const double revolutions = x * p.freq[pair];
         float s, co;
         sincospif(2.0f * (float)(revolutions - __builtin_rint(revolutions)), &s, &co);
-        turns[i] = float2_t{co, s};
+        table[wave][pair] = float2_t{co, s};
     }
-    __syncthreads();
-    for (;;) {
+    __builtin_amdgcn_wave_barrier();  // (LDS serves a wave in order)
+    // this lane's channels: of pair j cosine and sine; (1, 0) where channels pass
+    constexpr int PAIRS = HALVES ? 8 : 4;
+    const int half = p.pairs / 8;
+    const bool low = c < half;
+    float co[PAIRS], si[PAIRS];
+#pragma unroll
+    for (int j = 0; j < PAIRS; j++) {
+        const int pair = HALVES ? (low ? c : c - half) * 8 + j : c * 4 + j;
+        const bool turned = HALVES ? c < 2 * half : pair < p.pairs;
+        const float2_t cs = table[wave][turned ? pair : 0];
+        co[j] = turned ? cs[0] : 1.f;
+        si[j] = turned ? cs[1] : 0.f;
+        if (HALVES && low) si[j] = -si[j];
+    }
+    for (; turn < end; turn += ITEMS) {
+        if (turn != part * all / p.share) load(turn);
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
-            if (token[i] < 0) break;
+            if (turn + i >= end) break;
+            const int k = turn + i >= nq, head = (turn + i - (k ? nq : 0)) * SLOTS;
             float x[8], y[8];
             unpack<BF16>(w[i], x);
-            const bool norm = p.norm[0] || p.norm[1];
-            if (norm) {
-                // (the sum is everybody's, also where this head has no norm: lanes of other heads may have one)
+            if (NORM && p.norm[k]) {
                 float squares = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++) squares = __builtin_fmaf(x[j], x[j], squares);
                 squares = head_sum<LANES>(squares);
-                if (p.norm[which[i]]) {
-                    if (squares < 0x1p120f && squares >= p.tiny) {
-                        const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_d, p.eps));
+                if (squares < 0x1p120f && squares >= p.tiny) {
+                    const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, p.inv_d, p.eps));
 #pragma unroll
-                        for (int j = 0; j < 8; j++) x[j] *= r;
-                    } else {  // squares that leave fp32's range: once more in 64 bits (all lanes of the head)
-                        double s = 0.0;
+                    for (int j = 0; j < 8; j++) x[j] *= r;
+                } else {  // squares that leave fp32's range: once more in 64 bits (all lanes of the head)
+                    double s = 0.0;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) s += (double)x[j] * (double)x[j];
+                    for (int j = 0; j < 8; j++) s += (double)x[j] * (double)x[j];
 #pragma unroll
-                        for (int d = LANES / 2; d; d >>= 1) s += __shfl_xor(s, d);
-                        const double r = 1.0 / __builtin_sqrt(s / (double)p.D + (double)p.eps);
+                    for (int d = LANES / 2; d; d >>= 1) s += __shfl_xor(s, d);
+                    const double r = 1.0 / __builtin_sqrt(s / (double)p.D + (double)p.eps);
 #pragma unroll
-                        for (int j = 0; j < 8; j++) x[j] = (float)((double)x[j] * r);
-                    }
-                    unpack<BF16>(which[i] ? g[1] : g[0], y);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] *= y[j];
+                    for (int j = 0; j < 8; j++) x[j] = (float)((double)x[j] * r);
                 }
+                unpack<BF16>(g[k], y);
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] *= y[j];
             }
-            const float2_t *turn = turns + token[i] * p.pairs;
-            if (p.halves) {
-                const bool low = c < half;
+            if (HALVES) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) y[j] = __shfl(x[j], low ? c + half : c - half, LANES);
-                if (c < 2 * half) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float2_t cs = turn[(low ? c : c - half) * 8 + j];
-                        x[j] = low ? x[j] * cs[0] - y[j] * cs[1] : y[j] * cs[1] + x[j] * cs[0];
-                    }
-                }
+                for (int j = 0; j < 8; j++) x[j] = c < 2 * half ? x[j] * co[j] + y[j] * si[j] : x[j];
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int pair = c * 4 + j;
-                    if (pair < p.pairs) {
-                        const float2_t cs = turn[pair];
-                        const float a = x[2 * j], d = x[2 * j + 1];
-                        x[2 * j] = a * cs[0] - d * cs[1];
-                        x[2 * j + 1] = a * cs[1] + d * cs[0];
-                    }
+                    const float a = x[2 * j], d = x[2 * j + 1];
+                    x[2 * j] = a * co[j] - d * si[j];
+                    x[2 * j + 1] = a * si[j] + d * co[j];
                 }
             }
-            if (in) *(u32x4_t *)out[i] = pack<BF16>(x);
+            if (in && head + slot < p.heads[k]) *(u32x4_t *)(dst[k] + head * p.out_s[k][2]) = pack<BF16>(x);
         }
-        if (n >= count) return;
-        load();
     }
 }
 
+template <bool BF16, int LANES, bool NORM>
+void launch_pairs(const RotaryParams &p, unsigned blocks, hipStream_t st) {
+    if (p.halves) SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, NORM, true>), dim3(blocks), dim3(256), 0, st, p);
+    else SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, NORM, false>), dim3(blocks), dim3(256), 0, st, p);
+}
 template <bool BF16, int LANES>
 void launch_lanes(const RotaryParams &p, unsigned blocks, hipStream_t st) {
-    const dim3 grid(blocks), block(256);
-    if (p.tokens * (p.heads[0] + p.heads[1]) <= 256 / LANES) SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, 1>), grid, block, 0, st, p);
-    else SVDQ_LAUNCH((rotary_axes_kernel<BF16, LANES, 4>), grid, block, 0, st, p);
+    if (p.norm[0] || p.norm[1]) launch_pairs<BF16, LANES, true>(p, blocks, st);
+    else launch_pairs<BF16, LANES, false>(p, blocks, st);
 }
 template <bool BF16>
 void dispatch(const RotaryParams &p, unsigned blocks, hipStream_t st) {
@@ -247,12 +251,7 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
     }
     p.positions = a->positions;
     for (int j = 0; j < 3; j++) p.pos_s[j] = a->position_stride[j];
-    p.rows = a->batch * a->tokens;
-    // one row of tokens, where strides go on from an entry to the next
-    bool one = a->batch == 1 || a->position_stride[0] == a->tokens * a->position_stride[1];
-    for (int i = 0; i < 2; i++)
-        one = one && (a->batch == 1 || !ins[i] || (in_s[i][0] == a->tokens * in_s[i][1] && out_s[i][0] == a->tokens * out_s[i][1]));
-    p.T = one ? 0 : (int)a->tokens;
+    p.T = (int)a->tokens;
     p.heads[0] = (int)a->heads;
     p.heads[1] = a->k ? (int)a->kv_heads : 0;
     p.D = (int)a->head_dim;
@@ -273,16 +272,18 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
             p.axis[pair] = (uint8_t)i;
         }
     }
-    const int lanes = p.D <= 32 ? 4 : p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, heads = p.heads[0] + p.heads[1];
-    p.tokens = 1;
-    while (p.tokens < MOST_TOKENS && p.rows >= 2048 * p.tokens && p.tokens * heads < 4 * 256 / lanes) p.tokens *= 2;
-    p.once = p.rows * heads * p.D * 4 > 300000000;
-    // a launch takes fewer than 2^32 threads
-    const long long most = (1ll << 23) * p.tokens;
-    const long long all = p.rows;
+    const int lanes = p.D <= 32 ? 4 : p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, slots = 64 / lanes, turns = (p.heads[0] + slots - 1) / slots + (p.heads[1] + slots - 1) / slots;
+    const long long rows = a->batch * a->tokens;
+    // waves for every compute unit, as far as there is a turn for each
+    p.share = 1;
+    while (rows * p.share < 8192 && p.share < turns) p.share++;
+    p.work = rows * p.share;
+    p.once = rows * (p.heads[0] + p.heads[1]) * p.D * 4 > 300000000;
+    // a launch takes fewer than 2^32 threads, a wave is 64
+    const long long most = 1ll << 25, all = p.work;
     for (p.first = 0; p.first < all; p.first += most) {
-        p.rows = all - p.first < most ? all : p.first + most;
-        const unsigned blocks = (unsigned)((p.rows - p.first + p.tokens - 1) / p.tokens);
+        p.work = all - p.first < most ? all : p.first + most;
+        const unsigned blocks = (unsigned)((p.work - p.first + 3) / 4);
         if (a->dtype == SVDQ_BF16) dispatch<true>(p, blocks, (hipStream_t)stream);
         else dispatch<false>(p, blocks, (hipStream_t)stream);
         if (int rc = check_launch("rotary_axes")) return rc;
