@@ -18,7 +18,7 @@ struct NormParams {
     long long first, M, ld_x, ld_residual, ld_y, ld_h;   // bytes; rows first .. M are this launch's
     long long gate_s[2], scale_s[2], shift_s[2];        // bytes: entry, token
     long long tokens;                                   // rows of an entry
-    int sequences, pieces, zero_rest;                   // pieces of 8 elements per row
+    int sequences, pieces, zero_rest, once;             // pieces of 8 elements per row; once: what is read does not stay in the memory-side cache anyway
     float inv_k, tiny, eps, residual_scale;
 };
 
@@ -48,24 +48,51 @@ __device__ inline u32x4_t pack(const float (&f)[8]) {
     return w;
 }
 
-// The sum of x over a row's THREADS threads, in all of them.  `slot`: a place in LDS of its own for every sum, so that one barrier each is enough
-template <int THREADS, typename T>
-__device__ inline T row_sum(T x, T (*place)[16], int slot, int t) {
+// x of 16 lanes, of 64, added, in all of them
+template <int CONTROL>
+__device__ inline float moved(float x) {
+    return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), CONTROL, 0xF, 0xF, true));
+}
+__device__ inline float sum16(float x) {
+    x += moved<0xB1>(x);  // (quads, then mirrored halves of 8 and of 16)
+    x += moved<0x4E>(x);
+    x += moved<0x141>(x);
+    return x + moved<0x140>(x);
+}
+__device__ inline float sum64(float x) {
+    x = sum16(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(f32_bits(x), f32_bits(x), false, false);
+    x = bits_f32(a[0]) + bits_f32(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(x), false, false);
+    return bits_f32(b[0]) + bits_f32(b[1]);
+}
+__device__ inline double sum16(double x) {
 #pragma unroll
-    for (int d = THREADS < 64 ? THREADS / 2 : 32; d; d >>= 1) x += __shfl_xor(x, d);
-    if constexpr (THREADS > 64) {
-        if ((t & 63) == 0) place[slot][t >> 6] = x;
+    for (int d = 8; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ inline double sum64(double x) {
+    x = sum16(x);
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// The sum of x over a row's threads, in all of them.  WIDE: a workgroup has the row; `slot`: a place in LDS of its own for every sum, so that one barrier each is enough
+template <bool WIDE, typename T>
+__device__ inline T row_sum(T x, T (*place)[16], int slot) {
+    x = sum64(x);
+    if constexpr (WIDE) {
+        const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+        if (lane == 0) place[slot][threadIdx.x >> 6] = x;
         __syncthreads();
-        x = 0;
-#pragma unroll
-        for (int i = 0; i < THREADS / 64; i++) x += place[slot][i];
+        x = sum16((lane & 15) < waves ? place[slot][lane & 15] : (T)0);
     }
     return x;
 }
 
 // h <- (h - m) / sqrt(mean((h - m)^2) + eps), the pieces of this thread that lie in the row
-template <int THREADS, int VECS>
-__device__ inline void normalise(float (&h)[VECS][8], bool center, const NormParams &p, int t, int slot) {
+template <bool WIDE, int VECS>
+__device__ inline void normalise(float (&h)[VECS][8], bool center, const NormParams &p, int t, int threads, int slot) {
     __shared__ float sums[4][16];
     __shared__ double wide[4][16];
     float m = 0.f;
@@ -75,18 +102,18 @@ __device__ inline void normalise(float (&h)[VECS][8], bool center, const NormPar
         for (int i = 0; i < VECS; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) s += h[i][j];  // (zeros behind the row's end)
-        m = row_sum<THREADS>(s, sums, slot, t) * p.inv_k;
+        m = row_sum<WIDE>(s, sums, slot) * p.inv_k;
     }
     float squares = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-        if (t + i * THREADS >= p.pieces) break;
+        if (t + i * threads >= p.pieces) break;
 #pragma unroll
         for (int j = 0; j < 8; j++) squares = __builtin_fmaf(h[i][j] - m, h[i][j] - m, squares);
     }
-    squares = row_sum<THREADS>(squares, sums, slot + 1, t);
+    squares = row_sum<WIDE>(squares, sums, slot + 1);
     if (squares < 0x1p120f && squares >= p.tiny) {
-        const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(squares, p.inv_k, p.eps));
+        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, p.inv_k, p.eps));
 #pragma unroll
         for (int i = 0; i < VECS; i++)
 #pragma unroll
@@ -100,109 +127,125 @@ __device__ inline void normalise(float (&h)[VECS][8], bool center, const NormPar
         for (int i = 0; i < VECS; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) s += (double)h[i][j];
-        mean = row_sum<THREADS>(s, wide, slot, t) * inv_k;
+        mean = row_sum<WIDE>(s, wide, slot) * inv_k;
         s = 0.0;
     }
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-        if (t + i * THREADS >= p.pieces) break;
+        if (t + i * threads >= p.pieces) break;
 #pragma unroll
         for (int j = 0; j < 8; j++) s += ((double)h[i][j] - mean) * ((double)h[i][j] - mean);
     }
-    const double r = 1.0 / __builtin_sqrt(row_sum<THREADS>(s, wide, slot + 1, t) * inv_k + (double)p.eps);
+    const double r = 1.0 / __builtin_sqrt(row_sum<WIDE>(s, wide, slot + 1) * inv_k + (double)p.eps);
 #pragma unroll
     for (int i = 0; i < VECS; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) h[i][j] = (float)(((double)h[i][j] - mean) * r);
 }
 
-// The sequence of a row: how many offsets are not behind it, less one (-1 or the number of sequences: none).  THREADS threads look together.
-template <int THREADS>
-__device__ inline int sequence_of(const NormParams &p, long long row, int t) {
-    constexpr int L = THREADS < 64 ? THREADS : 64;
-    const int li = t % L;
+// The sequence of a row: how many offsets are not behind it, less one (-1 or the number of sequences: none), 64 at a time
+__device__ inline int sequence_of(const NormParams &p, long long row) {
+    const int lane = threadIdx.x & 63;
     int n = 0;
-    for (int base = 0; base <= p.sequences; base += L) {
-        uint64_t in = __ballot(base + li <= p.sequences && p.cu_seqlens[base + li] <= row);
-        if (L == 32) in = (threadIdx.x & 32 ? in >> 32 : in) & 0xFFFFFFFFull;
-        n += __popcll(in);
-    }
+    for (int base = 0; base <= p.sequences; base += 64) n += __popcll(__ballot(base + lane <= p.sequences && p.cu_seqlens[base + lane] <= row));
     return n - 1;
 }
 
-// THREADS per row (32 and 64: several rows per workgroup), each with up to VECS pieces of 8 elements
-template <bool BF16, int THREADS, int VECS, bool LAYER>
-__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) gated_norm_kernel(NormParams p) {
-    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
-    const int t = threadIdx.x % THREADS;
-    const long long row = p.first + (long long)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    if (row >= p.M) return;  // (all threads of a row; rows of several waves are one per workgroup)
-    long long entry = row / p.tokens, token = row - entry * p.tokens;
-    bool any = true;
-    if (p.cu_seqlens) {
-        entry = sequence_of<THREADS>(p, row, t);
-        token = 0;
-        any = entry >= 0 && entry < p.sequences;
+// A row to a wave, four to a workgroup, or (WIDE) to a workgroup; each thread up to VECS pieces of 8 elements.  Of rows of one piece a thread, everything is asked for
+// at once.
+template <bool BF16, bool WIDE, int VECS, bool LAYER>
+__global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormParams p) {
+    constexpr bool EARLY = VECS == 1;
+    const int threads = WIDE ? blockDim.x : 64, t = WIDE ? threadIdx.x : threadIdx.x & 63;
+    const long long row = p.first + (WIDE ? blockIdx.x : (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    if (row >= p.M) return;  // (all threads of a row)
+    u32x4_t w[VECS], r[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+        const int piece = t + i * threads;
+        w[i] = r[i] = u32x4_t{0, 0, 0, 0};
+        if (piece < p.pieces) {
+            const u32x4_t *x = (const u32x4_t *)(p.x + row * p.ld_x + (size_t)piece * 16), *res = (const u32x4_t *)(p.residual + row * p.ld_residual + (size_t)piece * 16);
+            if (p.once) {
+                w[i] = __builtin_nontemporal_load(x);
+                if (p.residual) r[i] = __builtin_nontemporal_load(res);
+            } else {
+                w[i] = *x;
+                if (p.residual) r[i] = *res;
+            }
+        }
     }
-    if (!any) {
-        if (p.zero_rest) {
+    int entry = 0, token = 0;
+    if (p.cu_seqlens) {
+        entry = sequence_of(p, row);
+        if (entry < 0 || entry >= p.sequences) {
 #pragma unroll
             for (int i = 0; i < VECS; i++) {
-                const int piece = t + i * THREADS;
+                const int piece = t + i * threads;
                 if (piece >= p.pieces) break;
                 if (p.zero_rest & 1) *(u32x4_t *)(p.y + row * p.ld_y + (size_t)piece * 16) = u32x4_t{0, 0, 0, 0};
                 if (p.h && (p.zero_rest & 2)) *(u32x4_t *)(p.h + row * p.ld_h + (size_t)piece * 16) = u32x4_t{0, 0, 0, 0};
             }
+            return;
         }
-        return;
+    } else if (p.gate || p.scale || p.shift) {
+        entry = (int)row / (int)p.tokens;
+        token = (int)row - entry * (int)p.tokens;
     }
-    u32x4_t w[VECS], r[VECS];
+    const char *vectors[5] = {p.branch_weight, p.gate, p.weight, p.scale, p.shift};
+    if (p.gate) vectors[1] += entry * p.gate_s[0] + token * p.gate_s[1];
+    if (p.scale) vectors[3] += entry * p.scale_s[0] + token * p.scale_s[1];
+    if (p.shift) vectors[4] += entry * p.shift_s[0] + token * p.shift_s[1];
+    u32x4_t early[EARLY ? 5 : 1];
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int v = 0; v < 5; v++) {
+            early[v] = u32x4_t{0, 0, 0, 0};
+            if (vectors[v] && t < p.pieces) early[v] = *(const u32x4_t *)(vectors[v] + (size_t)t * 16);
+        }
+    }
     float h[VECS][8], f[8];
 #pragma unroll
-    for (int i = 0; i < VECS; i++) {
-        const int piece = t + i * THREADS;
-        w[i] = r[i] = u32x4_t{0, 0, 0, 0};
-        if (piece < p.pieces) {
-            w[i] = *(const u32x4_t *)(p.x + row * p.ld_x + (size_t)piece * 16);
-            if (p.residual) r[i] = *(const u32x4_t *)(p.residual + row * p.ld_residual + (size_t)piece * 16);
-        }
-    }
-#pragma unroll
     for (int i = 0; i < VECS; i++) unpack<BF16>(w[i], h[i]);
-    auto times = [&](const char *v, float add) __attribute__((always_inline)) {
+    // f: of vector v, this thread's piece i
+    auto piece_of = [&](int v, int i) __attribute__((always_inline)) {
+        if constexpr (EARLY) unpack<BF16>(early[v], f);
+        else unpack<BF16>(*(const u32x4_t *)(vectors[v] + (size_t)(t + i * threads) * 16), f);
+    };
+    auto times = [&](int v, float add) __attribute__((always_inline)) {
+        if (!vectors[v]) return;
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
-            const int piece = t + i * THREADS;
-            if (piece >= p.pieces) break;
-            unpack<BF16>(*(const u32x4_t *)(v + (size_t)piece * 16), f);
+            if (t + i * threads >= p.pieces) break;
+            piece_of(v, i);
 #pragma unroll
             for (int j = 0; j < 8; j++) h[i][j] *= add + f[j];
         }
     };
     if (p.branch_weight) {
-        normalise<THREADS, VECS>(h, false, p, t, 0);
-        times(p.branch_weight, 0.f);
+        normalise<WIDE, VECS>(h, false, p, t, threads, 0);
+        times(0, 0.f);
     }
-    if (p.gate) times(p.gate + entry * p.gate_s[0] + token * p.gate_s[1], 0.f);
+    times(1, 0.f);
     if (p.residual) {
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
-            const int piece = t + i * THREADS;
+            const int piece = t + i * threads;
             unpack<BF16>(r[i], f);
 #pragma unroll
             for (int j = 0; j < 8; j++) h[i][j] = __builtin_fmaf(p.residual_scale, f[j], h[i][j]);
             if (piece < p.pieces && p.h) *(u32x4_t *)(p.h + row * p.ld_h + (size_t)piece * 16) = pack<BF16>(h[i]);
         }
     }
-    normalise<THREADS, VECS>(h, LAYER, p, t, 2);
-    if (p.weight) times(p.weight, 0.f);
-    if (p.scale) times(p.scale + entry * p.scale_s[0] + token * p.scale_s[1], 1.f);
+    normalise<WIDE, VECS>(h, LAYER, p, t, threads, 2);
+    times(2, 0.f);
+    times(3, 1.f);
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
-        const int piece = t + i * THREADS;
+        const int piece = t + i * threads;
         if (piece >= p.pieces) break;
         if (p.shift) {
-            unpack<BF16>(*(const u32x4_t *)(p.shift + entry * p.shift_s[0] + token * p.shift_s[1] + (size_t)piece * 16), f);
+            piece_of(4, i);
 #pragma unroll
             for (int j = 0; j < 8; j++) h[i][j] += f[j];
         }
@@ -210,25 +253,21 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) gated_norm_kern
     }
 }
 
-template <bool BF16, int THREADS, int VECS>
-void launch_rows(const NormParams &p, bool layer, hipStream_t st) {
-    constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1;
-    const dim3 grid((unsigned)((p.M - p.first + ROWS - 1) / ROWS)), block(THREADS < 256 ? 256 : THREADS);
-    if (layer) SVDQ_LAUNCH((gated_norm_kernel<BF16, THREADS, VECS, true>), grid, block, 0, st, p);
-    else SVDQ_LAUNCH((gated_norm_kernel<BF16, THREADS, VECS, false>), grid, block, 0, st, p);
+template <bool BF16, bool WIDE, int VECS>
+void launch_rows(const NormParams &p, int threads, bool layer, hipStream_t st) {
+    const long long rows = p.M - p.first;
+    const dim3 grid((unsigned)(WIDE ? rows : (rows + 3) / 4)), block(WIDE ? threads : 256);
+    if (layer) SVDQ_LAUNCH((gated_norm_kernel<BF16, WIDE, VECS, true>), grid, block, 0, st, p);
+    else SVDQ_LAUNCH((gated_norm_kernel<BF16, WIDE, VECS, false>), grid, block, 0, st, p);
 }
 
 template <bool BF16>
 void dispatch(const NormParams &p, bool layer, hipStream_t st) {
-    const int need = p.pieces;
-    if (need <= 32) launch_rows<BF16, 32, 1>(p, layer, st);
-    else if (need <= 64) launch_rows<BF16, 64, 1>(p, layer, st);
-    else if (need <= 128) launch_rows<BF16, 64, 2>(p, layer, st);
-    else if (need <= 256) launch_rows<BF16, 256, 1>(p, layer, st);
-    else if (need <= 512) launch_rows<BF16, 256, 2>(p, layer, st);
-    else if (need <= 1024) launch_rows<BF16, 512, 2>(p, layer, st);
-    else if (need <= 2048) launch_rows<BF16, 1024, 2>(p, layer, st);
-    else launch_rows<BF16, 1024, 4>(p, layer, st);
+    const int need = p.pieces, waves = (need + 63) / 64;
+    if (waves == 1) launch_rows<BF16, false, 1>(p, 64, layer, st);
+    else if (waves <= 16) launch_rows<BF16, true, 1>(p, waves * 64, layer, st);
+    else if (waves <= 32) launch_rows<BF16, true, 2>(p, (waves + 1) / 2 * 64, layer, st);
+    else launch_rows<BF16, true, 4>(p, (waves + 3) / 4 * 64, layer, st);
 }
 
 bool vector_ok(const void *v, const int64_t *s) { return !v || ((uintptr_t)v % 16 == 0 && s[0] >= 0 && s[1] >= 0 && (s[0] | s[1]) % 8 == 0); }
@@ -285,6 +324,7 @@ extern "C" int svdq_gated_norm(const svdq_gated_norm_args *a, void *stream) {
     p.tokens = a->cu_seqlens ? a->M : a->tokens;
     p.sequences = (int)a->sequences;
     p.pieces = (int)(a->K / 8);
+    p.once = a->M * a->K * (a->residual ? 8 : 4) > 300000000;
     p.zero_rest = a->zero_rest;
     p.inv_k = 1.0f / (float)a->K;
     // fp32 rounds a square by 2^-150 at most, K of them by K * 2^-150: from K * 2^-126 on 2^-24 of the sum, and nothing beside an eps of 2^-120
@@ -292,7 +332,7 @@ extern "C" int svdq_gated_norm(const svdq_gated_norm_args *a, void *stream) {
     p.eps = a->eps;
     p.residual_scale = a->residual_scale;
     // a launch takes fewer than 2^32 threads
-    const long long most = p.pieces <= 128 ? 1ll << 25 : 1ll << 21;
+    const long long most = 1ll << 21;
     for (p.first = 0; p.first < a->M; p.first += most) {
         p.M = a->M - p.first < most ? a->M : p.first + most;
         if (a->dtype == SVDQ_BF16) dispatch<true>(p, a->layer != 0, (hipStream_t)stream);
