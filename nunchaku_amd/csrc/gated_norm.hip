@@ -5,6 +5,8 @@
 // the first conversion to the last: y is made of h as it is, before h is rounded for the residual stream.
 // The mean is taken before the deviations' squares are summed, from registers: their difference in one pass would lose what a large mean leaves.
 // Squares whose sum leaves fp32's range, at either end, are summed once more in 64 bits: rows of finite numbers have finite norms.
+// Bound by the traffic, 8 bytes an element with a residual: 2 x 4608 x 5120 72 us, 5.3 TB/s (a copy reaches 5.1 here), 4096 x 4096 21.6, 6.2 TB/s; one row of 4096 with
+// both norms 3.0, launch and latencies.
 #include "svdq_common.h"
 
 using namespace svdq;
@@ -18,7 +20,7 @@ struct NormParams {
     long long first, M, ld_x, ld_residual, ld_y, ld_h;   // bytes; rows first .. M are this launch's
     long long gate_s[2], scale_s[2], shift_s[2];        // bytes: entry, token
     long long tokens;                                   // rows of an entry
-    int sequences, pieces, zero_rest, once;             // pieces of 8 elements per row; once: what is read does not stay in the memory-side cache anyway
+    int sequences, pieces, zero_rest;                   // pieces of 8 elements per row
     float inv_k, tiny, eps, residual_scale;
 };
 
@@ -165,14 +167,8 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormParam
         const int piece = t + i * threads;
         w[i] = r[i] = u32x4_t{0, 0, 0, 0};
         if (piece < p.pieces) {
-            const u32x4_t *x = (const u32x4_t *)(p.x + row * p.ld_x + (size_t)piece * 16), *res = (const u32x4_t *)(p.residual + row * p.ld_residual + (size_t)piece * 16);
-            if (p.once) {
-                w[i] = __builtin_nontemporal_load(x);
-                if (p.residual) r[i] = __builtin_nontemporal_load(res);
-            } else {
-                w[i] = *x;
-                if (p.residual) r[i] = *res;
-            }
+            w[i] = *(const u32x4_t *)(p.x + row * p.ld_x + (size_t)piece * 16);
+            if (p.residual) r[i] = *(const u32x4_t *)(p.residual + row * p.ld_residual + (size_t)piece * 16);
         }
     }
     int entry = 0, token = 0;
@@ -264,8 +260,11 @@ void launch_rows(const NormParams &p, int threads, bool layer, hipStream_t st) {
 template <bool BF16>
 void dispatch(const NormParams &p, bool layer, hipStream_t st) {
     const int need = p.pieces, waves = (need + 63) / 64;
+    // Two pieces a thread, where there is no residual to be asked for beside the row, if the rows are more than the card takes at once.  Us, two / one: 9000 x 5120 30.4 / 41.7,
+    // 4096 x 4096 13.3 / 14.4, 700 x 4096 4.9 / 5.0; 1500 x 1536 4.8 / 4.5; with a residual 16384 x 1536 32.5 / 30.2, 4096 x 4096 22.6 / 21.6
+    const bool two = !p.residual && waves > 2 && (p.M - p.first) * need > 320000;
     if (waves == 1) launch_rows<BF16, false, 1>(p, 64, layer, st);
-    else if (waves <= 16) launch_rows<BF16, true, 1>(p, waves * 64, layer, st);
+    else if (waves <= 16 && !two) launch_rows<BF16, true, 1>(p, waves * 64, layer, st);
     else if (waves <= 32) launch_rows<BF16, true, 2>(p, (waves + 1) / 2 * 64, layer, st);
     else launch_rows<BF16, true, 4>(p, (waves + 3) / 4 * 64, layer, st);
 }
@@ -324,7 +323,6 @@ extern "C" int svdq_gated_norm(const svdq_gated_norm_args *a, void *stream) {
     p.tokens = a->cu_seqlens ? a->M : a->tokens;
     p.sequences = (int)a->sequences;
     p.pieces = (int)(a->K / 8);
-    p.once = a->M * a->K * (a->residual ? 8 : 4) > 300000000;
     p.zero_rest = a->zero_rest;
     p.inv_k = 1.0f / (float)a->K;
     // fp32 rounds a square by 2^-150 at most, K of them by K * 2^-150: from K * 2^-126 on 2^-24 of the sum, and nothing beside an eps of 2^-120
