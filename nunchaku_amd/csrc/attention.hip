@@ -157,101 +157,6 @@ __device__ inline bool block_of(const AttentionParams &p, int groups, int &rb, i
     return true;
 }
 
-// The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
-template <typename H, int WAVES>
-struct Copies {
-    // Request i of a wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
-    // two steps: the wave's rows start on a multiple of 16 where there are four requests, of 8 where there are two).  With 12 pieces in a
-    // row a request is five rows and a third: each has its own rows, pieces and offsets.
-    static constexpr bool EVEN = H::PITCH != 192;
-    static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
-    static_assert(!EVEN || REQ == 1 || (REQ * H::RPR <= 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
-    static_assert(EVEN || (H::REQ % WAVES == 0 && H::fv(1) == 0 && H::fk(15) < 4), "");
-    static constexpr int OWN = EVEN ? 1 : REQ;
-    const char *kp, *vp;
-    long long k_token, v_token;
-    uint32_t dst, ok[OWN], ov[OWN], ck[OWN];
-    int row[OWN], count, bytes;
-    bool any, in_row[OWN];  // (whether V's piece lies in the head)
-    __device__ inline Copies(const AttentionParams &p, char *lds, int b, int hk, long long first, int count_, int wave, int lane, uint32_t one) {
-        kp = p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2];
-        vp = p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2];
-        k_token = p.ks[1];
-        v_token = p.vs[1];
-        count = count_;
-        bytes = p.D * 2;
-        any = wave < ACTIVE;
-        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
-#pragma unroll
-        for (int i = 0; i < OWN; i++) {
-            const int piece = (wave * REQ + i) * 64 + lane, place = piece % H::PIECES;
-            row[i] = piece / H::PIECES;
-            ck[i] = (place ^ H::fk(row[i])) * 16;
-            ok[i] = (uint32_t)(row[i] * k_token);
-            ov[i] = (uint32_t)(row[i] * v_token) + (place ^ H::fv(row[i])) * 16;
-            in_row[i] = (place ^ H::fv(row[i])) * 16 < bytes;
-            if (!EVEN) ok[i] += ck[i];
-        }
-        // columns behind the head's end, as far as they are multiplied, are zero in K for good: no copy writes there (all waves see it behind the
-        // first step's barrier)
-        zero_columns<H, 2 * KEYS>(lds, p.D / 8, threadIdx.x, WAVES * 64);
-        if constexpr (H::ONES) {
-            for (int r = threadIdx.x; r < 2 * KEYS; r += WAVES * 64)
-                *(u32x4_t *)(lds + 2 * H::TILE + r * H::PITCH + ((p.D / 8) ^ H::fv(r)) * 16) = u32x4_t{one, 0, 0, 0};
-        }
-    }
-    // K of step `step` to stage `slot`.  Rows behind the last key are not read: their scores are masked whatever they are.
-    __device__ __forceinline__ void k(int step, int slot) {
-        if (!any) return;
-        const char *k = kp + (long long)step * KEYS * k_token;
-        const int left = count - step * KEYS;
-        if constexpr (EVEN) {
-            uint32_t c0 = ck[0];
-            asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
-            if (left >= KEYS && bytes == H::PITCH) {
-#pragma unroll
-                for (int i = 0; i < REQ; i++) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + (c0 ^ (64 * i)));
-            } else {
-#pragma unroll
-                for (int i = 0; i < REQ; i++) {
-                    const uint32_t c = c0 ^ (64 * i);
-                    if ((int)c < bytes && row[0] < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + c);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < REQ; i++)
-                if ((int)ck[i] < bytes && row[i] < left) copy16(dst + slot * H::TILE + i * 1024, k, ok[i]);
-        }
-    }
-    // V: zeros for keys that do not count, since nothing times a NaN is one
-    __device__ __forceinline__ void v(int step, int slot, uint64_t bits) {
-        if (!any) return;
-        const char *v = vp + (long long)step * KEYS * v_token;
-        const uint32_t to = dst + (2 + slot) * H::TILE;
-        if constexpr (EVEN) {
-            if (!in_row[0]) return;
-            if (bits == ~0ull) {
-#pragma unroll
-                for (int i = 0; i < REQ; i++) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < REQ; i++) {
-                    if ((bits >> (i * H::RPR)) >> row[0] & 1) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
-                    else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < REQ; i++) {
-                if (!in_row[i]) continue;
-                if (bits == ~0ull || (bits >> row[i] & 1)) copy16(to + i * 1024, v, ov[i]);
-                else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
-            }
-        }
-    }
-};
-
 // ---- rows form: 128 rows per workgroup, 32 per wave; all waves share the keys through LDS, two steps of them -------------------
 // Bound by each wave's chain of scores, maximum, exponentials and second product: 4096 queries, 4573 keys, 24 heads of 128 in fp16 take 247 us,
 // 931 TFLOP/s, the matrix cores busy 46 % of the cycles.  A step takes a workgroup by itself 1.12 us, each of two on a compute unit 1.08: the second wave
@@ -274,7 +179,8 @@ __global__ void __launch_bounds__(256, 2) attention_rows_kernel(AttentionParams 
     State<BF16, H> st;
     load_q<BF16, H>(p, qf, b, hk, row, lane);
     st.clear();
-    Copies<H, 4> copies(p, lds, b, hk, first, count, wave, lane, E::ONE);
+    Copies<H, 4> copies(lds, p.k + b * p.ks[0] * (p.cu_seqlens ? 0 : 1) + first * p.ks[1] + hk * p.ks[2], p.v + b * p.vs[0] * (p.cu_seqlens ? 0 : 1) + first * p.vs[1] + hk * p.vs[2],
+                        p.ks[1], p.vs[1], p.D, count, wave, lane, E::ONE);
     Steps<MASK> list;
     int begin = 0, end = (count + KEYS - 1) / KEYS;
     share(p, part, begin, end);

@@ -228,5 +228,101 @@ __device__ inline void zero_columns(char *lds, int first, int thread, int thread
         for (int c = first; c < H::DP / 8; c++) *(u32x4_t *)(lds + r * H::PITCH + (c ^ H::fk(r % KEYS)) * 16) = u32x4_t{0, 0, 0, 0};
 }
 
+// The copies of K and V to LDS by the WAVES waves of a workgroup: stages 0 and 1 of K, then those of V.
+template <typename H, int WAVES>
+struct Copies {
+    // Request i of a wave brings rows row0 + i * RPR.  What a lane reads of them: V the same piece every time, K piece c ^ 4 i (f's
+    // two steps: the wave's rows start on a multiple of 16 where there are four requests, of 8 where there are two).  With 12 pieces in a
+    // row a request is five rows and a third: each has its own rows, pieces and offsets.
+    static constexpr bool EVEN = H::PITCH != 192;
+    static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
+    static_assert(!EVEN || REQ == 1 || (REQ * H::RPR <= 16 && H::fk(H::RPR) == 4 && H::fv(H::RPR) == 0), "");
+    static_assert(EVEN || (H::REQ % WAVES == 0 && H::fv(1) == 0 && H::fk(15) < 4), "");
+    static constexpr int OWN = EVEN ? 1 : REQ;
+    const char *kp, *vp;
+    long long k_token, v_token;
+    uint32_t dst, ok[OWN], ov[OWN], ck[OWN];
+    int row[OWN], count, bytes;
+    bool any, in_row[OWN];  // (whether V's piece lies in the head)
+    // keys and values of a head from the first one on, the bytes from one to the next, channels of a head, how many there are, 1 in the tensors' type
+    __device__ inline Copies(char *lds, const char *k_, const char *v_, long long k_token_, long long v_token_, int D, int count_, int wave, int lane, uint32_t one) {
+        kp = k_;
+        vp = v_;
+        k_token = k_token_;
+        v_token = v_token_;
+        count = count_;
+        bytes = D * 2;
+        any = wave < ACTIVE;
+        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const int piece = (wave * REQ + i) * 64 + lane, place = piece % H::PIECES;
+            row[i] = piece / H::PIECES;
+            ck[i] = (place ^ H::fk(row[i])) * 16;
+            ok[i] = (uint32_t)(row[i] * k_token);
+            ov[i] = (uint32_t)(row[i] * v_token) + (place ^ H::fv(row[i])) * 16;
+            in_row[i] = (place ^ H::fv(row[i])) * 16 < bytes;
+            if (!EVEN) ok[i] += ck[i];
+        }
+        // columns behind the head's end, as far as they are multiplied, are zero in K for good: no copy writes there (all waves see it behind the
+        // first step's barrier)
+        zero_columns<H, 2 * KEYS>(lds, D / 8, threadIdx.x, WAVES * 64);
+        if constexpr (H::ONES) {
+            for (int r = threadIdx.x; r < 2 * KEYS; r += WAVES * 64)
+                *(u32x4_t *)(lds + 2 * H::TILE + r * H::PITCH + ((D / 8) ^ H::fv(r)) * 16) = u32x4_t{one, 0, 0, 0};
+        }
+    }
+    // K of step `step` to stage `slot`.  Rows behind the last key are not read: their scores are masked whatever they are.
+    __device__ __forceinline__ void k(int step, int slot) {
+        if (!any) return;
+        const char *k = kp + (long long)step * KEYS * k_token;
+        const int left = count - step * KEYS;
+        if constexpr (EVEN) {
+            uint32_t c0 = ck[0];
+            asm volatile("" : "+v"(c0));  // (what differs between the requests is worked out anew: registers are short)
+            if (left >= KEYS && bytes == H::PITCH) {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + (c0 ^ (64 * i)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) {
+                    const uint32_t c = c0 ^ (64 * i);
+                    if ((int)c < bytes && row[0] < left - i * H::RPR) copy16(dst + slot * H::TILE + i * 1024, k + i * H::RPR * k_token, ok[0] + c);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < REQ; i++)
+                if ((int)ck[i] < bytes && row[i] < left) copy16(dst + slot * H::TILE + i * 1024, k, ok[i]);
+        }
+    }
+    // V: zeros for keys that do not count, since nothing times a NaN is one
+    __device__ __forceinline__ void v(int step, int slot, uint64_t bits) {
+        if (!any) return;
+        const char *v = vp + (long long)step * KEYS * v_token;
+        const uint32_t to = dst + (2 + slot) * H::TILE;
+        if constexpr (EVEN) {
+            if (!in_row[0]) return;
+            if (bits == ~0ull) {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) {
+                    if ((bits >> (i * H::RPR)) >> row[0] & 1) copy16(to + i * 1024, v + i * H::RPR * v_token, ov[0]);
+                    else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < REQ; i++) {
+                if (!in_row[i]) continue;
+                if (bits == ~0ull || (bits >> row[i] & 1)) copy16(to + i * 1024, v, ov[i]);
+                else clear16(to + i * 1024 + (threadIdx.x & 63) * 16);
+            }
+        }
+    }
+};
+
 }  // namespace attention
 }  // namespace svdq

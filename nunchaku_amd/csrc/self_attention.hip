@@ -449,7 +449,148 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     }
 }
 
-// ---- rows form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
+// The end of a wave's 32 rows: the quotients, or an item's share of them
+template <bool BF16, typename H, int BLOCK_ROWS>
+__device__ inline void finish(const Params &p, const Item &it, const Rows &r, State<BF16, H> &st, int hk, int wave, int lane) {
+    const int col = lane & 31, h = lane >> 5;
+    if constexpr (H::ONES) {
+#pragma unroll
+        for (int g = 0; g < 4 * H::DB; g++)
+            if (8 * g == p.D && h == 0) st.sum = st.o[g >> 2][4 * (g & 3)];
+    }
+    const float sum = across_sum(st.sum);
+    if (it.parts > 1) {
+        if (!r.in) return;
+        float *dst = share_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
+#pragma unroll
+        for (int d = 0; d < H::DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int c = 32 * d + 8 * g + 4 * h;
+                if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+            }
+        if (h == 0) {
+            float *ms = stats_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
+            ms[0] = st.top;
+            ms[1] = sum;
+        }
+        return;
+    }
+    const float inv = inverse(sum);
+#pragma unroll
+    for (int u = 0; u < 2 * H::DB; u++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = st.o[u >> 1][8 * (u & 1) + e];
+        store_columns<BF16>(r.out, x, inv, 16 * u, r.in ? p.D : 0, lane);
+    }
+}
+
+// ---- rows form: 128 rows per workgroup, 32 per wave; all four waves share the keys through LDS, 64 a step, two steps of them; two workgroups or three to a compute
+// unit.  Where rows are fewer than whole blocks of the turns form would have for every compute unit ---------------------------------------------------------------
+constexpr int HALF = 128;
+
+template <bool BF16, int DP, bool ONES>
+__global__ void __launch_bounds__(256, 2) self_attention_rows_kernel(Params p) {
+    using H = Head<DP, false, ONES>;
+    using E = Elem<BF16>;
+    using vec = typename E::vec;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    const Item it = p.target ? part_of<HALF, KEYS, false>(p, at, lane) : item_of<HALF>(p, at, lane);
+    if (!it.any) return;
+    const int wave0 = it.rb * HALF + wave * 32;
+    Rows r = rows_of(p, it.r, hk, wave0 + col);
+    int least, most, wave_least, wave_most, begin, end;
+    limits_of(p, r, it.rb * HALF, HALF, least, most);
+    limits_of(p, r, wave0, 32, wave_least, wave_most);
+    vec qf[H::KS];
+    load_q<BF16, H>(p, qf, r, lane);
+    // a part's keys: limits from its first one on
+    share<KEYS>(it, most, begin, end);
+    const int skip = begin * KEYS, stop = end * KEYS;
+    most = (most < stop ? most : stop) - skip;
+    wave_most = (wave_most < stop ? wave_most : stop) - skip;
+    wave_least -= skip;
+    r.limit -= skip;
+    const int steps = end > begin ? end - begin : 0;  // (a part may lie behind all keys that are seen)
+    Copies<H, 4> copies(lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], p.ks[1], p.vs[1], p.D, most, wave, lane, E::ONE);
+    State<BF16, H> st;
+    auto ask = [&](int step, int slot) __attribute__((always_inline)) {
+        const int left = most - step * KEYS;
+        copies.k(step, slot);
+        copies.v(step, slot, left >= KEYS ? ~0ull : (1ull << left) - 1);
+    };
+    float16_t s[2];
+    // operands of four matrix instructions at a time, the next four's on their way
+    constexpr int N = 2 * H::KS, GROUP = N % 4 == 0 ? 4 : 2;
+    auto score = [&](int slot) __attribute__((always_inline)) {
+        const char *k = lds + slot * H::TILE + col * H::PITCH;
+        vec kf[2][GROUP];
+        auto read_k = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                kf[g & 1][i] = __builtin_bit_cast(vec, *(const u32x4_t *)(k + kb * 32 * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16));
+            }
+        };
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+        read_k(0);
+#pragma unroll
+        for (int g = 0; g < N / GROUP; g++) {
+            if (g + 1 < N / GROUP) read_k(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
+                s[kb] = E::mfma(kf[g & 1][i], qf[ks], s[kb]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    st.clear();
+    if (steps > 0) ask(0, 0);
+    wait_for_q<BF16, H>(qf);
+    for (int step = 0; step < steps; step++) {
+        const int slot = step & 1;
+        // K and V of this step have landed, of all waves, and nobody reads what the next requests overwrite
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + 1 < steps) ask(step + 1, slot ^ 1);
+        if (step * KEYS >= wave_most) continue;
+        score(slot);
+        if (wave_least < (step + 1) * KEYS) hide(s, step * KEYS, r.limit, lane);
+        st.template attend<H::ONES>(s, ~0ull, p.scale2, lds + (2 + slot) * H::TILE, lane);
+    }
+    // Once more, key by key where rows do not see all keys, if sums turn out to hold a NaN: rows that see none of its causes have none then
+    if (p.causal && steps > 0) {
+        int *flags = (int *)(lds + 4 * H::TILE);
+        const bool nan = any_nan(st, p.D);
+        if (lane == 0) flags[wave] = nan;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3])) {
+            st.clear();
+#pragma unroll 1
+            for (int step = 0; step < steps; step++) {
+                asm volatile("s_barrier" ::: "memory");
+                ask(step, 0);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (step * KEYS >= wave_most) continue;
+                score(0);
+                const bool some = wave_least < (step + 1) * KEYS;
+                if (some) hide(s, step * KEYS, r.limit, lane);
+                if (some) attend_key_by_key(st, s, p.scale2, lds + 2 * H::TILE, step * KEYS, r.limit, lane);
+                else st.template attend<H::ONES>(s, ~0ull, p.scale2, lds + 2 * H::TILE, lane);
+            }
+        }
+    }
+    finish<BF16, H, HALF>(p, it, r, st, hk, wave, lane);
+}
+
+// ---- turns form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
 // The two waves of a SIMD take turns: while one makes probabilities of its scores (vector instructions), the other multiplies (the probabilities before
 // those with V, the next keys with Q).  A phase is one or the other; waves 4 .. 7 are one phase behind waves 0 .. 3, and a barrier ends a phase for all.
 // In phase 2 j the first four waves make the probabilities of step j, in phase 2 j + 1 they multiply them and score step j + 1.  Keys and values of step i are
@@ -524,7 +665,7 @@ struct RowCopies {
 };
 
 template <bool BF16, int DP, bool ONES>
-__global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
+__global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) {
     using H = Head<DP, true, ONES>;
     using E = Elem<BF16>;
     using vec = typename E::vec;
@@ -666,37 +807,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_rows_kernel(Params p) {
             }
         }
     }
-    if constexpr (H::ONES) {
-#pragma unroll
-        for (int g = 0; g < 4 * H::DB; g++)
-            if (8 * g == p.D && h == 0) st.sum = st.o[g >> 2][4 * (g & 3)];
-    }
-    const float sum = across_sum(st.sum);
-    if (it.parts > 1) {
-        if (!r.in) return;
-        float *dst = share_of<ROWS>(p, it.index, hk, wave * 32 + col);
-#pragma unroll
-        for (int d = 0; d < H::DB; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int c = 32 * d + 8 * g + 4 * h;
-                if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
-            }
-        if (h == 0) {
-            float *ms = stats_of<ROWS>(p, it.index, hk, wave * 32 + col);
-            ms[0] = st.top;
-            ms[1] = sum;
-        }
-        return;
-    }
-    const float inv = inverse(sum);
-#pragma unroll
-    for (int u = 0; u < 2 * H::DB; u++) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = st.o[u >> 1][8 * (u & 1) + e];
-        store_columns<BF16>(r.out, x, inv, 16 * u, r.in ? p.D : 0, lane);
-    }
+    finish<BF16, H, ROWS>(p, it, r, st, hk, wave, lane);
 }
 
 // Adds the parts of every row (at most 64): 32 rows of a block per workgroup, a wave to a row, two columns per lane; lane i holds part i's share of the row.
@@ -738,39 +849,44 @@ __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
     }
 }
 
+enum Form { BY_KEYS, BY_ROWS, BY_TURNS };
+
 template <bool BF16, int DP, bool ONES>
-int launch_kernels(const Params &p, bool keys, hipStream_t st) {
-    const int lds = keys ? 8 * Head<DP, true>::TILE : 2 * STAGES * Head<DP, true>::TILE + 64;
-    static bool reserved[2][64] = {{false}};
-    const void *kernel = keys ? (const void *)self_attention_keys_kernel<BF16, DP> : (const void *)self_attention_rows_kernel<BF16, DP, ONES>;
-    if (int rc = reserve_lds(kernel, lds, reserved[keys], "self_attention")) return rc;
+int launch_kernels(const Params &p, Form form, hipStream_t st) {
+    const int lds = form == BY_KEYS ? 8 * Head<DP, true>::TILE : form == BY_ROWS ? 4 * Head<DP>::TILE + 16 : 2 * STAGES * Head<DP, true>::TILE + 64;
+    static bool reserved[3][64] = {{false}};
+    const void *kernel = form == BY_KEYS   ? (const void *)self_attention_keys_kernel<BF16, DP>
+                         : form == BY_ROWS ? (const void *)self_attention_rows_kernel<BF16, DP, ONES> : (const void *)self_attention_turns_kernel<BF16, DP, ONES>;
+    if (int rc = reserve_lds(kernel, lds, reserved[form], "self_attention")) return rc;
     const dim3 grid((unsigned)((long long)p.items * p.Hkv));
-    if (keys) SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, dim3(256), lds, st, p);
-    else SVDQ_LAUNCH((self_attention_rows_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
+    if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, dim3(256), lds, st, p);
+    else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_rows_kernel<BF16, DP, ONES>), grid, dim3(256), lds, st, p);
+    else SVDQ_LAUNCH((self_attention_turns_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
     int rc = check_launch("self_attention");
     if (rc || !p.target) return rc;
-    if (keys) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * p.Hkv)), dim3(256), 0, st, p);
+    if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * p.Hkv)), dim3(256), 0, st, p);
+    else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, HALF, KEYS>), dim3((unsigned)(p.blocks * 4 * p.Hkv)), dim3(256), 0, st, p);
     else SVDQ_LAUNCH((self_attention_join_kernel<BF16, ROWS, KEYS>), dim3((unsigned)(p.blocks * WAVES * p.Hkv)), dim3(256), 0, st, p);
     return check_launch("self_attention");
 }
 
 template <bool BF16, int DP>
-int launch_head(const Params &p, bool keys, hipStream_t st) {
-    if (p.D < 32 * Head<DP>::DB) return launch_kernels<BF16, DP, true>(p, keys, st);
-    if constexpr (DP % 32 == 0) return launch_kernels<BF16, DP, false>(p, keys, st);
+int launch_head(const Params &p, Form form, hipStream_t st) {
+    if (p.D < 32 * Head<DP>::DB) return launch_kernels<BF16, DP, true>(p, form, st);
+    if constexpr (DP % 32 == 0) return launch_kernels<BF16, DP, false>(p, form, st);
     return SVDQ_EUNSUPPORTED;  // (not reached: the blocks of 80 end at 96)
 }
 template <bool BF16>
-int launch_heads(const Params &p, bool keys, hipStream_t st) {
-    if (p.D <= 32) return launch_head<BF16, 32>(p, keys, st);
-    if (p.D <= 64) return launch_head<BF16, 64>(p, keys, st);
-    if (p.D <= 80) return launch_head<BF16, 80>(p, keys, st);
-    if (p.D <= 96) return launch_head<BF16, 96>(p, keys, st);
-    return launch_head<BF16, 128>(p, keys, st);
+int launch_heads(const Params &p, Form form, hipStream_t st) {
+    if (p.D <= 32) return launch_head<BF16, 32>(p, form, st);
+    if (p.D <= 64) return launch_head<BF16, 64>(p, form, st);
+    if (p.D <= 80) return launch_head<BF16, 80>(p, form, st);
+    if (p.D <= 96) return launch_head<BF16, 96>(p, form, st);
+    return launch_head<BF16, 128>(p, form, st);
 }
 
 struct Plan {
-    bool keys;
+    Form form;
     long long blocks, items, target, least, workspace;
 };
 
@@ -783,13 +899,13 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
     Plan plan;
     const long long rows_each = (a->cu_seqlens_q ? (a->q_len + a->batch - 1) / a->batch : a->q_len) * (a->heads / a->kv_heads);
-    plan.keys = rows_each <= 128;
-    const int size = plan.keys ? 32 : ROWS;
+    plan.form = rows_each <= 128 ? BY_KEYS : blocks_of(a, HALF) * a->kv_heads < 4 * cus ? BY_ROWS : BY_TURNS;
+    const int size = plan.form == BY_KEYS ? 32 : plan.form == BY_ROWS ? HALF : ROWS;
     plan.blocks = plan.items = blocks_of(a, size);
     plan.target = plan.workspace = 0;
-    plan.least = 512 / (plan.keys ? 32 : KEYS);
-    const long long slots = plan.keys && a->head_dim <= 64 ? 2 * cus : cus;
-    if (plan.keys && a->batch + 2 <= MAX_REGIONS && plan.blocks * a->kv_heads < 2 * slots && a->k_len > 512) {
+    plan.least = 512 / (plan.form == BY_KEYS ? 32 : KEYS);
+    const long long slots = plan.form == BY_ROWS || (plan.form == BY_KEYS && a->head_dim <= 64) ? 2 * cus : cus;
+    if (plan.form == BY_KEYS && a->batch + 2 <= MAX_REGIONS && plan.blocks * a->kv_heads < 2 * slots && a->k_len > 512) {
         plan.target = (slots * 3 / 2 + a->kv_heads - 1) / a->kv_heads;
         plan.items = plan.blocks + plan.target + 1;
         plan.workspace = plan.items * a->kv_heads * size * (a->head_dim + 2) * 4;
@@ -878,5 +994,5 @@ extern "C" int svdq_self_attention(const svdq_self_attention_args *a, void *stre
     p.causal = a->causal != 0;
     p.zero_rest = a->zero_rest != 0;
     p.scale2 = a->scale * 1.44269504088896340736f;
-    return a->dtype == SVDQ_BF16 ? launch_heads<true>(p, plan.keys, (hipStream_t)stream) : launch_heads<false>(p, plan.keys, (hipStream_t)stream);
+    return a->dtype == SVDQ_BF16 ? launch_heads<true>(p, plan.form, (hipStream_t)stream) : launch_heads<false>(p, plan.form, (hipStream_t)stream);
 }
