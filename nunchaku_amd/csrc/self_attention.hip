@@ -63,6 +63,28 @@ __device__ inline int blocks_of(const Params &p, int count) {
     return (int)(((long long)count * p.G + ROWS - 1) / ROWS);
 }
 
+// op over this lane and those in front of it, by moves between lanes: 1, 2, 4 and 8 further in each 16, then the last of 16 and of 32 to those behind
+template <typename F>
+__device__ inline int up_to_lane(int x, F op) {  // (zero changes nothing)
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));
+    return op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));
+}
+// a sum, 2^29 at most: offsets that are not in order can make any
+__device__ inline int sum_up_to_lane(int x) {
+    return up_to_lane(x < 1 << 29 ? x : 1 << 29, [](int a, int b) __attribute__((always_inline)) { return a + b < 1 << 29 ? a + b : 1 << 29; });
+}
+__device__ inline int most_of(int x) {
+    return __builtin_amdgcn_readlane(up_to_lane(x, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; }), 63);
+}
+__device__ inline float sum_of(float x) {
+    return bits_f32(__builtin_amdgcn_readlane(
+        up_to_lane((int)f32_bits(x), [](int a, int b) __attribute__((always_inline)) { return (int)f32_bits(bits_f32((uint32_t)a) + bits_f32((uint32_t)b)); }), 63));
+}
+
 // A block of rows of a region and a part of its keys
 struct Item {
     Region r;
@@ -93,12 +115,7 @@ __device__ inline Item item_of(const Params &p, int at, int lane) {
         Region r = Region{0, 0, 0, 0, 0};
         if (lane < n) r = region_of(p, lane);
         const int blocks = blocks_of<ROWS>(p, r.count);
-        int upto = blocks;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d);
-            if (lane >= d) upto = upto + o < 1 << 29 ? upto + o : 1 << 29;  // (offsets that are not in order can make any sum)
-        }
+        const int upto = sum_up_to_lane(blocks);
         const uint64_t behind = __ballot(at < upto);
         const int l = behind ? __builtin_ctzll(behind) : 0;
         it.r = in_lane(r, l);
@@ -151,12 +168,8 @@ __device__ inline Item part_of(const Params &p, int at, int lane) {
         if (blocks[c]) most = steps[c] > most ? steps[c] : most;
         work += (float)blocks[c] * (float)steps[c];
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const int o = __shfl_xor(most, d);
-        most = o > most ? o : most;
-        work += __shfl_xor(work, d);
-    }
+    most = most_of(most);
+    work = sum_of(work);
     int chunk = (int)__builtin_fminf(work / (float)p.target, 1.0e9f) + 1;
     chunk = chunk < p.least ? p.least : chunk;
     chunk = chunk < (most + MAX_PARTS - 1) / MAX_PARTS ? (most + MAX_PARTS - 1) / MAX_PARTS : chunk;
@@ -167,16 +180,7 @@ __device__ inline Item part_of(const Params &p, int at, int lane) {
     for (int c = 0; c < C; c++) {
         if (c * 64 >= n || it.any) continue;
         const int parts = steps[c] > chunk ? (steps[c] + chunk - 1) / chunk : 1;
-        int upto = blocks[c], items = blocks[c] * parts;  // of this region and those in front of it
-        const int mine = items;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d), i = __shfl_up(items, d);
-            if (lane >= d) {  // (offsets that are not in order can make any sum)
-                upto = upto + o < 1 << 29 ? upto + o : 1 << 29;
-                items = items + i < 1 << 29 ? items + i : 1 << 29;
-            }
-        }
+        const int mine = blocks[c] * parts, items = sum_up_to_lane(mine), upto = BLOCK ? sum_up_to_lane(blocks[c]) : 0;  // of this region and those in front of it
         const uint64_t behind = __ballot(left < (BLOCK ? upto : items));
         if (behind) {
             const int l = __builtin_ctzll(behind), b = __builtin_amdgcn_readlane(blocks[c], l), before = __builtin_amdgcn_readlane(items, l) - __builtin_amdgcn_readlane(mine, l);
@@ -810,43 +814,52 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     finish<BF16, H, ROWS>(p, it, r, st, hk, wave, lane);
 }
 
-// Adds the parts of every row (at most 64): 32 rows of a block per workgroup, a wave to a row, two columns per lane; lane i holds part i's share of the row.
+// Adds the parts of every row (at most 64): four rows of a block per workgroup, a wave to a row, two columns per lane, 16 parts asked for at once; lane i holds part i's
+// share of the row.
 template <bool BF16, int BLOCK_ROWS, int SIZE>
 __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
-    constexpr int SUBS = BLOCK_ROWS / 32;
+    constexpr int SUBS = BLOCK_ROWS / 4, MOST = 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, sub = rest % SUBS;
     const Item it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
     if (!it.any || it.parts == 1 || (long long)it.index + (long long)(it.parts - 1) * it.next >= p.items) return;
+    const int at = sub * 4 + wave;
+    const Rows r = rows_of(p, it.r, hk, it.rb * BLOCK_ROWS + at);
+    if (!r.in) return;
     const int c = lane * 2 < p.D ? lane * 2 : 0;
     typedef float float2_t __attribute__((ext_vector_type(2)));
-    for (int i = wave; i < 32; i += 4) {
-        const int at = sub * 32 + i, row = it.rb * BLOCK_ROWS + at;
-        const Rows r = rows_of(p, it.r, hk, row);
-        if (!r.in) break;
-        float top = -__builtin_huge_valf(), sum = 0.f;
-        if (lane < it.parts) {
-            const float2_t t = *(const float2_t *)stats_of<BLOCK_ROWS>(p, it.index + lane * it.next, hk, at);
-            top = t[0];
-            sum = t[1];
-        }
-        float most = top;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
-        const float f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
-        sum *= f;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        float x = 0.f, y = 0.f;
-        for (int j = 0; j < it.parts; j++) {
-            const float2_t part = *(const float2_t *)(share_of<BLOCK_ROWS>(p, it.index + j * it.next, hk, at) + c);
-            const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), j));
-            x = __builtin_fmaf(part[0], g, x);
-            y = __builtin_fmaf(part[1], g, y);
-        }
-        const float inv = inverse(sum);
-        if (lane * 2 < p.D) *(uint32_t *)(r.out + c * 2) = Elem<BF16>::pair(x * inv, y * inv);
+    float top = -__builtin_huge_valf(), sum = 0.f;
+    if (lane < it.parts) {
+        const float2_t t = *(const float2_t *)stats_of<BLOCK_ROWS>(p, it.index + lane * it.next, hk, at);
+        top = t[0];
+        sum = t[1];
     }
+    float x = 0.f, y = 0.f, f = 0.f;
+    for (int first = 0; first < it.parts; first += MOST) {
+        float2_t part[MOST];
+#pragma unroll
+        for (int i = 0; i < MOST; i++) {
+            part[i] = float2_t{0.f, 0.f};
+            if (first + i < it.parts) part[i] = *(const float2_t *)(share_of<BLOCK_ROWS>(p, it.index + (first + i) * it.next, hk, at) + c);
+        }
+        if (first == 0) {
+            float most = top;
+#pragma unroll
+            for (int d = 32; d; d >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+            f = __builtin_amdgcn_exp2f(top - (most == -__builtin_huge_valf() ? 0.f : most));
+            sum *= f;
+#pragma unroll
+            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        }
+#pragma unroll
+        for (int i = 0; i < MOST; i++) {  // (zero times zero behind the last part)
+            const float g = bits_f32(__builtin_amdgcn_readlane(f32_bits(f), first + i));
+            x = __builtin_fmaf(part[i][0], g, x);
+            y = __builtin_fmaf(part[i][1], g, y);
+        }
+    }
+    const float inv = inverse(sum);
+    if (lane * 2 < p.D) *(uint32_t *)(r.out + c * 2) = Elem<BF16>::pair(x * inv, y * inv);
 }
 
 enum Form { BY_KEYS, BY_ROWS, BY_TURNS };
@@ -864,9 +877,9 @@ int launch_kernels(const Params &p, Form form, hipStream_t st) {
     else SVDQ_LAUNCH((self_attention_turns_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
     int rc = check_launch("self_attention");
     if (rc || !p.target) return rc;
-    if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * p.Hkv)), dim3(256), 0, st, p);
-    else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, HALF, KEYS>), dim3((unsigned)(p.blocks * 4 * p.Hkv)), dim3(256), 0, st, p);
-    else SVDQ_LAUNCH((self_attention_join_kernel<BF16, ROWS, KEYS>), dim3((unsigned)(p.blocks * WAVES * p.Hkv)), dim3(256), 0, st, p);
+    if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * 8 * p.Hkv)), dim3(256), 0, st, p);
+    else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, HALF, KEYS>), dim3((unsigned)(p.blocks * (HALF / 4) * p.Hkv)), dim3(256), 0, st, p);
+    else return fail(SVDQ_EUNSUPPORTED, "self_attention: parts of the keys of 256 rows");  // (no plan has them)
     return check_launch("self_attention");
 }
 
