@@ -909,17 +909,64 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
     return a->cu_seqlens_q ? rows / size + a->batch + 2 : (rows + size - 1) / size * a->batch;
 }
 
+// Which form a call takes and into how many parts it divides the keys of an average sequence: the least time by a model of the busiest compute unit, us.  Its constants are
+// those of 252 shapes (heads of 32 to 128, 1 .. 8192 queries, causal or not), each in every form and 1 .. 32 parts; what it chooses is 2 to 4 % behind the fastest on average,
+// 46 % at most (32 rows to 4096 keys, 17.2 us against 11.8).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.3 / keys 7.9, turns 7.0; 1024 tokens, 32 heads over 8 of
+// 128, causal rows 24.8 / keys 50.7, turns 33.1; 16384 tokens, 8 heads of 128 turns 995 / rows 1069; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128 29.9 in
+// eight parts / 143 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.2.
+// Sequences of other lengths than the average have parts in proportion.
+struct Cost {
+    int head_dim;                   // up to
+    float keys_base, round;         // keys form: first and last; a round of four waves' 32 keys
+    float rows_base, rows_step;     // rows form: the same; a step of 64 keys
+    float turns_base, turns_step;   // turns form
+    float join, join_bytes;         // parts: the second launch; bytes a us of their way there and back
+};
+constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.0f, 0.71f, 4.4f, 0.97f, 5.5f, 3.5e6f}, {96, 5.7f, 1.45f, 4.7f, 0.99f, 5.1f, 1.22f, 5.6f, 5.3e6f}, {128, 6.1f, 1.64f, 5.4f, 1.12f, 5.8f, 1.45f, 5.5f, 6.3e6f}};
+
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
-    Plan plan;
-    const long long rows_each = (a->cu_seqlens_q ? (a->q_len + a->batch - 1) / a->batch : a->q_len) * (a->heads / a->kv_heads);
-    plan.form = rows_each <= 128 ? BY_KEYS : blocks_of(a, HALF) * a->kv_heads < 4 * cus ? BY_ROWS : BY_TURNS;
+    const long long S = a->batch, q = a->cu_seqlens_q ? (a->q_len + S - 1) / S : a->q_len, k = a->cu_seqlens_k ? (a->k_len + S - 1) / S : a->k_len;
+    const long long rows = q * (a->heads / a->kv_heads);
+    const Cost &c = a->head_dim <= 64 ? costs[0] : a->head_dim <= 96 ? costs[1] : costs[2];
+    // of the keys that a whole row of scores would have, how many are seen
+    const float seen = !a->causal ? 1.f : q <= k ? 1.f - (float)(q - 1) / (2.f * (float)k) : (float)(k + 1) / (2.f * (float)q);
+    const bool even = seen > 0.95f;
+    static const int shares[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    Plan plan = {BY_TURNS, 0, 0, 0, 0, 0};
+    long long chosen = 1;
+    float best = 0.f;
+    for (int form = BY_KEYS; form <= BY_TURNS; form++) {
+        const int size = form == BY_KEYS ? 32 : form == BY_ROWS ? HALF : ROWS, step = form == BY_KEYS ? 32 : KEYS;
+        const long long groups = (rows + size - 1) / size * S * a->kv_heads, steps = (k + step - 1) / step;
+        for (int parts : shares) {
+            if (parts > 1 && (form == BY_TURNS || S + 2 > MAX_REGIONS || groups * parts > 4 * cus || steps < (form == BY_KEYS ? 4 : 1) * parts)) break;
+            const float w = (float)(groups * parts), each = (float)((steps + parts - 1) / parts), n = (float)cus;
+            float t;
+            if (form == BY_KEYS) {
+                // two workgroups to a compute unit with heads up to 64, one with wider ones (LDS)
+                const float slots = a->head_dim <= 64 ? 2.f * n : n, work = __builtin_ceilf(each / 4.f) * c.round * (w > n && a->head_dim <= 64 ? 1.3f : 1.f);
+                t = c.keys_base + work;
+                if (w > slots) {
+                    const float more = (c.keys_base + work * seen) * (even ? __builtin_ceilf(w / slots) : w / slots + 0.3f);
+                    t = more > t ? more : t;
+                }
+            } else {
+                const float load = even ? __builtin_ceilf(w / n) : w * seen / n, turns = w / n < 1.f ? 1.f : w / n > 3.f ? 3.f : w / n;
+                t = form == BY_ROWS ? c.rows_base + each * c.rows_step * (load > 1.f ? load : 1.f) : c.turns_base * turns + each * c.turns_step * (load > 1.f ? load : 1.f);
+            }
+            if (parts > 1) t += c.join + (float)(S * a->kv_heads * rows) * (float)(a->head_dim * 8 * parts) / c.join_bytes;
+            if (best == 0.f || t < best) {
+                best = t;
+                chosen = parts;
+                plan.form = (Form)form;
+            }
+        }
+    }
     const int size = plan.form == BY_KEYS ? 32 : plan.form == BY_ROWS ? HALF : ROWS;
     plan.blocks = plan.items = blocks_of(a, size);
-    plan.target = plan.workspace = 0;
-    plan.least = 512 / (plan.form == BY_KEYS ? 32 : KEYS);
-    const long long slots = plan.form == BY_ROWS || (plan.form == BY_KEYS && a->head_dim <= 64) ? 2 * cus : cus;
-    if (plan.form == BY_KEYS && a->batch + 2 <= MAX_REGIONS && plan.blocks * a->kv_heads < 2 * slots && a->k_len > 512) {
-        plan.target = (slots * 3 / 2 + a->kv_heads - 1) / a->kv_heads;
+    if (chosen > 1) {
+        plan.least = plan.form == BY_KEYS ? 4 : 1;
+        plan.target = (rows + size - 1) / size * S * chosen;
         plan.items = plan.blocks + plan.target + 1;
         plan.workspace = plan.items * a->kv_heads * size * (a->head_dim + 2) * 4;
     }
