@@ -270,16 +270,14 @@ __device__ inline float *stats_of(const Params &p, int index, int hk, int row) {
 
 // A step in which some rows do not see some keys, where what such a key has in V is an infinity or a NaN: zero times it is a NaN, too.  A key at a time; rows that
 // do not see it keep what they have.
-template <bool BF16, typename H, int NB>
-__device__ inline void attend_key_by_key(State<BF16, H> &st, float16_t (&s)[NB], float scale2, const char *v, int first, int limit, int lane) {
+template <bool BF16, typename H, int NB, typename S, typename F>
+__device__ inline void attend_key_by_key(S &st, const float16_t (&s)[NB], const char *v, int first, int limit, int lane, F &&probabilities) {
     using vec = typename Elem<BF16>::vec;
-    st.raise(st.highest(s), scale2);
-    const float ref = st.reference();
 #pragma unroll
     for (int n = 0; n < 2 * NB; n++) {
         vec vf[H::DB];
         st.read_v(vf, v, n, lane);
-        const u32x4_t pr = __builtin_bit_cast(u32x4_t, st.template exponentials<NB, H::ONES>(s, n, scale2, ref));
+        const u32x4_t pr = __builtin_bit_cast(u32x4_t, probabilities(n));
 #pragma unroll 1
         for (int j = 0; j < 16; j++) {  // (element 4 (j / 8) + j % 4 of the half-wave j / 4 % 2)
             const int at = 4 * (j >> 3) + (j & 3);
@@ -391,7 +389,11 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
             }
             const bool some = least < (step + 1) * SIZE;
             if (some) hide(s, step * SIZE, r.limit, lane);
-            if (some && careful) attend_key_by_key(st, s, p.scale2, v, step * SIZE, r.limit, lane);
+            if (some && careful) {
+                st.raise(st.highest(s), p.scale2);
+                const float ref = st.reference();
+                attend_key_by_key<BF16, H>(st, s, v, step * SIZE, r.limit, lane, [&](int n) __attribute__((always_inline)) { return st.template exponentials<1, false>(s, n, p.scale2, ref); });
+            }
             else st.template attend<false>(s, 0xFFFFFFFFull, p.scale2, v, lane);
             step = next;
         }
@@ -453,16 +455,127 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     }
 }
 
+// ---- the running softmax of 32 rows, as the forms below have it that are bound by their vector instructions ----------------------------
+// The sums of the (rounded) probabilities come from the matrix cores, too: v_mfma_f32_16x16x32 takes the same registers for sixteen rows' 32 keys, of which lanes 16 .. 31 and 48 .. 63
+// hold those of sixteen other rows; a left operand whose row 0 has ones for the first and third eight keys, and row 1 for the others, adds both apart.  16 cycles
+// of the matrix cores for 8 additions of 4 cycles, and both sides of the division have the same roundings.  (A NaN of one of two such rows is a NaN in both their sums, since
+// nothing times it is one: then the wave's rows are worked out once more, with sums of their own.)
+template <bool BF16>
+__device__ inline float4_t add_up(typename Elem<BF16>::vec ones, typename Elem<BF16>::vec p, float4_t c) {
+    if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p, c, 0, 0, 0);
+}
+template <bool BF16, typename H>
+struct Softmax : State<BF16, H> {
+    using E = Elem<BF16>;
+    using vec = typename E::vec;
+    using Base = State<BF16, H>;
+    float4_t sums;  // lanes 0 .. 15: of rows 0 .. 15 and 16 .. 31
+    vec ones;
+    __device__ inline void start(int lane) {
+        const uint32_t w = (lane & 15) == ((lane >> 4) & 1) ? E::ONE * 0x10001u : 0u;
+        ones = __builtin_bit_cast(vec, u32x4_t{w, w, w, w});
+    }
+    __device__ inline void clear() {
+        Base::clear();
+        sums = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    // (a maximum that a NaN stays in takes no instructions of its own to make quiet ones of others)
+    static __device__ inline float highest(const float16_t (&s)[2]) {
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            m[i] = s[i >> 1][8 * (i & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; e++) m[i] = __builtin_elementwise_maximum(m[i], s[i >> 1][8 * (i & 1) + e]);
+        }
+        return across_max(__builtin_elementwise_maximum(__builtin_elementwise_maximum(m[0], m[1]), __builtin_elementwise_maximum(m[2], m[3])));
+    }
+    __device__ inline void raise(float high, float scale2, int lane) {
+        if (__any(__builtin_fmaf(high, scale2, -this->top) > E::RAISED + 8.f)) {
+            const float m = high * scale2 - E::RAISED, now = m > this->top ? m : this->top;
+            const float f = this->top == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(this->top - now);
+            this->top = now;
+#pragma unroll
+            for (int d = 0; d < H::DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) this->o[d][e] *= f;
+            if (!H::ONES) {
+                sums[0] *= f;
+                sums[1] *= __shfl(f, (lane & 15) + 16);
+            }
+        }
+    }
+    // the right operand: probabilities of 16 keys, rounded
+    __device__ inline vec exponentials(const float16_t (&s)[2], int n, float scale2, float ref) { return Base::template exponentials<2, true>(s, n, scale2, ref); }
+    __device__ inline void add(vec p) {
+        if (!H::ONES) sums = add_up<BF16>(ones, p, sums);
+    }
+    // A step's scores and values (v in LDS) join the sums, 16 keys at a time: while the matrix cores multiply the probabilities of one 16, those of the next are made and
+    // the operands of the one behind it are on their way.
+    __device__ inline void attend(const float16_t (&s)[2], float scale2, const char *v, int lane) {
+        vec vf[2][H::DB], pr[2];
+        Base::read_v(vf[0], v, 0, lane);
+        raise(highest(s), scale2, lane);
+        const float ref = this->reference();
+        pr[0] = exponentials(s, 0, scale2, ref);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            if (n < 3) {
+                Base::read_v(vf[(n + 1) & 1], v, n + 1, lane);
+                pr[(n + 1) & 1] = exponentials(s, n + 1, scale2, ref);
+            }
+#pragma unroll
+            for (int d = 0; d < H::DB; d++) this->o[d] = E::mfma(vf[n & 1][d], pr[n & 1], this->o[d]);
+            add(pr[n & 1]);
+            if (n < 3) {
+#pragma unroll
+                for (int d = 0; d < H::DB; d++) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 16 / H::DB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x400, 8 / H::DB, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // the same with sums by additions, and, where some rows do not see all keys, key by key
+    __device__ inline void attend_carefully(float16_t (&s)[2], float scale2, const char *v, int first, int limit, bool some, int lane) {
+        if (!some) {
+            Base::template attend<H::ONES>(s, ~0ull, scale2, v, lane);
+            return;
+        }
+        Base::raise(Base::highest(s), scale2);
+        const float ref = this->reference();
+        attend_key_by_key<BF16, H>(*this, s, v, first, limit, lane, [&](int n) __attribute__((always_inline)) { return Base::template exponentials<2, H::ONES>(s, n, scale2, ref); });
+    }
+    // whether what there is may hold a NaN that belongs to another row, or to a key that a row does not see
+    __device__ inline bool doubtful(bool causal, int D, int lane) const {
+        float x = H::ONES || lane >= 16 ? 0.f : sums[0] * 0.f + sums[1] * 0.f;
+        return __any(x != x) || (causal && any_nan(*(const Base *)this, D));
+    }
+    // of this lane's row
+    __device__ inline float whole_sum(int D, bool careful, int lane) const {
+        if constexpr (H::ONES) {
+            float x = 0.f;
+#pragma unroll
+            for (int g = 0; g < 4 * H::DB; g++)
+                if (8 * g == D && lane < 32) x = this->o[g >> 2][4 * (g & 3)];
+            return across_sum(x);
+        }
+        if (careful) return across_sum(this->sum);
+        const float low = __shfl(sums[0], lane & 15), high = __shfl(sums[1], lane & 15);
+        return lane & 16 ? high : low;
+    }
+};
+
 // The end of a wave's 32 rows: the quotients, or an item's share of them
 template <bool BF16, typename H, int BLOCK_ROWS>
-__device__ inline void finish(const Params &p, const Item &it, const Rows &r, State<BF16, H> &st, int hk, int wave, int lane) {
+__device__ inline void finish(const Params &p, const Item &it, const Rows &r, const Softmax<BF16, H> &st, bool careful, int hk, int wave, int lane) {
     const int col = lane & 31, h = lane >> 5;
-    if constexpr (H::ONES) {
-#pragma unroll
-        for (int g = 0; g < 4 * H::DB; g++)
-            if (8 * g == p.D && h == 0) st.sum = st.o[g >> 2][4 * (g & 3)];
-    }
-    const float sum = across_sum(st.sum);
+    const float sum = st.whole_sum(p.D, careful, lane);
     if (it.parts > 1) {
         if (!r.in) return;
         float *dst = share_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
@@ -495,7 +608,7 @@ __device__ inline void finish(const Params &p, const Item &it, const Rows &r, St
 constexpr int HALF = 128;
 
 template <bool BF16, int DP, bool ONES>
-__global__ void __launch_bounds__(256, 2) self_attention_rows_kernel(Params p) {
+__global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_attention_rows_kernel(Params p) {
     using H = Head<DP, false, ONES>;
     using E = Elem<BF16>;
     using vec = typename E::vec;
@@ -520,7 +633,8 @@ __global__ void __launch_bounds__(256, 2) self_attention_rows_kernel(Params p) {
     r.limit -= skip;
     const int steps = end > begin ? end - begin : 0;  // (a part may lie behind all keys that are seen)
     Copies<H, 4> copies(lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], p.ks[1], p.vs[1], p.D, most, wave, lane, E::ONE);
-    State<BF16, H> st;
+    Softmax<BF16, H> st;
+    st.start(lane);
     auto ask = [&](int step, int slot) __attribute__((always_inline)) {
         const int left = most - step * KEYS;
         copies.k(step, slot);
@@ -567,15 +681,17 @@ __global__ void __launch_bounds__(256, 2) self_attention_rows_kernel(Params p) {
         if (step * KEYS >= wave_most) continue;
         score(slot);
         if (wave_least < (step + 1) * KEYS) hide(s, step * KEYS, r.limit, lane);
-        st.template attend<H::ONES>(s, ~0ull, p.scale2, lds + (2 + slot) * H::TILE, lane);
+        st.attend(s, p.scale2, lds + (2 + slot) * H::TILE, lane);
     }
-    // Once more, key by key where rows do not see all keys, if sums turn out to hold a NaN: rows that see none of its causes have none then
-    if (p.causal && steps > 0) {
+    // Once more, and key by key where rows do not see all keys, if there turns out to be a NaN: rows that see none of its causes have none then
+    bool careful = false;
+    if (steps > 0) {
         int *flags = (int *)(lds + 4 * H::TILE);
-        const bool nan = any_nan(st, p.D);
+        const bool nan = st.doubtful(p.causal, p.D, lane);
         if (lane == 0) flags[wave] = nan;
         __syncthreads();
-        if (__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3])) {
+        careful = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+        if (careful) {
             st.clear();
 #pragma unroll 1
             for (int step = 0; step < steps; step++) {
@@ -586,12 +702,11 @@ __global__ void __launch_bounds__(256, 2) self_attention_rows_kernel(Params p) {
                 score(0);
                 const bool some = wave_least < (step + 1) * KEYS;
                 if (some) hide(s, step * KEYS, r.limit, lane);
-                if (some) attend_key_by_key(st, s, p.scale2, lds + 2 * H::TILE, step * KEYS, r.limit, lane);
-                else st.template attend<H::ONES>(s, ~0ull, p.scale2, lds + 2 * H::TILE, lane);
+                st.attend_carefully(s, p.scale2, lds + 2 * H::TILE, step * KEYS, r.limit, some, lane);
             }
         }
     }
-    finish<BF16, H, HALF>(p, it, r, st, hk, wave, lane);
+    finish<BF16, H, HALF>(p, it, r, st, careful, hk, wave, lane);
 }
 
 // ---- turns form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
@@ -702,60 +817,76 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
         for (int i = threadIdx.x; i < STAGES * KEYS; i += 64 * WAVES)
             *(u32x4_t *)(lds + STAGES * H::TILE + i * H::PITCH + ((p.D / 8) ^ H::fv(i)) * 16) = u32x4_t{E::ONE, 0, 0, 0};
     }
-    State<BF16, H> st;
+    Softmax<BF16, H> st;
+    st.start(lane);
     st.clear();
     float16_t s[2];
-    vec pr[4], vf[2][H::DB], kf[2][4];
-    constexpr int N = 2 * H::KS, GROUP = N % 4 == 0 ? 4 : 2;
-    const char *k0 = lds + col * H::PITCH, *v0 = lds + STAGES * H::TILE;
-    auto read_k = [&](int slot, int g) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < GROUP; i++) {
-            const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
-            kf[g & 1][i] = __builtin_bit_cast(vec, *(const u32x4_t *)(k0 + slot * H::TILE + kb * 32 * H::PITCH + ((2 * ks + h) ^ H::fk(col)) * 16));
+    // Operands of the matrix instructions of a phase: 0 .. VALUES - 1 sixteen keys' values of 32 columns, for their probabilities, then 32 keys of the next step.  Eight are there
+    // or on their way; where one has been multiplied, that of the eighth instruction behind takes its place.
+    constexpr int VALUES = 4 * H::DB, ALL = VALUES + 2 * H::KS, AHEAD = 8;
+    vec pr[4], ops[AHEAD];
+    // Where this lane's operands stand in LDS: with what differs between the instructions of a phase by an exclusive or, worked out anew each time (registers are short)
+    typedef __attribute__((address_space(3))) char *lds_t;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t)lds;
+    const uint32_t k_lane = lds0 + col * H::PITCH + (h ^ H::fk(col)) * 16;
+    const uint32_t v_lane = lds0 + STAGES * H::TILE + (4 * h + ((lane & 15) >> 2)) * H::PITCH + (lane & 1) * 8 + ((((lane >> 4) & 1) * 2 + ((lane >> 1) & 1)) ^ H::fv((lane & 15) >> 2)) * 16;
+    uint32_t k_at, v_at;  // of the next step's keys, of a step's values
+    auto read = [&](int i) __attribute__((always_inline)) {
+        if (i < VALUES) {
+            typedef short short4_t __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) short4_t *tr_t;
+            const lds_t at = (lds_t)(uintptr_t)((v_at ^ (i % H::DB * 64)) + i / H::DB * 16 * H::PITCH);
+            const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(at + 8 * H::PITCH));
+            ops[i % AHEAD] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int n = i - VALUES, kb = n & 1, ks = n >> 1;
+            ops[i % AHEAD] = __builtin_bit_cast(vec, *(__attribute__((address_space(3))) u32x4_t *)(uintptr_t)((k_at ^ (ks * 32)) + kb * 32 * H::PITCH));
         }
     };
-    // the scores of a step; its first operands are there or on their way
-    auto score = [&](int slot) __attribute__((always_inline)) {
+    auto stand = [&](int slot) __attribute__((always_inline)) {
+        v_at = v_lane + slot * H::TILE;
+        k_at = k_lane + (slot + 1) % STAGES * H::TILE;
+        asm volatile("" : "+v"(v_at), "+v"(k_at));
+    };
+    auto multiply = [&](auto from, auto to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+        for (int i = from; i < to; i++) {
+            if (i == VALUES) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+                for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int g = 0; g < N / GROUP; g++) {
-            if (g + 1 < N / GROUP) read_k(slot, g + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < GROUP; i++) {
-                const int n = g * GROUP + i, kb = n & 1, ks = n >> 1;
-                s[kb] = E::mfma(kf[g & 1][i], qf[ks], s[kb]);
+                    for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
             }
+            if (i < VALUES) {
+                st.o[i % H::DB] = E::mfma(ops[i % AHEAD], pr[i / H::DB], st.o[i % H::DB]);
+                if (i % H::DB == H::DB - 1) st.add(pr[i / H::DB]);
+            } else {
+                const int n = i - VALUES, kb = n & 1, ks = n >> 1;
+                s[kb] = E::mfma(ops[i % AHEAD], qf[ks], s[kb]);
+            }
+            if (i + AHEAD < ALL) read(i + AHEAD);  // (behind a row's last step, of keys that are not multiplied)
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // the probabilities of a step times its values, the first of these there or on their way
-    auto weigh = [&](int slot) __attribute__((always_inline)) {
+    constexpr std::integral_constant<int, 0> FIRST;
+    constexpr std::integral_constant<int, VALUES> SCORES;
+    constexpr std::integral_constant<int, ALL> END;
+    // the scores of the step in `slot`, from nothing
+    auto score = [&](int slot) __attribute__((always_inline)) {
+        stand((slot + STAGES - 1) % STAGES);
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-            if (n < 3) st.read_v(vf[(n + 1) & 1], v0 + slot * H::TILE, n + 1, lane);
-            else read_k((slot + 1) % STAGES, 0);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int d = 0; d < H::DB; d++) st.o[d] = E::mfma(vf[n & 1][d], pr[n], st.o[d]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int i = 0; i < AHEAD && VALUES + i < ALL; i++) read(VALUES + i);
+        multiply(SCORES, END);
     };
     const bool late = wave >= WAVES / 2;
+    bool careful = false;
     if (steps > 0) {
         wait_for_q<BF16, H>(qf);
         if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RowCopies<H>::REQ * (STAGES - 2)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         phase_ends();
         if (late) phase_ends();
-        if (wave_most > 0) {
-            read_k(0, 0);
-            score(0);
-        }
+        if (wave_most > 0) score(0);
         if (late) copies.wait_for_next(0);
         phase_ends();
         for (int j = 0; j < steps; j++) {
@@ -764,18 +895,22 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
             if (late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
             if (here) {
                 if (wave_least < (j + 1) * KEYS) hide(s, j * KEYS, r.limit, lane);
-                st.raise(st.highest(s), p.scale2);
+                st.raise(st.highest(s), p.scale2, lane);
                 const float ref = st.reference();
 #pragma unroll
-                for (int n = 0; n < 4; n++) pr[n] = st.template exponentials<2, H::ONES>(s, n, p.scale2, ref);
-                st.read_v(vf[0], v0 + slot * H::TILE, 0, lane);
+                for (int n = 0; n < 4; n++) pr[n] = st.exponentials(s, n, p.scale2, ref);
+                stand(slot);
+#pragma unroll
+                for (int i = 0; i < AHEAD && i < VALUES; i++) read(i);
             }
             if (!late) copies.wait_for_next(j);
             phase_ends();
             if (!late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
             if (here) {
-                weigh(slot);
-                if ((j + 1) * KEYS < wave_most) score((j + 1) % STAGES);
+#pragma unroll
+                for (int i = VALUES; i < AHEAD && i < ALL; i++) read(i);  // (heads up to 32: keys that had not landed before)
+                multiply(FIRST, SCORES);
+                if ((j + 1) * KEYS < wave_most) multiply(SCORES, END);
             }
             if (late) {
                 if (j + 1 == steps) break;
@@ -783,35 +918,32 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
             }
             phase_ends();
         }
-        // Once more, key by key where rows do not see all keys, if sums turn out to hold a NaN: rows that see none of its causes have none then
-        if (p.causal) {
-            int *flags = (int *)(lds + 2 * STAGES * H::TILE);
-            const bool nan = any_nan(st, p.D);
-            if (lane == 0) flags[wave] = nan;
-            __syncthreads();
-            bool any = false;
+        // Once more, and key by key where rows do not see all keys, if there turns out to be a NaN: rows that see none of its causes have none then
+        int *flags = (int *)(lds + 2 * STAGES * H::TILE);
+        const bool nan = st.doubtful(p.causal, p.D, lane);
+        if (lane == 0) flags[wave] = nan;
+        __syncthreads();
+        int any = 0;
 #pragma unroll
-            for (int i = 0; i < WAVES; i++) any |= flags[i] != 0;
-            if (__builtin_amdgcn_readfirstlane(any)) {
-                st.clear();
+        for (int i = 0; i < WAVES; i++) any |= flags[i];
+        careful = __builtin_amdgcn_readfirstlane(any) != 0;
+        if (careful) {
+            st.clear();
 #pragma unroll 1
-                for (int j = 0; j < steps; j++) {
-                    phase_ends();
-                    copies.ask(j, 0);
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                    phase_ends();
-                    if (j * KEYS >= wave_most) continue;
-                    read_k(0, 0);
-                    score(0);
-                    const bool some = wave_least < (j + 1) * KEYS;
-                    if (some) hide(s, j * KEYS, r.limit, lane);
-                    if (some) attend_key_by_key(st, s, p.scale2, v0, j * KEYS, r.limit, lane);
-                    else st.template attend<H::ONES>(s, ~0ull, p.scale2, v0, lane);
-                }
+            for (int j = 0; j < steps; j++) {
+                phase_ends();
+                copies.ask(j, 0);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                phase_ends();
+                if (j * KEYS >= wave_most) continue;
+                score(0);
+                const bool some = wave_least < (j + 1) * KEYS;
+                if (some) hide(s, j * KEYS, r.limit, lane);
+                st.attend_carefully(s, p.scale2, lds + STAGES * H::TILE, j * KEYS, r.limit, some, lane);
             }
         }
     }
-    finish<BF16, H, ROWS>(p, it, r, st, hk, wave, lane);
+    finish<BF16, H, ROWS>(p, it, r, st, careful, hk, wave, lane);
 }
 
 // Adds the parts of every row (at most 64): four rows of a block per workgroup, a wave to a row, two columns per lane, 16 parts asked for at once; lane i holds part i's

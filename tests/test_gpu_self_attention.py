@@ -235,3 +235,31 @@ def test_far_scores(dev, dtype, scale):
     got = self_attention(k.to(dev)[None], k.to(dev)[None], v.to(dev)[None], causal=True, scale=scale)
     u = torch.finfo(dtype).eps / 2
     assert ((got[0].cpu().double() - v.double()).abs() <= 1.01 * (2 * u + 4 * U32) * v.double().abs() + 2.0**-24).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [(40, 2, 2, 64), (300, 4, 1, 128), (700, 8, 8, 64), (90, 3, 1, 72), (1030, 2, 1, 96), (2100, 16, 16, 128), (2100, 16, 16, 32)])
+def test_a_nan_of_one_query_stays_with_it(dev, shape, causal):
+    """Infinities and NaN in some queries and one head: all other rows are right."""
+    from nunchaku_amd.ops import self_attention
+
+    T, H, Hkv, D = shape
+    announce(f"self_attention query nan {shape} {causal}")
+    q, k, v = rand(T, H, D, dtype=torch.bfloat16, seed=1), rand(T, Hkv, D, dtype=torch.bfloat16, seed=2), rand(T, Hkv, D, dtype=torch.bfloat16, seed=3)
+    bad = q.clone()
+    rows = sorted({0, 7, T // 2, T - 1})
+    for i, t in enumerate(rows):
+        bad[t, i % H, 3] = (math.nan, math.inf)[i % 2]
+    got = self_attention(bad[None].to(dev), k[None].to(dev), v[None].to(dev), causal=causal)[0].cpu()
+    for i, t in enumerate(rows):
+        if t or not causal:  # (a query that sees itself alone has no other score to compare with: NaN or its value)
+            assert got[t, i % H].isnan().all()
+        got[t, i % H] = 0
+        q[t, i % H] = 0
+    heads = sorted({0, H - 1} | {i % H for i in range(len(rows))})
+    want, b = (f(q[:, heads], k, v, causal) if Hkv == 1 else f(q[:, heads], k[:, [h * Hkv // H for h in heads]], v[:, [h * Hkv // H for h in heads]], causal)
+               for f in (blocks.self_attention, lambda q, k, v, c: bound(blocks.self_attention(q, k, v, c), q, k, v, c)))
+    off = (got[:, heads].double() - want).abs() - b
+    for i, t in enumerate(rows):
+        off[t, heads.index(i % H)] = -1
+    assert (off <= 0).all(), (off.max().item(), (~(off <= 0)).sum().item())
