@@ -679,7 +679,9 @@ __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_att
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (step + 1 < steps) ask(step + 1, slot ^ 1);
         if (step * KEYS >= wave_most) continue;
+        if (DP > 64) __builtin_amdgcn_s_setprio(1);  // (8 heads of 128, 16384 tokens 1001 -> 984 us; heads of 64 301 -> 303)
         score(slot);
+        if (DP > 64) __builtin_amdgcn_s_setprio(0);
         if (wave_least < (step + 1) * KEYS) hide(s, step * KEYS, r.limit, lane);
         st.attend(s, p.scale2, lds + (2 + slot) * H::TILE, lane);
     }
@@ -713,7 +715,8 @@ __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_att
 // The two waves of a SIMD take turns: while one makes probabilities of its scores (vector instructions), the other multiplies (the probabilities before
 // those with V, the next keys with Q).  A phase is one or the other; waves 4 .. 7 are one phase behind waves 0 .. 3, and a barrier ends a phase for all.
 // In phase 2 j the first four waves make the probabilities of step j, in phase 2 j + 1 they multiply them and score step j + 1.  Keys and values of step i are
-// read in phases 2 i - 1 .. 2 i + 2; those of step i + 4 take their place, asked for in phase 2 i + 3, by all waves, and waited for at the end of phase 2 i + 6.
+// read in phases 2 i - 1 .. 2 i + 2; those of step i + 4 take their place.  Every wave asks for its share of them where it makes probabilities, in phases 2 i + 3 and 2 i + 4, and
+// waits for it at the end of phase 2 i + 6 (asking between the matrix instructions: 8 heads of 128, 16384 tokens 953 -> 922 us).
 constexpr int STAGES = 4, WAVES = 8, ROWS = 32 * WAVES;
 
 __device__ inline void phase_ends() {
@@ -809,8 +812,9 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     r.limit -= skip;
     const RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], most, wave, lane);
     const int steps = copies.steps;
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) copies.ask(i, i);
+    const bool late = wave >= WAVES / 2;
+    const int ahead = late ? STAGES - 1 : STAGES - 2;  // steps
+    for (int i = 0; i < ahead; i++) copies.ask(i, i);
     // columns behind the head's end, as far as they are multiplied, are zero in K for good: no copy writes there
     zero_columns<H, STAGES * KEYS>(lds, p.D / 8, threadIdx.x, 64 * WAVES);
     if constexpr (H::ONES) {
@@ -824,6 +828,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     // Operands of the matrix instructions of a phase: 0 .. VALUES - 1 sixteen keys' values of 32 columns, for their probabilities, then 32 keys of the next step.  Eight are there
     // or on their way; where one has been multiplied, that of the eighth instruction behind takes its place.
     constexpr int VALUES = 4 * H::DB, ALL = VALUES + 2 * H::KS, AHEAD = 8;
+    static_assert(VALUES >= AHEAD, "");  // (keys have not landed where the first operands are asked for)
     vec pr[4], ops[AHEAD];
     // Where this lane's operands stand in LDS: with what differs between the instructions of a phase by an exclusive or, worked out anew each time (registers are short)
     typedef __attribute__((address_space(3))) char *lds_t;
@@ -878,11 +883,10 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
         for (int i = 0; i < AHEAD && VALUES + i < ALL; i++) read(VALUES + i);
         multiply(SCORES, END);
     };
-    const bool late = wave >= WAVES / 2;
     bool careful = false;
     if (steps > 0) {
         wait_for_q<BF16, H>(qf);
-        if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RowCopies<H>::REQ * (STAGES - 2)) : "memory");
+        if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RowCopies<H>::REQ * (STAGES - 3)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         phase_ends();
         if (late) phase_ends();
@@ -892,7 +896,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
         for (int j = 0; j < steps; j++) {
             const int slot = j % STAGES;
             const bool here = j * KEYS < wave_most;
-            if (late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
+            copies.ask(j + ahead, (j + ahead) % STAGES);
             if (here) {
                 if (wave_least < (j + 1) * KEYS) hide(s, j * KEYS, r.limit, lane);
                 st.raise(st.highest(s), p.scale2, lane);
@@ -905,10 +909,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
             }
             if (!late) copies.wait_for_next(j);
             phase_ends();
-            if (!late) copies.ask(j + STAGES - 1, (j + STAGES - 1) % STAGES);
             if (here) {
-#pragma unroll
-                for (int i = VALUES; i < AHEAD && i < ALL; i++) read(i);  // (heads up to 32: keys that had not landed before)
                 multiply(FIRST, SCORES);
                 if ((j + 1) * KEYS < wave_most) multiply(SCORES, END);
             }
@@ -1000,13 +1001,17 @@ template <bool BF16, int DP, bool ONES>
 int launch_kernels(const Params &p, Form form, hipStream_t st) {
     const int lds = form == BY_KEYS ? 8 * Head<DP, true>::TILE : form == BY_ROWS ? 4 * Head<DP>::TILE + 16 : 2 * STAGES * Head<DP, true>::TILE + 64;
     static bool reserved[3][64] = {{false}};
-    const void *kernel = form == BY_KEYS   ? (const void *)self_attention_keys_kernel<BF16, DP>
-                         : form == BY_ROWS ? (const void *)self_attention_rows_kernel<BF16, DP, ONES> : (const void *)self_attention_turns_kernel<BF16, DP, ONES>;
+    const void *kernel = form == BY_KEYS ? (const void *)self_attention_keys_kernel<BF16, DP> : (const void *)self_attention_rows_kernel<BF16, DP, ONES>;
+    if constexpr (DP > 64) {
+        if (form == BY_TURNS) kernel = (const void *)self_attention_turns_kernel<BF16, DP, ONES>;
+    }
     if (int rc = reserve_lds(kernel, lds, reserved[form], "self_attention")) return rc;
     const dim3 grid((unsigned)((long long)p.items * p.Hkv));
     if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_keys_kernel<BF16, DP>), grid, dim3(256), lds, st, p);
     else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_rows_kernel<BF16, DP, ONES>), grid, dim3(256), lds, st, p);
-    else SVDQ_LAUNCH((self_attention_turns_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
+    if constexpr (DP > 64) {
+        if (form == BY_TURNS) SVDQ_LAUNCH((self_attention_turns_kernel<BF16, DP, ONES>), grid, dim3(64 * WAVES), lds, st, p);
+    }
     int rc = check_launch("self_attention");
     if (rc || !p.target) return rc;
     if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * 8 * p.Hkv)), dim3(256), 0, st, p);
@@ -1051,10 +1056,10 @@ struct Cost {
     int head_dim;                   // up to
     float keys_base, round;         // keys form: first and last; a round of four waves' 32 keys
     float rows_base, rows_step;     // rows form: the same; a step of 64 keys
-    float turns_base, turns_step;   // turns form
+    float turns_base, turns_step;   // turns form, which heads up to 64 never take: 8192 tokens, 16 heads of 64 307 us by turns, 300 by rows, causal 632 and 573; of 32 255 and 212
     float join, join_bytes;         // parts: the second launch; bytes a us of their way there and back
 };
-constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.0f, 0.71f, 4.4f, 0.97f, 5.5f, 3.5e6f}, {96, 5.7f, 1.45f, 4.7f, 0.99f, 5.1f, 1.22f, 5.6f, 5.3e6f}, {128, 6.1f, 1.64f, 5.4f, 1.12f, 5.8f, 1.45f, 5.5f, 6.3e6f}};
+constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.3f, 0.69f, 0.f, 0.f, 5.4f, 3.5e6f}, {96, 5.7f, 1.45f, 4.8f, 0.95f, 5.5f, 1.17f, 5.6f, 5.2e6f}, {128, 6.1f, 1.65f, 5.6f, 1.06f, 7.0f, 1.31f, 5.5f, 6.2e6f}};
 
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
     const long long S = a->batch, q = a->cu_seqlens_q ? (a->q_len + S - 1) / S : a->q_len, k = a->cu_seqlens_k ? (a->k_len + S - 1) / S : a->k_len;
@@ -1067,7 +1072,7 @@ Plan plan_of(const svdq_self_attention_args *a, int cus) {
     Plan plan = {BY_TURNS, 0, 0, 0, 0, 0};
     long long chosen = 1;
     float best = 0.f;
-    for (int form = BY_KEYS; form <= BY_TURNS; form++) {
+    for (int form = BY_KEYS; form <= (a->head_dim > 64 ? BY_TURNS : BY_ROWS); form++) {
         const int size = form == BY_KEYS ? 32 : form == BY_ROWS ? HALF : ROWS, step = form == BY_KEYS ? 32 : KEYS;
         const long long groups = (rows + size - 1) / size * S * a->kv_heads, steps = (k + step - 1) / step;
         for (int parts : shares) {
