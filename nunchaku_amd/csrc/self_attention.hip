@@ -147,11 +147,10 @@ __device__ inline Item item_of(const Params &p, int at, int lane) {
 }
 
 // Item `at` where keys are divided into parts, or (BLOCK) the first of block `at`.  All regions' work together, in steps of SIZE keys, is divided by the number of items that
-// is aimed at: longer keys than that are divided, evenly.  At most 4 x 64 regions, four to a lane.
+// is aimed at: longer keys than that are divided, evenly.  C regions to a lane.
 constexpr int MAX_PARTS = 64, MAX_REGIONS = 256;
-template <int ROWS, int SIZE, bool BLOCK>
-__device__ inline Item part_of(const Params &p, int at, int lane) {
-    constexpr int C = MAX_REGIONS / 64;
+template <int ROWS, int SIZE, bool BLOCK, int C>
+__device__ inline Item part_among(const Params &p, int at, int lane) {
     Region r[C];
     int blocks[C], steps[C], most = 0;
     float work = 0.f;
@@ -198,6 +197,11 @@ __device__ inline Item part_of(const Params &p, int at, int lane) {
         }
     }
     return it;
+}
+
+template <int ROWS, int SIZE, bool BLOCK>
+__device__ inline Item part_of(const Params &p, int at, int lane) {
+    return regions(p) <= 64 ? part_among<ROWS, SIZE, BLOCK, 1>(p, at, lane) : part_among<ROWS, SIZE, BLOCK, MAX_REGIONS / 64>(p, at, lane);
 }
 
 // This lane's row, and the keys that rows see
