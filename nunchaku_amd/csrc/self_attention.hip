@@ -19,6 +19,7 @@ struct Params {
     long long qs[3], ks[3], vs[3], os[3];  // bytes: batch, token, head
     int S, Hkv, G, D, Tq, Tk, causal, zero_rest;
     int items, blocks;                     // per key head, at most
+    int mirror;                            // rows form: the second so many items in the opposite order, see plan_of
     int target, least;                     // keys in parts (target > 0): about how many items in all, steps of one at least
     float scale2;                          // scale * log2(e)
 };
@@ -251,16 +252,25 @@ __device__ inline void wait_for_q(typename Elem<BF16>::vec (&qf)[H::KS]) {
     for (int ks = 0; ks < H::KS; ks++) asm volatile("" : "+v"(qf[ks]));
 }
 
-// The steps of a part, of those that all of the sequence's keys make; no more than the first `most` keys
+// The first step of a part, of those that all of the sequence's keys make
 template <int SIZE>
-__device__ inline void share(const Item &it, int most, int &begin, int &end) {
+__device__ inline int first_step(const Item &it, int part) {
+    const int all = (it.r.keys + SIZE - 1) / SIZE, each = all / it.parts, more = all - each * it.parts;
+    return part * each + (part < more ? part : more);
+}
+// The steps of an item, no more than those of the first `most` keys, which its block sees.  With a causal mask parts may lie behind those: nobody has to do anything for them
+// (false), and a block whose keys end in its first part is whole.
+template <int SIZE>
+__device__ inline bool share(Item &it, int most, int &begin, int &end) {
     begin = 0;
     end = (most + SIZE - 1) / SIZE;
-    if (it.parts == 1) return;
-    const int all = (it.r.keys + SIZE - 1) / SIZE, each = all / it.parts, more = all - each * it.parts;
-    begin = it.part * each + (it.part < more ? it.part : more);
-    const int stop = begin + each + (it.part < more);
+    if (it.parts == 1) return true;
+    begin = first_step<SIZE>(it, it.part);
+    const int stop = first_step<SIZE>(it, it.part + 1);
+    if (it.part == 0 && stop >= end) it.parts = 1;
+    if (it.part > 0 && begin >= end) return false;
     end = stop < end ? stop : end;
+    return true;
 }
 // Where an item's share of a row goes, and its maximum and sum behind all of those
 template <int ROWS>
@@ -332,12 +342,12 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) self_attention_keys_ker
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
     constexpr int SIZE = 32;
-    const Item it = p.target ? part_of<32, SIZE, false>(p, at, lane) : item_of<32>(p, at, lane);
+    Item it = p.target ? part_of<32, SIZE, false>(p, at, lane) : item_of<32>(p, at, lane);
     if (!it.any) return;
     const Rows r = rows_of(p, it.r, hk, it.rb * 32 + col);
     int least, most, begin, end;
     limits_of(p, r, it.rb * 32, 32, least, most);
-    share<SIZE>(it, most, begin, end);
+    if (!share<SIZE>(it, most, begin, end)) return;
     typename E::vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
     const char *kp = first_key(p, it.r, p.k, p.ks, hk), *vp = first_key(p, it.r, p.v, p.vs, hk);
@@ -618,8 +628,10 @@ __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_att
     using vec = typename E::vec;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
-    const Item it = p.target ? part_of<HALF, KEYS, false>(p, at, lane) : item_of<HALF>(p, at, lane);
+    const int hk = blockIdx.x % p.Hkv;
+    int at = blockIdx.x / p.Hkv;
+    if (at >= p.mirror && at < 2 * p.mirror) at = p.mirror + (2 * p.mirror < p.items ? 2 * p.mirror : p.items) - 1 - at;
+    Item it = p.target ? part_of<HALF, KEYS, false>(p, at, lane) : item_of<HALF>(p, at, lane);
     if (!it.any) return;
     const int wave0 = it.rb * HALF + wave * 32;
     Rows r = rows_of(p, it.r, hk, wave0 + col);
@@ -629,13 +641,13 @@ __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_att
     vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
     // a part's keys: limits from its first one on
-    share<KEYS>(it, most, begin, end);
+    if (!share<KEYS>(it, most, begin, end)) return;
     const int skip = begin * KEYS, stop = end * KEYS;
     most = (most < stop ? most : stop) - skip;
     wave_most = (wave_most < stop ? wave_most : stop) - skip;
     wave_least -= skip;
     r.limit -= skip;
-    const int steps = end > begin ? end - begin : 0;  // (a part may lie behind all keys that are seen)
+    const int steps = end > begin ? end - begin : 0;
     Copies<H, 4> copies(lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], p.ks[1], p.vs[1], p.D, most, wave, lane, E::ONE);
     Softmax<BF16, H> st;
     st.start(lane);
@@ -744,7 +756,7 @@ struct RowCopies {
         k_step = KEYS * p.ks[1];
         v_step = KEYS * p.vs[1];
         most = most_;
-        steps = most > 0 ? (most + KEYS - 1) / KEYS : 0;  // (a part may lie behind all keys that are seen)
+        steps = most > 0 ? (most + KEYS - 1) / KEYS : 0;
         any = wave < ACTIVE;
         dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
 #pragma unroll
@@ -798,7 +810,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
-    const Item it = p.target ? part_of<ROWS, KEYS, false>(p, at, lane) : item_of<ROWS>(p, at, lane);
+    Item it = p.target ? part_of<ROWS, KEYS, false>(p, at, lane) : item_of<ROWS>(p, at, lane);
     if (!it.any) return;
     const int wave0 = it.rb * ROWS + wave * 32;
     Rows r = rows_of(p, it.r, hk, wave0 + col);
@@ -808,7 +820,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
     // a part's keys: limits from its first one on
-    share<KEYS>(it, most, begin, end);
+    if (!share<KEYS>(it, most, begin, end)) return;
     const int skip = begin * KEYS, stop = end * KEYS;
     most = (most < stop ? most : stop) - skip;
     wave_most = (wave_most < stop ? wave_most : stop) - skip;
@@ -958,11 +970,15 @@ __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
     constexpr int SUBS = BLOCK_ROWS / 4, MOST = 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, sub = rest % SUBS;
-    const Item it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
+    Item it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
     if (!it.any || it.parts == 1 || (long long)it.index + (long long)(it.parts - 1) * it.next >= p.items) return;
     const int at = sub * 4 + wave;
     const Rows r = rows_of(p, it.r, hk, it.rb * BLOCK_ROWS + at);
     if (!r.in) return;
+    int least, most;
+    limits_of(p, r, it.rb * BLOCK_ROWS, BLOCK_ROWS, least, most);
+    it.parts = __popcll(__ballot(lane < it.parts && first_step<SIZE>(it, lane) * SIZE < most));  // (those that `share` has something for, but the first)
+    if (it.parts < 2) return;
     const int c = lane * 2 < p.D ? lane * 2 : 0;
     typedef float float2_t __attribute__((ext_vector_type(2)));
     float top = -__builtin_huge_valf(), sum = 0.f;
@@ -1041,7 +1057,7 @@ int launch_heads(const Params &p, Form form, hipStream_t st) {
 
 struct Plan {
     Form form;
-    long long blocks, items, target, least, workspace;
+    long long blocks, items, target, least, mirror, workspace;
 };
 
 long long blocks_of(const svdq_self_attention_args *a, long long size) {
@@ -1051,10 +1067,11 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
 }
 
 // Which form a call takes and into how many parts it divides the keys of an average sequence: the least time by a model of the busiest compute unit, us.  Its constants are
-// those of 252 shapes (heads of 32 to 128, 1 .. 8192 queries, causal or not), each in every form and 1 .. 32 parts; what it chooses is 2 to 4 % behind the fastest on average,
-// 46 % at most (32 rows to 4096 keys, 17.2 us against 11.8).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.3 / keys 7.9, turns 7.0; 1024 tokens, 32 heads over 8 of
-// 128, causal rows 24.8 / keys 50.7, turns 33.1; 16384 tokens, 8 heads of 128 turns 995 / rows 1069; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128 29.9 in
-// eight parts / 143 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.2.
+// those of 252 shapes (heads of 32 to 128, 1 .. 8192 queries, causal or not), each in every form and 1 .. 32 parts; what it chooses is 1 to 2 % behind the fastest on average,
+// 39 % at most (2 x 100 tokens behind 1000, 8 heads of 80, 17.2 us against 12.3).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.3 / keys 7.9, turns 7.0; 1024 tokens,
+// 32 heads over 8 of 128, causal rows 24.3 / keys 51, turns 31; 16384 tokens, 8 heads of 128 turns 930 / rows 1069; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128
+// 29.9 in eight parts / 143 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.2; 4096 tokens, 8 heads of 128, causal rows in two parts
+// 64.5 / whole 73, turns 94.
 // Sequences of other lengths than the average have parts in proportion.
 struct Cost {
     int head_dim;                   // up to
@@ -1073,7 +1090,7 @@ Plan plan_of(const svdq_self_attention_args *a, int cus) {
     const float seen = !a->causal ? 1.f : q <= k ? 1.f - (float)(q - 1) / (2.f * (float)k) : (float)(k + 1) / (2.f * (float)q);
     const bool even = seen > 0.95f;
     static const int shares[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
-    Plan plan = {BY_TURNS, 0, 0, 0, 0, 0};
+    Plan plan = {BY_TURNS, 0, 0, 0, 0, 0, 0};
     long long chosen = 1;
     float best = 0.f;
     for (int form = BY_KEYS; form <= (a->head_dim > 64 ? BY_TURNS : BY_ROWS); form++) {
@@ -1085,7 +1102,7 @@ Plan plan_of(const svdq_self_attention_args *a, int cus) {
             float t;
             if (form == BY_KEYS) {
                 // two workgroups to a compute unit with heads up to 64, one with wider ones (LDS)
-                const float slots = a->head_dim <= 64 ? 2.f * n : n, work = __builtin_ceilf(each / 4.f) * c.round * (w > n && a->head_dim <= 64 ? 1.3f : 1.f);
+                const float slots = a->head_dim <= 64 ? 2.f * n : n, work = __builtin_ceilf(each / 4.f) * c.round * (w > n && a->head_dim <= 64 && even ? 1.3f : 1.f);
                 t = c.keys_base + work;
                 if (w > slots) {
                     const float more = (c.keys_base + work * seen) * (even ? __builtin_ceilf(w / slots) : w / slots + 0.3f);
@@ -1095,7 +1112,7 @@ Plan plan_of(const svdq_self_attention_args *a, int cus) {
                 const float load = even ? __builtin_ceilf(w / n) : w * seen / n, turns = w / n < 1.f ? 1.f : w / n > 3.f ? 3.f : w / n;
                 t = form == BY_ROWS ? c.rows_base + each * c.rows_step * (load > 1.f ? load : 1.f) : c.turns_base * turns + each * c.turns_step * (load > 1.f ? load : 1.f);
             }
-            if (parts > 1) t += c.join + (float)(S * a->kv_heads * rows) * (float)(a->head_dim * 8 * parts) / c.join_bytes;
+            if (parts > 1) t += c.join + (float)(S * a->kv_heads * rows) * (float)(a->head_dim * 8) * (1.f + (float)(parts - 1) * seen) / c.join_bytes;
             if (best == 0.f || t < best) {
                 best = t;
                 chosen = parts;
@@ -1104,6 +1121,11 @@ Plan plan_of(const svdq_self_attention_args *a, int cus) {
         }
     }
     const int size = plan.form == BY_KEYS ? 32 : plan.form == BY_ROWS ? HALF : ROWS;
+    // A compute unit gets its first workgroup and one of the second round at once.  With a causal mask the first have the most keys: those of the second round then come in the
+    // opposite order, the longest with the shortest (4096 tokens, 8 heads of 128, causal, in two parts 75.6 -> 64.5 us; 16384, 2 heads of 64 155 -> 119).  Not where all have
+    // about the same keys (chunks of new tokens behind long caches 34 -> 42), or where more rounds follow, which are given out as compute units come free (8 x 512 tokens, 32 heads over 8
+    // of 128 35.1 -> 36.8).
+    if (plan.form == BY_ROWS && !even && (rows + size - 1) / size * S * a->kv_heads * chosen <= 3 * cus) plan.mirror = cus / a->kv_heads;
     plan.blocks = plan.items = blocks_of(a, size);
     if (chosen > 1) {
         plan.least = plan.form == BY_KEYS ? 4 : 1;
@@ -1192,6 +1214,7 @@ extern "C" int svdq_self_attention(const svdq_self_attention_args *a, void *stre
     p.blocks = (int)plan.blocks;
     p.target = (int)plan.target;
     p.least = (int)plan.least;
+    p.mirror = (int)plan.mirror;
     p.causal = a->causal != 0;
     p.zero_rest = a->zero_rest != 0;
     p.scale2 = a->scale * 1.44269504088896340736f;

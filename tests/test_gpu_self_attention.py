@@ -263,3 +263,27 @@ def test_a_nan_of_one_query_stays_with_it(dev, shape, causal):
     for i, t in enumerate(rows):
         off[t, heads.index(i % H)] = -1
     assert (off <= 0).all(), (off.max().item(), (~(off <= 0)).sum().item())
+
+
+# (queries, keys) of each entry or sequence, heads, heads of keys, head size: causal, so few heads that the keys are divided, blocks whose keys end in the first part, and rows in
+# front of all keys
+@pytest.mark.parametrize("case", [([(2300, 2300)], 1, 1, 128), ([(1500, 1500)], 2, 1, 64), ([(1100, 1900)] * 2, 1, 1, 96), ([(1300, 700)], 2, 2, 72), ([(129, 4200), (1, 64), (900, 900)], 3, 1, 128),
+                                  ([(1024, 1024)] * 2, 2, 2, 32)])
+def test_parts_of_keys_under_a_causal_mask(dev, case):
+    from nunchaku_amd.ops import self_attention
+
+    lens, H, Hkv, D = case
+    announce(f"self_attention parts {case}")
+    new, keys = ([n[i] for n in lens] for i in (0, 1))
+    q = rand(sum(new), H, D, dtype=torch.bfloat16, seed=5, scale=1.5)
+    k, v = (rand(sum(keys), Hkv, D, dtype=torch.bfloat16, seed=s) for s in (6, 7))
+    out = Guarded((sum(new), H, D), torch.bfloat16, dev)
+    self_attention(q.to(dev), k.to(dev), v.to(dev), offsets(new).to(dev), offsets(keys).to(dev), causal=True, out=out.t)
+    out.check("out")
+    results = [out.t]
+    if len(set(lens)) == 1:
+        S = len(lens)
+        results.append(self_attention(*(t.to(dev).unflatten(0, (S, -1)) for t in (q, k, v)), causal=True).flatten(0, 1))
+    for got in results:
+        for a, m, b, n in zip(offsets(new).tolist(), new, offsets(keys).tolist(), keys):
+            check(got[a:a + m], q[a:a + m], k[b:b + n], v[b:b + n], True)
