@@ -741,70 +741,96 @@ __device__ inline void phase_ends() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// A wave's share of the copies of K and V: the same requests at every step, one or two of K and as many of V
+// A wave's share of the copies: the same requests at every step, of K by the first four waves, of V by the others
 template <typename H>
 struct RowCopies {
-    static constexpr int REQ = H::REQ / WAVES > 0 ? H::REQ / WAVES : 1, ACTIVE = H::REQ / REQ;  // per wave; waves that make any
-    const char *k, *v;
-    long long k_step, v_step;
-    uint32_t dst, ok[REQ], ov[REQ];
-    int row[REQ], most, steps;
-    bool any, in_k[REQ], in_v[REQ];  // whether the piece lies in the head
+    static constexpr int REQ = 2 * H::REQ / WAVES;
+    static_assert(REQ * WAVES == 2 * H::REQ && H::REQ % REQ == 0, "");
+    const char *first, *next;  // of the first step, of the one to be asked for next
+    long long bytes;           // a step
+    uint32_t dst, off[REQ];
+    uint64_t in[REQ];  // lanes whose piece lies in the head
+    int row[REQ], most, steps, whole;
+    bool values;
     __device__ inline RowCopies(const Params &p, char *lds, const char *kp, const char *vp, int most_, int wave, int lane) {
-        k = kp;
-        v = vp;
-        k_step = KEYS * p.ks[1];
-        v_step = KEYS * p.vs[1];
+        values = wave >= WAVES / 2;
+        first = next = values ? vp : kp;
+        const long long token = values ? p.vs[1] : p.ks[1];
+        bytes = KEYS * token;
         most = most_;
+        whole = most > 0 ? most / KEYS : 0;
         steps = most > 0 ? (most + KEYS - 1) / KEYS : 0;
-        any = wave < ACTIVE;
-        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * REQ * 1024;
+        const int request = (wave - (values ? WAVES / 2 : 0)) * REQ;
+        dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (values ? STAGES * H::TILE : 0) + request * 1024;
 #pragma unroll
         for (int i = 0; i < REQ; i++) {
-            const int piece = (wave * REQ + i) * 64 + lane, place = piece % H::PIECES;
+            const int piece = (request + i) * 64 + lane, place = piece % H::PIECES;
             row[i] = piece / H::PIECES;
-            const int ck = (place ^ H::fk(row[i])) * 16, cv = (place ^ H::fv(row[i])) * 16;
-            ok[i] = (uint32_t)(row[i] * p.ks[1]) + ck;
-            ov[i] = (uint32_t)(row[i] * p.vs[1]) + cv;
-            in_k[i] = ck < p.D * 2;
-            in_v[i] = cv < p.D * 2;
+            const int c = (place ^ (values ? H::fv(row[i]) : H::fk(row[i]))) * 16;
+            off[i] = (uint32_t)(row[i] * token) + c;
+            in[i] = __ballot(c < p.D * 2);
         }
     }
     // Rows behind the last key are not read: their scores are masked whatever K holds, and V holds zeros there, since nothing times a NaN is one.
-    __device__ inline void ask(int step, int slot) const {
-        if (!any || step >= steps) return;
-        const char *ks = k + step * k_step, *vs = v + step * v_step;
+    __device__ inline void ask_at(const char *src, int step, int slot) const {
         const uint32_t to = dst + slot * H::TILE;
-        const int left = most - step * KEYS;
-        if (left >= KEYS) {
+        const int left = most - step * KEYS, lane = threadIdx.x & 63;
 #pragma unroll
-            for (int i = 0; i < REQ; i++)
-                if (in_k[i]) copy16(to + i * 1024, ks, ok[i]);
-#pragma unroll
-            for (int i = 0; i < REQ; i++)
-                if (in_v[i]) copy16(to + STAGES * H::TILE + i * 1024, vs, ov[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < REQ; i++) {
-                if (in_k[i] && row[i] < left) copy16(to + i * 1024, ks, ok[i]);
-                if (in_v[i]) {
-                    if (row[i] < left) copy16(to + STAGES * H::TILE + i * 1024, vs, ov[i]);
-                    else clear16(to + STAGES * H::TILE + i * 1024 + (threadIdx.x & 63) * 16);
-                }
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a barrier alone does not wait for LDS)
+        for (int i = 0; i < REQ; i++) {
+            if (!(in[i] >> lane & 1)) continue;
+            if (row[i] < left) copy16(to + i * 1024, src, off[i]);
+            else if (values) clear16(to + i * 1024 + lane * 16);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a barrier alone does not wait for LDS)
+    }
+    // The next step.  Of a whole one, all lanes of all requests, or (a head that ends inside a row of LDS) all requests in one piece, without branches around those lanes that
+    // have none.  What a request costs is its issue, about 25 cycles of the compute unit whatever its lanes bring: rows of 192 bytes instead of 256 for heads of 72 .. 96 are
+    // three requests a wave instead of four (4608 tokens, 24 heads of 72 199 -> 186 us, 8192 tokens, 16 heads of 96 383 -> 363).
+    __device__ inline void ask(int step, int slot) {
+        if (step < whole) {
+            const uint32_t to = dst + slot * H::TILE;
+            [[maybe_unused]] uint64_t lanes;
+            if constexpr (!H::ONES) {
+#pragma unroll
+                for (int i = 0; i < REQ; i++) copy16(to + i * 1024, next, off[i]);
+            } else if constexpr (REQ == 4) {
+                asm volatile(
+                    "s_mov_b64 %0, exec\n\t"
+                    "s_mov_b32 m0, %1\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %7, %2\n\t"
+                    "s_add_u32 m0, m0, 0x400\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %8, %2\n\t"
+                    "s_add_u32 m0, m0, 0x400\n\ts_mov_b64 exec, %5\n\tglobal_load_lds_dwordx4 %9, %2\n\t"
+                    "s_add_u32 m0, m0, 0x400\n\ts_mov_b64 exec, %6\n\tglobal_load_lds_dwordx4 %10, %2\n\t"
+                    "s_mov_b64 exec, %0"
+                    : "=&s"(lanes)
+                    : "s"(to), "s"(next), "s"(in[0]), "s"(in[1]), "s"(in[2]), "s"(in[3]), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3])
+                    : "memory", "m0", "scc");
+            } else {
+                static_assert(REQ == 3, "");
+                asm volatile(
+                    "s_mov_b64 %0, exec\n\t"
+                    "s_mov_b32 m0, %1\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %6, %2\n\t"
+                    "s_add_u32 m0, m0, 0x400\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %7, %2\n\t"
+                    "s_add_u32 m0, m0, 0x400\n\ts_mov_b64 exec, %5\n\tglobal_load_lds_dwordx4 %8, %2\n\t"
+                    "s_mov_b64 exec, %0"
+                    : "=&s"(lanes)
+                    : "s"(to), "s"(next), "s"(in[0]), "s"(in[1]), "s"(in[2]), "v"(off[0]), "v"(off[1]), "v"(off[2])
+                    : "memory", "m0", "scc");
+            }
+        } else if (step < steps) {
+            ask_at(next, step, slot);
+        }
+        next += bytes;
     }
     // Step j + 1 has landed.  Step j + 2 alone has been asked for behind it; of the last step some requests may have had no lane to make them.
     __device__ inline void wait_for_next(int j) const {
-        if (j + 3 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * REQ) : "memory");
+        if (j + 3 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQ) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 };
 
 template <bool BF16, int DP, bool ONES>
 __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) {
-    using H = Head<DP, true, ONES>;
+    using H = Head<DP, false, ONES>;
     using E = Elem<BF16>;
     using vec = typename E::vec;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -826,7 +852,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     wave_most = (wave_most < stop ? wave_most : stop) - skip;
     wave_least -= skip;
     r.limit -= skip;
-    const RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], most, wave, lane);
+    RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], most, wave, lane);
     const int steps = copies.steps;
     const bool late = wave >= WAVES / 2;
     const int ahead = late ? STAGES - 1 : STAGES - 2;  // steps
@@ -856,12 +882,12 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
         if (i < VALUES) {
             typedef short short4_t __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) short4_t *tr_t;
-            const lds_t at = (lds_t)(uintptr_t)((v_at ^ (i % H::DB * 64)) + i / H::DB * 16 * H::PITCH);
+            const lds_t at = (lds_t)(uintptr_t)((H::PITCH == 256 ? v_at ^ (i % H::DB * 64) : v_at + i % H::DB * 64) + i / H::DB * 16 * H::PITCH);
             const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(at + 8 * H::PITCH));
             ops[i % AHEAD] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             const int n = i - VALUES, kb = n & 1, ks = n >> 1;
-            ops[i % AHEAD] = __builtin_bit_cast(vec, *(__attribute__((address_space(3))) u32x4_t *)(uintptr_t)((k_at ^ (ks * 32)) + kb * 32 * H::PITCH));
+            ops[i % AHEAD] = __builtin_bit_cast(vec, *(__attribute__((address_space(3))) u32x4_t *)(uintptr_t)((H::PITCH == 256 ? k_at ^ (ks * 32) : (k_at ^ (ks % 2 * 32)) + ks / 2 * 64) + kb * 32 * H::PITCH));
         }
     };
     auto stand = [&](int slot) __attribute__((always_inline)) {
@@ -902,7 +928,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     bool careful = false;
     if (steps > 0) {
         wait_for_q<BF16, H>(qf);
-        if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RowCopies<H>::REQ * (STAGES - 3)) : "memory");
+        if (steps > STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(RowCopies<H>::REQ * (STAGES - 3)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         phase_ends();
         if (late) phase_ends();
@@ -949,7 +975,7 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
 #pragma unroll 1
             for (int j = 0; j < steps; j++) {
                 phase_ends();
-                copies.ask(j, 0);
+                copies.ask_at(copies.first + j * copies.bytes, j, 0);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 phase_ends();
                 if (j * KEYS >= wave_most) continue;
@@ -1019,7 +1045,7 @@ enum Form { BY_KEYS, BY_ROWS, BY_TURNS };
 
 template <bool BF16, int DP, bool ONES>
 int launch_kernels(const Params &p, Form form, hipStream_t st) {
-    const int lds = form == BY_KEYS ? 8 * Head<DP, true>::TILE : form == BY_ROWS ? 4 * Head<DP>::TILE + 16 : 2 * STAGES * Head<DP, true>::TILE + 64;
+    const int lds = form == BY_KEYS ? 8 * Head<DP, true>::TILE : form == BY_ROWS ? 4 * Head<DP>::TILE + 16 : 2 * STAGES * Head<DP>::TILE + 64;
     static bool reserved[3][64] = {{false}};
     const void *kernel = form == BY_KEYS ? (const void *)self_attention_keys_kernel<BF16, DP> : (const void *)self_attention_rows_kernel<BF16, DP, ONES>;
     if constexpr (DP > 64) {
@@ -1080,7 +1106,7 @@ struct Cost {
     float turns_base, turns_step;   // turns form, which heads up to 64 never take: 8192 tokens, 16 heads of 64 307 us by turns, 300 by rows, causal 632 and 573; of 32 255 and 212
     float join, join_bytes;         // parts: the second launch; bytes a us of their way there and back
 };
-constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.3f, 0.69f, 0.f, 0.f, 5.4f, 3.5e6f}, {96, 5.7f, 1.45f, 4.8f, 0.95f, 5.5f, 1.17f, 5.6f, 5.2e6f}, {128, 6.1f, 1.65f, 5.6f, 1.06f, 7.0f, 1.31f, 5.5f, 6.2e6f}};
+constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.3f, 0.69f, 0.f, 0.f, 5.4f, 3.5e6f}, {96, 5.7f, 1.45f, 4.8f, 0.95f, 5.5f, 1.10f, 5.6f, 5.2e6f}, {128, 6.1f, 1.65f, 5.6f, 1.06f, 7.0f, 1.30f, 5.5f, 6.2e6f}};
 
 Plan plan_of(const svdq_self_attention_args *a, int cus) {
     const long long S = a->batch, q = a->cu_seqlens_q ? (a->q_len + S - 1) / S : a->q_len, k = a->cu_seqlens_k ? (a->k_len + S - 1) / S : a->k_len;

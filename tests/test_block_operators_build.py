@@ -55,7 +55,7 @@ def test_registers(compiled):
 def test_main_loops(compiled):
     _, lines = compiled["self_attention.hip"]
     seen = {"rows": 0, "turns": 0}
-    for form, barriers, waits in (("rows", 1, {"s_waitcnt vmcnt(0) lgkmcnt(0)"}), ("turns", 2, {"s_waitcnt vmcnt(0)", "s_waitcnt vmcnt(4)"})):
+    for form, barriers, waits in (("rows", 1, {"s_waitcnt vmcnt(0) lgkmcnt(0)"}), ("turns", 2, {"s_waitcnt vmcnt(0)", "s_waitcnt vmcnt(3)", "s_waitcnt vmcnt(4)"})):
         for name, body in bodies(lines, f"self_attention_{form}_kernel"):
             mains = []
             for loop in innermost_loops(body):
