@@ -320,7 +320,7 @@ extern "C" int svdq_gated_norm(const svdq_gated_norm_args *a, void *stream) {
         p.scale_s[i] = a->scale_stride[i] * 2;
         p.shift_s[i] = a->shift_stride[i] * 2;
     }
-    p.tokens = a->cu_seqlens ? a->M : a->tokens;
+    p.tokens = a->cu_seqlens || a->tokens > a->M ? a->M : a->tokens;  // (32 bits hold it)
     p.sequences = (int)a->sequences;
     p.pieces = (int)(a->K / 8);
     p.zero_rest = a->zero_rest;

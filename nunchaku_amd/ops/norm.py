@@ -8,9 +8,14 @@ import math
 import torch
 
 from .. import _native as nv
-from .w8a8 import DTYPES, _row_stride, _rows
+from .w8a8 import DTYPES, _row_stride
+from .w8a8 import _rows as _filled_rows
 
 NORMS = {"rms": 0, "layer": 1}
+
+
+def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    return _filled_rows(x if x.numel() or x.dim() < 3 else x.flatten(0, -2), name)
 
 
 def _vector(v: torch.Tensor | None, name: str, x: torch.Tensor, entries: int | None) -> tuple[int, int]:
@@ -31,7 +36,7 @@ def _vector(v: torch.Tensor | None, name: str, x: torch.Tensor, entries: int | N
     if v.shape == x.shape:  # one for each token
         rows = _rows(v, name)
         ld = rows.stride(0) if rows.shape[0] > 1 else 0
-        return ld * (x.numel() // K // x.shape[0] if x.dim() > 2 else 1), ld
+        return ld * math.prod(x.shape[1:-1]), ld
     if x.dim() > 2 and v.numel() == x.shape[0] * K and v.shape[0] == x.shape[0]:  # one for each batch entry
         return (v.stride(0) if v.shape[0] > 1 else 0), 0
     raise ValueError(f"{name} must be [{K}], [{x.shape[0]}, {K}] or {tuple(x.shape)}, got {tuple(v.shape)}")

@@ -170,3 +170,32 @@ def test_zero_rows(dev):
         assert torch.equal(gated_norm(x, norm=norm, shift=s)[0], s.expand(3, 256))
     y, h = gated_norm(x[:0], x[:0])
     assert y.shape == h.shape == (0, 256)
+
+
+def test_no_rows(dev):
+    """Empty batches and entries: empty results, vectors of their shape taken all the same."""
+    from nunchaku_amd.ops import gated_norm
+
+    for shape in ((0, 16), (0, 5, 16), (3, 0, 16), (2, 0, 4, 16)):
+        x = torch.empty(shape, dtype=torch.float16, device=dev)
+        y, h = gated_norm(x, x.clone(), gate=x.clone(), scale=torch.ones(16, dtype=x.dtype, device=dev))
+        assert y.shape == h.shape == x.shape
+        out = torch.empty_like(x)
+        assert gated_norm(x, out=out)[0] is out
+    with pytest.raises(ValueError):
+        gated_norm(torch.empty(2, 3, 0, dtype=torch.float16, device=dev), gate=torch.empty(2, 3, 0, dtype=torch.float16, device=dev))
+
+
+@pytest.mark.parametrize("tokens", [5, 2**32, 2**40 + 1])
+def test_entries_longer_than_the_rows(dev, tokens):
+    """The C entry: all rows belong to the first entry, however many rows one would have."""
+    import ctypes
+
+    from nunchaku_amd import _native as nv
+
+    x, gate, y = rand(5, 64, dtype=torch.float16, seed=1), rand(5, 64, dtype=torch.float16, seed=2), torch.empty(5, 64, dtype=torch.float16, device=dev)
+    gx, gg, two = x.to(dev), gate.to(dev), ctypes.c_int64 * 2
+    args = nv.GatedNormArgs(gx.data_ptr(), None, y.data_ptr(), None, None, None, gg.data_ptr(), None, None, None, 5, 64, tokens, 0, 64, 0, 64, 0, two(1 << 40, 64), two(0, 0), two(0, 0),
+                            1.0, 1e-6, 0, 0, 1)
+    assert nv.lib().svdq_gated_norm(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    check((y, None), x, gate=gate)
