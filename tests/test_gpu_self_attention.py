@@ -287,3 +287,18 @@ def test_parts_of_keys_under_a_causal_mask(dev, case):
     for got in results:
         for a, m, b, n in zip(offsets(new).tolist(), new, offsets(keys).tolist(), keys):
             check(got[a:a + m], q[a:a + m], k[b:b + n], v[b:b + n], True)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [(3, 5, 2, 1, 64), (2, 300, 4, 4, 72), (4, 1, 8, 2, 128)])
+def test_a_batch_of_queries_over_packed_keys(dev, shape, causal):
+    from nunchaku_amd.ops import self_attention
+
+    S, T, H, Hkv, D = shape
+    lens = [0, 700, 33, 129][:S]
+    q = rand(S, T, H, D, dtype=torch.float16, seed=1)
+    k, v = (rand(sum(lens), Hkv, D, dtype=torch.float16, seed=s) for s in (2, 3))
+    cu = offsets(lens)
+    got = self_attention(q.to(dev), k.to(dev), v.to(dev), cu_seqlens_k=cu.to(dev), causal=causal)
+    for s, (a, n) in enumerate(zip(cu.tolist(), lens)):
+        check(got[s], q[s], k[a:a + n], v[a:a + n], causal)
