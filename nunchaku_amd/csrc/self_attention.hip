@@ -951,10 +951,12 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
             }
             if (!late) copies.wait_for_next(j);
             phase_ends();
+            if (DP > 96) __builtin_amdgcn_s_setprio(1);  // (16384 tokens, 8 heads of 128 930 -> 916 us; 8192 tokens, 16 heads of 96 379 -> 382)
             if (here) {
                 multiply(FIRST, SCORES);
                 if ((j + 1) * KEYS < wave_most) multiply(SCORES, END);
             }
+            if (DP > 96) __builtin_amdgcn_s_setprio(0);
             if (late) {
                 if (j + 1 == steps) break;
                 copies.wait_for_next(j + 1);
