@@ -86,24 +86,34 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
     const int nq = (p.heads[0] + SLOTS - 1) / SLOTS, all = nq + (p.heads[1] + SLOTS - 1) / SLOTS;
     int turn = part * all / p.share;
     const int end = (part + 1) * all / p.share;
-    const char *src[2];
-    char *dst[2];
+    // This lane's piece of a turn's head, in and out, moved on turn by turn: from q's last one to k's first
+    const char *first_in[2];
+    char *first_out[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        src[k] = p.in[k] + b * p.in_s[k][0] + t * p.in_s[k][1] + (slot * p.in_s[k][2] + c * 16);
-        dst[k] = p.out[k] + b * p.out_s[k][0] + t * p.out_s[k][1] + (slot * p.out_s[k][2] + c * 16);
+        first_in[k] = p.in[k] + b * p.in_s[k][0] + t * p.in_s[k][1] + (slot * p.in_s[k][2] + c * 16);
+        first_out[k] = p.out[k] + b * p.out_s[k][0] + t * p.out_s[k][1] + (slot * p.out_s[k][2] + c * 16);
     }
+    const int begun = turn < nq ? turn : turn - nq;
+    const char *src = (turn < nq ? first_in[0] : first_in[1]) + begun * SLOTS * (turn < nq ? p.in_s[0][2] : p.in_s[1][2]);
+    char *dst = (turn < nq ? first_out[0] : first_out[1]) + begun * SLOTS * (turn < nq ? p.out_s[0][2] : p.out_s[1][2]);
+    // whether this lane has a piece of turn x
+    auto has = [&](int x) __attribute__((always_inline)) {
+        const int left = x < nq ? p.heads[0] - x * SLOTS : p.heads[1] - (x - nq) * SLOTS;
+        return in && slot < left;
+    };
     u32x4_t w[ITEMS];
     auto load = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
-            const int k = first + i >= nq, head = (first + i - (k ? nq : 0)) * SLOTS;
             w[i] = u32x4_t{0, 0, 0, 0};
-            if (first + i < end && in && head + slot < p.heads[k]) {
-                const u32x4_t *from = (const u32x4_t *)(src[k] + head * p.in_s[k][2]);
-                if (p.once) w[i] = __builtin_nontemporal_load(from);
-                else w[i] = *from;
+            if (first + i >= end) continue;
+            if (has(first + i)) {
+                if (p.once) w[i] = __builtin_nontemporal_load((const u32x4_t *)src);
+                else w[i] = *(const u32x4_t *)src;
             }
+            src += SLOTS * (first + i < nq ? p.in_s[0][2] : p.in_s[1][2]);
+            if (first + i == nq - 1) src = first_in[1];
         }
     };
     load(turn);
@@ -144,7 +154,7 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             if (turn + i >= end) break;
-            const int k = turn + i >= nq, head = (turn + i - (k ? nq : 0)) * SLOTS;
+            const int k = turn + i >= nq;
             float x[8], y[8];
             unpack<BF16>(w[i], x);
             if (NORM && p.norm[k]) {
@@ -183,7 +193,9 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
                     x[2 * j + 1] = a * si[j] + d * co[j];
                 }
             }
-            if (in && head + slot < p.heads[k]) *(u32x4_t *)(dst[k] + head * p.out_s[k][2]) = pack<BF16>(x);
+            if (has(turn + i)) *(u32x4_t *)dst = pack<BF16>(x);
+            dst += SLOTS * (k ? p.out_s[1][2] : p.out_s[0][2]);
+            if (turn + i == nq - 1) dst = first_out[1];
         }
     }
 }
