@@ -272,3 +272,19 @@ def test_attention_refusals(dev):
         self_attention(q.float(), k.float(), k.float())
     with pytest.raises(RuntimeError, match="GPU"):
         self_attention(q.cpu(), k.cpu(), k.cpu())
+
+
+@pytest.mark.parametrize("D", [72, 128])
+def test_keys_beyond_32_bits_of_many_rows(dev, D):
+    """Tokens 8 MiB apart: the last keys of a sequence are more than 2^32 bytes behind its first ones."""
+    from nunchaku_amd.ops import self_attention
+
+    announce(f"keys beyond 32 bits {D}")
+    T, H, token = 700, 64, 2**22
+    q, k, v = (attention_test.rand(1, T, H, D, dtype=torch.bfloat16, seed=s) for s in (1, 2, 3))
+    big = torch.empty(T * token, dtype=torch.bfloat16, device=dev)  # 5.9 GB
+    g = [big.as_strided((1, T, H, D), (0, token, D, 1), i * H * D) for i in range(2)]
+    for a, t in zip(g, (k, v)):
+        a.copy_(t)
+    for causal in (False, True):
+        attention_test.check(self_attention(q.to(dev), *g, causal=causal)[0], q[0], k[0], v[0], causal)
