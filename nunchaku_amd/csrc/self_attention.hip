@@ -998,7 +998,25 @@ __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
     constexpr int SUBS = BLOCK_ROWS / 4, MOST = 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, sub = rest % SUBS;
-    Item it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
+    Item it;
+    if constexpr (BLOCK_ROWS > 32) {
+        // one wave finds the block for all four: with many workgroups the search is most of their instructions (8192 tokens, one head of 64 30.4 -> 28.9 us, 304 workgroups in
+        // parts 34.3 -> 33.5; a single token to 4096 keys, 32 heads over 8 of 128, 13.3 -> 13.5)
+        __shared__ Item found;
+        if (wave == 0) {
+            const Item first = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
+            if (lane == 0) found = first;
+        }
+        __syncthreads();
+        it.r = in_lane(found.r, 0);
+        it.rb = __builtin_amdgcn_readfirstlane(found.rb);
+        it.parts = __builtin_amdgcn_readfirstlane(found.parts);
+        it.index = __builtin_amdgcn_readfirstlane(found.index);
+        it.next = __builtin_amdgcn_readfirstlane(found.next);
+        it.any = __builtin_amdgcn_readfirstlane((int)found.any) != 0;
+    } else {
+        it = part_of<BLOCK_ROWS, SIZE, true>(p, rest / SUBS, lane);
+    }
     if (!it.any || it.parts == 1 || (long long)it.index + (long long)(it.parts - 1) * it.next >= p.items) return;
     const int at = sub * 4 + wave;
     const Rows r = rows_of(p, it.r, hk, it.rb * BLOCK_ROWS + at);
