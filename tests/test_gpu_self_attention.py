@@ -302,3 +302,37 @@ def test_a_batch_of_queries_over_packed_keys(dev, shape, causal):
     got = self_attention(q.to(dev), k.to(dev), v.to(dev), cu_seqlens_k=cu.to(dev), causal=causal)
     for s, (a, n) in enumerate(zip(cu.tolist(), lens)):
         check(got[s], q[s], k[a:a + n], v[a:a + n], causal)
+
+
+# heads of every kernel of blocks of 128 and of 256 rows, with and without a column of ones
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [(900, 2, 2, 64), (900, 1, 1, 72), (700, 2, 1, 128), (600, 4, 4, 24), (700, 64, 64, 128), (700, 64, 64, 72), (700, 48, 48, 96)])
+def test_scores_that_rise_along_the_keys(dev, shape, causal):
+    """By 30, 80, 100 and 3000 over all keys, or by 90 at one key between two others: within fp32's range of an old maximum's exponentials, at its end and beyond."""
+    from nunchaku_amd.ops import self_attention
+
+    T, H, Hkv, D = shape
+    dtype = torch.bfloat16
+    announce(f"self_attention rising {shape} {causal}")
+    way = torch.sign(rand(1, 1, D, dtype=torch.float32, seed=1))
+    q = (way * (1 + 0.05 * rand(T, H, 1, dtype=torch.float32, seed=2))).to(dtype)
+    v = rand(T, Hkv, D, dtype=dtype, seed=3)
+    at = torch.arange(T, dtype=torch.float32)[:, None, None] / T
+    for rise in (30.0, 80.0, 100.0, 3000.0, None):
+        size = rise * at if rise else 90.0 * (at == 333 / T) - 3.0 * at
+        k = (way * size / math.sqrt(D) + 0.02 * rand(T, Hkv, D, dtype=torch.float32, seed=4)).to(dtype)
+        check(self_attention(*(t.to(dev)[None] for t in (q, k, v)), causal=causal)[0], q, k, v, causal)
+
+
+@pytest.mark.parametrize("shape", [(500, 2, 2, 64), (700, 64, 64, 128), (700, 64, 64, 72)])
+def test_first_keys_of_no_weight(dev, shape):
+    """Scores of minus infinity for more than a block's first keys: as if those keys were not there."""
+    from nunchaku_amd.ops import self_attention
+
+    T, H, Hkv, D = shape
+    for dtype in DTYPES:
+        q, v = rand(T, H, D, dtype=dtype, seed=1).abs() + 0.125, rand(T, Hkv, D, dtype=dtype, seed=3)
+        k = rand(T, Hkv, D, dtype=dtype, seed=2)
+        for first in (40, 130):
+            k[:first] = -math.inf
+            check(self_attention(*(t.to(dev)[None] for t in (q, k, v)))[0], q, k[first:], v[first:], False)
