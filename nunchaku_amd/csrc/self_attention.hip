@@ -1121,10 +1121,10 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
 
 // Which form a call takes and into how many parts it divides the keys of an average sequence: the least time by a model of the busiest compute unit, us.  Its constants are
 // those of 252 shapes (heads of 32 to 128, 1 .. 8192 queries, causal or not), each in every form and 1 .. 32 parts; what it chooses is 1 to 2 % behind the fastest on average,
-// 28 % at most (1024 tokens, 32 heads over 8 of 32, causal, 14.4 us against 11.4).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.3 / keys 7.9, turns 7.0; 1024 tokens,
-// 32 heads over 8 of 128, causal rows 24.3 / keys 51, turns 31; 16384 tokens, 8 heads of 128 turns 930 / rows 1069; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128
-// 29.9 in eight parts / 143 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.2; 4096 tokens, 8 heads of 128, causal rows in two parts
-// 64.5 / whole 73, turns 94.
+// 26 % at most (1024 tokens, 32 heads over 8 of 32, causal, 14.4 us against 11.4).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.5 / keys 7.9, turns 7.3; 1024 tokens,
+// 32 heads over 8 of 128, causal rows 24.9 / keys 54, turns 29; 16384 tokens, 8 heads of 128 turns 920 / rows 1020; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128
+// 29.6 in eight parts / 116 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.3; 4096 tokens, 8 heads of 128, causal rows in two parts
+// 64.8 / whole 75, turns 83.
 // Sequences of other lengths than the average have parts in proportion.
 struct Cost {
     int head_dim;                   // up to
