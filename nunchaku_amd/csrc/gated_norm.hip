@@ -3,7 +3,8 @@
 //   y = (h - m) / sqrt(mean((h - m)^2) + eps) * weight * (1 + scale) + shift,   m = 0 (RMS norm) or mean(h) (layer norm)
 // Vectors that are not given are left out.  gate, scale and shift belong to a batch entry, a packed sequence or a token.  All of it is fp32 from
 // the first conversion to the last: y is made of h as it is, before h is rounded for the residual stream.
-// The mean is taken before the deviations' squares are summed, from registers: their difference in one pass would lose what a large mean leaves.
+// The mean is taken before the deviations' squares are summed, from registers: their difference in one pass would lose what a large mean leaves.  So would the
+// mean's own rounding, 2^-24 of it beside a spread that may be less: the deviations are summed with their squares, and what they have in common is taken out of both.
 // Squares whose sum leaves fp32's range, at either end, are summed once more in 64 bits: rows of finite numbers have finite norms.
 // Bound by the traffic, 8 bytes an element with a residual: 2 x 4608 x 5120 72 us, 5.3 TB/s (a copy reaches 5.1 here), 4096 x 4096 21.6, 6.2 TB/s; one row of 4096 with
 // both norms 3.0, launch and latencies.
@@ -92,13 +93,32 @@ __device__ inline T row_sum(T x, T (*place)[16], int slot) {
     return x;
 }
 
+// Those of x and y, in places `slot` and the next.  The half-waves exchange first, so that one has x left and the other y: both cost what one does
+// (two sums one beside the other: 2 x 1157 x 2304 7.2 us, this 7.0; 9000 x 5120 33.2, 32.4)
+template <bool WIDE>
+__device__ inline void row_sums(float &x, float &y, float (*place)[16], int slot) {
+    const auto a = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(y), false, false);
+    float s = sum16(bits_f32(a[0]) + bits_f32(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(f32_bits(s), f32_bits(s), false, false);
+    s = bits_f32(b[0]) + bits_f32(b[1]);
+    if constexpr (WIDE) {
+        const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+        float *mine = place[slot + (lane >> 5)];
+        if ((lane & 31) == 0) mine[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = sum16((lane & 15) < waves ? mine[lane & 15] : 0.f);
+    }
+    x = bits_f32(__builtin_amdgcn_readlane(f32_bits(s), 0));
+    y = bits_f32(__builtin_amdgcn_readlane(f32_bits(s), 32));
+}
+
 // h <- (h - m) / sqrt(mean((h - m)^2) + eps), the pieces of this thread that lie in the row
-template <bool WIDE, int VECS>
-__device__ inline void normalise(float (&h)[VECS][8], bool center, const NormParams &p, int t, int threads, int slot) {
-    __shared__ float sums[4][16];
+template <bool WIDE, int VECS, bool CENTER>
+__device__ inline void normalise(float (&h)[VECS][8], const NormParams &p, int t, int threads, int slot) {
+    __shared__ float sums[5][16];
     __shared__ double wide[4][16];
     float m = 0.f;
-    if (center) {
+    if constexpr (CENTER) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < VECS; i++)
@@ -106,25 +126,38 @@ __device__ inline void normalise(float (&h)[VECS][8], bool center, const NormPar
             for (int j = 0; j < 8; j++) s += h[i][j];  // (zeros behind the row's end)
         m = row_sum<WIDE>(s, sums, slot) * p.inv_k;
     }
-    float squares = 0.f;
+    float squares = 0.f, rest = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
         if (t + i * threads >= p.pieces) break;
 #pragma unroll
-        for (int j = 0; j < 8; j++) squares = __builtin_fmaf(h[i][j] - m, h[i][j] - m, squares);
+        for (int j = 0; j < 8; j++) {
+            const float d = h[i][j] - m;
+            squares = __builtin_fmaf(d, d, squares);
+            if (CENTER) rest += d;
+        }
     }
-    squares = row_sum<WIDE>(squares, sums, slot + 1);
-    if (squares < 0x1p120f && squares >= p.tiny) {
-        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, p.inv_k, p.eps));
+    bool good = true;
+    if constexpr (CENTER) {
+        row_sums<WIDE>(squares, rest, sums, slot + 1);
+        const float common = rest * (rest * p.inv_k);
+        good = common <= 0.5f * squares;  // (else next to nothing is left of the squares, as of a row of equal numbers; or a NaN)
+        rest *= p.inv_k;
+        squares -= common;
+    } else {
+        squares = row_sum<WIDE>(squares, sums, slot + 1);
+    }
+    if (good && squares < 0x1p120f && squares >= p.tiny) {
+        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, p.inv_k, p.eps)), c = -rest * r;
 #pragma unroll
         for (int i = 0; i < VECS; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) h[i][j] = (h[i][j] - m) * r;
+            for (int j = 0; j < 8; j++) h[i][j] = CENTER ? __builtin_fmaf(h[i][j] - m, r, c) : h[i][j] * r;
         return;
     }
     const double inv_k = 1.0 / (8.0 * p.pieces);
     double mean = 0.0, s = 0.0;
-    if (center) {
+    if constexpr (CENTER) {
 #pragma unroll
         for (int i = 0; i < VECS; i++)
 #pragma unroll
@@ -219,7 +252,7 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormParam
         }
     };
     if (p.branch_weight) {
-        normalise<WIDE, VECS>(h, false, p, t, threads, 0);
+        normalise<WIDE, VECS, false>(h, p, t, threads, 0);
         times(0, 0.f);
     }
     times(1, 0.f);
@@ -233,7 +266,7 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256) gated_norm_kernel(NormParam
             if (piece < p.pieces && p.h) *(u32x4_t *)(p.h + row * p.ld_h + (size_t)piece * 16) = pack<BF16>(h[i]);
         }
     }
-    normalise<WIDE, VECS>(h, LAYER, p, t, threads, 2);
+    normalise<WIDE, VECS, LAYER>(h, p, t, threads, 2);
     times(2, 0.f);
     times(3, 1.f);
 #pragma unroll
