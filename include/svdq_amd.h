@@ -433,7 +433,7 @@ typedef struct svdq_self_attention_args {
     const void *k, *v;      /* [batch][k_len][kv_heads][head_dim] by strides; with cu_seqlens_k the same */
     void *out;              /* as q                                                                  */
     const int32_t *cu_seqlens_q, *cu_seqlens_k; /* [batch + 1] ascending offsets or NULL (offsets out of range or order give
-                               fewer rows or keys, never others)                                      */
+                               fewer rows or keys, never others, and no row of q to two sequences)    */
     const int32_t *key_lengths; /* [batch] or NULL, without cu_seqlens_k; values outside 0..k_len count as the nearer of the two */
     void *workspace;        /* svdq_self_attention_workspace bytes (16-byte aligned), not shared with a call that may run at the same
                                time; NULL if that is 0                                               */

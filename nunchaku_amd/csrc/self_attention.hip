@@ -27,25 +27,24 @@ struct Params {
 __device__ inline int clamped(int x, int lo, int hi) { return x < lo ? lo : x < hi ? x : hi; }
 
 // Rows of q that belong together: those of a sequence (s in 0 .. S - 1), or, packed, those in front of the first (region 0) and behind the last, which are in none.
-// Offsets that are not in order give fewer rows and keys, never others.
+// A launch has as many blocks as regions need that lie one behind the other, and nobody but its own region's workgroups may store a row: an offset below one in front of it
+// counts as that one.  Offsets that are not in order so give fewer rows (and keys), never others, and every row is in one region.
 struct Region {
     int s, first, count;  // sequence, its first query's row of q (of its batch entry, if they are not packed), its queries
     int key, keys;        // the same of k and v
 };
 __device__ inline int regions(const Params &p) { return p.cu_q ? p.S + 2 : p.S; }
 __device__ inline int region_start(const Params &p, int i) { return i == 0 ? 0 : i > p.S + 1 ? p.Tq : clamped(p.cu_q[i - 1], 0, p.Tq); }  // (packed)
-__device__ inline Region region_of(const Params &p, int i) {
+__device__ inline Region region_of(const Params &p, int i) {  // (packed: by its offsets as they stand)
     Region r;
     r.s = p.cu_q ? i - 1 : i;
     r.first = r.key = r.keys = 0;
     r.count = p.Tq;
-    const bool any = r.s >= 0 && r.s < p.S;
     if (p.cu_q) {
         r.first = region_start(p, i);
-        const int n = region_start(p, i + 1) - r.first;
-        r.count = (any || p.zero_rest) && n > 0 ? n : 0;
+        r.count = region_start(p, i + 1) - r.first;
     }
-    if (any) {
+    if (r.s >= 0 && r.s < p.S) {
         if (p.cu_k) {
             r.key = clamped(p.cu_k[r.s], 0, p.Tk);
             r.keys = clamped(p.cu_k[r.s + 1], r.key, p.Tk) - r.key;
@@ -74,16 +73,24 @@ __device__ inline int up_to_lane(int x, F op) {  // (zero changes nothing)
     x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));
     return op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));
 }
-// a sum, 2^29 at most: offsets that are not in order can make any
+// (blocks are fewer than 2^24, parts 64 of each at most)
 __device__ inline int sum_up_to_lane(int x) {
-    return up_to_lane(x < 1 << 29 ? x : 1 << 29, [](int a, int b) __attribute__((always_inline)) { return a + b < 1 << 29 ? a + b : 1 << 29; });
+    return up_to_lane(x, [](int a, int b) __attribute__((always_inline)) { return a + b; });
 }
-__device__ inline int most_of(int x) {
-    return __builtin_amdgcn_readlane(up_to_lane(x, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; }), 63);
+__device__ inline int most_up_to_lane(int x) {
+    return up_to_lane(x, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; });
 }
+__device__ inline int most_of(int x) { return __builtin_amdgcn_readlane(most_up_to_lane(x), 63); }
 __device__ inline float sum_of(float x) {
     return bits_f32(__builtin_amdgcn_readlane(
         up_to_lane((int)f32_bits(x), [](int a, int b) __attribute__((always_inline)) { return (int)f32_bits(bits_f32((uint32_t)a) + bits_f32((uint32_t)b)); }), 63));
+}
+
+// Packed, a region to a lane, in the order of the lanes: the one in front of them all begins at `before`
+__device__ inline void put_in_order(const Params &p, Region &r, int before) {
+    const int end = r.first + r.count, most = most_up_to_lane(r.first);
+    r.first = most > before ? most : before;
+    r.count = end > r.first && (p.zero_rest || (r.s >= 0 && r.s < p.S)) ? end - r.first : 0;
 }
 
 // A block of rows of a region and a part of its keys
@@ -98,7 +105,7 @@ struct Item {
 // Packed, up to 64 regions: their blocks one behind the other, which takes the sums over the regions in front of each.  (The workgroups without a block are the last ones
 // then: between the others they leave some compute units with two and some with none, 16 sequences of 256, 12 heads of 64 20.8 us against 11.5.)
 // More: region i has the numbers from f(i) = floor(start(i) * G / ROWS) + i to f(i + 1), as many as it needs or one or two more, without sums.  Its own is the last
-// region whose f is not behind `at`, found among 64 at a time.
+// region whose f is not behind `at`, found among 64 at a time; in order are put the starts that are looked at, between those found before, so that all workgroups see the same ones.
 template <int ROWS>
 __device__ inline Item item_of(const Params &p, int at, int lane) {
     Item it;
@@ -115,6 +122,7 @@ __device__ inline Item item_of(const Params &p, int at, int lane) {
     if (n <= 64) {
         Region r = Region{0, 0, 0, 0, 0};
         if (lane < n) r = region_of(p, lane);
+        put_in_order(p, r, 0);
         const int blocks = blocks_of<ROWS>(p, r.count);
         const int upto = sum_up_to_lane(blocks);
         const uint64_t behind = __ballot(at < upto);
@@ -124,22 +132,29 @@ __device__ inline Item item_of(const Params &p, int at, int lane) {
         it.any = behind && it.rb < __builtin_amdgcn_readlane(blocks, l);
         return it;
     }
+    int low = 0, high = p.Tq;  // where region `lo` begins and the last of the n ends
     for (;;) {
         const int step = (n + 63) / 64, i = lo + lane * step;
         Region r = Region{0, 0, 0, 0, 0};
         bool in = i < lo + n;
+        int start = high;
         if (in) {
             if (step == 1) r = region_of(p, i);
             else r.first = region_start(p, i);
-            in = (int)((long long)r.first * p.G / ROWS) + i <= at;
+            start = clamped(r.first, low, high);
         }
-        const uint64_t found = __ballot(in);
-        const int l = found ? 63 - __builtin_clzll(found) : 0;
+        start = most_up_to_lane(start);
+        in = in && (int)((long long)start * p.G / ROWS) + i <= at;
+        const int l = 63 - __builtin_clzll(__ballot(in));  // (region `lo` itself is)
+        low = __builtin_amdgcn_readlane(start, l);
+        high = l < 63 ? __builtin_amdgcn_readlane(start, l + 1) : high;
         if (step == 1) {
             it.r = in_lane(r, l);
-            const int blocks = blocks_of<ROWS>(p, it.r.count), rel = at - ((int)((long long)it.r.first * p.G / ROWS) + lo + l);
+            it.r.first = low;
+            it.r.count = p.zero_rest || (it.r.s >= 0 && it.r.s < p.S) ? high - low : 0;
+            const int blocks = blocks_of<ROWS>(p, it.r.count), rel = at - ((int)((long long)low * p.G / ROWS) + lo + l);
             it.rb = blocks - 1 - rel;
-            it.any = found && rel >= 0 && rel < blocks;
+            it.any = rel < blocks;
             return it;
         }
         lo += l * step;
@@ -161,8 +176,13 @@ __device__ inline Item part_among(const Params &p, int at, int lane) {
         r[c] = Region{0, 0, 0, 0, 0};
         if (c * 64 + lane < n) r[c] = region_of(p, c * 64 + lane);
     }
+    int before = 0;
 #pragma unroll
     for (int c = 0; c < C; c++) {
+        if (p.cu_q) {
+            put_in_order(p, r[c], before);
+            before = __builtin_amdgcn_readlane(r[c].first, 63);
+        }
         blocks[c] = blocks_of<ROWS>(p, r[c].count);
         steps[c] = (r[c].keys + SIZE - 1) / SIZE;
         if (blocks[c]) most = steps[c] > most ? steps[c] : most;
