@@ -392,8 +392,8 @@ int svdq_gated_norm(const svdq_gated_norm_args *args, void *stream);
  * Rotary positions with up to four axes, for the queries and keys of a layer in one launch, behind the RMS norm of every head where its
  * weights are given.  Of the R = sum(axis_dim) rotated channels of a head, pair i is (2 i, 2 i + 1) or, with `halves`, (i, i + R / 2); axis a
  * has the next axis_dim[a] / 2 pairs.  Pair j of axis a turns by positions[b][t][a] * theta[a]^(-2 j / axis_dim[a]); with
- * `whole_spectrum` pair i of the head by positions[b][t][a] * theta[a]^(-2 i / R).  Angles are 64 bits, the rest fp32.  The channels behind
- * the R are not turned.
+ * `whole_spectrum` pair i of the head by positions[b][t][a] * theta[a]^(-2 i / R).  An angle is right to 2^-55 of itself (2^-24
+ * radians at a position of 2^31), the rest is fp32.  The channels behind the R are not turned.
  * ------------------------------------------------------------------------------------------ */
 #define SVDQ_POSITION_INT32 0
 #define SVDQ_POSITION_INT64 1

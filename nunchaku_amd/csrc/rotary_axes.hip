@@ -2,9 +2,9 @@
 // (i, i + R / 2) of the R rotated channels of a head, and the pairs in runs, one for each axis of the positions (time, height, width).  With the
 // angle phi = position[axis] * frequency[pair] a pair (x, y) becomes (x cos phi - y sin phi, x sin phi + y cos phi).  Channels behind the R pass.
 //
-// Angles.  A frequency in revolutions, theta^(-e) / (2 pi), comes from the host in 64 bits; position times frequency, less the nearest whole number of
-// revolutions, is right to 2^-24 revolutions for positions of 2^31 and to 2^-34 for those of 2^21, where 32 bits would have lost all but 2^-6.  Sine and
-// cosine see half a revolution at most.
+// Angles.  A frequency in revolutions, theta^(-e) / (2 pi), comes from the host in two parts, 64 bits and the next ones: one of 53 bits alone would leave 2^-22
+// radians of a position of 2^31 open, more than fp32 rounds by.  The product's high part loses its whole revolutions before the low ones are added.  What is
+// left open is what 80 bits leave of the frequency on the host, 2^-55 of the angle at most (2^-24 radians at 2^31).  Sine and cosine see half a revolution at most.
 // They are the same for all heads of a token: a wave makes those of its token once, a pair to a lane, and hands them round through LDS.
 #include <math.h>
 
@@ -27,6 +27,7 @@ struct RotaryParams {
     int once;                           // the tensors do not fit the memory-side cache: what is read is not kept there
     float inv_d, eps, tiny;
     double freq[MAX_PAIRS];  // revolutions per position
+    float low[MAX_PAIRS];    // what 64 bits leave of them
     uint8_t axis[MAX_PAIRS];
 };
 
@@ -127,11 +128,24 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(RotaryParams p) {
     }
     for (int pair = lane; pair < p.pairs; pair += 64) {
         const long long from = b * p.pos_s[0] + t * p.pos_s[1] + p.axis[pair] * p.pos_s[2];
-        const double x = p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[from]
-                         : p.position_type == SVDQ_POSITION_INT64 ? (double)((const int64_t *)p.positions)[from] : (double)((const float *)p.positions)[from];
-        const double revolutions = x * p.freq[pair];
+        const double freq = p.freq[pair], low = (double)p.low[pair];
+        auto fraction = [&](double x) __attribute__((always_inline)) {  // of x positions' revolutions
+            const double whole = x * freq, r = (whole - __builtin_rint(whole)) + (__builtin_fma(x, freq, -whole) + x * low);
+            return r - __builtin_rint(r);
+        };
+        double r;
+        if (p.position_type == SVDQ_POSITION_INT64) {
+            const int64_t x = ((const int64_t *)p.positions)[from], rest = x < 1ll << 53 && x > -(1ll << 53) ? 0 : x & 2047;  // (the rest fits 64 bits)
+            r = fraction((double)(x - rest));
+            if (rest) {
+                r += fraction((double)rest);
+                r -= __builtin_rint(r);
+            }
+        } else {
+            r = fraction(p.position_type == SVDQ_POSITION_INT32 ? (double)((const int32_t *)p.positions)[from] : (double)((const float *)p.positions)[from]);
+        }
         float s, co;
-        sincospif(2.0f * (float)(revolutions - __builtin_rint(revolutions)), &s, &co);
+        sincospif(2.0f * (float)r, &s, &co);
         table[wave][pair] = float2_t{co, s};
     }
     __builtin_amdgcn_wave_barrier();  // (LDS serves a wave in order)
@@ -273,7 +287,8 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
     p.inv_d = 1.0f / (float)a->head_dim;
     p.eps = a->eps;
     p.tiny = a->eps >= 0x1p-120f ? 0.f : 0x1p-100f;
-    // An axis' frequencies are a geometric series; its products in 80 bits are right to more than the 64 bits they are rounded to
+    // An axis' frequencies are a geometric series.  80 bits round by 2^-64: number j is off by 3 j of that for the products and the step's exponential, by 3 e log(theta) for the
+    // logarithm and the exponent, and by 4, which for 128 pairs and any theta up to 10^15 is less than 2^-55
     int pair = 0;
     for (int i = 0; i < a->axes; i++) {
         const long double span = a->whole_spectrum ? (long double)rotated : (long double)a->axis_dim[i], rate = -logl((long double)a->theta[i]);
@@ -281,6 +296,7 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
         long double f = (a->whole_spectrum ? expl(rate * 2.0L * pair / span) : 1.0L) / 6.283185307179586476925286766559L;
         for (int j = 0; j < a->axis_dim[i] / 2; j++, pair++, f *= step) {
             p.freq[pair] = (double)f;
+            p.low[pair] = (float)(f - (long double)p.freq[pair]);
             p.axis[pair] = (uint8_t)i;
         }
     }

@@ -44,8 +44,8 @@ def rotary_axes(
     them is (2 i, 2 i + 1), or (i, i + R / 2) with ``interleaved`` false (R is then a multiple of 16).  Axis a has the next axes[a] / 2 pairs.  Pair j of an
     axis of n channels turns by position * theta^(-2 j / n) (``spectrum`` "axis"); with "head" pair i of the head turns by its axis' position *
     theta^(-2 i / R), as where the axes share one spectrum.  ``theta``: one number, or one for each axis.
-    ``positions`` int32, int64 or fp32 (between whole numbers, too) [B, T, len(axes)] or [T, len(axes)], by any strides; far positions lose nothing: angles
-    are 64 bits.  The rest is fp32, rounded once.
+    ``positions`` int32, int64 or fp32 (between whole numbers, too) [B, T, len(axes)] or [T, len(axes)], by any strides.  An angle is right to 2^-55 of
+    itself before its whole revolutions are dropped: positions up to 2^31 lose nothing that fp32 could hold, one of 2^40 up to 3e-5 radians.  The rest is fp32, rounded once.
 
     D is a multiple of 8 up to 256.  q and k go by their strides (multiples of 8, elements of a head next to each other), as parts of a fused
     projection do.  ``out_q`` and ``out_k`` take the results when given; they may be ``q`` and ``k`` themselves.  Forward only."""
