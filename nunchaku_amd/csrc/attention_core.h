@@ -155,15 +155,6 @@ struct State {
             vf[d] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
-    // that of block d alone
-    static __device__ inline vec read_v(const char *v, int n, int d, int lane) {
-        const int g = lane >> 4, i = lane & 15, h = lane >> 5;
-        typedef short short4_t __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) short4_t *lds_t;
-        const char *at = v + (4 * h + (i >> 2)) * H::PITCH + (i & 1) * 8 + 16 * n * H::PITCH + ((4 * d + (g & 1) * 2 + ((i >> 1) & 1)) ^ H::fv(i >> 2)) * 16;
-        const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at + 8 * H::PITCH));
-        return __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
     // the right operand: probabilities of 16 keys, rounded
     template <int NB, bool ONES>
     __device__ inline vec exponentials(const float16_t (&s)[NB], int n, float scale2, float ref) {

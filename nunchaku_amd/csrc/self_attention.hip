@@ -612,35 +612,36 @@ struct Softmax : State<BF16, H> {
     }
 };
 
-// The end of a wave's 32 rows: the quotients, or an item's share of them
-template <bool BF16, typename H, int BLOCK_ROWS>
-__device__ inline void finish(const Params &p, const Item &it, const Rows &r, const Softmax<BF16, H> &st, bool careful, int hk, int wave, int lane) {
-    const int col = lane & 31, h = lane >> 5;
-    const float sum = st.whole_sum(p.D, careful, lane);
-    if (it.parts > 1) {
-        if (!r.in) return;
-        float *dst = share_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
-#pragma unroll
-        for (int d = 0; d < H::DB; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int c = 32 * d + 8 * g + 4 * h;
-                if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
-            }
-        if (h == 0) {
-            float *ms = stats_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
-            ms[0] = st.top;
-            ms[1] = sum;
-        }
-        return;
-    }
-    const float inv = inverse(sum);
+// The end of a wave's 32 rows: the quotients
+template <bool BF16, typename H>
+__device__ inline void finish(const Params &p, const Rows &r, const Softmax<BF16, H> &st, bool careful, int lane) {
+    const float inv = inverse(st.whole_sum(p.D, careful, lane));
 #pragma unroll
     for (int u = 0; u < 2 * H::DB; u++) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = st.o[u >> 1][8 * (u & 1) + e];
         store_columns<BF16>(r.out, x, inv, 16 * u, r.in ? p.D : 0, lane);
+    }
+}
+// or an item's share of them
+template <bool BF16, typename H, int BLOCK_ROWS>
+__device__ inline void finish_part(const Params &p, const Item &it, const Rows &r, const Softmax<BF16, H> &st, bool careful, int hk, int wave, int lane) {
+    const int col = lane & 31, h = lane >> 5;
+    const float sum = st.whole_sum(p.D, careful, lane);
+    if (!r.in) return;
+    float *dst = share_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
+#pragma unroll
+    for (int d = 0; d < H::DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int c = 32 * d + 8 * g + 4 * h;
+            if (c < p.D) *(float4_t *)(dst + c) = float4_t{st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]};
+        }
+    if (h == 0) {
+        float *ms = stats_of<BLOCK_ROWS>(p, it.index, hk, wave * 32 + col);
+        ms[0] = st.top;
+        ms[1] = sum;
     }
 }
 
@@ -751,7 +752,8 @@ __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) self_att
             }
         }
     }
-    finish<BF16, H, HALF>(p, it, r, st, careful, hk, wave, lane);
+    if (it.parts > 1) finish_part<BF16, H, HALF>(p, it, r, st, careful, hk, wave, lane);
+    else finish<BF16, H>(p, r, st, careful, lane);
 }
 
 // ---- turns form: 256 rows per workgroup, 32 per wave; all eight waves share the keys through LDS, 64 a step, four steps of them -----------
@@ -863,23 +865,16 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
-    Item it = p.target ? part_of<ROWS, KEYS, false>(p, at, lane) : item_of<ROWS>(p, at, lane);
+    const Item it = item_of<ROWS>(p, at, lane);
     if (!it.any) return;
     const int wave0 = it.rb * ROWS + wave * 32;
-    Rows r = rows_of(p, it.r, hk, wave0 + col);
-    int least, most, wave_least, wave_most, begin, end;
+    const Rows r = rows_of(p, it.r, hk, wave0 + col);
+    int least, most, wave_least, wave_most;
     limits_of(p, r, it.rb * ROWS, ROWS, least, most);
     limits_of(p, r, wave0, 32, wave_least, wave_most);
     vec qf[H::KS];
     load_q<BF16, H>(p, qf, r, lane);
-    // a part's keys: limits from its first one on
-    if (!share<KEYS>(it, most, begin, end)) return;
-    const int skip = begin * KEYS, stop = end * KEYS;
-    most = (most < stop ? most : stop) - skip;
-    wave_most = (wave_most < stop ? wave_most : stop) - skip;
-    wave_least -= skip;
-    r.limit -= skip;
-    RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk) + skip * p.ks[1], first_key(p, it.r, p.v, p.vs, hk) + skip * p.vs[1], most, wave, lane);
+    RowCopies<H> copies(p, lds, first_key(p, it.r, p.k, p.ks, hk), first_key(p, it.r, p.v, p.vs, hk), most, wave, lane);
     const int steps = copies.steps;
     const bool late = wave >= WAVES / 2;
     const int ahead = late ? STAGES - 1 : STAGES - 2;  // steps
@@ -1015,7 +1010,9 @@ __global__ void __launch_bounds__(512, 2) self_attention_turns_kernel(Params p) 
             }
         }
     }
-    finish<BF16, H, ROWS>(p, it, r, st, careful, hk, wave, lane);
+    int row = wave0 + col;
+    asm volatile("" : "+v"(row));  // (where the row goes is worked out anew: two registers through the loop are two too many)
+    finish<BF16, H>(p, rows_of(p, it.r, hk, row), st, careful, lane);
 }
 
 // Adds the parts of every row (at most 64): four rows of a block per workgroup, a wave to a row, two columns per lane, 16 parts asked for at once; lane i holds part i's
@@ -1088,7 +1085,7 @@ __global__ void __launch_bounds__(256) self_attention_join_kernel(Params p) {
     if (lane * 2 < p.D) *(uint32_t *)(r.out + c * 2) = Elem<BF16>::pair(x * inv, y * inv);
 }
 
-enum Form { BY_KEYS, BY_ROWS, BY_TURNS };
+enum Form { BY_KEYS, BY_ROWS, BY_TURNS };  // (keys in parts: the first two alone)
 
 template <bool BF16, int DP, bool ONES>
 int launch_kernels(const Params &p, Form form, hipStream_t st) {
@@ -1108,8 +1105,7 @@ int launch_kernels(const Params &p, Form form, hipStream_t st) {
     int rc = check_launch("self_attention");
     if (rc || !p.target) return rc;
     if (form == BY_KEYS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, 32, 32>), dim3((unsigned)(p.blocks * 8 * p.Hkv)), dim3(256), 0, st, p);
-    else if (form == BY_ROWS) SVDQ_LAUNCH((self_attention_join_kernel<BF16, HALF, KEYS>), dim3((unsigned)(p.blocks * (HALF / 4) * p.Hkv)), dim3(256), 0, st, p);
-    else return fail(SVDQ_EUNSUPPORTED, "self_attention: parts of the keys of 256 rows");  // (no plan has them)
+    else SVDQ_LAUNCH((self_attention_join_kernel<BF16, HALF, KEYS>), dim3((unsigned)(p.blocks * (HALF / 4) * p.Hkv)), dim3(256), 0, st, p);
     return check_launch("self_attention");
 }
 
