@@ -6,8 +6,8 @@
 // The mean is taken before the deviations' squares are summed, from registers: their difference in one pass would lose what a large mean leaves.  So would the
 // mean's own rounding, 2^-24 of it beside a spread that may be less: the deviations are summed with their squares, and what they have in common is taken out of both.
 // Squares whose sum leaves fp32's range, at either end, are summed once more in 64 bits: rows of finite numbers have finite norms.
-// Bound by the traffic, 8 bytes an element with a residual: 2 x 4608 x 5120 72 us, 5.3 TB/s (a copy reaches 5.1 here), 4096 x 4096 21.6, 6.2 TB/s; one row of 4096 with
-// both norms 3.0, launch and latencies.
+// Bound by the traffic, 8 bytes an element with a residual: 2 x 4608 x 5120 72 us, 5.2 TB/s (a copy reaches 5.1 here), 4096 x 4096 21.6, 6.2 TB/s; one row of 4096 with
+// both norms 2.8, launch and latencies.
 #include "svdq_common.h"
 
 using namespace svdq;

@@ -527,8 +527,9 @@ struct Softmax : State<BF16, H> {
     }
     // Whether a step's maximum has to be looked for.  In bf16, every LOOKS-th alone: probabilities have fp32's range, and sums of 2^64 or more, or an infinity or a NaN among the
     // outputs, send the rows through `attend_carefully`, which looks at every step.  As long as a row has no reference at all, at every step, so that its sums are zero when it gets
-    // one.  (In fp16 a rise of 2^9 between two looks would be beyond the range.)  16384 tokens, 8 heads of 128 885 -> 856 us, 8192 tokens, 16 heads of 64
-    // 296 -> 288, 4608 tokens, 24 heads of 72 186 -> 176, 1024 tokens, 24 heads of 128 23.3 -> 23.4.
+    // one.  (In fp16 a rise of 2^9 between two looks would be beyond the range.)  16384 tokens, 8 heads of 128 897 -> 863 us, 8192 tokens, 16 heads of 64
+    // 299 -> 284, 4608 tokens, 24 heads of 72 189 -> 180, 1024 tokens, 24 heads of 128 23.8 -> 23.4.  The price: finite scores that rise by 44 or more between two looks are
+    // worked out twice, the second time without overlap.  The same three, one key 90 above those in front of it: 860 -> 1980, 283 -> 651, 178 -> 425.
     static constexpr int LOOKS = 8;
     __device__ inline bool due(int step) const { return !BF16 || step % LOOKS == 0 || __any(this->top == -__builtin_huge_valf()); }
     __device__ inline void raise(float high, float scale2, int lane) {
@@ -1137,16 +1138,17 @@ long long blocks_of(const svdq_self_attention_args *a, long long size) {
 
 // Which form a call takes and into how many parts it divides the keys of an average sequence: the least time by a model of the busiest compute unit, us.  Its constants are
 // those of 252 shapes (heads of 32 to 128, 1 .. 8192 queries, causal or not), each in every form and 1 .. 32 parts; what it chooses is 1 to 2 % behind the fastest on average,
-// 26 % at most (1024 tokens, 32 heads over 8 of 32, causal, 14.4 us against 11.4).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.5 / keys 7.9, turns 7.3; 1024 tokens,
-// 32 heads over 8 of 128, causal rows 24.9 / keys 54, turns 29; 16384 tokens, 8 heads of 128 turns 920 / rows 1020; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128
-// 29.6 in eight parts / 116 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 25.0 / keys in four 39.3; 4096 tokens, 8 heads of 128, causal rows in two parts
-// 64.8 / whole 75, turns 83.
-// Sequences of other lengths than the average have parts in proportion.
+// 27 % at most (1024 tokens, 32 heads over 8 of 32, causal, 14.3 us against 11.3).  Chosen / others, us: 4 x 64 tokens, 8 heads of 128 rows 6.4 / keys 7.9, turns 7.3; 1024 tokens,
+// 32 heads over 8 of 128, causal rows 24.6 / keys 54, turns 29; 16384 tokens, 8 heads of 128 turns 863 / rows 961; single tokens of 4 sequences of 8192 keys, 32 heads over 8 of 128
+// 29.6 in eight parts / 115 whole; 64 tokens behind 8192, 32 over 8 heads of 128 rows in 16 parts 24.4 / keys in four 38.7; 4096 tokens, 8 heads of 128, causal rows in two parts
+// 62.9 / whole 74, turns 82.
+// Sequences of other lengths than the average have parts in proportion; of a cache the average is what it has room for.  One model for bf16 and fp16, whose steps take 3 to 6 %
+// more, and without the memory's rate: 100 single tokens over 8192 keys of two heads of 128, 840 MB, are 112 us by it and take 160 (in parts 168 or more).
 struct Cost {
     int head_dim;                   // up to
     float keys_base, round;         // keys form: first and last; a round of four waves' 32 keys
     float rows_base, rows_step;     // rows form: the same; a step of 64 keys
-    float turns_base, turns_step;   // turns form, which heads up to 64 never take: 8192 tokens, 16 heads of 64 307 us by turns, 300 by rows, causal 632 and 573; of 32 255 and 212
+    float turns_base, turns_step;   // turns form, which heads up to 64 never take: 8192 tokens, 16 heads of 64 307 us by turns, 300 by rows, causal 632 and 573; of 32 255 and 212 (maxima at every step)
     float join, join_bytes;         // parts: the second launch; bytes a us of their way there and back
 };
 constexpr Cost costs[] = {{64, 4.2f, 0.72f, 4.3f, 0.69f, 0.f, 0.f, 5.4f, 3.5e6f}, {96, 5.7f, 1.45f, 4.8f, 0.95f, 5.5f, 1.10f, 5.6f, 5.2e6f}, {128, 6.1f, 1.65f, 5.6f, 1.06f, 7.0f, 1.30f, 5.5f, 6.2e6f}};

@@ -131,7 +131,10 @@ def self_attention(
 
     D is a multiple of 8 up to 128.  Tensors go by their strides (multiples of 8, elements of a head next to each other).  ``out`` takes the result
     when given and must not overlap the inputs.  ``scale``: 1 / sqrt(D) by default, positive.  Forward only: the result carries no gradient.  Precision
-    and range of scores are those of ``cross_attention``."""
+    and range of scores are those of ``cross_attention``; finite bf16 scores of a row that rise by more than 44 within 448 keys take 2.4 times as long.
+
+    Batches without a causal mask can go to either operator: from about a thousand queries and keys on this one is faster (4608 tokens, 24 heads of 128 244 us,
+    ``cross_attention`` 293), with some hundred keys or single tokens the other (300 tokens 9.4 us, this 11.1)."""
     if out is None:
         y = nv.host().self_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, key_lengths, causal, scale)
         if y is not None:
