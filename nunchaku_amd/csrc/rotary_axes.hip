@@ -296,7 +296,7 @@ extern "C" int svdq_rotary_axes(const svdq_rotary_axes_args *a, void *stream) {
         long double f = (a->whole_spectrum ? expl(rate * 2.0L * pair / span) : 1.0L) / 6.283185307179586476925286766559L;
         for (int j = 0; j < a->axis_dim[i] / 2; j++, pair++, f *= step) {
             p.freq[pair] = (double)f;
-            p.low[pair] = (float)(f - (long double)p.freq[pair]);
+            p.low[pair] = f < 0x1p170L ? (float)(f - (long double)p.freq[pair]) : 0.f;  // (those beyond, of a theta near zero, have nothing left of their angles)
             p.axis[pair] = (uint8_t)i;
         }
     }

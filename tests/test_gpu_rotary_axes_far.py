@@ -65,3 +65,14 @@ def test_far_positions(dev, kind, theta, interleaved):
     if kind == "int64_31":  # whole numbers of another type: the same bits
         again = rotary_axes(q[3:].to(dev), None, pos[3:, None].int().to(dev), (D,), theta=theta, interleaved=interleaved)[0]
         assert torch.equal(again[:, 0].cpu().double(), got[3:])
+
+
+@pytest.mark.parametrize("theta", [1e-30, 1e-60, 1e-200])
+def test_theta_near_zero(dev, theta):
+    """Frequencies beyond fp32: position zero turns nothing, others stay finite."""
+    from nunchaku_amd.ops import rotary_axes
+
+    q = torch.randn(4, 2, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    pos = torch.tensor([0, 1, 5, -7], dtype=torch.int32, device=dev)[:, None]
+    got = rotary_axes(q, None, pos, (64,), theta=theta)[0]
+    assert torch.equal(got[0], q[0]) and got.isfinite().all()
